@@ -305,6 +305,11 @@ enum KernelKind : int {
   K_GATHER,
   K_DECODE,
   K_STREAM_READ,
+  K_ROPE,
+  K_KV_STORE,
+  K_KV_READ,
+  K_KV_PAGES,
+  K_KV_ATTENTION,
   K_KINDS
 };
 

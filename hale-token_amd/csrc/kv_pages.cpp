@@ -1,0 +1,290 @@
+// kv_pages.cpp -- page bookkeeping and step plans of the key/value cache.
+#include "kv_pages.h"
+
+#include <algorithm>
+#include <cstdio>
+
+namespace hale {
+
+namespace {
+
+KvPages::Status refuse(std::string* err, KvPages::Status s, const char* fmt, size_t a, size_t b = 0, size_t c = 0) {
+  char buf[192];
+  std::snprintf(buf, sizeof buf, fmt, a, b, c);
+  *err = buf;
+  return s;
+}
+
+size_t ceil_div(size_t a, size_t b) { return (a + b - 1) / b; }
+
+}  // namespace
+
+void KvPages::init(size_t pages, size_t max_seqs, size_t max_len) {
+  max_len_ = max_len;
+  max_pages_ = ceil_div(max_len, KV_PAGE);
+  refs_.assign(pages, 0);
+  free_.resize(pages);
+  for (size_t i = 0; i < pages; i++) free_[i] = (uint32_t)(pages - 1 - i);  // the lowest is taken first
+  seqs_.resize(max_seqs);
+  for (Seq& s : seqs_) s.pages.reserve(max_pages_ < 64 ? max_pages_ : 64);
+  free_seqs_.resize(max_seqs);
+  for (size_t i = 0; i < max_seqs; i++) free_seqs_[i] = (uint32_t)(max_seqs - 1 - i);
+  mark_.assign(max_seqs, 0);
+}
+
+KvPages::Status KvPages::find(uint32_t seq, std::string* err) const {
+  if (live(seq)) return OK;
+  return refuse(err, BAD, "no sequence %zu", seq);
+}
+
+uint32_t KvPages::take() {
+  const uint32_t p = free_.back();
+  free_.pop_back();
+  refs_[p] = 1;
+  return p;
+}
+
+void KvPages::drop(uint32_t page) {
+  if (--refs_[page] == 0) free_.push_back(page);
+}
+
+void KvPages::set(uint32_t seq, size_t index) { dirty.push_back((uint32_t)(seq * max_pages_ + index)); }
+
+KvPages::Status KvPages::create(uint32_t* seq, std::string* err) {
+  if (free_seqs_.empty()) return refuse(err, FULL, "all %zu sequences are in use", seqs_.size());
+  *seq = free_seqs_.back();
+  free_seqs_.pop_back();
+  Seq& s = seqs_[*seq];
+  s.live = true;
+  s.len = 0;
+  s.pages.clear();
+  return OK;
+}
+
+KvPages::Status KvPages::free(uint32_t seq, std::string* err) {
+  const Status st = find(seq, err);
+  if (st) return st;
+  free_seqs_.push_back(seq);  // reserved at init: holds every sequence
+  Seq& s = seqs_[seq];
+  for (uint32_t p : s.pages) drop(p);
+  s.pages.clear();
+  s.live = false;
+  s.len = 0;
+  return OK;
+}
+
+KvPages::Status KvPages::fork(uint32_t seq, size_t n, uint32_t* out, std::string* err) {
+  const Status st = find(seq, err);
+  if (st) return st;
+  if (n > free_seqs_.size()) return refuse(err, FULL, "%zu forks, but only %zu of %zu sequences are free", n, free_seqs_.size(), seqs_.size());
+  const size_t np = seqs_[seq].pages.size();
+  dirty.reserve(dirty.size() + n * np);
+  for (size_t i = 0; i < n; i++) seqs_[free_seqs_[free_seqs_.size() - 1 - i]].pages.reserve(np);
+  for (size_t i = 0; i < n; i++) {
+    uint32_t id = 0;
+    (void)create(&id, err);
+    Seq& s = seqs_[id];
+    s.pages = seqs_[seq].pages;
+    s.len = seqs_[seq].len;
+    for (size_t j = 0; j < np; j++) {
+      refs_[s.pages[j]]++;
+      set(id, j);
+    }
+    out[i] = id;
+  }
+  return OK;
+}
+
+KvPages::Status KvPages::copy(uint32_t seq, uint32_t* out, std::vector<KvCopy>* copies, std::string* err) {
+  const Status st = find(seq, err);
+  if (st) return st;
+  const size_t np = seqs_[seq].pages.size();
+  if (np > free_.size()) return refuse(err, FULL, "a copy of %zu pages, but only %zu of %zu are free", np, free_.size(), refs_.size());
+  if (free_seqs_.empty()) return refuse(err, FULL, "all %zu sequences are in use", seqs_.size());
+  dirty.reserve(dirty.size() + np);
+  copies->reserve(copies->size() + np);
+  seqs_[free_seqs_.back()].pages.reserve(np);
+  (void)create(out, err);
+  Seq& s = seqs_[*out];
+  s.len = seqs_[seq].len;
+  for (size_t j = 0; j < np; j++) {
+    const uint32_t p = take();
+    s.pages.push_back(p);
+    copies->push_back({seqs_[seq].pages[j], p});
+    set(*out, j);
+  }
+  return OK;
+}
+
+KvPages::Status KvPages::truncate(uint32_t seq, size_t len, std::string* err) {
+  const Status st = find(seq, err);
+  if (st) return st;
+  Seq& s = seqs_[seq];
+  if (len > s.len) return refuse(err, BAD, "sequence %zu holds %zu positions, not %zu", seq, s.len, len);
+  while (s.pages.size() > ceil_div(len, KV_PAGE)) {
+    drop(s.pages.back());
+    s.pages.pop_back();
+  }
+  s.len = len;
+  return OK;
+}
+
+KvPages::Status KvPages::len(uint32_t seq, size_t* len, std::string* err) const {
+  const Status st = find(seq, err);
+  if (st) return st;
+  *len = seqs_[seq].len;
+  return OK;
+}
+
+KvPages::Status KvPages::check_step(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, std::string* err) {
+  if (++stamp_ == 0) {  // wrapped: no mark may equal the new stamp
+    std::fill(mark_.begin(), mark_.end(), 0u);
+    stamp_ = 1;
+  }
+  need_ = copies_ = 0;
+  for (size_t i = 0; i < nseq; i++) {
+    const Status st = find(seqs[i], err);
+    if (st) return st;
+    if (mark_[seqs[i]] == stamp_) return refuse(err, BAD, "sequence %zu twice in one step", seqs[i]);
+    mark_[seqs[i]] = stamp_;
+    const Seq& s = seqs_[seqs[i]];
+    if (ntok[i] > max_len_ - s.len)
+      return refuse(err, BAD, "sequence %zu: context overflow, %zu positions needed, at most %zu", seqs[i], s.len + ntok[i], max_len_);
+    need_ += ceil_div(s.len + ntok[i], KV_PAGE) - s.pages.size();
+  }
+  // Shared pages that are written to.  Of k sequences of this step on a page
+  // that r sequences hold, k copy it where r > k; where r == k the last one
+  // writes in place.  Counted by taking the references off and putting them back.
+  for (size_t i = 0; i < nseq; i++) {
+    const Seq& s = seqs_[seqs[i]];
+    if (ntok[i] && s.len % KV_PAGE && refs_[s.pages.back()] > 1) {
+      refs_[s.pages.back()]--;
+      copies_++;
+      mark_[seqs[i]] = 0;  // copies
+    }
+  }
+  for (size_t i = 0; i < nseq; i++)
+    if (mark_[seqs[i]] == 0) refs_[seqs_[seqs[i]].pages.back()]++;
+  need_ += copies_;
+  if (need_ > free_.size()) return refuse(err, FULL, "%zu pages needed, but only %zu of %zu are free", need_, free_.size(), refs_.size());
+  return OK;
+}
+
+KvPages::Status KvPages::step(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, std::vector<KvStepSeq>* plan,
+                              std::vector<KvCopy>* copies, std::string* err) {
+  const Status st = check_step(nseq, seqs, ntok, err);
+  if (st) return st;
+  plan->resize(nseq);
+  copies->reserve(copies->size() + copies_);
+  dirty.reserve(dirty.size() + need_);
+  for (size_t i = 0; i < nseq; i++) {
+    Seq& s = seqs_[seqs[i]];
+    s.pages.reserve(ceil_div(s.len + ntok[i], KV_PAGE));
+  }
+  uint32_t tok0 = 0;
+  for (size_t i = 0; i < nseq; i++) {
+    Seq& s = seqs_[seqs[i]];
+    (*plan)[i] = {seqs[i], (uint32_t)s.len, ntok[i], tok0};
+    tok0 += ntok[i];
+    if (mark_[seqs[i]] == 0) {
+      const uint32_t p = take();
+      copies->push_back({s.pages.back(), p});
+      refs_[s.pages.back()]--;  // others hold it: it never becomes free here
+      s.pages.back() = p;
+      set(seqs[i], s.pages.size() - 1);
+    }
+    s.len += ntok[i];
+    while (s.pages.size() * KV_PAGE < s.len) {
+      s.pages.push_back(take());
+      set(seqs[i], s.pages.size() - 1);
+    }
+  }
+  return OK;
+}
+
+void KvPages::compact(std::vector<KvCopy>* copies) {
+  const size_t n = used();
+  std::vector<uint32_t> to(refs_.size());
+  size_t hole = 0, moved = 0;
+  for (size_t p = n; p < refs_.size(); p++) moved += refs_[p] != 0;
+  copies->reserve(copies->size() + moved);
+  size_t entries = 0;
+  for (const Seq& s : seqs_)
+    for (uint32_t p : s.pages) entries += p >= n;
+  dirty.reserve(dirty.size() + entries);
+  for (size_t p = n; p < refs_.size(); p++) {
+    if (!refs_[p]) continue;
+    while (refs_[hole]) hole++;
+    to[p] = (uint32_t)hole;
+    copies->push_back({(uint32_t)p, (uint32_t)hole});
+    refs_[hole] = refs_[p];
+    refs_[p] = 0;
+  }
+  for (uint32_t id = 0; id < seqs_.size(); id++)
+    for (size_t j = 0; j < seqs_[id].pages.size(); j++)
+      if (seqs_[id].pages[j] >= n) {
+        seqs_[id].pages[j] = to[seqs_[id].pages[j]];
+        set(id, j);
+      }
+  free_.clear();  // keeps its room
+  for (size_t p = refs_.size(); p > n; p--) free_.push_back((uint32_t)(p - 1));
+}
+
+void KvPages::resize(size_t pages) {
+  const size_t n = used();
+  std::vector<uint32_t> refs(pages, 0), rest;
+  rest.reserve(pages);  // drop() never allocates
+  std::copy(refs_.begin(), refs_.begin() + n, refs.begin());
+  for (size_t p = pages; p > n; p--) rest.push_back((uint32_t)(p - 1));
+  refs_.swap(refs);
+  free_.swap(rest);
+}
+
+void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window, KvPlan* out) {
+  out->items.clear();
+  out->joins.clear();
+  out->parts = 0;
+  const size_t group = s.group();
+  size_t most = 0;
+  for (const KvStepSeq& q : seqs) most = std::max(most, q.ntok * group);
+  out->cols = most <= 16 ? 1 : kv_max_cols(s.head_dim);
+  const size_t rows = 16 * (size_t)out->cols;
+  // the pages that rows row0 .. row0 + n - 1 of sequence q see
+  auto range = [&](const KvStepSeq& q, size_t row0, size_t n, size_t* first, size_t* last) {
+    const size_t low = q.len0 + row0 / group, high = q.len0 + (row0 + n - 1) / group;
+    *first = window && low + 1 > window ? (low + 1 - window) / KV_PAGE : 0;
+    *last = high / KV_PAGE + 1;
+  };
+  size_t total = 0, a, b;
+  for (const KvStepSeq& q : seqs)
+    for (size_t r = 0; r < q.ntok * group; r += rows) {
+      range(q, r, std::min(rows, q.ntok * group - r), &a, &b);
+      total += b - a;
+    }
+  total *= s.kv_heads;
+  // a work-group's waves take a page each: fewer than four leave some idle
+  const size_t each = std::max<size_t>(4, ceil_div(total, KV_TARGET_GROUPS));
+  for (uint32_t i = 0; i < seqs.size(); i++) {
+    const KvStepSeq& q = seqs[i];
+    // the rows with the most pages first, so that the last work-groups are short
+    const size_t tiles = ceil_div(q.ntok * group, rows);
+    for (size_t t = tiles; t-- > 0;) {
+      const size_t r = t * rows, n = std::min(rows, q.ntok * group - r);
+      range(q, r, n, &a, &b);
+      const size_t parts = ceil_div(b - a, each);
+      for (uint32_t h = 0; h < s.kv_heads; h++) {
+        if (parts > 1) out->joins.push_back({i, h, (uint32_t)r, (uint32_t)n, out->parts, (uint32_t)parts, {0, 0}});
+        for (size_t k = 0; k < parts; k++)
+          out->items.push_back({i, h, (uint32_t)r, (uint32_t)n, (uint32_t)(a + (b - a) * k / parts),
+                                (uint32_t)(a + (b - a) * (k + 1) / parts), parts > 1 ? out->parts++ : KV_WHOLE, 0});
+      }
+    }
+  }
+}
+
+size_t kv_max_items(const KvShape& s, size_t tokens, size_t nseq) {
+  // tiles of 16 rows or more, one more per sequence for the last, and the further parts of divided ones
+  return (tokens * s.group() / 16 + nseq) * s.kv_heads + KV_MAX_PARTS;
+}
+
+}  // namespace hale

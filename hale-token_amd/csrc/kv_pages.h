@@ -1,0 +1,151 @@
+// kv_pages.h -- the pages of a key/value cache and the plan of one step over
+// it: which page holds which positions of which sequence, how many sequences
+// share it, and how the attention of a step is divided.  Host-only C++: no
+// entry here touches the device; what has to move there is returned as lists.
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include <string>
+#include <vector>
+
+namespace hale {
+
+constexpr size_t KV_PAGE = 64;   // positions per page (HALE_KV_PAGE)
+constexpr size_t KV_BLOCK = 16;  // positions per scale (HALE_KV_BLOCK)
+
+// One sequence's share of a step, as the kernels read it.
+struct KvStepSeq {
+  uint32_t row;    // its row of the page table
+  uint32_t len0;   // positions held before the step
+  uint32_t ntok;   // new tokens
+  uint32_t tok0;   // the first one's index among the step's tokens
+};
+
+// A block of 16 positions that the step's tokens touch.
+struct KvBlock {
+  uint32_t seq, block;  // index into the step's sequences; position / 16
+};
+
+// One work-group's share of the attention: rows row0 .. row0 + rows - 1 of a
+// sequence's queries of one key/value head (row r is token r / group, head
+// r % group of the group) over pages page0 .. page1 - 1.
+struct KvItem {
+  uint32_t seq, head, row0, rows;
+  uint32_t page0, page1;
+  uint32_t part;  // its slot among the partial results, or KV_WHOLE
+  uint32_t pad;
+};
+constexpr uint32_t KV_WHOLE = 0xffffffffu;
+
+// Partial results part0 .. part0 + parts - 1 to be joined, the rows of one item.
+struct KvJoin {
+  uint32_t seq, head, row0, rows;
+  uint32_t part0, parts;
+  uint32_t pad[2];
+};
+
+// The attention of a step under one window.
+struct KvPlan {
+  int cols = 1;  // groups of 16 rows per work-group: 1 or 2
+  std::vector<KvItem> items;
+  std::vector<KvJoin> joins;
+  uint32_t parts = 0;
+};
+
+struct KvCopy {
+  uint32_t src, dst;
+};
+
+struct KvShape {
+  size_t heads, kv_heads, head_dim;
+  size_t group() const { return heads / kv_heads; }
+};
+
+// Work-groups that a step's attention is divided into where its length allows,
+// and with it the most partial results (see kv_plan).
+constexpr size_t KV_TARGET_GROUPS = 512;
+constexpr size_t KV_MAX_PARTS = 2 * KV_TARGET_GROUPS;
+
+// Most groups of 16 rows that the attention kernels hold at once.
+inline int kv_max_cols(size_t head_dim) { return head_dim <= 192 ? 2 : 1; }
+
+// Divides the attention of a step: rows of 16 * cols per work-group, few
+// enough pages each that all compute units take part.  Window 0 sees every
+// earlier position.
+void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window, KvPlan* out);
+
+// Most items and blocks that a plan of so many tokens and sequences can have.
+size_t kv_max_items(const KvShape& s, size_t tokens, size_t nseq);
+inline size_t kv_max_blocks(size_t tokens, size_t nseq) { return tokens / KV_BLOCK + 2 * nseq; }
+
+// The pool's pages, their owners and the sequences.
+class KvPages {
+ public:
+  // Throws std::bad_alloc.
+  void init(size_t pages, size_t max_seqs, size_t max_len);
+
+  size_t pages() const { return refs_.size(); }
+  size_t used() const { return refs_.size() - free_.size(); }
+  size_t max_seqs() const { return seqs_.size(); }
+  size_t max_pages() const { return max_pages_; }  // a page table row's entries
+  size_t max_len() const { return max_len_; }
+
+  // Every call either succeeds or leaves everything as it was, with a message.
+  enum Status { OK, BAD, FULL };
+  Status create(uint32_t* seq, std::string* err);
+  Status free(uint32_t seq, std::string* err);
+  // n new sequences that share the pages of `seq`
+  Status fork(uint32_t seq, size_t n, uint32_t* out, std::string* err);
+  // one new sequence with pages of its own; copies: what they are filled from
+  Status copy(uint32_t seq, uint32_t* out, std::vector<KvCopy>* copies, std::string* err);
+  Status truncate(uint32_t seq, size_t len, std::string* err);
+  Status len(uint32_t seq, size_t* len, std::string* err) const;
+  // Whether step() would succeed, and a message if not.
+  Status check_step(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, std::string* err);
+  // Room for ntok[i] more positions of seqs[i]: new pages, and copies of
+  // shared, partly filled pages that the step writes to.
+  Status step(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, std::vector<KvStepSeq>* plan,
+              std::vector<KvCopy>* copies, std::string* err);
+  // Moves the pages behind the first used() into the holes before.
+  void compact(std::vector<KvCopy>* copies);
+  // Another number of pages, at least used(), of a compacted pool.  Throws
+  // std::bad_alloc, leaving everything as it was.
+  void resize(size_t pages);
+
+  // The page that holds a sequence's position (which it holds).
+  uint32_t page_of(uint32_t seq, size_t pos) const { return seqs_[seq].pages[pos / KV_PAGE]; }
+  bool live(uint32_t seq) const { return seq < seqs_.size() && seqs_[seq].live; }
+  uint32_t refs(uint32_t page) const { return refs_[page]; }
+
+  // Page table entries (row * max_pages + index) that changed since they were
+  // last sent, some perhaps several times, and an entry's page now (0 where the
+  // sequence has none there).
+  std::vector<uint32_t> dirty;
+  uint32_t entry(uint32_t index) const {
+    const Seq& s = seqs_[index / max_pages_];
+    return index % max_pages_ < s.pages.size() ? s.pages[index % max_pages_] : 0;
+  }
+
+ private:
+  struct Seq {
+    bool live = false;
+    size_t len = 0;
+    std::vector<uint32_t> pages;
+  };
+  Status find(uint32_t seq, std::string* err) const;
+  uint32_t take();
+  void drop(uint32_t page);
+  void set(uint32_t seq, size_t index);
+  std::vector<uint32_t> refs_, free_;
+  std::vector<Seq> seqs_;
+  std::vector<uint32_t> free_seqs_;
+  // check_step(): what it saw of each sequence in its last call, and its counts
+  std::vector<uint32_t> mark_;
+  uint32_t stamp_ = 0;
+  size_t need_ = 0, copies_ = 0;
+  size_t max_len_ = 0, max_pages_ = 0;
+};
+
+}  // namespace hale

@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "../../include/hale_moe.h"
+#include "context.h"
 #include "hale_device.h"
 #include "kernels.h"
 #include "pack.h"
@@ -29,51 +30,6 @@ using namespace hale;
 // ---------------------------------------------------------------------------
 // handles
 // ---------------------------------------------------------------------------
-
-struct ProfRecord {
-  int kind;
-  hipEvent_t start, stop;
-};
-
-struct hale_ctx {
-  int device = 0;
-  hipStream_t stream = nullptr;
-  std::recursive_mutex mu;
-  std::string err;
-  // scratch of the synchronous single-matrix / single-expert entry points
-  void* scratch = nullptr;
-  size_t scratch_bytes = 0;
-  // wall timer
-  hipEvent_t t0 = nullptr, t1 = nullptr;
-  // per-kernel profiler
-  bool prof_on = false;
-  std::vector<hipEvent_t> ev_pool;
-  std::vector<ProfRecord> recs;
-  int open_kind = -1;
-  bool prof_saved = false;  // prof_on while a capture runs (profiling is off then)
-  double prof_ms[K_KINDS] = {};
-  uint64_t prof_n[K_KINDS] = {};
-  // Graphs keep the device addresses they were captured with.  While any
-  // graph of this context exists, scratch that a call outgrows is retired
-  // here instead of freed, so that replaying an older graph never touches
-  // freed memory; the last hale_graph_destroy frees it.
-  int live_graphs = 0;
-  std::vector<void*> retired;
-  // this device's copy of the fixed scratch array (forward without allocation)
-  void* fixed_scratch = nullptr;
-  // pinned host staging of the synchronous host-slice entry points: inputs
-  // are copied in and outputs out of it by the CPU, the GPU copies from and
-  // to it (every such call ends with a stream synchronize, so the next one
-  // may reuse it)
-  void* pinned = nullptr;
-  size_t pinned_bytes = 0;
-};
-
-struct hale_graph {
-  hale_ctx* ctx = nullptr;
-  hipGraph_t graph = nullptr;
-  hipGraphExec_t exec = nullptr;
-};
 
 struct hale_matrix {
   hale_ctx* ctx = nullptr;
@@ -425,6 +381,9 @@ static void prof_end(hale_ctx* c) {
   }
   pe = ProfEvents{};
 }
+
+void hale::ctx_prof_begin(hale_ctx* c, int kind) { prof_begin(c, kind); }
+void hale::ctx_prof_end(hale_ctx* c) { prof_end(c); }
 
 static void hook_begin(void* self, int kind) { prof_begin((hale_ctx*)self, kind); }
 static void hook_end(void* self) { prof_end((hale_ctx*)self); }
@@ -2568,7 +2527,8 @@ extern "C" const char* hale_kernel_name(int kind) {
   static const char* names[K_KINDS] = {"route", "gate_up", "down", "act_quant", "gemv", "encode",
                                        "repack", "fill", "group", "grouped_gate_up",
                                        "grouped_down", "combine", "copy", "rms_norm",
-                                       "attention", "gather", "decode", "stream_read"};
+                                       "attention", "gather", "decode", "stream_read",
+                                       "rope", "kv_store", "kv_read", "kv_pages", "kv_attention"};
   return kind >= 0 && kind < K_KINDS ? names[kind] : "";
 }
 
@@ -2583,6 +2543,7 @@ extern "C" int hale_graph_begin(hale_ctx* c) {
   }
   c->prof_saved = c->prof_on;  // profiler events are not captured into graphs
   c->prof_on = false;
+  c->kv_uses.clear();
   return HALE_OK;
 }
 
@@ -2592,6 +2553,8 @@ extern "C" int hale_graph_end(hale_ctx* c, hale_graph** out) {
   hipGraph_t graph = nullptr;
   hipError_t e = hipStreamEndCapture(c->stream, &graph);
   c->prof_on = c->prof_saved;
+  std::vector<KvUse> uses;
+  uses.swap(c->kv_uses);
   c->mu.unlock();
   if (e != hipSuccess) return fail(c, HALE_EHIP, "end capture: %s", hipGetErrorString(e));
   hale_graph* g = new (std::nothrow) hale_graph;
@@ -2601,6 +2564,7 @@ extern "C" int hale_graph_end(hale_ctx* c, hale_graph** out) {
   }
   g->ctx = c;
   g->graph = graph;
+  g->kv_uses.swap(uses);
   e = hipGraphInstantiate(&g->exec, graph, nullptr, nullptr, 0);
   if (e != hipSuccess) {
     (void)hipGraphDestroy(graph);
@@ -2627,6 +2591,10 @@ extern "C" int hale_graph_launch(hale_graph* g) {
   if (!g) return HALE_EINVAL;
   hale_ctx* c = g->ctx;
   std::lock_guard<std::recursive_mutex> lk(c->mu);
+  if (!g->kv_uses.empty()) {
+    const int rc = kv_check_replay(c, g->kv_uses);
+    if (rc) return rc;
+  }
   HIPCHK(c, hipSetDevice(c->device));
   HIPCHK(c, hipGraphLaunch(g->exec, c->stream));
   return HALE_OK;

@@ -12,6 +12,11 @@ names and argument meaning:
 ``MoeLayer``           ``MoeLayer::{route, forward}`` (src/model/moe.rs:36-70)
 ``HbmExpertProvider``  ``ExpertProvider::{fetch, stats, routing_stats}``
                        (src/expert/mod.rs:128-137), all experts resident in HBM
+``Rope``               rotary positions of many rows (beyond ``Rope::apply``,
+                       src/ops/rope.rs)
+``KvCache``            keys and values of many sequences in 8 bits, in pages, and
+                       their attention (beyond ``LayerCache``,
+                       src/model/kv_cache.rs)
 =====================  ==========================================================
 
 Errors follow the reference: shape and length violations (which panic in
@@ -114,6 +119,27 @@ SIGNATURES = {
     "hale_attention_len": (C.c_int, [_vp, C.POINTER(_sz)]),
     "hale_attention_forward": (C.c_int, [_vp, _fp, _sz, _fp, _fp, _fp]),
     "hale_attention_forward_device": (C.c_int, [_vp, _vp, _sz, _vp, _vp, _vp]),
+    "hale_rope_create": (C.c_int, [_vp, _vp, C.POINTER(_vp)]),
+    "hale_rope_destroy": (None, [_vp]),
+    "hale_rope_frequencies": (C.c_int, [_vp, C.POINTER(C.c_double), _sz]),
+    "hale_rope_device": (C.c_int, [_vp, C.c_int, _sz, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _vp, _sz]),
+    "hale_kv_create": (C.c_int, [_vp, _sz, _sz, _sz, _sz, _sz, _sz, _sz, C.POINTER(_vp)]),
+    "hale_kv_destroy": (None, [_vp]),
+    "hale_kv_seq_create": (C.c_int, [_vp, _u32p]),
+    "hale_kv_seq_free": (C.c_int, [_vp, C.c_uint32]),
+    "hale_kv_seq_fork": (C.c_int, [_vp, C.c_uint32, _sz, _u32p]),
+    "hale_kv_seq_copy": (C.c_int, [_vp, C.c_uint32, _u32p]),
+    "hale_kv_seq_truncate": (C.c_int, [_vp, C.c_uint32, _sz]),
+    "hale_kv_seq_len": (C.c_int, [_vp, C.c_uint32, C.POINTER(_sz)]),
+    "hale_kv_pages": (C.c_int, [_vp, C.POINTER(_sz), C.POINTER(_sz)]),
+    "hale_kv_compact": (C.c_int, [_vp, C.POINTER(_sz)]),
+    "hale_kv_resize": (C.c_int, [_vp, _sz]),
+    "hale_kv_step": (C.c_int, [_vp, _sz, _u32p, _u32p]),
+    "hale_kv_reserve": (C.c_int, [_vp, _sz]),
+    "hale_kv_positions": (C.c_int, [_vp, C.POINTER(_vp)]),
+    "hale_kv_append_device": (C.c_int, [_vp, _sz, C.c_int, _sz, _vp, _sz, _vp, _sz]),
+    "hale_kv_attention_device": (C.c_int, [_vp, _sz, C.c_int, _sz, _vp, _sz, C.c_float, _sz, _vp, _sz]),
+    "hale_kv_read_device": (C.c_int, [_vp, _sz, C.c_uint32, _sz, _sz, _vp, _vp]),
     "hale_device_malloc": (C.c_int, [_vp, _sz, C.POINTER(_vp)]),
     "hale_device_free": (C.c_int, [_vp, _vp]),
     "hale_memcpy_htod": (C.c_int, [_vp, _vp, _vp, _sz]),
@@ -765,6 +791,191 @@ class Attention:
     def close(self):
         if getattr(self, "handle", None) and self.ctx.alive:
             lib().hale_attention_destroy(self.handle)
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class _RopeConfigC(C.Structure):
+    _fields_ = [("layout", C.c_int), ("scaling", C.c_int), ("head_dim", _sz), ("rotary_dim", _sz),
+                ("base", C.c_double), ("factor", C.c_double), ("original_len", C.c_double), ("low", C.c_double),
+                ("high", C.c_double), ("attention_factor", C.c_double)]
+
+
+class Rope:
+    """Rotary positions of any number of rows (hale_rope_*): the rotation of
+    Rope::apply (src/ops/rope.rs) with both pair layouts, part of the head,
+    and frequencies scaled for long contexts."""
+
+    LAYOUTS = {"half": 0, "interleaved": 1}
+    SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "parts": 3}
+
+    def __init__(self, ctx: "Context", head_dim: int, base: float = 10000.0, *, rotary_dim: int | None = None,
+                 layout: str = "half", scaling: str = "none", factor: float = 1.0, original_len: float = 0.0,
+                 low: float = 1.0, high: float = 32.0, attention_factor: float = 1.0):
+        self.ctx, self.head_dim = ctx, head_dim
+        self.rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        if layout not in self.LAYOUTS or scaling not in self.SCALINGS:
+            raise ValueError(f"unknown layout {layout!r} or scaling {scaling!r}")
+        c = _RopeConfigC(self.LAYOUTS[layout], self.SCALINGS[scaling], head_dim, self.rotary_dim, base, factor,
+                         original_len, low, high, attention_factor)
+        h = _vp()
+        ctx.check(lib().hale_rope_create(ctx.handle, C.byref(c), C.byref(h)), "Rope")
+        self.handle = h
+        ctx.adopt(self)
+
+    def frequencies(self) -> np.ndarray:
+        """The angle per position of each pair, in radians."""
+        out = np.zeros(self.rotary_dim // 2, dtype=np.float64)
+        self.ctx.check(lib().hale_rope_frequencies(self.handle, _p(out, C.POINTER(C.c_double)), out.size), "Rope")
+        return out
+
+    def apply_device(self, dtype, rows: int, d_positions: int, d_q: int, q_heads: int, d_q_out: int, d_k: int = 0,
+                     k_heads: int = 0, d_k_out: int = 0, *, q_stride: int = 0, q_out_stride: int = 0,
+                     k_stride: int = 0, k_out_stride: int = 0):
+        """Turns the heads of `rows` rows on device buffers, enqueued on the
+        context stream.  Strides count elements from row to row (0: the heads'
+        numbers lie one behind the other); outputs may be their inputs."""
+        nq, nk = q_heads * self.head_dim, k_heads * self.head_dim
+        self.ctx.check(lib().hale_rope_device(self.handle, parse_dtype(dtype), rows, _vp(d_positions), _vp(d_q), q_heads,
+                                              q_stride or nq, _vp(d_q_out), q_out_stride or nq, _vp(d_k), k_heads,
+                                              k_stride or nk, _vp(d_k_out), k_out_stride or nk), "Rope")
+
+    def close(self):
+        if getattr(self, "handle", None) and self.ctx.alive:
+            lib().hale_rope_destroy(self.handle)
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+KV_PAGE, KV_BLOCK = 64, 16
+
+
+class KvCache:
+    """Keys and values of many sequences in 8 bits, in pages (hale_kv_*), with
+    the causal attention that reads them.  A step is `step`, then for every
+    layer `append_device` and `attention_device`; between steps sequences are
+    made, forked, copied, cut and freed.  Sequences are numbers below
+    max_seqs."""
+
+    def __init__(self, ctx: "Context", layers: int, num_heads: int, num_kv_heads: int, head_dim: int, num_pages: int,
+                 max_seqs: int, max_len: int):
+        self.ctx, self.layers = ctx, layers
+        self.num_heads, self.num_kv_heads, self.head_dim = num_heads, num_kv_heads, head_dim
+        h = _vp()
+        ctx.check(lib().hale_kv_create(ctx.handle, layers, num_heads, num_kv_heads, head_dim, num_pages, max_seqs,
+                                       max_len, C.byref(h)), "KvCache")
+        self.handle = h
+        ctx.adopt(self)
+
+    def _check(self, rc: int, what: str):
+        self.ctx.check(rc, what)
+
+    def seq_create(self) -> int:
+        s = C.c_uint32()
+        self._check(lib().hale_kv_seq_create(self.handle, C.byref(s)), "seq_create")
+        return int(s.value)
+
+    def seq_free(self, seq: int):
+        self._check(lib().hale_kv_seq_free(self.handle, seq), "seq_free")
+
+    def seq_fork(self, seq: int, n: int = 1) -> list:
+        """n new sequences that share seq's pages until they store to them."""
+        out = np.zeros(max(n, 1), dtype=np.uint32)
+        self._check(lib().hale_kv_seq_fork(self.handle, seq, n, _p(out, _u32p)), "seq_fork")
+        return [int(s) for s in out[:n]]
+
+    def seq_copy(self, seq: int) -> int:
+        """A new sequence with seq's contents in pages of its own."""
+        s = C.c_uint32()
+        self._check(lib().hale_kv_seq_copy(self.handle, seq, C.byref(s)), "seq_copy")
+        return int(s.value)
+
+    def seq_truncate(self, seq: int, length: int):
+        self._check(lib().hale_kv_seq_truncate(self.handle, seq, length), "seq_truncate")
+
+    def seq_len(self, seq: int) -> int:
+        n = _sz()
+        self._check(lib().hale_kv_seq_len(self.handle, seq, C.byref(n)), "seq_len")
+        return int(n.value)
+
+    def pages(self) -> tuple:
+        """(pages of the pool, pages in use)."""
+        total, used = _sz(), _sz()
+        self._check(lib().hale_kv_pages(self.handle, C.byref(total), C.byref(used)), "pages")
+        return int(total.value), int(used.value)
+
+    def compact(self) -> int:
+        """Moves the pages in use to the pool's front; how many were moved."""
+        n = _sz()
+        self._check(lib().hale_kv_compact(self.handle, C.byref(n)), "compact")
+        return int(n.value)
+
+    def resize(self, num_pages: int):
+        self._check(lib().hale_kv_resize(self.handle, num_pages), "resize")
+
+    def reserve(self, max_tokens: int):
+        self._check(lib().hale_kv_reserve(self.handle, max_tokens), "reserve")
+
+    def step(self, seqs, ntok):
+        """Begins a step: ntok[i] new tokens for sequence seqs[i]."""
+        s, n = (np.ascontiguousarray(a, dtype=np.uint32).reshape(-1) for a in (seqs, ntok))
+        if s.size != n.size:
+            raise ValueError("step: as many token counts as sequences")
+        self._check(lib().hale_kv_step(self.handle, s.size, _p(s, _u32p), _p(n, _u32p)), "step")
+
+    @property
+    def positions(self) -> int:
+        """Device address of the step's positions ([tokens] int32)."""
+        p = _vp()
+        self._check(lib().hale_kv_positions(self.handle, C.byref(p)), "positions")
+        return int(p.value or 0)
+
+    def append_device(self, layer: int, dtype, ntok: int, d_k: int, d_v: int, *, k_stride: int = 0,
+                      v_stride: int = 0):
+        """Stores the step's keys and values of a layer (device buffers,
+        strides in elements per token; 0: without gaps)."""
+        n = self.num_kv_heads * self.head_dim
+        self._check(lib().hale_kv_append_device(self.handle, layer, parse_dtype(dtype), ntok, _vp(d_k), k_stride or n,
+                                                _vp(d_v), v_stride or n), "append")
+
+    def attention_device(self, layer: int, dtype, ntok: int, d_q: int, d_out: int, *, scale: float | None = None,
+                         window: int = 0, q_stride: int = 0, out_stride: int = 0):
+        """Causal attention of the step's tokens over their sequences (scale:
+        1 / sqrt(head_dim) unless given; window 0: all earlier positions)."""
+        n = self.num_heads * self.head_dim
+        s = self.head_dim ** -0.5 if scale is None else scale
+        self._check(lib().hale_kv_attention_device(self.handle, layer, parse_dtype(dtype), ntok, _vp(d_q), q_stride or n,
+                                                   s, window, _vp(d_out), out_stride or n), "attention")
+
+    def read_device(self, layer: int, seq: int, first: int, count: int, d_k: int, d_v: int):
+        """Positions first .. first + count - 1 as f32 into device buffers."""
+        self._check(lib().hale_kv_read_device(self.handle, layer, seq, first, count, _vp(d_k), _vp(d_v)), "read")
+
+    def read(self, layer: int, seq: int, first: int, count: int) -> tuple:
+        """(keys, values) [count][kv_heads][head_dim] of those positions."""
+        shape = (count, self.num_kv_heads, self.head_dim)
+        n = int(np.prod(shape))
+        bufs = [self.ctx.malloc(max(4 * n, 4)) for _ in range(2)]
+        try:
+            self.read_device(layer, seq, first, count, bufs[0].address, bufs[1].address)
+            return tuple(b.download(np.float32, n).reshape(shape) for b in bufs)
+        finally:
+            for b in bufs:
+                b.free()
+
+    def close(self):
+        if getattr(self, "handle", None) and self.ctx.alive:
+            lib().hale_kv_destroy(self.handle)
         self.handle = None
 
     def __del__(self):

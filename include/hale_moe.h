@@ -503,6 +503,162 @@ int hale_attention_forward_device(hale_attention *attn, const float *d_x,
                                   size_t position, const float *d_cos,
                                   const float *d_sin, float *d_out);
 
+/* ---- rotary positions -------------------------------------------------
+ * No counterpart in the reference beyond Rope::{angles, apply}
+ * (src/ops/rope.rs), whose rotation hale_attention_* computes itself from the
+ * caller's cos and sin.  This form takes any number of rows, both pair
+ * layouts, part of the head, scaled frequencies and f32 / f16 / bf16. */
+
+typedef struct hale_rope hale_rope;
+
+#define HALE_ROPE_HALF 0        /* pairs (i, i + rotary_dim / 2)             */
+#define HALE_ROPE_INTERLEAVED 1 /* pairs (2 i, 2 i + 1)                      */
+
+#define HALE_ROPE_NONE 0   /* f_i = base^(-2 i / rotary_dim)                 */
+#define HALE_ROPE_LINEAR 1 /* f_i / factor: positions interpolated           */
+#define HALE_ROPE_NTK 2    /* base * factor^(rotary_dim / (rotary_dim - 2))  */
+/* by parts: a pair of t_i = original_len * f_i / (2 pi) turns keeps f_i from
+ * t_i = high on, takes f_i / factor up to t_i = low, and between them
+ * f_i g + f_i / factor (1 - g) with g = (t_i - low) / (high - low) */
+#define HALE_ROPE_PARTS 3
+
+typedef struct {
+  int layout;
+  int scaling;
+  size_t head_dim;         /* 1..1024                                        */
+  size_t rotary_dim;       /* even, 2..head_dim; numbers behind it pass      */
+  double base;             /* above 1                                        */
+  double factor;           /* from 1 on (unless HALE_ROPE_NONE)              */
+  double original_len;     /* HALE_ROPE_PARTS                                */
+  double low, high;        /* HALE_ROPE_PARTS: 0 <= low < high               */
+  double attention_factor; /* multiplies cos and sin; 1 for none             */
+} hale_rope_config;
+
+int hale_rope_create(hale_ctx *ctx, const hale_rope_config *config,
+                     hale_rope **out);
+void hale_rope_destroy(hale_rope *rope);
+/* The angle per position of each pair, in radians: freq[rotary_dim / 2]. */
+int hale_rope_frequencies(const hale_rope *rope, double *freq, size_t n);
+/* Turns the heads of `rows` rows: queries [rows][q_heads][head_dim] and keys
+ * [rows][k_heads][head_dim] of `dtype` (HALE_F32, HALE_F16, HALE_BF16), row r at
+ * position d_positions[r] (any int32; negative positions turn back, which is
+ * also the gradient of turning forth).  Strides count elements from row to row,
+ * at least heads * head_dim.  Either side may be left out (heads 0, pointers
+ * NULL).  Each output may be its own input with the same stride (in place);
+ * otherwise no output may overlap an input or the other output.  Angles are formed
+ * in 64 bits, products in f32, and rounded once.  Enqueued on the context's
+ * stream. */
+int hale_rope_device(hale_rope *rope, int dtype, size_t rows,
+                     const int32_t *d_positions, const void *d_q,
+                     size_t q_heads, size_t q_stride, void *d_q_out,
+                     size_t q_out_stride, const void *d_k, size_t k_heads,
+                     size_t k_stride, void *d_k_out, size_t k_out_stride);
+
+/* ---- paged 8-bit key/value cache and its attention ----------------------
+ * No counterpart in the reference, whose LayerCache (src/model/kv_cache.rs)
+ * holds one sequence's f32 keys and values; for callers that serve many
+ * sequences.
+ *
+ * A cache holds the keys and values of all layers of up to max_seqs sequences
+ * in a pool of pages of HALE_KV_PAGE positions.  A sequence's pages may lie
+ * anywhere in the pool, and sequences may share pages (hale_kv_seq_fork).
+ * Keys and values are held as whole numbers -127..127 with one f32 scale for each
+ * block of HALE_KV_BLOCK positions, head, and keys or values:
+ *   scale = max |x| / 127 over the block's numbers, rounded to f32, or the
+ *           block's former scale where that is larger;
+ *   code  = x / scale, rounded to the nearest whole number (ties to even).
+ * A block that is stored to in several steps rounds the codes it already holds
+ * anew when its scale grows.  Numbers that are not finite are stored as 0.  After
+ * hale_kv_seq_truncate a block keeps the scale it had, unless nothing of it is
+ * left.
+ *
+ * A step is what a serving loop computes at once: hale_kv_step makes room for
+ * each sequence's new tokens and lays out the work, then for every layer
+ * hale_kv_append_device stores their keys and values and
+ * hale_kv_attention_device attends.  Tokens lie one behind the other, sequence by
+ * sequence in the order given.  Attention of a layer whose new tokens were not
+ * stored, and the positions of a step that was followed by another without it,
+ * read what the page held before.
+ *
+ * Calls return HALE_EINVAL for arguments they refuse and HALE_ENOMEM where
+ * pages, sequences or memory run out; either way nothing has changed. */
+
+#define HALE_KV_PAGE 64
+#define HALE_KV_BLOCK 16
+#define HALE_KV_MAX_WINDOWS 4
+
+typedef struct hale_kv_cache hale_kv_cache;
+
+/* head_dim: a multiple of 16 from 16 to 256 (key rows are padded to 64, 96, 128,
+ * 192 or 256); num_heads a multiple of num_kv_heads.  max_len: most positions
+ * of one sequence.  num_pages pages of
+ * layers * num_kv_heads * (64 * padded + 64 * head_dim + 128) bytes. */
+int hale_kv_create(hale_ctx *ctx, size_t layers, size_t num_heads,
+                   size_t num_kv_heads, size_t head_dim, size_t num_pages,
+                   size_t max_seqs, size_t max_len, hale_kv_cache **out);
+/* Graphs that use the cache can no longer be launched. */
+void hale_kv_destroy(hale_kv_cache *kv);
+
+/* A new, empty sequence: its number, below max_seqs. */
+int hale_kv_seq_create(hale_kv_cache *kv, uint32_t *seq);
+/* Gives the sequence and the pages that only it holds back. */
+int hale_kv_seq_free(hale_kv_cache *kv, uint32_t seq);
+/* n new sequences with seq's contents, which share its pages: nothing is
+ * copied until one of them stores to a partly filled page that others hold,
+ * which the step then copies first. */
+int hale_kv_seq_fork(hale_kv_cache *kv, uint32_t seq, size_t n, uint32_t *out);
+/* One new sequence with seq's contents in pages of its own (copied on the
+ * context's stream). */
+int hale_kv_seq_copy(hale_kv_cache *kv, uint32_t seq, uint32_t *out);
+/* Drops the positions from len on (drafted tokens that were not accepted). */
+int hale_kv_seq_truncate(hale_kv_cache *kv, uint32_t seq, size_t len);
+int hale_kv_seq_len(const hale_kv_cache *kv, uint32_t seq, size_t *len);
+/* Pages of the pool, and how many are in use. */
+int hale_kv_pages(const hale_kv_cache *kv, size_t *total, size_t *used);
+/* Moves pages from the pool's end into its holes, on the context's stream:
+ * afterwards the pages in use are the first ones.  moved (may be NULL): how
+ * many were moved. */
+int hale_kv_compact(hale_kv_cache *kv, size_t *moved);
+/* Gives the pool num_pages pages, at least those in use, which are compacted:
+ * returns memory to the device or takes more.  Synchronous; refused while a
+ * graph of the context exists, since graphs keep the pool's address. */
+int hale_kv_resize(hale_kv_cache *kv, size_t num_pages);
+
+/* Begins a step: ntok[i] new tokens (0 allowed) for sequence seqs[i], all
+ * different.  Refused while the context's stream is being captured. */
+int hale_kv_step(hale_kv_cache *kv, size_t nseq, const uint32_t *seqs,
+                 const uint32_t *ntok);
+/* Room for steps of up to max_tokens tokens, so that none grows the plan's
+ * buffers (which graphs hold: growing them makes older graphs unusable). */
+int hale_kv_reserve(hale_kv_cache *kv, size_t max_tokens);
+/* Device address of the positions of the step's tokens, [tokens] int32, for
+ * hale_rope_device.  The same for every step until the buffers grow. */
+int hale_kv_positions(const hale_kv_cache *kv, const int32_t **d_positions);
+
+/* Stores the step's keys and values into a layer: d_k and d_v
+ * [ntok][num_kv_heads][head_dim] of `dtype` (HALE_F32, HALE_F16, HALE_BF16),
+ * strides in elements from token to token.  ntok must be the step's tokens. */
+int hale_kv_append_device(hale_kv_cache *kv, size_t layer, int dtype,
+                          size_t ntok, const void *d_k, size_t k_stride,
+                          const void *d_v, size_t v_stride);
+/* Causal grouped-query attention of the step's tokens over their sequences:
+ * d_q and d_out [ntok][num_heads][head_dim] of `dtype`; query head h reads
+ * key/value head h / (num_heads / num_kv_heads).  A token at position p sees the
+ * positions up to p, with window > 0 only those above p - window.  Scores are
+ * scale (positive) times q . k.  At most HALE_KV_MAX_WINDOWS different windows
+ * (0 among them) per cache.  Sums and the softmax's statistics are f32; queries
+ * of f16 and bf16 enter exactly, of f32 to 2^-23 of the row's largest; probabilities
+ * are rounded to 2^-11 of their value for f16 and bf16 and 2^-23 for f32.  The
+ * order of all sums is fixed: equal calls give equal bits. */
+int hale_kv_attention_device(hale_kv_cache *kv, size_t layer, int dtype,
+                             size_t ntok, const void *d_q, size_t q_stride,
+                             float scale, size_t window, void *d_out,
+                             size_t out_stride);
+/* Positions first .. first + count - 1 of a sequence as f32 (code times
+ * scale): d_k and d_v [count][num_kv_heads][head_dim]. */
+int hale_kv_read_device(hale_kv_cache *kv, size_t layer, uint32_t seq,
+                        size_t first, size_t count, float *d_k, float *d_v);
+
 /* ---- support entry points -------------------------------------------
  * No counterpart in the reference: device memory, timing and graph capture
  * for benchmarks and tests, so that a caller needs no second HIP runtime. */
@@ -557,7 +713,13 @@ const char *hale_kernel_name(int kind);
  *     later call outgrows while any graph of the context exists is kept,
  *     not freed, until the last of those graphs is destroyed, so an older
  *     graph replays correctly after a larger call.
- *   - Matrices, layers and attention blocks a graph uses must outlive it. */
+ *   - Matrices, layers and attention blocks a graph uses must outlive it.
+ *   - hale_kv_append_device and hale_kv_attention_device may be captured (call
+ *     each window once before).  A launch then works on the cache's step of
+ *     that moment, which must have the same tokens per sequence as the captured
+ *     one (lengths and pages may differ); hale_graph_launch is refused
+ *     (HALE_EINVAL) for another step, or once the cache's buffers grew or the
+ *     cache is gone. */
 typedef struct hale_graph hale_graph;
 int hale_graph_begin(hale_ctx *ctx);
 int hale_graph_end(hale_ctx *ctx, hale_graph **out);
