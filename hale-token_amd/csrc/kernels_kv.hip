@@ -63,23 +63,32 @@ hipError_t launch_rope(int dtype, const RopeArgs& a, hipStream_t st) {
 // plan upload, page copies
 // ---------------------------------------------------------------------------
 
-__global__ __launch_bounds__(256) void k_kv_upload(KvUploadArgs a) {
-  const unsigned id = blockIdx.x * 256 + threadIdx.x, step = gridDim.x * 256;
-  const u32x4* src = (const u32x4*)a.src;
-  for (int p = 0; p < a.pieces; p++) {
-    const unsigned n = a.words[p] / 4;
-    u32x4* dst = (u32x4*)a.dst[p];
-    for (unsigned i = id; i < n; i += step) dst[i] = src[i];
-    src += n;
+// A thread per 16 bytes, all of them read at once: the host's memory is a
+// microsecond away, once.
+__global__ __launch_bounds__(256) void k_kv_upload(KvUploadArgs a, unsigned n4) {
+  const unsigned id = blockIdx.x * 256 + threadIdx.x;
+  if (id < n4) {
+    const u32x4 x = ((const u32x4*)a.src)[id];
+    unsigned at = id;
+    for (int p = 0; p < a.pieces; p++) {
+      const unsigned n = a.words[p] / 4;
+      if (at < n) {
+        ((u32x4*)a.dst[p])[at] = x;
+        break;
+      }
+      at -= n;
+    }
+  } else if (id - n4 < a.npairs) {
+    const unsigned i = id - n4;
+    a.table[a.pairs[2 * i]] = a.pairs[2 * i + 1];
   }
-  for (unsigned i = id; i < a.npairs; i += step) a.table[a.pairs[2 * i]] = a.pairs[2 * i + 1];
 }
 
 hipError_t launch_kv_upload(const KvUploadArgs& a, hipStream_t st) {
-  size_t most = a.npairs;
-  for (int p = 0; p < a.pieces; p++) most = std::max<size_t>(most, a.words[p] / 4);
-  if (most == 0) return hipSuccess;
-  return launch(k_kv_upload, (unsigned)std::min<size_t>((most + 255) / 256, 64), 256, 0, st, a);
+  unsigned n4 = 0;
+  for (int p = 0; p < a.pieces; p++) n4 += a.words[p] / 4;
+  if (n4 + a.npairs == 0) return hipSuccess;
+  return launch(k_kv_upload, (n4 + a.npairs + 255) / 256, 256, 0, st, a, n4);
 }
 
 constexpr unsigned COPY_BYTES = 16384;  // per work-group: four 16-byte pieces a thread
@@ -113,75 +122,148 @@ hipError_t launch_kv_copy_pages(uint8_t* pool, size_t page_bytes, const KvCopy* 
 // storing
 // ---------------------------------------------------------------------------
 //
-// One wave per block of 16 positions, head, and keys or values: the largest
-// magnitude of the new numbers, the block's scale from it and the former one,
-// the codes.  Quotients are rounded to whole numbers from their exact values:
-// x / s is formed in f64, whose rounding cannot carry a quotient of two f32
-// onto a half (they are at least 2^-25 of it apart from one, or on it).
-template <typename T, int NI>
-__device__ __forceinline__ void append_block(const KvAppendArgs& a, KvBlock blk) {
-  const KvStepSeq sq = a.seqs[blk.seq];
-  const int head = blockIdx.y, lane = threadIdx.x, values = threadIdx.y, hd = a.g.hd;
-  const unsigned pos0 = blk.block * KV_BLOCK;
-  const int old = sq.len0 > pos0 ? (int)(sq.len0 - pos0) : 0;  // positions held; < 16
-  const int end = sq.len0 + sq.ntok - pos0 < KV_BLOCK ? (int)(sq.len0 + sq.ntok - pos0) : (int)KV_BLOCK;
-  const size_t stride = values ? a.v_stride : a.k_stride;
-  // the token of the block's position 0 (it may lie before the step's first)
-  const long long tok = (long long)sq.tok0 + pos0 - sq.len0;
-  const T* src = (const T*)(values ? a.v : a.k) + (size_t)head * hd;
-  const uint32_t page = a.g.table[(size_t)sq.row * a.g.max_pages + pos0 / KV_PAGE];
-  uint8_t* region = a.g.pool + page * a.g.page_bytes + a.layer * a.g.layer_bytes + (size_t)head * a.g.head_bytes;
-  const unsigned t0 = pos0 % KV_PAGE;
-  float* scale = (float*)(region + a.g.s_off) + values * 4 + t0 / KV_BLOCK;
+// One work-group per block of 16 positions, head, and keys or values: the new
+// rows go to LDS as f32 on the way to the largest magnitude; the block's scale
+// from it and the former one; then the codes, each thread those of the bytes it writes:
+// 8 consecutive numbers of one position of the keys, four positions of one number
+// of the values, so that no thread's bytes depend on another's.  A decode step's
+// call is a chain of latencies (the block, its page, scale and codes, the
+// rounding of held codes where the scale grew, about 20 dependent instructions
+// each): four waves share a block, 8 codes a thread at head dimension 128.
 
-  float x[NI][KV_BLOCK], top = 0.0f;
-#pragma unroll
-  for (int n = 0; n < NI; n++) {
-    const int d = lane + 64 * n;
-#pragma unroll
-    for (int t = 0; t < (int)KV_BLOCK; t++) {
-      float v = 0.0f;
-      if (t >= old && t < end && d < hd) v = to_f32(src[(size_t)(tok + t) * stride + d]);
-      v = __builtin_isfinite(v) ? v : 0.0f;  // what is not finite is stored as 0 and raises no scale
-      x[n][t] = v;
-      top = fmaxf(top, fabsf(v));
-    }
-  }
-  top = wave_max_f32(top);
-  const float had = old ? *scale : 0.0f;
-  const float s = fmaxf(had, top / 127.0f);
-  const bool grown = old && s > had;
-  const double wide = (double)s;
-#pragma unroll
-  for (int n = 0; n < NI; n++) {
-    const int d = lane + 64 * n;
-    if (d >= hd) break;
-#pragma unroll
-    for (int t = 0; t < (int)KV_BLOCK; t++) {
-      uint8_t* at = region + (values ? a.g.v_off + kv_value_byte(t0 + t, d) : kv_key_byte(a.g.chunks, t0 + t, d));
-      if (t < old) {
-        if (grown) *at = (uint8_t)((int)rint((double)((int)*at - 128) * had / wide) + 128);
-      } else if (t < end) {
-        const double q = s > 0.0f ? rint((double)x[n][t] / wide) : 0.0;
-        *at = (uint8_t)((int)fmin(fmax(q, -127.0), 127.0) + 128);
-      }
-    }
-  }
-  if (lane == 0) *scale = s;
+// The whole number nearest to (p + e) / s, ties to even, where |p / s| < 200, e is
+// the rest of a product rounded to p (or 0), and inv is within 2^-21 of 1 / s
+// relative.  p inv is off by less than 2^-13, so its nearest whole number c is
+// the quotient's or the one beside it; p - c s, of at most half of s and a little,
+// is a multiple of the smaller of both ulps and so exact, as is 2 |p - c s| - s
+// where it is near 0; the sign of that with e decides.
+__device__ __forceinline__ unsigned nearest_code(float p, float e, float s, float inv) {
+  float c = rintf(p * inv);
+  const float r = __builtin_fmaf(-c, s, p);
+  const float over = (2.0f * fabsf(r) - s) + 2.0f * (r < 0.0f ? -e : e);
+  const bool odd = ((int)c & 1) != 0;
+  c += over > 0.0f || (over == 0.0f && odd) ? (r > 0.0f ? 1.0f : -1.0f) : 0.0f;
+  return (unsigned)((int)fminf(fmaxf(c, -127.0f), 127.0f) + 128);
 }
 
-template <typename T, int NI>
-__global__ __launch_bounds__(128) void k_kv_append(KvAppendArgs a) {
+// A lane's number n of the keys, n a multiple of 8: which of the dimension
+// it is (lane group g), and where its code and the next seven go.
+__device__ __forceinline__ int key_dim(int kc, int n, int g) {
+  return n / 16 < kc / 2 ? 64 * (n / 16) + 16 * g + n % 16 : 64 * (kc / 2) + 8 * g;
+}
+__device__ __forceinline__ unsigned key_at(int kc, int n, int block, int lane) {
+  return n / 16 < kc / 2 ? ((n / 16 * 4 + block) * 64 + lane) * 16 + n % 16 : kc / 2 * 4096 + (block * 64 + lane) * 8;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
+  extern __shared__ float x[];  // [16][hd + 4]
+  __shared__ float red[4];
+  const int tid = threadIdx.x, hd = a.g.hd, ldx = hd + 4;
+  const bool values = blockIdx.z;
+  const size_t stride = values ? a.v_stride : a.k_stride;
+  const T* base = (const T*)(values ? a.v : a.k) + (size_t)blockIdx.y * hd;
   const unsigned nblocks = a.count ? *a.count : a.nblocks;
-  for (unsigned b = blockIdx.x; b < nblocks; b += gridDim.x) append_block<T, NI>(a, a.blocks[b]);
+  for (unsigned b = blockIdx.x; b < nblocks; b += gridDim.x) {
+    const KvBlock blk = a.blocks[b];
+    const int old = blk.old, end = blk.end;
+    const uint32_t page = a.g.table[blk.entry];
+    const T* src = base + (long long)blk.tok * (long long)stride;
+    uint8_t* region = a.g.pool + page * a.g.page_bytes + a.layer * a.g.layer_bytes + (size_t)blockIdx.y * a.g.head_bytes;
+    float* scale = (float*)(region + a.g.s_off) + (values ? 4 : 0) + blk.block;
+    const float had = old ? *scale : 0.0f;
+
+    float top = 0.0f;
+    auto keep = [&](int t, int d, float v) {
+      v = __builtin_isfinite(v) ? v : 0.0f;  // what is not finite is stored as 0 and raises no scale
+      top = fmaxf(top, fabsf(v));
+      x[t * ldx + d] = v;
+    };
+    if (a.vec) {
+      constexpr int PER = 16 / sizeof(T);
+      const int row = hd / PER, n = (end - old) * row;  // 16-byte pieces
+      for (int e = tid; e < n; e += 256) {
+        const int t = old + e / row, d = e % row * PER;
+        union {
+          u32x4 u;
+          T v[PER];
+        } r;
+        r.u = *(const u32x4*)(src + (size_t)t * stride + d);
+#pragma unroll
+        for (int j = 0; j < PER; j++) keep(t, d + j, to_f32(r.v[j]));
+      }
+    } else {
+      const int n = (end - old) * hd;
+#pragma unroll 4
+      for (int e = tid; e < n; e += 256) {
+        const int t = old + e / hd, d = e % hd;
+        keep(t, d, to_f32(src[(size_t)t * stride + d]));
+      }
+    }
+    top = wave_max_f32(top);
+    if (tid % 64 == 0) red[tid / 64] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float s = fmaxf(had, top / 127.0f);
+    const bool grown = old && s > had;
+    // the reciprocal of a very small scale overflows: both sides times 2^64, exactly
+    const float up = s < 0x1p-64f ? 0x1p64f : 1.0f, su = s * up, hu = had * up;
+    const float inv = s > 0.0f ? 1.0f / su : 0.0f;  // scale 0: all numbers are 0, and so are their quotients
+    auto code = [&](bool held, unsigned was, float v) {
+      const float c = (float)((int)was - 128), m = c * hu;
+      return nearest_code(held ? m : v * up, held ? __builtin_fmaf(c, hu, -m) : 0.0f, su, inv);
+    };
+    if (!values) {
+      // thread: position i, numbers d .. d + 7 (lane and piece as in kv_key_byte)
+      for (int e = tid; e < a.g.chunks * 64; e += 256) {
+        const int lane = e % 64, i = lane % 16, n = e / 64 * 8;
+        const int d = key_dim(a.g.chunks, n, lane / 16);
+        const bool held = i < old;
+        if (d >= hd || !(held ? grown : i < end)) continue;
+        u32x2* at = (u32x2*)(region + key_at(a.g.chunks, n, blk.block, lane));
+        u32x2 o = {0, 0}, w;
+        f32x4 v[2] = {};
+        if (held) {
+          o = *at;
+        } else {
+          v[0] = *(const f32x4*)(x + i * ldx + d);
+          v[1] = *(const f32x4*)(x + i * ldx + d + 4);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          w[j] = 0;
+#pragma unroll
+          for (int k = 0; k < 4; k++) w[j] |= code(held, o[j] >> (8 * k) & 255, v[j][k]) << (8 * k);
+        }
+        *at = w;
+      }
+    } else {
+      // thread: number d = 16 n + i, positions 4 g .. 4 g + 3
+#pragma unroll 2
+      for (int e = tid; e < hd * 4; e += 256) {
+        const int lane = e % 64, i = lane % 16, g = lane / 16, n = e / 64;
+        if (4 * g >= end || !(grown || 4 * g + 3 >= old)) continue;
+        unsigned* at = (unsigned*)(region + a.g.v_off + e * 16 + 4 * blk.block);
+        const unsigned o = 4 * g < old ? *at : 0;
+        unsigned w = 0;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int t = 4 * g + r;
+          const float v = t >= old && t < end ? x[t * ldx + 16 * n + i] : 0.0f;
+          w |= code(t < old, o >> (8 * r) & 255, v) << (8 * r);
+        }
+        *at = w;
+      }
+    }
+    if (tid == 0) *scale = s;
+    __syncthreads();  // the next block's rows may overwrite these
+  }
 }
 
 template <typename T>
 static hipError_t append_typed(const KvAppendArgs& a, unsigned n, hipStream_t st) {
-  const dim3 grid(std::min(n, 1u << 20), (unsigned)a.g.kv_heads), block(64, 2);
-  if (a.g.hd <= 64) return launch(k_kv_append<T, 1>, grid, block, 0, st, a);
-  if (a.g.hd <= 128) return launch(k_kv_append<T, 2>, grid, block, 0, st, a);
-  return launch(k_kv_append<T, 4>, grid, block, 0, st, a);
+  const dim3 grid(std::min(n, 1u << 20), (unsigned)a.g.kv_heads, 2);
+  return launch(k_kv_append<T>, grid, 256, (uint32_t)(KV_BLOCK * (a.g.hd + 4) * 4), st, a);
 }
 
 hipError_t launch_kv_append(int dtype, const KvAppendArgs& a, unsigned grid, hipStream_t st) {

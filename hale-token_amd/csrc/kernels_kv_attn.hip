@@ -29,7 +29,6 @@ namespace hale {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int ATT_WAVES = 4;
 constexpr float P_SHIFT = 15.0f;  // probabilities are held times 2^15
@@ -75,43 +74,10 @@ __device__ __forceinline__ float pow2(int k) { return __uint_as_float((unsigned)
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Eight numbers of a row from p on, by its type.
-__device__ __forceinline__ void load8(int dtype, const void* base, size_t at, bool vec, float* x) {
-  if (dtype == F32) {
-    const float* p = (const float*)base + at;
-    if (vec) {
-      const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        x[i] = a[i];
-        x[i + 4] = b[i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = p[i];
-    }
-    return;
-  }
-  union {
-    u32x2 u[2];
-    uint16_t h[8];
-    _Float16 f[8];
-  } r;
-  const uint16_t* p = (const uint16_t*)base + at;
-  if (vec) {
-    r.u[0] = *(const u32x2*)p;
-    r.u[1] = *(const u32x2*)(p + 4);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) r.h[i] = p[i];
-  }
-  if (dtype == F16) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = (float)r.f[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = __uint_as_float((unsigned)r.h[i] << 16);
-  }
+// The first of eight numbers of the dimension that a lane of group g holds of
+// the query operand kk, in the order of the keys' layout.
+__device__ __forceinline__ int query_dim(int kc, int kk, int g) {
+  return kk / 2 < kc / 2 ? 64 * (kk / 2) + 16 * g + 8 * (kk & 1) : 64 * (kc / 2) + 8 * g;
 }
 
 // Four numbers to a row of the output.
@@ -147,10 +113,11 @@ __device__ __forceinline__ void store4(int dtype, void* base, size_t at, bool ve
   }
 }
 
-// KC: padded head dimension / 32; C: groups of 16 query rows; P: f16 parts per
-// query number and probability.
-template <int KC, int C, int P>
+// T: type of queries and results; KC: padded head dimension / 32; C: groups of
+// 16 query rows.
+template <typename T, int KC, int C>
 __global__ __launch_bounds__(64 * ATT_WAVES) void k_kv_attend(KvAttnArgs a) {
+  constexpr int P = sizeof(T) == 4 ? 2 : 1;  // f16 parts per query number and probability
   constexpr int ND = 2 * KC;          // groups of 16 numbers of the head dimension
   constexpr int LDO = 32 * KC + 4;    // floats per row of the waves' results
   // head dimensions that share this padding: their groups of 16 from NDMIN on may be missing
@@ -163,64 +130,8 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_kv_attend(KvAttnArgs a) {
   const unsigned nitems = a.nitems != 0xffffffffu ? a.nitems : a.counts[0];
   for (unsigned it = blockIdx.x; it < nitems; it += gridDim.x) {
     const KvItem item = a.items[it];
-    const KvStepSeq sq = a.seqs[item.seq];
-    const uint32_t* table = a.g.table + (size_t)sq.row * a.g.max_pages;
+    const uint32_t* table = a.g.table + (size_t)item.row * a.g.max_pages;
     const uint8_t* pool = a.g.pool + a.layer * a.g.layer_bytes + (size_t)item.head * a.g.head_bytes;
-
-    // ---- the query rows ------------------------------------------------------
-    f16x8 q[C][P][KC];
-    float rs[C];      // what a score is multiplied with, but for the keys' scale
-    int hi[C], lo[C];  // visible: lo < position <= hi
-#pragma unroll
-    for (int c = 0; c < C; c++) {
-      const unsigned r = 16 * c + i;
-      const bool valid = r < item.rows;
-      const unsigned row = item.row0 + (valid ? r : 0), tok = row / (unsigned)a.g.group;
-      hi[c] = valid ? (int)(sq.len0 + tok) : -1;
-      lo[c] = a.window ? (int)(sq.len0 + tok) - a.window : -1;
-      const size_t at = (size_t)(sq.tok0 + tok) * a.q_stride +
-                        ((size_t)item.head * a.g.group + row % (unsigned)a.g.group) * a.g.hd;
-      float x[KC][8], top = 0.0f;
-#pragma unroll
-      for (int kk = 0; kk < KC; kk++) {
-        const int d0 = kk / 2 < KC / 2 ? 64 * (kk / 2) + 16 * g + 8 * (kk & 1) : 64 * (KC / 2) + 8 * g;
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[kk][e] = 0.0f;
-        if (valid && d0 < a.g.hd) load8(a.dtype, a.q, at + d0, a.vec, x[kk]);
-#pragma unroll
-        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[kk][e]));
-      }
-      top = row_max(top);
-      int ex = 0;
-      if (top > 0.0f && top < __builtin_inff()) (void)frexpf(top, &ex);
-      ex = ex < -100 ? -100 : ex;
-      const float up = ldexpf(1.0f, 14 - ex);
-      rs[c] = a.scale * ldexpf(1.0f, ex - 14);
-#pragma unroll
-      for (int kk = 0; kk < KC; kk++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float y = x[kk][e] * up;
-          const _Float16 h = (_Float16)y;
-          q[c][0][kk][e] = h;
-          if constexpr (P == 2) q[c][1][kk][e] = (_Float16)(y - (float)h);
-        }
-    }
-    // pages that every row sees whole: from position `first` to `last`
-    const int last = (int)(sq.len0 + item.row0 / (unsigned)a.g.group);
-    const int first = a.window ? (int)(sq.len0 + (item.row0 + item.rows - 1) / (unsigned)a.g.group) - a.window + 1 : 0;
-
-    float m[C], l[C];
-    int vk[C];  // 2^vk is above the values' scales so far, and what probabilities are relative to
-    f32x4 o[C][ND];
-#pragma unroll
-    for (int c = 0; c < C; c++) {
-      m[c] = -__builtin_inff();
-      l[c] = 0.0f;
-      vk[c] = -126;
-#pragma unroll
-      for (int n = 0; n < ND; n++) o[c][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
 
     // ---- the pages -------------------------------------------------------------
     u32x4 kreg[KC / 2][4];
@@ -244,13 +155,94 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_kv_attend(KvAttnArgs a) {
         if (n < NDMIN || n < nd) vreg[n] = *(const u32x4*)(base + a.g.v_off + n * 1024 + lane * 16);
       vs = *(const f32x4*)(base + a.g.s_off + 16);
     };
+    // a page's place is read one page ahead of its keys, these one page ahead of
+    // their use, its values behind the use of the last ones
     unsigned p = item.page0 + wave;
-    const uint8_t* base = nullptr;
+    uint32_t ahead = 0;
     if (p < item.page1) {
-      base = pool + (size_t)table[p] * a.g.page_bytes;
+      const uint8_t* base = pool + (size_t)table[p] * a.g.page_bytes;
+      if (p + ATT_WAVES < item.page1) ahead = table[p + ATT_WAVES];
       load_k(base);
       load_v(base);
     }
+    // ---- the query rows ------------------------------------------------------
+    // loaded whole before any is used; rows and numbers that are missing read others
+    T raw[C][KC][8];
+    int hi[C], lo[C];  // visible: lo < position <= hi
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      const unsigned r = 16 * c + i;
+      const bool valid = r < item.rows;
+      const unsigned row = item.row0 + (valid ? r : 0), tok = row / (unsigned)a.g.group;
+      hi[c] = valid ? (int)(item.len0 + tok) : -1;
+      lo[c] = a.window ? (int)(item.len0 + tok) - a.window : -1;
+      const T* x = (const T*)a.q + (size_t)(item.tok0 + tok) * a.q_stride +
+                   ((size_t)item.head * a.g.group + row % (unsigned)a.g.group) * a.g.hd;
+      if (a.vec) {
+#pragma unroll
+        for (int kk = 0; kk < KC; kk++) {
+          const int d = query_dim(KC, kk, g);
+          const T* p8 = x + (d < a.g.hd ? d : 0);
+          *(u32x2*)&raw[c][kk][0] = *(const u32x2*)p8;
+          *(u32x2*)&raw[c][kk][8 / sizeof(T)] = *(const u32x2*)(p8 + 8 / sizeof(T));
+          if constexpr (sizeof(T) == 4) {
+            *(u32x2*)&raw[c][kk][4] = *(const u32x2*)(p8 + 4);
+            *(u32x2*)&raw[c][kk][6] = *(const u32x2*)(p8 + 6);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < KC; kk++) {
+          const int d = query_dim(KC, kk, g);
+#pragma unroll
+          for (int e = 0; e < 8; e++) raw[c][kk][e] = x[(d < a.g.hd ? d : 0) + e];
+        }
+      }
+    }
+    f16x8 q[C][P][KC];
+    float rs[C];  // what a score is multiplied with, but for the keys' scale
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      float x[KC][8], top = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < KC; kk++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          x[kk][e] = 16 * c + i < item.rows && query_dim(KC, kk, g) < a.g.hd ? to_f32(raw[c][kk][e]) : 0.0f;
+          top = fmaxf(top, fabsf(x[kk][e]));
+        }
+      top = row_max(top);
+      // the power of two that takes the row's largest to [2^13, 2^14)
+      int ex = (int)(__float_as_uint(top) >> 23) - 126;
+      ex = ex < -100 ? -100 : ex > 128 ? 128 : ex;
+      const float up = ex > 100 ? pow2(-100) * pow2(114 - ex) : pow2(14 - ex);
+      rs[c] = ex > 100 ? a.scale * pow2(100) * pow2(ex - 114) : a.scale * pow2(ex - 14);
+#pragma unroll
+      for (int kk = 0; kk < KC; kk++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float y = x[kk][e] * up;
+          const _Float16 h = (_Float16)y;
+          q[c][0][kk][e] = h;
+          if constexpr (P == 2) q[c][1][kk][e] = (_Float16)(y - (float)h);
+        }
+    }
+    // pages that every row sees whole: from position `first` to `last`
+    const int last = (int)(item.len0 + item.row0 / (unsigned)a.g.group);
+    const int first = a.window ? (int)(item.len0 + (item.row0 + item.rows - 1) / (unsigned)a.g.group) - a.window + 1 : 0;
+
+    float m[C], l[C];
+    int vk[C];  // 2^vk is above the values' scales so far, and what probabilities are relative to
+    f32x4 o[C][ND];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      m[c] = -__builtin_inff();
+      l[c] = 0.0f;
+      vk[c] = -126;
+#pragma unroll
+      for (int n = 0; n < ND; n++) o[c][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
     while (p < item.page1) {
       f32x4 s[C][4];
 #pragma unroll
@@ -276,7 +268,8 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_kv_attend(KvAttnArgs a) {
       const unsigned pn = p + ATT_WAVES;
       const uint8_t* next = nullptr;
       if (pn < item.page1) {
-        next = pool + (size_t)table[pn] * a.g.page_bytes;
+        next = pool + (size_t)ahead * a.g.page_bytes;
+        if (pn + ATT_WAVES < item.page1) ahead = table[pn + ATT_WAVES];
         load_k(next);
       }
       const int pos0 = (int)(p * KV_PAGE);
@@ -349,7 +342,6 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_kv_attend(KvAttnArgs a) {
       }
       if (next) load_v(next);
       p = pn;
-      base = next;
     }
 
     // ---- the waves' results joined, 16 rows at a time --------------------------
@@ -383,7 +375,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_kv_attend(KvAttnArgs a) {
 #pragma unroll
           for (int w = 0; w < ATT_WAVES; w++) v = v + *(const f32x4*)&so[w][r][d] * f[w];
           if (item.part == KV_WHOLE)
-            store4(a.dtype, a.out, (size_t)(sq.tok0 + tok) * a.out_stride + (size_t)h * a.g.hd + d, a.vec, v * inv);
+            store4(a.dtype, a.out, (size_t)(item.tok0 + tok) * a.out_stride + (size_t)h * a.g.hd + d, a.vec, v * inv);
           else
             *(f32x4*)(a.part_o + prow * a.g.hd + d) = v;
         }
@@ -393,81 +385,83 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_kv_attend(KvAttnArgs a) {
   }
 }
 
-// Joins the partial results of an item's rows: a work-group per 16 rows, 16
-// threads per row, the parts in their order.
+// Joins the partial results of one row: a work-group, whose threads take four
+// numbers each of every so many'th part; the slices are added in their order.
 __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a, int rows_per_part) {
-  __shared__ float sw[16][65];
-  const int r = threadIdx.x / 16, j = threadIdx.x % 16;
+  __shared__ float sw[KV_MAX_PARTS];
+  __shared__ float red[8];
+  __shared__ f32x4 sv[256];
+  const int t = threadIdx.x, wave = t >> 6;
+  const int quads = a.g.hd / 4, lanes = quads <= 16 ? 16 : quads <= 32 ? 32 : 64, slices = 256 / lanes;
+  const int x = t % lanes, slice = t / lanes;
   const unsigned njoins = a.njoins != 0xffffffffu ? a.njoins : a.counts[1];
   for (unsigned it = blockIdx.x; it < njoins; it += gridDim.x) {
     const KvJoin join = a.joins[it];
-    const unsigned row = 16 * blockIdx.y + r;
-    const bool valid = row < join.rows;
+    const unsigned row = blockIdx.y;
+    if (row >= join.rows) continue;
     const float2* ml = a.part_ml + (size_t)join.part0 * rows_per_part + row;
-    const float* po = a.part_o + ((size_t)join.part0 * rows_per_part + row) * a.g.hd;
-    float top = -__builtin_inff();
-    if (valid)
-      for (unsigned k = j; k < join.parts; k += 16) top = fmaxf(top, ml[(size_t)k * rows_per_part].x);
+    const float* po = a.part_o + ((size_t)join.part0 * rows_per_part + row) * a.g.hd + 4 * x;
+    const size_t step = (size_t)rows_per_part * a.g.hd;
+    float2 mine[KV_MAX_PARTS / 256];
+    float top = -__builtin_inff(), total = 0.0f;
 #pragma unroll
-    for (int x = 1; x < 16; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+    for (int k = 0; k < (int)KV_MAX_PARTS / 256; k++) {
+      const unsigned part = t + 256 * k;
+      mine[k] = part < join.parts ? ml[(size_t)part * rows_per_part] : float2{-__builtin_inff(), 0.0f};
+      top = fmaxf(top, mine[k].x);
+    }
+    top = wave_max_f32(top);
+    __syncthreads();  // the row before is read
+    if (t % 64 == 0) red[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float base2 = top == -__builtin_inff() ? 0.0f : top;
-    float total = 0.0f;
-    f32x4 v[4];
 #pragma unroll
-    for (int n = 0; n < 4; n++) v[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (unsigned k0 = 0; k0 < join.parts; k0 += 64) {
-      const unsigned n = join.parts - k0 < 64 ? join.parts - k0 : 64;
-      __syncthreads();
-      if (valid)
-        for (unsigned k = j; k < n; k += 16) {
-          const float2 x = ml[(size_t)(k0 + k) * rows_per_part];
-          const float w = exp2_fast(x.x - base2);
-          sw[r][k] = w;
-          total += w * x.y;
-        }
-      __syncthreads();
-      if (valid)
-        for (unsigned k = 0; k < n; k++) {
-          const float w = sw[r][k];
-          const float* src = po + (size_t)(k0 + k) * rows_per_part * a.g.hd;
-#pragma unroll
-          for (int x = 0; x < 4; x++)
-            if (64 * x + 4 * j < a.g.hd) v[x] = v[x] + *(const f32x4*)(src + 64 * x + 4 * j) * w;
-        }
+    for (int k = 0; k < (int)KV_MAX_PARTS / 256; k++) {
+      const unsigned part = t + 256 * k;
+      const float w = exp2_fast(mine[k].x - base2);
+      if (part < join.parts) sw[part] = w;
+      total += w * mine[k].y;
     }
 #pragma unroll
-    for (int x = 1; x < 16; x *= 2) total += __shfl_xor(total, x);
-    if (valid) {
-      const KvStepSeq sq = a.seqs[join.seq];
+    for (int o = 32; o; o /= 2) total += __shfl_xor(total, o);
+    if (t % 64 == 0) red[4 + wave] = total;
+    __syncthreads();
+    total = (red[4] + red[5]) + (red[6] + red[7]);
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (x < quads) {
+#pragma unroll 4
+      for (unsigned k = slice; k < join.parts; k += slices) v = v + *(const f32x4*)(po + k * step) * sw[k];
+    }
+    sv[t] = v;
+    __syncthreads();
+    if (slice == 0 && x < quads) {
+      for (int k = 1; k < slices; k++) v = v + sv[x + lanes * k];
       const unsigned tok = (join.row0 + row) / (unsigned)a.g.group;
       const unsigned h = join.head * a.g.group + (join.row0 + row) % (unsigned)a.g.group;
       const float inv = total > 0.0f ? 1.0f / total : 0.0f;
-#pragma unroll
-      for (int x = 0; x < 4; x++)
-        if (64 * x + 4 * j < a.g.hd)
-          store4(a.dtype, a.out, (size_t)(sq.tok0 + tok) * a.out_stride + (size_t)h * a.g.hd + 64 * x + 4 * j, a.vec,
-                 v[x] * inv);
+      store4(a.dtype, a.out, (size_t)(join.tok0 + tok) * a.out_stride + (size_t)h * a.g.hd + 4 * x, a.vec, v * inv);
     }
   }
 }
 
-template <int KC, int P>
+template <typename T, int KC>
 static hipError_t attend_cols(const KvAttnArgs& a, int cols, unsigned grid, hipStream_t st) {
-  if (cols == 1) return launch(k_kv_attend<KC, 1, P>, grid, 64 * ATT_WAVES, 0, st, a);
-  if constexpr (KC <= 6) {
-    if (cols == 2) return launch(k_kv_attend<KC, 2, P>, grid, 64 * ATT_WAVES, 0, st, a);
+  if (cols == 1) return launch(k_kv_attend<T, KC, 1>, grid, 64 * ATT_WAVES, 0, st, a);
+  if constexpr (KC <= 4) {
+    if (cols == 2) return launch(k_kv_attend<T, KC, 2>, grid, 64 * ATT_WAVES, 0, st, a);
   }
   return hipErrorInvalidValue;
 }
 
-template <int P>
-static hipError_t attend_parts(const KvAttnArgs& a, int cols, unsigned grid, hipStream_t st) {
+template <typename T>
+static hipError_t attend_typed(const KvAttnArgs& a, int cols, unsigned grid, hipStream_t st) {
   switch (a.g.chunks) {
-    case 2: return attend_cols<2, P>(a, cols, grid, st);
-    case 3: return attend_cols<3, P>(a, cols, grid, st);
-    case 4: return attend_cols<4, P>(a, cols, grid, st);
-    case 6: return attend_cols<6, P>(a, cols, grid, st);
-    case 8: return attend_cols<8, P>(a, cols, grid, st);
+    case 2: return attend_cols<T, 2>(a, cols, grid, st);
+    case 3: return attend_cols<T, 3>(a, cols, grid, st);
+    case 4: return attend_cols<T, 4>(a, cols, grid, st);
+    case 6: return attend_cols<T, 6>(a, cols, grid, st);
+    case 8: return attend_cols<T, 8>(a, cols, grid, st);
     default: return hipErrorInvalidValue;
   }
 }
@@ -475,9 +469,11 @@ static hipError_t attend_parts(const KvAttnArgs& a, int cols, unsigned grid, hip
 hipError_t launch_kv_attention(const KvAttnArgs& a, int cols, unsigned grid_items, unsigned grid_joins,
                                hipStream_t st) {
   if (grid_items == 0) return hipSuccess;
-  hipError_t e = a.dtype == F32 ? attend_parts<2>(a, cols, grid_items, st) : attend_parts<1>(a, cols, grid_items, st);
+  hipError_t e = a.dtype == F32   ? attend_typed<float>(a, cols, grid_items, st)
+                 : a.dtype == F16 ? attend_typed<_Float16>(a, cols, grid_items, st)
+                                  : attend_typed<Bf16>(a, cols, grid_items, st);
   if (e == hipSuccess && grid_joins)
-    e = launch(k_kv_join, dim3(grid_joins, (unsigned)cols), 256, 0, st, a, 16 * cols);
+    e = launch(k_kv_join, dim3(grid_joins, 16u * cols), 256, 0, st, a, 16 * cols);
   return e;
 }
 

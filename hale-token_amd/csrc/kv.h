@@ -79,12 +79,12 @@ hipError_t launch_kv_copy_pages(uint8_t* pool, size_t page_bytes, const KvCopy* 
 struct KvAppendArgs {
   KvGeom g;
   size_t layer;
-  const KvStepSeq* seqs;
   const KvBlock* blocks;
   const uint32_t* count;  // blocks of the step, on the device (captured calls), or null
   unsigned nblocks;       // the same
   const void *k, *v;  // [tokens][kv_heads][hd], a stride of so many elements per token
   size_t k_stride, v_stride;
+  bool vec;               // all rows start at multiples of 16 bytes
 };
 // grid: blocks launched for at least (they loop over the step's)
 hipError_t launch_kv_append(int dtype, const KvAppendArgs& a, unsigned grid, hipStream_t st);
@@ -103,7 +103,6 @@ struct KvAttnArgs {
   size_t q_stride, out_stride;
   float scale;                 // times log2(e)
   int window;                  // 0: none
-  const KvStepSeq* seqs;
   const KvItem* items;
   const KvJoin* joins;
   const uint32_t* counts;      // {items, joins} of the plan, on the device

@@ -181,7 +181,7 @@ struct View {  // the plan of the current step under one window
 // Sections of the plan's device buffer, in 32-bit words (multiples of four).
 // Their places hold until the buffer grows, so captured kernels keep them.
 struct Sections {
-  size_t counts = 0, seqs = 0, positions = 0, blocks = 0, items[HALE_KV_MAX_WINDOWS] = {},
+  size_t counts = 0, positions = 0, blocks = 0, items[HALE_KV_MAX_WINDOWS] = {},
          joins[HALE_KV_MAX_WINDOWS] = {}, words = 0;
 };
 constexpr size_t COUNT_WORDS = 4 + 4 * HALE_KV_MAX_WINDOWS;  // blocks; then items and joins per window
@@ -319,7 +319,6 @@ static Sections sections(const hale_kv_cache* kv, size_t tokens) {
   Sections s;
   const size_t n = kv->pages.max_seqs(), items = kv_max_items(kv->shape, tokens, n), joins = items - KV_MAX_PARTS;
   size_t w = COUNT_WORDS;
-  s.seqs = w, w += n * sizeof(KvStepSeq) / 4;
   s.positions = w, w += round_up(tokens, 4);
   s.blocks = w, w += round_up(kv_max_blocks(tokens, n) * sizeof(KvBlock) / 4, 4);
   for (int v = 0; v < HALE_KV_MAX_WINDOWS; v++) {
@@ -659,12 +658,11 @@ extern "C" int hale_kv_step(hale_kv_cache* kv, size_t nseq, const uint32_t* seqs
     const KvStepSeq& s = kv->seqs[i];
     mix(s.ntok);
     for (uint32_t t = 0; t < s.ntok; t++) positions[s.tok0 + t] = (int32_t)(s.len0 + t);
-    if (s.ntok)
-      for (uint32_t b = s.len0 / KV_BLOCK; b <= (s.len0 + s.ntok - 1) / KV_BLOCK; b++) blocks.push_back({i, b});
   }
+  kv_blocks(kv->seqs, kv->pages.max_pages(), &blocks);
   kv->step_shape = shape;
   kv->blocks = blocks.size();
-  size_t bytes = kv->copies.size() * sizeof(KvCopy) + nseq * sizeof(KvStepSeq) + tokens * 4 + blocks.size() * sizeof(KvBlock) + 64;
+  size_t bytes = kv->copies.size() * sizeof(KvCopy) + tokens * 4 + blocks.size() * sizeof(KvBlock) + 64;
   for (int i = 0; i < kv->nviews; i++) {
     build_view(kv, kv->views[i]);
     bytes += view_bytes(kv->views[i]);
@@ -674,7 +672,6 @@ extern "C" int hale_kv_step(hale_kv_cache* kv, size_t nseq, const uint32_t* seqs
   if (rc) return rc;
   const uint32_t n[4] = {(uint32_t)blocks.size(), (uint32_t)tokens, 0, 0};
   u.put(kv->plan + kv->at.counts, n, sizeof n);
-  u.put(kv->plan + kv->at.seqs, kv->seqs.data(), nseq * sizeof(KvStepSeq));
   u.put(kv->plan + kv->at.positions, positions.data(), tokens * 4);
   u.put(kv->plan + kv->at.blocks, blocks.data(), blocks.size() * sizeof(KvBlock));
   u.put(kv->list, kv->copies.data(), kv->copies.size() * sizeof(KvCopy));
@@ -751,7 +748,6 @@ extern "C" int hale_kv_append_device(hale_kv_cache* kv, size_t layer, int dtype,
   KvAppendArgs a{};
   a.g = kv->geom;
   a.layer = layer;
-  a.seqs = (const KvStepSeq*)(kv->plan + kv->at.seqs);
   a.blocks = (const KvBlock*)(kv->plan + kv->at.blocks);
   a.count = cap ? kv->plan + kv->at.counts : nullptr;
   a.nblocks = (unsigned)kv->blocks;
@@ -759,6 +755,8 @@ extern "C" int hale_kv_append_device(hale_kv_cache* kv, size_t layer, int dtype,
   a.v = v;
   a.k_stride = k_stride;
   a.v_stride = v_stride;
+  const size_t both = (uintptr_t)k | (uintptr_t)v | k_stride * type_bytes(dtype) | v_stride * type_bytes(dtype);
+  a.vec = both % 16 == 0;  // head_dim is a multiple of 16
   // later steps of these tokens may touch one block more per sequence
   const size_t grid = cap ? kv_max_blocks(ntok, kv->seqs.size()) : kv->blocks;
   KV_LAUNCH(c, K_KV_STORE, launch_kv_append(dtype, a, (unsigned)grid, c->stream));
@@ -812,7 +810,6 @@ extern "C" int hale_kv_attention_device(hale_kv_cache* kv, size_t layer, int dty
   a.out_stride = out_stride;
   a.scale = scale * 1.44269504088896340736f;
   a.window = (int)window;
-  a.seqs = (const KvStepSeq*)(kv->plan + kv->at.seqs);
   a.items = (const KvItem*)(kv->plan + kv->at.items[i]);
   a.joins = (const KvJoin*)(kv->plan + kv->at.joins[i]);
   a.counts = kv->plan + kv->at.counts + 4 + 4 * i;

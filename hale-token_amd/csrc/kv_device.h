@@ -6,7 +6,11 @@
 
 #include <algorithm>
 
+#include "hale_device.h"
+
 namespace hale {
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 // A bf16 number: the upper half of an f32.
 struct Bf16 {

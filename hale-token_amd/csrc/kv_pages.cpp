@@ -264,8 +264,7 @@ void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window
   total *= s.kv_heads;
   // a work-group's waves take a page each: fewer than four leave some idle
   const size_t each = std::max<size_t>(4, ceil_div(total, KV_TARGET_GROUPS));
-  for (uint32_t i = 0; i < seqs.size(); i++) {
-    const KvStepSeq& q = seqs[i];
+  for (const KvStepSeq& q : seqs) {
     // the rows with the most pages first, so that the last work-groups are short
     const size_t tiles = ceil_div(q.ntok * group, rows);
     for (size_t t = tiles; t-- > 0;) {
@@ -273,11 +272,26 @@ void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window
       range(q, r, n, &a, &b);
       const size_t parts = ceil_div(b - a, each);
       for (uint32_t h = 0; h < s.kv_heads; h++) {
-        if (parts > 1) out->joins.push_back({i, h, (uint32_t)r, (uint32_t)n, out->parts, (uint32_t)parts, {0, 0}});
+        if (parts > 1) out->joins.push_back({q.tok0, (uint16_t)h, (uint16_t)n, (uint32_t)r, out->parts, (uint32_t)parts, {0, 0, 0}});
         for (size_t k = 0; k < parts; k++)
-          out->items.push_back({i, h, (uint32_t)r, (uint32_t)n, (uint32_t)(a + (b - a) * k / parts),
-                                (uint32_t)(a + (b - a) * (k + 1) / parts), parts > 1 ? out->parts++ : KV_WHOLE, 0});
+          out->items.push_back({q.row, q.len0, q.tok0, (uint16_t)h, (uint16_t)n, (uint32_t)r,
+                                (uint32_t)(a + (b - a) * k / parts), (uint32_t)(a + (b - a) * (k + 1) / parts),
+                                parts > 1 ? out->parts++ : KV_WHOLE});
       }
+    }
+  }
+}
+
+void kv_blocks(const std::vector<KvStepSeq>& seqs, size_t max_pages, std::vector<KvBlock>* out) {
+  out->clear();
+  for (const KvStepSeq& q : seqs) {
+    if (!q.ntok) continue;
+    const uint32_t end = q.len0 + q.ntok;
+    for (uint32_t b = q.len0 / KV_BLOCK; b * KV_BLOCK < end; b++) {
+      const uint32_t pos = b * KV_BLOCK;
+      out->push_back({(uint32_t)(q.row * max_pages + pos / KV_PAGE), (int32_t)(q.tok0 + pos - q.len0),
+                      (uint8_t)(pos % KV_PAGE / KV_BLOCK), (uint8_t)(q.len0 > pos ? q.len0 - pos : 0),
+                      (uint8_t)(end - pos < KV_BLOCK ? end - pos : KV_BLOCK), 0, 0});
     }
   }
 }

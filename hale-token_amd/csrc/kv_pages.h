@@ -23,27 +23,36 @@ struct KvStepSeq {
   uint32_t tok0;   // the first one's index among the step's tokens
 };
 
-// A block of 16 positions that the step's tokens touch.
+// A block of 16 positions that the step's tokens touch: positions old .. end -
+// 1 of it are new, the one at j is token tok + j.
 struct KvBlock {
-  uint32_t seq, block;  // index into the step's sequences; position / 16
+  uint32_t entry;  // of its page in the page table
+  int32_t tok;     // may be negative
+  uint8_t block;   // of the page: 0..3
+  uint8_t old, end, pad;
+  uint32_t pad2;
 };
 
 // One work-group's share of the attention: rows row0 .. row0 + rows - 1 of a
 // sequence's queries of one key/value head (row r is token r / group, head
 // r % group of the group) over pages page0 .. page1 - 1.
 struct KvItem {
-  uint32_t seq, head, row0, rows;
+  uint32_t row;    // of the page table
+  uint32_t len0, tok0;  // as in KvStepSeq
+  uint16_t head, rows;
+  uint32_t row0;
   uint32_t page0, page1;
   uint32_t part;  // its slot among the partial results, or KV_WHOLE
-  uint32_t pad;
 };
 constexpr uint32_t KV_WHOLE = 0xffffffffu;
 
 // Partial results part0 .. part0 + parts - 1 to be joined, the rows of one item.
 struct KvJoin {
-  uint32_t seq, head, row0, rows;
+  uint32_t tok0;
+  uint16_t head, rows;
+  uint32_t row0;
   uint32_t part0, parts;
-  uint32_t pad[2];
+  uint32_t pad[3];
 };
 
 // The attention of a step under one window.
@@ -69,12 +78,15 @@ constexpr size_t KV_TARGET_GROUPS = 512;
 constexpr size_t KV_MAX_PARTS = 2 * KV_TARGET_GROUPS;
 
 // Most groups of 16 rows that the attention kernels hold at once.
-inline int kv_max_cols(size_t head_dim) { return head_dim <= 192 ? 2 : 1; }
+inline int kv_max_cols(size_t head_dim) { return head_dim <= 128 ? 2 : 1; }
 
 // Divides the attention of a step: rows of 16 * cols per work-group, few
 // enough pages each that all compute units take part.  Window 0 sees every
 // earlier position.
 void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window, KvPlan* out);
+
+// The blocks that a step's tokens touch.
+void kv_blocks(const std::vector<KvStepSeq>& seqs, size_t max_pages, std::vector<KvBlock>* out);
 
 // Most items and blocks that a plan of so many tokens and sequences can have.
 size_t kv_max_items(const KvShape& s, size_t tokens, size_t nseq);

@@ -197,7 +197,7 @@ void plans() {
     std::vector<KvStepSeq> seqs(below(below(3) ? 4 : 40));
     uint32_t tok = 0;
     for (auto& q : seqs) {
-      q = {0, (uint32_t)(below(3) ? below(3000) : below(200000)), (uint32_t)(below(2) ? below(8) : below(400)), tok};
+      q = {(uint32_t)(&q - seqs.data()), (uint32_t)(below(3) ? below(3000) : below(200000)), (uint32_t)(below(2) ? below(8) : below(400)), tok};
       tok += q.ntok;
     }
     const size_t window = below(2) ? 0 : 1 + below(below(2) ? 100 : 5000);
@@ -207,16 +207,30 @@ void plans() {
     CHECK(plan.parts <= KV_MAX_PARTS);
     CHECK(plan.items.size() <= kv_max_items(s, tok, seqs.size()));
     CHECK(plan.joins.size() + KV_MAX_PARTS <= kv_max_items(s, tok, seqs.size()));
-    size_t blocks = 0;
-    for (auto& q : seqs)
-      if (q.ntok) blocks += (q.len0 + q.ntok - 1) / KV_BLOCK - q.len0 / KV_BLOCK + 1;
-    CHECK(blocks <= kv_max_blocks(tok, seqs.size()));
+    // every new token is in one block, at its position, and no other is
+    std::vector<KvBlock> blocks;
+    const size_t max_pages = 4096;
+    kv_blocks(seqs, max_pages, &blocks);
+    CHECK(blocks.size() <= kv_max_blocks(tok, seqs.size()));
+    std::vector<int> seen(tok, 0);
+    for (const KvBlock& b : blocks) {
+      const KvStepSeq& q = seqs[b.entry / max_pages];
+      CHECK(b.block < 4 && b.old < b.end && b.end <= KV_BLOCK);
+      const size_t pos = b.entry % max_pages * KV_PAGE + b.block * KV_BLOCK;
+      CHECK(b.old == (q.len0 > pos ? q.len0 - pos : 0));
+      for (int j = b.old; j < b.end; j++) {
+        const long long t = (long long)b.tok + j;
+        CHECK(t == (long long)q.tok0 + (long long)(pos + j) - q.len0 && t >= q.tok0 && t < (long long)q.tok0 + q.ntok);
+        seen[t]++;
+      }
+    }
+    for (int n : seen) CHECK(n == 1);
     std::map<std::pair<std::pair<uint32_t, uint32_t>, uint32_t>, std::vector<const KvItem*>> tiles;
     for (const KvItem& it : plan.items) {
-      CHECK(it.seq < seqs.size() && it.head < s.kv_heads && it.rows >= 1 && it.rows <= 16u * plan.cols);
-      CHECK(it.row0 % (16 * plan.cols) == 0 && it.row0 + it.rows <= seqs[it.seq].ntok * s.group());
+      CHECK(it.row < seqs.size() && it.len0 == seqs[it.row].len0 && it.tok0 == seqs[it.row].tok0 && it.head < s.kv_heads && it.rows >= 1 && it.rows <= 16u * plan.cols);
+      CHECK(it.row0 % (16 * plan.cols) == 0 && it.row0 + it.rows <= seqs[it.row].ntok * s.group());
       CHECK(it.page0 < it.page1);
-      tiles[{{it.seq, it.head}, it.row0}].push_back(&it);
+      tiles[{{it.row, it.head}, it.row0}].push_back(&it);
     }
     size_t want = 0;
     for (auto& q : seqs) want += (q.ntok * s.group() + 16 * plan.cols - 1) / (16 * plan.cols) * s.kv_heads;
@@ -230,7 +244,7 @@ void plans() {
     size_t divided = 0;
     for (auto& t : tiles) {
       auto& v = t.second;
-      const KvStepSeq& q = seqs[v[0]->seq];
+      const KvStepSeq& q = seqs[v[0]->row];
       std::sort(v.begin(), v.end(), [](const KvItem* a, const KvItem* b) { return a->page0 < b->page0; });
       const size_t low = q.len0 + v[0]->row0 / s.group(), high = q.len0 + (v[0]->row0 + v[0]->rows - 1) / s.group();
       CHECK(v.back()->page1 == high / KV_PAGE + 1);
@@ -246,7 +260,7 @@ void plans() {
       if (v.size() > 1) {
         divided++;
         const KvJoin* j = joins.at(v[0]->part);
-        CHECK(j->parts == v.size() && j->seq == v[0]->seq && j->head == v[0]->head && j->row0 == v[0]->row0 && j->rows == v[0]->rows);
+        CHECK(j->parts == v.size() && j->tok0 == v[0]->tok0 && j->head == v[0]->head && j->row0 == v[0]->row0 && j->rows == v[0]->rows);
       }
     }
     CHECK(divided == plan.joins.size() && parts.size() == plan.parts);
