@@ -19,6 +19,62 @@ namespace hale {
 // the f32 argument of sin and cos is exact to 2^-24 of a turn's fraction at any
 // position an int32 holds; in f32 the angle of position 10^6 would be off by
 // 0.03.
+// Rows of 16-byte pieces: a work-group per row (blockIdx.y: its share of the
+// heads) finds the row's cosines and sines once, a thread then turns eight pairs of
+// a head at a time, or copies eight numbers behind them.
+template <typename T, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void k_rope_vec(RopeArgs a) {
+  __shared__ float2 cs[512];
+  const size_t row = blockIdx.x;
+  const int pos = a.pos[row], turned = a.half / 8, rest = (a.hd - 2 * a.half) / 8, per = turned + rest;
+  const int units = (a.heads[0] + a.heads[1]) * per;
+  for (int e = threadIdx.x; e < a.half; e += 256) rope_angle(pos, a.turns[e], a.factor, &cs[e].x, &cs[e].y);
+  __syncthreads();
+  union Piece {
+    u32x4 u[sizeof(T) / 2];
+    T v[8];
+  };
+  auto load = [](Piece& p, const T* x) {
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T) / 2; j++) p.u[j] = ((const u32x4*)x)[j];
+  };
+  auto store = [](const Piece& p, T* x) {
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T) / 2; j++) ((u32x4*)x)[j] = p.u[j];
+  };
+#pragma unroll 2
+  for (int u = blockIdx.y * 256 + threadIdx.x; u < units; u += 256 * gridDim.y) {
+    int h = u / per;
+    const int j = u % per, which = h >= a.heads[0];
+    if (which) h -= a.heads[0];
+    const T* x = (const T*)a.src[which] + row * a.src_stride[which] + (size_t)h * a.hd;
+    T* y = (T*)a.dst[which] + row * a.dst_stride[which] + (size_t)h * a.hd;
+    Piece p, q;
+    if (j >= turned) {
+      const int d = 2 * a.half + (j - turned) * 8;
+      if (x == y) continue;
+      load(p, x + d);
+      store(p, y + d);
+      continue;
+    }
+    const int d0 = INTERLEAVED ? 16 * j : 8 * j, d1 = INTERLEAVED ? 16 * j + 8 : 8 * j + a.half;
+    load(p, x + d0);
+    load(q, x + d1);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const float2 t = cs[8 * j + e];
+      T& s0 = INTERLEAVED ? (e < 4 ? p.v[2 * (e & 3)] : q.v[2 * (e & 3)]) : p.v[e];
+      T& s1 = INTERLEAVED ? (e < 4 ? p.v[2 * (e & 3) + 1] : q.v[2 * (e & 3) + 1]) : q.v[e];
+      const float f = to_f32(s0), g = to_f32(s1);
+      s0 = from_f32<T>(f * t.x - g * t.y);
+      s1 = from_f32<T>(g * t.x + f * t.y);
+    }
+    store(p, y + d0);
+    store(q, y + d1);
+  }
+}
+
+// Any strides, alignments and dimensions: a thread per pair or copied number.
 template <typename T>
 __global__ __launch_bounds__(256) void k_rope(RopeArgs a) {
   // a thread per pair or untouched number of one head, its rows apart
@@ -47,14 +103,29 @@ __global__ __launch_bounds__(256) void k_rope(RopeArgs a) {
   }
 }
 
-hipError_t launch_rope(int dtype, const RopeArgs& a, hipStream_t st) {
+template <typename T>
+static hipError_t rope_typed(const RopeArgs& a, hipStream_t st) {
+  size_t bits = 0;
+  for (int i = 0; i < 2; i++)
+    if (a.heads[i]) bits |= (uintptr_t)a.src[i] | (uintptr_t)a.dst[i] | (a.src_stride[i] | a.dst_stride[i]) * sizeof(T);
+  if (bits % 16 == 0 && a.hd % 8 == 0 && a.half % 8 == 0) {
+    const int units = (a.heads[0] + a.heads[1]) * (a.half / 8 + (a.hd - 2 * a.half) / 8);
+    // few rows: their heads spread over more work-groups
+    const unsigned split = a.rows >= 512 ? 1 : (unsigned)(units + 255) / 256;
+    const dim3 grid((unsigned)a.rows, split);
+    return a.interleaved ? launch(k_rope_vec<T, true>, grid, 256, 0, st, a) : launch(k_rope_vec<T, false>, grid, 256, 0, st, a);
+  }
   const size_t total = a.rows * (size_t)(a.heads[0] + a.heads[1]) * (a.hd - a.half);
   if (total == 0) return hipSuccess;
   const unsigned grid = (unsigned)std::min<size_t>((total + 255) / 256, 1u << 20);
+  return launch(k_rope<T>, grid, 256, 0, st, a);
+}
+
+hipError_t launch_rope(int dtype, const RopeArgs& a, hipStream_t st) {
   switch (dtype) {
-    case F32: return launch(k_rope<float>, grid, 256, 0, st, a);
-    case F16: return launch(k_rope<_Float16>, grid, 256, 0, st, a);
-    case BF16: return launch(k_rope<Bf16>, grid, 256, 0, st, a);
+    case F32: return rope_typed<float>(a, st);
+    case F16: return rope_typed<_Float16>(a, st);
+    case BF16: return rope_typed<Bf16>(a, st);
     default: return hipErrorInvalidValue;
   }
 }
@@ -280,29 +351,72 @@ hipError_t launch_kv_append(int dtype, const KvAppendArgs& a, unsigned grid, hip
 // reading back
 // ---------------------------------------------------------------------------
 
+// A work-group per page, head, and keys or values; a lane reads 16 bytes as they
+// lie: 16 numbers of one position of the keys (four 16-byte stores, 64 bytes of
+// a row), 16 positions of one number of the values (16 stores, of which a wave's
+// make 64-byte pieces of four rows).
 __global__ __launch_bounds__(256) void k_kv_read(KvGeom g, size_t layer, uint32_t row, size_t first, size_t count,
                                                  float* k, float* v) {
-  const size_t total = count * g.kv_heads * g.hd;
-  for (size_t id = (size_t)blockIdx.x * 256 + threadIdx.x; id < total; id += (size_t)gridDim.x * 256) {
-    const unsigned d = (unsigned)(id % g.hd);
-    const size_t rest = id / g.hd;
-    const unsigned head = (unsigned)(rest % g.kv_heads);
-    const size_t pos = first + rest / g.kv_heads;
-    const uint32_t page = g.table[(size_t)row * g.max_pages + pos / KV_PAGE];
-    const uint8_t* region = g.pool + page * g.page_bytes + layer * g.layer_bytes + (size_t)head * g.head_bytes;
-    const unsigned t = (unsigned)(pos % KV_PAGE);
-    const float* scale = (const float*)(region + g.s_off) + t / KV_BLOCK;
-    k[id] = (float)((int)region[kv_key_byte(g.chunks, t, d)] - 128) * scale[0];
-    v[id] = (float)((int)region[g.v_off + kv_value_byte(t, d)] - 128) * scale[4];
+  const size_t p = first / KV_PAGE + blockIdx.x;
+  const int head = blockIdx.y, hd = g.hd;
+  const uint8_t* region = g.pool + g.table[(size_t)row * g.max_pages + p] * g.page_bytes + layer * g.layer_bytes +
+                          (size_t)head * g.head_bytes;
+  const long long base = (long long)(p * KV_PAGE) - (long long)first;  // output row of the page's position 0
+  const size_t stride = (size_t)g.kv_heads * hd;
+  const f32x4 s = *(const f32x4*)(region + g.s_off + (blockIdx.z ? 16 : 0));
+  auto row_of = [&](int t) { return base + t; };
+  auto wanted = [&](long long r) { return r >= 0 && r < (long long)count; };
+  if (blockIdx.z == 0) {
+    float* out = k + (size_t)head * hd;
+    const int whole = g.chunks / 2 * 256;
+    for (int e = threadIdx.x; e < whole; e += 256) {
+      const int lane = e % 64, mm = e / 64 % 4, d = e / 256 * 64 + lane / 16 * 16;
+      const long long r = row_of(16 * mm + lane % 16);
+      if (!wanted(r) || d >= hd) continue;
+      const u32x4 w = *(const u32x4*)(region + e * 16);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        f32x4 x;
+#pragma unroll
+        for (int b = 0; b < 4; b++) x[b] = (float)((int)(w[j] >> (8 * b) & 255) - 128) * s[mm];
+        *(f32x4u*)(out + r * stride + d + 4 * j) = x;
+      }
+    }
+    if (g.chunks & 1) {
+      const int lane = threadIdx.x % 64, mm = threadIdx.x / 64, d = g.chunks / 2 * 64 + lane / 16 * 8;
+      const long long r = row_of(16 * mm + lane % 16);
+      if (wanted(r) && d < hd) {
+        const u32x2 w = *(const u32x2*)(region + whole * 16 + threadIdx.x * 8);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          f32x4 x;
+#pragma unroll
+          for (int b = 0; b < 4; b++) x[b] = (float)((int)(w[j] >> (8 * b) & 255) - 128) * s[mm];
+          *(f32x4u*)(out + r * stride + d + 4 * j) = x;
+        }
+      }
+    }
+  } else {
+    for (int e = threadIdx.x; e < hd * 4; e += 256) {
+      const int lane = e % 64, d = e / 64 * 16 + lane % 16;
+      const u32x4 w = *(const u32x4*)(region + g.v_off + e * 16);
+      float* out = v + (size_t)head * hd + d;
+#pragma unroll
+      for (int mm = 0; mm < 4; mm++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const long long r = row_of(16 * mm + lane / 16 * 4 + j);
+          if (wanted(r)) out[r * stride] = (float)((int)(w[mm] >> (8 * j) & 255) - 128) * s[mm];
+        }
+    }
   }
 }
 
 hipError_t launch_kv_read(const KvGeom& g, size_t layer, uint32_t row, size_t first, size_t count, float* k, float* v,
                           hipStream_t st) {
-  const size_t total = count * g.kv_heads * g.hd;
-  if (total == 0) return hipSuccess;
-  return launch(k_kv_read, (unsigned)std::min<size_t>((total + 255) / 256, 1u << 20), 256, 0, st, g, layer, row, first,
-                count, k, v);
+  if (count == 0) return hipSuccess;
+  const size_t pages = (first + count - 1) / KV_PAGE - first / KV_PAGE + 1;
+  return launch(k_kv_read, dim3((unsigned)pages, (unsigned)g.kv_heads, 2), 256, 0, st, g, layer, row, first, count, k, v);
 }
 
 }  // namespace hale

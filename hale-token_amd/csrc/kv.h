@@ -103,16 +103,22 @@ struct KvAttnArgs {
   size_t q_stride, out_stride;
   float scale;                 // times log2(e)
   int window;                  // 0: none
-  const KvItem* items;
+  const KvItem* items;         // of one kind
   const KvJoin* joins;
-  const uint32_t* counts;      // {items, joins} of the plan, on the device
+  const uint32_t* counts;      // {few, many, joins of few, of many} of the plan, on the device
   unsigned nitems, njoins;     // the same, or 0xffffffff: read counts (captured calls)
-  float* part_o;               // [part][16 cols][hd]
-  float2* part_ml;             // [part][16 cols] running maximum (base 2) and sum
+  int kind;                    // 0: items and joins of few rows, 1: of many
+  float* part_o;               // [row][hd]
+  float2* part_ml;             // [row] running maximum (base 2) and sum
   bool vec;                    // q and out rows start at multiples of four elements
 };
-// grid_items / grid_joins: work-groups launched (they loop over the plan)
-hipError_t launch_kv_attention(const KvAttnArgs& a, int cols, unsigned grid_items, unsigned grid_joins, hipStream_t st);
+// Sequences of few rows: cols groups of 16 per work-group.  grid: work-groups
+// launched (they loop over the plan).
+hipError_t launch_kv_attend_few(const KvAttnArgs& a, int cols, unsigned grid, hipStream_t st);
+// Of many rows: kv_many_rows per work-group.
+hipError_t launch_kv_attend_many(const KvAttnArgs& a, unsigned grid, hipStream_t st);
+// Joins of one kind, of at most `rows` rows each.
+hipError_t launch_kv_join(const KvAttnArgs& a, unsigned grid, unsigned rows, hipStream_t st);
 
 // ---- rotary positions --------------------------------------------------------
 

@@ -181,10 +181,11 @@ struct View {  // the plan of the current step under one window
 // Sections of the plan's device buffer, in 32-bit words (multiples of four).
 // Their places hold until the buffer grows, so captured kernels keep them.
 struct Sections {
-  size_t counts = 0, positions = 0, blocks = 0, items[HALE_KV_MAX_WINDOWS] = {},
-         joins[HALE_KV_MAX_WINDOWS] = {}, words = 0;
+  size_t counts = 0, positions = 0, blocks = 0, items[HALE_KV_MAX_WINDOWS] = {},  // few, `many` words on many
+         many = 0, joins[HALE_KV_MAX_WINDOWS] = {},                         // likewise
+         many_joins = 0, words = 0;
 };
-constexpr size_t COUNT_WORDS = 4 + 4 * HALE_KV_MAX_WINDOWS;  // blocks; then items and joins per window
+constexpr size_t COUNT_WORDS = 4 + 4 * HALE_KV_MAX_WINDOWS;  // blocks; then few, many and their joins per window
 
 }  // namespace
 
@@ -318,12 +319,14 @@ static void free_device(hale_kv_cache* kv) {
 static Sections sections(const hale_kv_cache* kv, size_t tokens) {
   Sections s;
   const size_t n = kv->pages.max_seqs(), items = kv_max_items(kv->shape, tokens, n), joins = items - KV_MAX_PARTS;
+  s.many = items * sizeof(KvItem) / 4;
+  s.many_joins = joins * sizeof(KvJoin) / 4;
   size_t w = COUNT_WORDS;
   s.positions = w, w += round_up(tokens, 4);
   s.blocks = w, w += round_up(kv_max_blocks(tokens, n) * sizeof(KvBlock) / 4, 4);
   for (int v = 0; v < HALE_KV_MAX_WINDOWS; v++) {
-    s.items[v] = w, w += items * sizeof(KvItem) / 4;
-    s.joins[v] = w, w += joins * sizeof(KvJoin) / 4;
+    s.items[v] = w, w += 2 * s.many;
+    s.joins[v] = w, w += 2 * s.many_joins;
   }
   s.words = w;
   return s;
@@ -414,7 +417,7 @@ extern "C" int hale_kv_create(hale_ctx* c, size_t layers, size_t heads, size_t k
   g.page_bytes = g.layer_bytes * layers;
   g.max_pages = (unsigned)row;
   rc = make_pool(c, g.page_bytes * num_pages, &g.pool);
-  const size_t part_rows = KV_MAX_PARTS * 16 * kv_max_cols(hd);
+  const size_t part_rows = kv_part_rows(hd);
   if (!rc && (hipMalloc(&kv->table, row * max_seqs * 4) != hipSuccess ||
               hipMalloc(&kv->list, num_pages * sizeof(KvCopy) + 16) != hipSuccess ||
               hipMalloc(&kv->part_o, part_rows * hd * 4) != hipSuccess ||
@@ -601,14 +604,17 @@ static void build_view(hale_kv_cache* kv, View& v) {
   kv_plan(kv->shape, kv->seqs, v.window, &v.plan);
 }
 static size_t view_bytes(const View& v) {
-  return v.plan.items.size() * sizeof(KvItem) + v.plan.joins.size() * sizeof(KvJoin) + 32;
+  return (v.plan.few.size() + v.plan.many.size()) * sizeof(KvItem) + (v.plan.few_joins.size() + v.plan.many_joins.size()) * sizeof(KvJoin) + 32;
 }
 static void put_view(hale_kv_cache* kv, Upload& u, int i) {
   View& v = kv->views[i];
-  const uint32_t n[4] = {(uint32_t)v.plan.items.size(), (uint32_t)v.plan.joins.size(), 0, 0};
+  const uint32_t n[4] = {(uint32_t)v.plan.few.size(), (uint32_t)v.plan.many.size(), (uint32_t)v.plan.few_joins.size(),
+                         (uint32_t)v.plan.many_joins.size()};
   u.put(kv->plan + kv->at.counts + 4 + 4 * i, n, sizeof n);
-  u.put(kv->plan + kv->at.items[i], v.plan.items.data(), v.plan.items.size() * sizeof(KvItem));
-  u.put(kv->plan + kv->at.joins[i], v.plan.joins.data(), v.plan.joins.size() * sizeof(KvJoin));
+  u.put(kv->plan + kv->at.items[i], v.plan.few.data(), v.plan.few.size() * sizeof(KvItem));
+  u.put(kv->plan + kv->at.items[i] + kv->at.many, v.plan.many.data(), v.plan.many.size() * sizeof(KvItem));
+  u.put(kv->plan + kv->at.joins[i], v.plan.few_joins.data(), v.plan.few_joins.size() * sizeof(KvJoin));
+  u.put(kv->plan + kv->at.joins[i] + kv->at.many_joins, v.plan.many_joins.data(), v.plan.many_joins.size() * sizeof(KvJoin));
   v.built = true;
 }
 
@@ -810,25 +816,34 @@ extern "C" int hale_kv_attention_device(hale_kv_cache* kv, size_t layer, int dty
   a.out_stride = out_stride;
   a.scale = scale * 1.44269504088896340736f;
   a.window = (int)window;
-  a.items = (const KvItem*)(kv->plan + kv->at.items[i]);
-  a.joins = (const KvJoin*)(kv->plan + kv->at.joins[i]);
+  const KvItem* items = (const KvItem*)(kv->plan + kv->at.items[i]);
+  const KvJoin* joins = (const KvJoin*)(kv->plan + kv->at.joins[i]);
   a.counts = kv->plan + kv->at.counts + 4 + 4 * i;
-  a.nitems = cap ? 0xffffffffu : (unsigned)v.plan.items.size();
-  a.njoins = cap ? 0xffffffffu : (unsigned)v.plan.joins.size();
   a.part_o = kv->part_o;
   a.part_ml = kv->part_ml;
   const size_t quad = 4 * type_bytes(dtype);
   a.vec = (uintptr_t)q % quad == 0 && (uintptr_t)out % quad == 0 && q_stride % 4 == 0 && out_stride % 4 == 0;
   // captured: later steps of these tokens may have more items, which the
   // work-groups then take in turn, and joins of the same rows
-  size_t gi = v.plan.items.size(), gj = v.plan.joins.size();
-  if (cap) {
-    const size_t tiles = kv_max_items(kv->shape, ntok, kv->seqs.size()) - KV_MAX_PARTS;
-    gi = std::max(gi, std::min<size_t>(tiles + KV_MAX_PARTS, 1024));
-    gj = std::max(gj, std::min<size_t>(tiles, 1024));
+  auto grid = [&](size_t now, size_t most) {
+    return (unsigned)std::min<size_t>(cap && now ? std::max(now, std::min<size_t>(most, 1024)) : now, 1u << 20);
+  };
+  const size_t tiles = kv_max_items(kv->shape, ntok, kv->seqs.size()) - KV_MAX_PARTS;
+  bool few = false, many = false;
+  for (const KvStepSeq& s : kv->seqs) (s.ntok * kv->shape.group() <= kv_few_rows(kv->shape.head_dim) ? few : many) |= s.ntok > 0;
+  for (int kind = 0; kind < 2; kind++) {
+    if (!(kind ? many : few)) continue;
+    const size_t nitems = (kind ? v.plan.many : v.plan.few).size(), njoins = (kind ? v.plan.many_joins : v.plan.few_joins).size();
+    a.kind = kind;
+    a.items = kind ? items + kv->at.many * 4 / sizeof(KvItem) : items;
+    a.joins = kind ? joins + kv->at.many_joins * 4 / sizeof(KvJoin) : joins;
+    a.nitems = cap ? 0xffffffffu : (unsigned)nitems;
+    a.njoins = cap ? 0xffffffffu : (unsigned)njoins;
+    const unsigned gi = grid(nitems, tiles + KV_MAX_PARTS), gj = cap ? (unsigned)std::min<size_t>(tiles, 256) : grid(njoins, 0);
+    const unsigned rows = kind ? (unsigned)kv_many_rows(kv->shape.head_dim) : 16u * v.plan.cols;
+    KV_LAUNCH(c, K_KV_ATTENTION, kind ? launch_kv_attend_many(a, gi, c->stream) : launch_kv_attend_few(a, v.plan.cols, gi, c->stream));
+    KV_LAUNCH(c, K_KV_ATTENTION, launch_kv_join(a, gj, rows, c->stream));
   }
-  KV_LAUNCH(c, K_KV_ATTENTION, launch_kv_attention(a, v.plan.cols, (unsigned)std::min<size_t>(gi, 1u << 20),
-                                                   (unsigned)std::min<size_t>(gj, 1u << 20), c->stream));
   return HALE_OK;
   KV_CATCH(c)
 }

@@ -11,6 +11,7 @@
 namespace hale {
 
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // at any float's address
 
 // A bf16 number: the upper half of an f32.
 struct Bf16 {

@@ -240,46 +240,122 @@ void KvPages::resize(size_t pages) {
   free_.swap(rest);
 }
 
-void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window, KvPlan* out) {
-  out->items.clear();
-  out->joins.clear();
-  out->parts = 0;
-  const size_t group = s.group();
-  size_t most = 0;
-  for (const KvStepSeq& q : seqs) most = std::max(most, q.ntok * group);
-  out->cols = most <= 16 ? 1 : kv_max_cols(s.head_dim);
-  const size_t rows = 16 * (size_t)out->cols;
-  // the pages that rows row0 .. row0 + n - 1 of sequence q see
-  auto range = [&](const KvStepSeq& q, size_t row0, size_t n, size_t* first, size_t* last) {
-    const size_t low = q.len0 + row0 / group, high = q.len0 + (row0 + n - 1) / group;
-    *first = window && low + 1 > window ? (low + 1 - window) / KV_PAGE : 0;
-    *last = high / KV_PAGE + 1;
-  };
-  size_t total = 0, a, b;
-  for (const KvStepSeq& q : seqs)
-    for (size_t r = 0; r < q.ntok * group; r += rows) {
-      range(q, r, std::min(rows, q.ntok * group - r), &a, &b);
-      total += b - a;
-    }
-  total *= s.kv_heads;
-  // a work-group's waves take a page each: fewer than four leave some idle
-  const size_t each = std::max<size_t>(4, ceil_div(total, KV_TARGET_GROUPS));
-  for (const KvStepSeq& q : seqs) {
-    // the rows with the most pages first, so that the last work-groups are short
-    const size_t tiles = ceil_div(q.ntok * group, rows);
-    for (size_t t = tiles; t-- > 0;) {
-      const size_t r = t * rows, n = std::min(rows, q.ntok * group - r);
-      range(q, r, n, &a, &b);
-      const size_t parts = ceil_div(b - a, each);
-      for (uint32_t h = 0; h < s.kv_heads; h++) {
-        if (parts > 1) out->joins.push_back({q.tok0, (uint16_t)h, (uint16_t)n, (uint32_t)r, out->parts, (uint32_t)parts, {0, 0, 0}});
-        for (size_t k = 0; k < parts; k++)
-          out->items.push_back({q.row, q.len0, q.tok0, (uint16_t)h, (uint16_t)n, (uint32_t)r,
-                                (uint32_t)(a + (b - a) * k / parts), (uint32_t)(a + (b - a) * (k + 1) / parts),
-                                parts > 1 ? out->parts++ : KV_WHOLE});
-      }
+namespace {
+
+struct Tile {
+  const KvStepSeq* q;
+  uint32_t head, row0, rows, page0, page1;
+};
+
+// Tiles into items of at most `each` pages, and the joins of those divided.
+void divide(const std::vector<Tile>& tiles, size_t each, size_t step, std::vector<KvItem>* items, std::vector<KvJoin>* joins,
+            uint32_t* part_rows) {
+  for (const Tile& t : tiles) {
+    const size_t n = t.page1 - t.page0, parts = ceil_div(n, each);
+    if (parts > 1)
+      joins->push_back({t.q->tok0, (uint16_t)t.head, (uint16_t)t.rows, t.row0, *part_rows, (uint32_t)parts, (uint32_t)step, {0, 0}});
+    for (size_t k = 0; k < parts; k++) {
+      items->push_back({t.q->row, t.q->len0, t.q->tok0, (uint16_t)t.head, (uint16_t)t.rows, t.row0,
+                        (uint32_t)(t.page0 + n * k / parts), (uint32_t)(t.page0 + n * (k + 1) / parts),
+                        parts > 1 ? *part_rows : KV_WHOLE});
+      if (parts > 1) *part_rows += (uint32_t)step;
     }
   }
+}
+
+size_t count_pages(const std::vector<Tile>& tiles) {
+  size_t total = 0;
+  for (const Tile& t : tiles) total += t.page1 - t.page0;
+  return total;
+}
+
+// Most pages of an item of many rows.  The work-groups that run at once take the
+// items in rounds; with the longest tile cut into 1, 2, .. parts, the time is about
+// the rounds times an item's mean pages (at least the longest item), and a
+// part costs about four pages for its partial result.  The cut of the least time.
+size_t many_each(const std::vector<Tile>& tiles) {
+  const size_t total = count_pages(tiles), least = ceil_div(total, KV_MANY_GROUPS);
+  size_t longest = 0, best = 0;
+  for (const Tile& t : tiles) longest = std::max<size_t>(longest, t.page1 - t.page0);
+  double best_time = 0;
+  for (size_t cut = 1; cut <= 64; cut++) {
+    const size_t each = std::max<size_t>(4, ceil_div(longest, cut));
+    if (cut > 1 && each < least) break;
+    size_t items = 0, parts = 0;
+    for (const Tile& t : tiles) {
+      const size_t n = ceil_div(t.page1 - t.page0, each);
+      items += n;
+      parts += n > 1 ? n : 0;
+    }
+    if (parts > 2 * KV_MANY_GROUPS) break;
+    const double mean = (double)(total + 4 * parts) / (double)items;
+    const double time = std::max((double)each, (double)ceil_div(items, KV_MANY_GROUPS) * mean) + (parts ? 4 : 0);
+    if (cut == 1 || time < best_time) {
+      best = each;
+      best_time = time;
+    }
+    if (each == 4) break;
+  }
+  return best;
+}
+
+// Work-group i runs on accelerator die i % 8, each of which has its own L2: the
+// items of one sequence and head, which read the same pages, go to one die (or
+// as few as keep all eight busy), the longest first.
+void spread(std::vector<KvItem>* items) {
+  constexpr size_t DIES = 8;
+  if (items->size() < 2 * DIES) return;
+  size_t streams = 0;
+  std::vector<std::vector<KvItem>> die(DIES);
+  std::vector<size_t> first;  // items of a stream lie one behind the other
+  for (size_t i = 0; i < items->size(); i++)
+    if (i == 0 || (*items)[i].tok0 != (*items)[i - 1].tok0 || (*items)[i].head != (*items)[i - 1].head) {
+      streams++;
+      first.push_back(i);
+    }
+  first.push_back(items->size());
+  const size_t share = streams < DIES ? DIES / streams : 1;  // dies per stream
+  for (size_t s = 0; s < streams; s++)
+    for (size_t i = first[s]; i < first[s + 1]; i++) die[(s * share + (i - first[s]) % share) % DIES].push_back((*items)[i]);
+  for (auto& d : die)
+    std::stable_sort(d.begin(), d.end(), [](const KvItem& a, const KvItem& b) { return a.page1 - a.page0 > b.page1 - b.page0; });
+  size_t n = 0;
+  for (size_t k = 0; n < items->size(); k++)
+    for (auto& d : die)
+      if (k < d.size()) (*items)[n++] = d[k];
+}
+
+}  // namespace
+
+void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window, KvPlan* out) {
+  out->few.clear();
+  out->many.clear();
+  out->few_joins.clear();
+  out->many_joins.clear();
+  out->part_rows = 0;
+  const size_t group = s.group(), few_rows = kv_few_rows(s.head_dim), many_rows = kv_many_rows(s.head_dim);
+  size_t most = 0;
+  for (const KvStepSeq& q : seqs)
+    if (q.ntok * group <= few_rows) most = std::max(most, q.ntok * group);
+  out->cols = most <= 16 ? 1 : 2;
+  std::vector<Tile> few, many;
+  for (const KvStepSeq& q : seqs) {
+    const bool is_few = q.ntok * group <= few_rows;
+    const size_t rows = is_few ? few_rows : many_rows;
+    for (uint32_t h = 0; h < s.kv_heads; h++)
+      // the rows with the most pages first, so that the last work-groups are short
+      for (size_t t = ceil_div(q.ntok * group, rows); t-- > 0;) {
+        const size_t r = t * rows, n = std::min(rows, q.ntok * group - r);
+        const size_t low = q.len0 + r / group, high = q.len0 + (r + n - 1) / group;
+        const size_t page0 = window && low + 1 > window ? (low + 1 - window) / KV_PAGE : 0;
+        (is_few ? few : many).push_back({&q, h, (uint32_t)r, (uint32_t)n, (uint32_t)page0, (uint32_t)(high / KV_PAGE + 1)});
+      }
+  }
+  // few rows: a work-group's waves take a page each, fewer than four leave some idle
+  divide(few, std::max<size_t>(4, ceil_div(count_pages(few), KV_FEW_GROUPS)), 16 * (size_t)out->cols, &out->few, &out->few_joins,
+         &out->part_rows);
+  if (!many.empty()) divide(many, many_each(many), many_rows, &out->many, &out->many_joins, &out->part_rows);
+  spread(&out->many);
 }
 
 void kv_blocks(const std::vector<KvStepSeq>& seqs, size_t max_pages, std::vector<KvBlock>* out) {

@@ -42,25 +42,27 @@ struct KvItem {
   uint16_t head, rows;
   uint32_t row0;
   uint32_t page0, page1;
-  uint32_t part;  // its slot among the partial results, or KV_WHOLE
+  uint32_t part;  // the first of its rows among the partial results, or KV_WHOLE
 };
 constexpr uint32_t KV_WHOLE = 0xffffffffu;
 
-// Partial results part0 .. part0 + parts - 1 to be joined, the rows of one item.
+// Partial results of `rows` rows to be joined: `parts` of them, part0, part0 +
+// step, .. their first rows.
 struct KvJoin {
   uint32_t tok0;
   uint16_t head, rows;
   uint32_t row0;
-  uint32_t part0, parts;
-  uint32_t pad[3];
+  uint32_t part0, parts, step;
+  uint32_t pad[2];
 };
 
-// The attention of a step under one window.
+// The attention of a step under one window: sequences of few rows (the waves of
+// a work-group share their pages) and of many (the waves share their rows).
 struct KvPlan {
-  int cols = 1;  // groups of 16 rows per work-group: 1 or 2
-  std::vector<KvItem> items;
-  std::vector<KvJoin> joins;
-  uint32_t parts = 0;
+  int cols = 1;  // few: groups of 16 rows per work-group, 1 or 2
+  std::vector<KvItem> few, many;
+  std::vector<KvJoin> few_joins, many_joins;
+  uint32_t part_rows = 0;
 };
 
 struct KvCopy {
@@ -73,22 +75,27 @@ struct KvShape {
 };
 
 // Work-groups that a step's attention is divided into where its length allows,
-// and with it the most partial results (see kv_plan).
-constexpr size_t KV_TARGET_GROUPS = 512;
-constexpr size_t KV_MAX_PARTS = 2 * KV_TARGET_GROUPS;
+// for few and for many rows apart.  A tile of pages that is divided has more
+// than total / groups of them, so there are at most twice as many parts.
+constexpr size_t KV_FEW_GROUPS = 512, KV_MANY_GROUPS = 512;
+constexpr size_t KV_MAX_PARTS = 2 * (KV_FEW_GROUPS + KV_MANY_GROUPS);
 
-// Most groups of 16 rows that the attention kernels hold at once.
-inline int kv_max_cols(size_t head_dim) { return head_dim <= 128 ? 2 : 1; }
+// Rows per work-group for sequences of few rows, at most, and of many.
+inline size_t kv_few_rows(size_t head_dim) { return head_dim <= 128 ? 32 : 16; }
+inline size_t kv_many_rows(size_t head_dim) { return head_dim <= 128 ? 128 : 64; }
+inline size_t kv_part_rows(size_t head_dim) {
+  return 2 * KV_FEW_GROUPS * kv_few_rows(head_dim) + 2 * KV_MANY_GROUPS * kv_many_rows(head_dim);
+}
 
-// Divides the attention of a step: rows of 16 * cols per work-group, few
-// enough pages each that all compute units take part.  Window 0 sees every
-// earlier position.
+// Divides the attention of a step: tiles of rows, and few enough pages each
+// that all compute units take part.  Window 0 sees every earlier position.
 void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window, KvPlan* out);
 
 // The blocks that a step's tokens touch.
 void kv_blocks(const std::vector<KvStepSeq>& seqs, size_t max_pages, std::vector<KvBlock>* out);
 
-// Most items and blocks that a plan of so many tokens and sequences can have.
+// Most items (of both kinds together) and blocks that a plan of so many tokens and
+// sequences can have.
 size_t kv_max_items(const KvShape& s, size_t tokens, size_t nseq);
 inline size_t kv_max_blocks(size_t tokens, size_t nseq) { return tokens / KV_BLOCK + 2 * nseq; }
 

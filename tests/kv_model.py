@@ -148,9 +148,11 @@ def attention_bound(dtype, mag, prod, total, vtop, dim):
     Small probabilities: a probability, times 2^15 over the row's largest and
     times its block's scale over a power of two of at most twice the largest, is held
     in f16, whose step ends at 2^-24: off by 2^-25 more, times a code of up to 127.  Over
-    the sum (at least 2^15) that is 2^-39 vtop for each key."""
+    the sum (at least 2^15) that is 2^-39 vtop for each key.  For f16 and bf16 the
+    probabilities of many rows are relative to a reference that may lie 2^8 below the
+    largest score's: the sum is at least 2^7, and it is 2^-31 vtop."""
     s = prod * (3 * dim + 8) * 2.0 ** -24
     p = np.expm1(s) + 2.0 ** -22 + (2.0 ** -23 if dtype == "f32" else 2.0 ** -11) + 3 * 2.0 ** -24
     rel = 2 * p + (total + 64) * 2.0 ** -24
-    floor = total * 2.0 ** -39 * vtop[..., None] + (2.0 ** -25 if dtype == "f16" else 0.0)
+    floor = total * 2.0 ** (-39 if dtype == "f32" else -31) * vtop[..., None] + (2.0 ** -25 if dtype == "f16" else 0.0)
     return mag * rel[..., None] * 1.01 + EPS[dtype] * mag + floor

@@ -203,10 +203,10 @@ void plans() {
     const size_t window = below(2) ? 0 : 1 + below(below(2) ? 100 : 5000);
     KvPlan plan;
     kv_plan(s, seqs, window, &plan);
-    CHECK(plan.cols >= 1 && plan.cols <= kv_max_cols(s.head_dim));
-    CHECK(plan.parts <= KV_MAX_PARTS);
-    CHECK(plan.items.size() <= kv_max_items(s, tok, seqs.size()));
-    CHECK(plan.joins.size() + KV_MAX_PARTS <= kv_max_items(s, tok, seqs.size()));
+    CHECK(plan.cols >= 1 && 16 * (size_t)plan.cols <= kv_few_rows(s.head_dim));
+    CHECK(plan.few.size() + plan.many.size() <= kv_max_items(s, tok, seqs.size()));
+    CHECK(plan.few_joins.size() + plan.many_joins.size() + KV_MAX_PARTS <= kv_max_items(s, tok, seqs.size()));
+    CHECK(plan.part_rows <= kv_part_rows(s.head_dim));
     // every new token is in one block, at its position, and no other is
     std::vector<KvBlock> blocks;
     const size_t max_pages = 4096;
@@ -226,19 +226,28 @@ void plans() {
     }
     for (int n : seen) CHECK(n == 1);
     std::map<std::pair<std::pair<uint32_t, uint32_t>, uint32_t>, std::vector<const KvItem*>> tiles;
-    for (const KvItem& it : plan.items) {
-      CHECK(it.row < seqs.size() && it.len0 == seqs[it.row].len0 && it.tok0 == seqs[it.row].tok0 && it.head < s.kv_heads && it.rows >= 1 && it.rows <= 16u * plan.cols);
-      CHECK(it.row0 % (16 * plan.cols) == 0 && it.row0 + it.rows <= seqs[it.row].ntok * s.group());
-      CHECK(it.page0 < it.page1);
-      tiles[{{it.row, it.head}, it.row0}].push_back(&it);
-    }
+    for (int kind = 0; kind < 2; kind++)
+      for (const KvItem& it : kind ? plan.many : plan.few) {
+        CHECK(it.row < seqs.size() && it.len0 == seqs[it.row].len0 && it.tok0 == seqs[it.row].tok0);
+        const size_t all = seqs[it.row].ntok * s.group(), tile = kind ? kv_many_rows(s.head_dim) : 16 * (size_t)plan.cols;
+        CHECK((all > kv_few_rows(s.head_dim)) == (kind == 1));
+        CHECK(it.head < s.kv_heads && it.rows >= 1 && it.rows <= tile);
+        CHECK(it.row0 % tile == 0 && it.row0 + it.rows <= all && (it.rows == tile || it.row0 + it.rows == all));
+        CHECK(it.page0 < it.page1);
+        tiles[{{it.row, it.head}, it.row0}].push_back(&it);
+      }
     size_t want = 0;
-    for (auto& q : seqs) want += (q.ntok * s.group() + 16 * plan.cols - 1) / (16 * plan.cols) * s.kv_heads;
+    for (auto& q : seqs) {
+      const size_t all = q.ntok * s.group(), tile = all > kv_few_rows(s.head_dim) ? kv_many_rows(s.head_dim) : kv_few_rows(s.head_dim);
+      want += (all + tile - 1) / tile * s.kv_heads;
+    }
     CHECK(tiles.size() == want);
-    std::set<uint32_t> parts;
+    std::vector<char> taken(plan.part_rows, 0);  // rows of partial results, each written by one item
     std::map<uint32_t, const KvJoin*> joins;
-    for (const KvJoin& j : plan.joins) {
-      CHECK(j.parts > 1);
+    for (int kind = 0; kind < 2; kind++)
+    for (const KvJoin& j : kind ? plan.many_joins : plan.few_joins) {
+      CHECK(j.step == (kind ? kv_many_rows(s.head_dim) : 16 * (size_t)plan.cols));
+      CHECK(j.parts > 1 && j.parts <= 2 * KV_FEW_GROUPS && j.parts <= 2 * KV_MANY_GROUPS && j.rows <= j.step);
       joins[j.part0] = &j;
     }
     size_t divided = 0;
@@ -249,21 +258,22 @@ void plans() {
       const size_t low = q.len0 + v[0]->row0 / s.group(), high = q.len0 + (v[0]->row0 + v[0]->rows - 1) / s.group();
       CHECK(v.back()->page1 == high / KV_PAGE + 1);
       CHECK(v[0]->page0 == (window && low + 1 > window ? (low + 1 - window) / KV_PAGE : 0));
-      for (size_t i = 0; i < v.size(); i++) {
-        if (i) CHECK(v[i]->page0 == v[i - 1]->page1);
-        if (v.size() == 1) {
-          CHECK(v[i]->part == KV_WHOLE);
-        } else {
-          CHECK(v[i]->part < plan.parts && parts.insert(v[i]->part).second && v[i]->part == v[0]->part + i);
-        }
-      }
-      if (v.size() > 1) {
+      const KvJoin* j = v.size() > 1 ? joins.at(v[0]->part) : nullptr;
+      if (j) {
         divided++;
-        const KvJoin* j = joins.at(v[0]->part);
         CHECK(j->parts == v.size() && j->tok0 == v[0]->tok0 && j->head == v[0]->head && j->row0 == v[0]->row0 && j->rows == v[0]->rows);
       }
+      for (size_t i = 0; i < v.size(); i++) {
+        if (i) CHECK(v[i]->page0 == v[i - 1]->page1);
+        if (!j) {
+          CHECK(v[i]->part == KV_WHOLE);
+          continue;
+        }
+        CHECK(v[i]->part == j->part0 + i * j->step && v[i]->part + v[i]->rows <= plan.part_rows);
+        for (uint32_t r = 0; r < v[i]->rows; r++) CHECK(!taken[v[i]->part + r]++);
+      }
     }
-    CHECK(divided == plan.joins.size() && parts.size() == plan.parts);
+    CHECK(divided == plan.few_joins.size() + plan.many_joins.size());
   }
 }
 
