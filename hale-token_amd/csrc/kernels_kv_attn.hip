@@ -426,10 +426,9 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_kv_attend_few(KvAttnArgs a) 
 // positions and 16 rows at head dimension 128 the matrix instructions take 512
 // cycles and the softmax about 500, so two work-groups on a compute unit, whose
 // waves are in different phases, keep both busy (f32 at dimensions 96 and 128 needs the
-// registers of both for one, dimension 256 the LDS).  For f16 and bf16 the softmax is
-// kept short: the values' scale goes into the exponent (and out of the sum by one
-// product per 16 positions), and the reference m follows the maximum only where this is
-// more than 2^8 above it (probabilities are then up to 2^15 from 2^7).
+// registers of both for one, dimension 256 the LDS).  For f16 and bf16 the reference m
+// follows the maximum only where this is more than 2^8 above it (probabilities are then
+// up to 2^15 from 2^7), so that the sums are seldom rescaled.
 constexpr int many_waves(size_t size, int kc) { return (size == 4 ? kc == 2 || kc == 6 : kc <= 6) ? 2 : 1; }
 
 template <typename T, int KC, int C>
@@ -528,55 +527,64 @@ __global__ __launch_bounds__(256, many_waves(sizeof(T), KC)) void k_kv_attend_ma
       if (more) fetch(pages.place(places, turn));
       const int pos0 = (int)(p * KV_PAGE);
       if (present && pos0 <= end && pos0 + (int)KV_PAGE > begin) {
-        // operands are read from LDS one group ahead of their products
+        // operands are read from LDS one group ahead of their products, and products
+        // of one sum are several others apart
         f32x4 s[C][4];
-        f16x8 kf[2][KC], vf[2][2];
-#pragma unroll
-        for (int kk = 0; kk < KC; kk++) kf[0][kk] = buf[kk * 64 + lane];
+        f16x8 kf[2][4], vf[2][2][2];
 #pragma unroll
         for (int mm = 0; mm < 4; mm++) {
-          if (mm < 3) {
+          kf[0][mm] = buf[mm * KC * 64 + lane];
 #pragma unroll
-            for (int kk = 0; kk < KC; kk++) kf[(mm + 1) & 1][kk] = buf[((mm + 1) * KC + kk) * 64 + lane];
-          } else {
-            vf[0][0] = buf[KC * 4 * 64 + lane];
-            vf[0][1] = buf[(KC * 4 + 1) * 64 + lane];
+          for (int c = 0; c < C; c++) s[c][mm] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int kk = 0; kk < KC; kk++) {
+          if (kk + 1 < KC) {
+#pragma unroll
+            for (int mm = 0; mm < 4; mm++) kf[(kk + 1) & 1][mm] = buf[(mm * KC + kk + 1) * 64 + lane];
           }
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int c = 0; c < C; c++) s[c][mm] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          for (int h = 0; h < P; h++)
 #pragma unroll
-          for (int kk = 0; kk < KC; kk++)
+            for (int mm = 0; mm < 4; mm++)
 #pragma unroll
-            for (int c = 0; c < C; c++)
-#pragma unroll
-              for (int h = 0; h < P; h++) s[c][mm] = mfma(kf[mm & 1][kk], q[c][h][kk], s[c][mm]);
+              for (int c = 0; c < C; c++) s[c][mm] = mfma(kf[kk & 1][mm], q[c][h][kk], s[c][mm]);
           __builtin_amdgcn_sched_barrier(0);
         }
-        const bool edge = pos0 + (int)KV_PAGE - 1 > last || pos0 < first;
-        float lg[4];  // log2 of the values' scales; a block of zeros as one of scale 2^-126
+        __builtin_amdgcn_s_setprio(0);
+        auto read_v = [&](int pair) {  // groups 2 pair and 2 pair + 1 of the dimension
 #pragma unroll
-        for (int mm = 0; mm < 4; mm++) lg[mm] = vs_now[mm] > 0x1p-126f ? __builtin_amdgcn_logf(vs_now[mm]) : -126.0f;
+          for (int x = 0; x < 4; x++) vf[pair & 1][x / 2][x % 2] = buf[(KC * 4 + 4 * pair + x) * 64 + lane];
+        };
+        read_v(0);
+        const bool edge = pos0 + (int)KV_PAGE - 1 > last || pos0 < first;
+        const float vall = fmaxf(fmaxf(vs_now[0], vs_now[1]), fmaxf(vs_now[2], vs_now[3]));
         f16x8 pf[C][P][2];
 #pragma unroll
         for (int c = 0; c < C; c++) {
-          f32x4 vr = vs_now;
-          float f[4], top = -__builtin_inff();
+          f32x4 vr = vs_now, f = ks_now * rs[c];
+          float vtop = vall;
+          if (edge) {
 #pragma unroll
-          for (int mm = 0; mm < 4; mm++) {
-            f[mm] = fmaxf(rs[c] * ks_now[mm], 0x1p-120f);  // not 0: hidden scores stay -inf
-            if (edge) {
+            for (int mm = 0; mm < 4; mm++) {
+              // blocks that the row sees nothing of may hold anything
               vr[mm] = pos0 + 16 * mm <= hi[c] && pos0 + 16 * mm + 15 > lo[c] ? vr[mm] : 0.0f;
+              f[mm] = fmaxf(f[mm], 0x1p-120f);  // not 0: hidden scores stay -inf
 #pragma unroll
               for (int r = 0; r < 4; r++) {
                 const int t = pos0 + 16 * mm + 4 * g + r;
                 s[c][mm][r] = t <= hi[c] && t > lo[c] ? s[c][mm][r] : -__builtin_inff();
               }
             }
-            top = fmaxf(top, f[mm] * fmaxf(fmaxf(s[c][mm][0], s[c][mm][1]), fmaxf(s[c][mm][2], s[c][mm][3])));
+            vtop = fmaxf(fmaxf(vr[0], vr[1]), fmaxf(vr[2], vr[3]));
           }
+          float top = -__builtin_inff();
+#pragma unroll
+          for (int mm = 0; mm < 4; mm++)
+            top = fmaxf(top, f[mm] * fmaxf(fmaxf(s[c][mm][0], s[c][mm][1]), fmaxf(s[c][mm][2], s[c][mm][3])));
           top = row_max(top);
-          const float vtop = fmaxf(fmaxf(vr[0], vr[1]), fmaxf(vr[2], vr[3]));
           const int k_now = (int)(__float_as_uint(vtop) >> 23) - 126, k_new = k_now > vk[c] ? k_now : vk[c];
           const float mnew = top > m[c] + (float)SLACK ? top : m[c];
           const float ref = mnew == -__builtin_inff() ? 0.0f : mnew;
@@ -584,55 +592,46 @@ __global__ __launch_bounds__(256, many_waves(sizeof(T), KC)) void k_kv_attend_ma
           m[c] = mnew;
           vk[c] = k_new;
           l[c] *= alpha;
+          vr = vr * pow2(SHIFT - k_new);
+          float sum = 0.0f;
 #pragma unroll
-          for (int mm = 0; mm < 4; mm++) {
-            float sum = 0.0f;
-            if constexpr (P == 1) {
-              // the scale over the largest, times 2^SHIFT; one 2^60 below the largest counts
-              // as that: nothing against the rest
-              const float lv = fmaxf(lg[mm] - (float)(k_new - SHIFT), (float)(SHIFT - 60)), at = lv - ref;
+          for (int mm = 0; mm < 4; mm++)
 #pragma unroll
-              for (int r = 0; r < 4; r++) {
-                const float w = exp2_fast(__builtin_fmaf(s[c][mm][r], f[mm], at));
-                sum += w;
-                pf[c][0][mm / 2][(mm & 1) * 4 + r] = (_Float16)w;
-              }
-              l[c] = __builtin_fmaf(sum, exp2_fast(-lv), l[c]);
-            } else {
-              const float v = vr[mm] * pow2(SHIFT - k_new);
-#pragma unroll
-              for (int r = 0; r < 4; r++) {
-                const float e = exp2_fast(__builtin_fmaf(s[c][mm][r], f[mm], -ref)), w = rounded(e * v);
+            for (int r = 0; r < 4; r++) {
+              const float e = exp2_fast(__builtin_fmaf(s[c][mm][r], f[mm], -ref));
+              sum += e;
+              if constexpr (P == 1) {
+                pf[c][0][mm / 2][(mm & 1) * 4 + r] = (_Float16)(e * vr[mm]);
+              } else {
+                const float w = rounded(e * vr[mm]);
                 const _Float16 h = (_Float16)w;
-                sum += e;
                 pf[c][0][mm / 2][(mm & 1) * 4 + r] = h;
                 pf[c][P - 1][mm / 2][(mm & 1) * 4 + r] = (_Float16)(w - (float)h);
               }
-              l[c] += sum;
             }
-          }
+          l[c] += sum;
           if (__builtin_amdgcn_ballot_w64(scale != 1.0f)) {
 #pragma unroll
             for (int n = 0; n < ND; n++) o[c][n] = o[c][n] * scale;
           }
         }
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int n = 0; n < ND; n++) {
-          if (n + 1 < ND) {
-            vf[(n + 1) & 1][0] = buf[(KC * 4 + 2 * n + 2) * 64 + lane];
-            vf[(n + 1) & 1][1] = buf[(KC * 4 + 2 * n + 3) * 64 + lane];
-          }
+        for (int pair = 0; pair < ND / 2; pair++) {
+          if (pair + 1 < ND / 2) read_v(pair + 1);
           __builtin_amdgcn_sched_barrier(0);
-          if (n < NDMIN || n < nd) {
+          // (a last group that the head dimension has not takes what lies in its place, and is not stored)
+#pragma unroll
+          for (int h = 0; h < P; h++)
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
-              for (int c = 0; c < C; c++)
+              for (int x = 0; x < 2; x++)
 #pragma unroll
-                for (int h = 0; h < P; h++) o[c][n] = mfma(vf[n & 1][j], pf[c][h][j], o[c][n]);
-          }
+                for (int c = 0; c < C; c++) o[c][2 * pair + x] = mfma(vf[pair & 1][x][j], pf[c][h][j], o[c][2 * pair + x]);
           __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
       }
       if (more) convert(other);
       __syncthreads();

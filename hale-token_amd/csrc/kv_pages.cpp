@@ -317,8 +317,11 @@ void spread(std::vector<KvItem>* items) {
   const size_t share = streams < DIES ? DIES / streams : 1;  // dies per stream
   for (size_t s = 0; s < streams; s++)
     for (size_t i = first[s]; i < first[s + 1]; i++) die[(s * share + (i - first[s]) % share) % DIES].push_back((*items)[i]);
-  for (auto& d : die)
+  for (auto& d : die) {
     std::stable_sort(d.begin(), d.end(), [](const KvItem& a, const KvItem& b) { return a.page1 - a.page0 > b.page1 - b.page0; });
+    // all of them running at once, two to a compute unit: a long one beside a short one
+    if (d.size() <= KV_MANY_GROUPS / DIES) std::reverse(d.begin() + (d.size() + 1) / 2, d.end());
+  }
   size_t n = 0;
   for (size_t k = 0; n < items->size(); k++)
     for (auto& d : die)
