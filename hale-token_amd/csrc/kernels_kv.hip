@@ -103,12 +103,16 @@ __global__ __launch_bounds__(256) void k_rope(RopeArgs a) {
   }
 }
 
+constexpr size_t ROPE_VEC_PAIRS = 65536;
+
 template <typename T>
 static hipError_t rope_typed(const RopeArgs& a, hipStream_t st) {
   size_t bits = 0;
   for (int i = 0; i < 2; i++)
     if (a.heads[i]) bits |= (uintptr_t)a.src[i] | (uintptr_t)a.dst[i] | (a.src_stride[i] | a.dst_stride[i]) * sizeof(T);
-  if (bits % 16 == 0 && a.hd % 8 == 0 && a.half % 8 == 0) {
+  // few rows are a matter of latency, where a thread per pair is the shorter way
+  const size_t pairs = a.rows * (size_t)(a.heads[0] + a.heads[1]) * a.half;
+  if (pairs >= ROPE_VEC_PAIRS && bits % 16 == 0 && a.hd % 8 == 0 && a.half % 8 == 0) {
     const int units = (a.heads[0] + a.heads[1]) * (a.half / 8 + (a.hd - 2 * a.half) / 8);
     // few rows: their heads spread over more work-groups
     const unsigned split = a.rows >= 512 ? 1 : (unsigned)(units + 255) / 256;
@@ -138,6 +142,8 @@ hipError_t launch_rope(int dtype, const RopeArgs& a, hipStream_t st) {
 // microsecond away, once.
 __global__ __launch_bounds__(256) void k_kv_upload(KvUploadArgs a, unsigned n4) {
   const unsigned id = blockIdx.x * 256 + threadIdx.x;
+  // that this kernel runs says that the one before it has ended
+  if (id == 0) __hip_atomic_store(a.done, a.number, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
   if (id < n4) {
     const u32x4 x = ((const u32x4*)a.src)[id];
     unsigned at = id;
@@ -234,9 +240,10 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
   const bool values = blockIdx.z;
   const size_t stride = values ? a.v_stride : a.k_stride;
   const T* base = (const T*)(values ? a.v : a.k) + (size_t)blockIdx.y * hd;
+  const KvBlock first = a.blocks[blockIdx.x];  // read beside the count: the plan has room for the whole grid
   const unsigned nblocks = a.count ? *a.count : a.nblocks;
   for (unsigned b = blockIdx.x; b < nblocks; b += gridDim.x) {
-    const KvBlock blk = a.blocks[b];
+    const KvBlock blk = b == blockIdx.x ? first : a.blocks[b];
     const int old = blk.old, end = blk.end;
     const uint32_t page = a.g.table[blk.entry];
     const T* src = base + (long long)blk.tok * (long long)stride;

@@ -207,9 +207,10 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_kv_attend_few(KvAttnArgs a) 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, g = lane >> 4;
   const int nd = a.g.hd / 16;
+  KvItem item = a.items[blockIdx.x];  // read beside the count: the plan has room for the whole grid
   const unsigned nitems = a.nitems != 0xffffffffu ? a.nitems : a.counts[a.kind];
   for (unsigned it = blockIdx.x; it < nitems; it += gridDim.x) {
-    const KvItem item = a.items[it];
+    if (it != blockIdx.x) item = a.items[it];
     const uint32_t* table = a.g.table + (size_t)item.row * a.g.max_pages;
     const uint8_t* pool = a.g.pool + a.layer * a.g.layer_bytes + (size_t)item.head * a.g.head_bytes;
 

@@ -70,6 +70,8 @@ struct KvUploadArgs {
   const uint32_t* pairs;
   unsigned npairs;
   uint32_t* table;
+  uint32_t* done;   // host memory: receives `number`, the last upload before this one
+  uint32_t number;
 };
 hipError_t launch_kv_upload(const KvUploadArgs& a, hipStream_t st);
 

@@ -162,15 +162,16 @@ extern "C" int hale_rope_device(hale_rope* r, int dtype, size_t rows, const int3
 
 namespace {
 
-// Pinned host memory that the device reads plans from.  Each upload takes the
-// next of a few buffers and waits for the kernel that read it last.
+// Pinned host memory that the device reads plans from: a ring of buffers, one
+// per upload.  Upload n, when it runs, reports that upload n - 1 has been read,
+// so a buffer's next use waits (for the stream) only where the host is a whole
+// ring ahead.
 struct Staging {
   char* base = nullptr;
   size_t bytes = 0;
-  hipEvent_t read = nullptr;  // recorded behind the kernel that reads it
-  bool pending = false;
+  uint32_t number = 0;  // the upload that read it last
 };
-constexpr int STAGINGS = 4;
+constexpr int STAGINGS = 32;
 
 struct View {  // the plan of the current step under one window
   size_t window = 0;
@@ -204,7 +205,8 @@ struct hale_kv_cache {
   float* part_o = nullptr;
   float2* part_ml = nullptr;
   Staging staging[STAGINGS];
-  int turn = 0;
+  uint32_t uploads = 0;       // so far
+  uint32_t* done = nullptr;   // pinned: the last upload known to have been read
   // the current step
   bool stepped = false;
   size_t tokens = 0, blocks = 0;
@@ -231,11 +233,10 @@ struct Upload {
 
   int begin(size_t bytes) {
     hale_ctx* c = kv->ctx;
-    s = &kv->staging[kv->turn];
-    kv->turn = (kv->turn + 1) % STAGINGS;
-    if (s->pending) KVCHK(c, hipEventSynchronize(s->read));
-    s->pending = false;
-    if (!s->read) KVCHK(c, hipEventCreateWithFlags(&s->read, hipEventDisableTiming));
+    s = &kv->staging[kv->uploads % STAGINGS];
+    if (s->number && (int32_t)(__atomic_load_n(kv->done, __ATOMIC_ACQUIRE) - s->number) < 0)
+      KVCHK(c, hipStreamSynchronize(c->stream));
+    s->number = 0;
     if (s->bytes < bytes) {
       if (s->base) (void)hipHostFree(s->base);
       s->base = nullptr;
@@ -277,9 +278,10 @@ struct Upload {
       pairs[2 * i + 1] = kv->pages.entry(dirty[i]);
     }
     a.src = (const uint32_t*)s->base;
+    a.done = kv->done;
+    a.number = kv->uploads++;  // from the first one's 0 on: numbers count from 1
     KV_LAUNCH(c, K_KV_PAGES, launch_kv_upload(a, c->stream));
-    KVCHK(c, hipEventRecord(s->read, c->stream));
-    s->pending = true;
+    s->number = kv->uploads;
     dirty.clear();
     return HALE_OK;
   }
@@ -312,8 +314,8 @@ static void free_device(hale_kv_cache* kv) {
     (void)hipFree(p);
   for (Staging& s : kv->staging) {
     if (s.base) (void)hipHostFree(s.base);
-    if (s.read) (void)hipEventDestroy(s.read);
   }
+  if (kv->done) (void)hipHostFree(kv->done);
 }
 
 static Sections sections(const hale_kv_cache* kv, size_t tokens) {
@@ -423,6 +425,11 @@ extern "C" int hale_kv_create(hale_ctx* c, size_t layers, size_t heads, size_t k
               hipMalloc(&kv->part_o, part_rows * hd * 4) != hipSuccess ||
               hipMalloc(&kv->part_ml, part_rows * sizeof(float2)) != hipSuccess))
     rc = ctx_fail(c, HALE_ENOMEM, "kv_create: page table and workspace");
+  if (!rc && hipHostMalloc(&kv->done, 64, hipHostMallocDefault) != hipSuccess) {
+    kv->done = nullptr;
+    rc = ctx_fail(c, HALE_ENOMEM, "kv_create: pinned memory");
+  }
+  if (!rc) *kv->done = 0;
   if (!rc && (hipMemsetAsync(kv->table, 0, row * max_seqs * 4, c->stream) != hipSuccess ||
               hipStreamSynchronize(c->stream) != hipSuccess))
     rc = ctx_fail(c, HALE_EHIP, "kv_create: clearing the page table");
@@ -826,7 +833,7 @@ extern "C" int hale_kv_attention_device(hale_kv_cache* kv, size_t layer, int dty
   // captured: later steps of these tokens may have more items, which the
   // work-groups then take in turn, and joins of the same rows
   auto grid = [&](size_t now, size_t most) {
-    return (unsigned)std::min<size_t>(cap && now ? std::max(now, std::min<size_t>(most, 1024)) : now, 1u << 20);
+    return (unsigned)std::min<size_t>(cap && now ? std::max(now, std::min<size_t>(most, KV_FEW_GROUPS)) : now, 1u << 20);
   };
   const size_t tiles = kv_max_items(kv->shape, ntok, kv->seqs.size()) - KV_MAX_PARTS;
   bool few = false, many = false;
