@@ -208,19 +208,35 @@ hipError_t launch_kv_copy_pages(uint8_t* pool, size_t page_bytes, const KvCopy* 
 // rounding of held codes where the scale grew, about 20 dependent instructions
 // each): four waves share a block, 8 codes a thread at head dimension 128.
 
-// The whole number nearest to (p + e) / s, ties to even, where |p / s| < 200, e is
-// the rest of a product rounded to p (or 0), and inv is within 2^-21 of 1 / s
-// relative.  p inv is off by less than 2^-13, so its nearest whole number c is
-// the quotient's or the one beside it; p - c s, of at most half of s and a little,
-// is a multiple of the smaller of both ulps and so exact, as is 2 |p - c s| - s
-// where it is near 0; the sign of that with e decides.
-__device__ __forceinline__ unsigned nearest_code(float p, float e, float s, float inv) {
-  float c = rintf(p * inv);
-  const float r = __builtin_fmaf(-c, s, p);
-  const float over = (2.0f * fabsf(r) - s) + 2.0f * (r < 0.0f ? -e : e);
-  const bool odd = ((int)c & 1) != 0;
-  c += over > 0.0f || (over == 0.0f && odd) ? (r > 0.0f ? 1.0f : -1.0f) : 0.0f;
-  return (unsigned)((int)fminf(fmaxf(c, -127.0f), 127.0f) + 128);
+// The whole numbers nearest to (p + e) / s, ties to even, as four codes of a word,
+// where |p / s| < 200, e is the rest of a product rounded to p (or 0), and inv is
+// within 2^-21 of 1 / s relative.  p inv is off by less than 2^-13: where it is
+// farther than that from a half, its nearest whole number c is the quotient's.  Else
+// (one number in 2500) c or the one beside it is: p - c s, of at most half of s and a
+// little, is a multiple of the smaller of both ulps and so exact, as is 2 |p - c s|
+// - s where it is near 0; the sign of that with e decides.
+__device__ __forceinline__ unsigned nearest_codes(const float (&p)[4], const float (&e)[4], float s, float inv) {
+  float c[4];
+  unsigned far = 0;  // magnitudes are ordered as their bits are
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const float t = p[k] * inv;
+    c[k] = rintf(t);
+    far = max(far, __float_as_uint(fabsf(t - c[k])));
+  }
+  if (__builtin_amdgcn_ballot_w64(far > __float_as_uint(0.4998f))) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const float r = __builtin_fmaf(-c[k], s, p[k]);
+      const float over = (2.0f * fabsf(r) - s) + 2.0f * (r < 0.0f ? -e[k] : e[k]);
+      const bool odd = ((int)c[k] & 1) != 0;
+      c[k] += over > 0.0f || (over == 0.0f && odd) ? (r > 0.0f ? 1.0f : -1.0f) : 0.0f;
+    }
+  }
+  unsigned w = 0;
+#pragma unroll
+  for (int k = 0; k < 4; k++) w = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_amdgcn_fmed3f(c[k], -127.0f, 127.0f) + 128.0f, k, w);
+  return w;
 }
 
 // A lane's number n of the keys, n a multiple of 8: which of the dimension
@@ -232,18 +248,27 @@ __device__ __forceinline__ unsigned key_at(int kc, int n, int block, int lane) {
   return n / 16 < kc / 2 ? ((n / 16 * 4 + block) * 64 + lane) * 16 + n % 16 : kc / 2 * 4096 + (block * 64 + lane) * 8;
 }
 
-template <typename T>
+//
+// W: waves per block, 4 or 1.  Four where few blocks leave the chain to be shortened; one
+// where more blocks than the compute units hold work-groups would wait for each
+// other (a bf16 prompt of 4090 tokens, 8 heads of 128: 17.7 us with four, XX with one).
+template <typename T, int W>
 __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
-  extern __shared__ float x[];  // [16][hd + 4]
+  extern __shared__ float lds[];  // [4 / W][16][hd + 4]
   __shared__ float red[4];
-  const int tid = threadIdx.x, hd = a.g.hd, ldx = hd + 4;
+  constexpr int N = 64 * W;  // threads of a block
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), mine = wave / W;
+  const int tid = threadIdx.x % N, hd = a.g.hd, ldx = hd + 4;
+  float* x = lds + mine * (int)KV_BLOCK * ldx;
   const bool values = blockIdx.z;
   const size_t stride = values ? a.v_stride : a.k_stride;
   const T* base = (const T*)(values ? a.v : a.k) + (size_t)blockIdx.y * hd;
-  const KvBlock first = a.blocks[blockIdx.x];  // read beside the count: the plan has room for the whole grid
+  // read beside the count: the plan has room for the whole grid
+  const unsigned b0 = blockIdx.x * (4 / W) + mine;
+  KvBlock blk = a.blocks[b0];
   const unsigned nblocks = a.count ? *a.count : a.nblocks;
-  for (unsigned b = blockIdx.x; b < nblocks; b += gridDim.x) {
-    const KvBlock blk = b == blockIdx.x ? first : a.blocks[b];
+  for (unsigned b = b0; b < nblocks; b += gridDim.x * (4 / W)) {
+    if (b != b0) blk = a.blocks[b];
     const int old = blk.old, end = blk.end;
     const uint32_t page = a.g.table[blk.entry];
     const T* src = base + (long long)blk.tok * (long long)stride;
@@ -251,17 +276,20 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
     float* scale = (float*)(region + a.g.s_off) + (values ? 4 : 0) + blk.block;
     const float had = old ? *scale : 0.0f;
 
-    float top = 0.0f;
+    unsigned bits = 0;  // of the largest magnitude
     auto keep = [&](int t, int d, float v) {
-      v = __builtin_isfinite(v) ? v : 0.0f;  // what is not finite is stored as 0 and raises no scale
-      top = fmaxf(top, fabsf(v));
-      x[t * ldx + d] = v;
+      // what is not finite is stored as 0 and raises no scale
+      const unsigned u = __float_as_uint(v) & 0x7fffffffu, m = u < 0x7f800000u ? u : 0u;
+      bits = max(bits, m);
+      x[t * ldx + d] = u < 0x7f800000u ? v : 0.0f;
     };
     if (a.vec) {
       constexpr int PER = 16 / sizeof(T);
       const int row = hd / PER, n = (end - old) * row;  // 16-byte pieces
-      for (int e = tid; e < n; e += 256) {
-        const int t = old + e / row, d = e % row * PER;
+      const unsigned inv_row = (1u << 20) / row + 1;     // e / row exactly for e row < 2^20
+#pragma unroll 4
+      for (int e = tid; e < n; e += N) {
+        const int q = (int)(e * inv_row >> 20), t = old + q, d = (e - q * row) * PER;
         union {
           u32x4 u;
           T v[PER];
@@ -273,27 +301,70 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
     } else {
       const int n = (end - old) * hd;
 #pragma unroll 4
-      for (int e = tid; e < n; e += 256) {
+      for (int e = tid; e < n; e += N) {
         const int t = old + e / hd, d = e % hd;
         keep(t, d, to_f32(src[(size_t)t * stride + d]));
       }
     }
-    top = wave_max_f32(top);
-    if (tid % 64 == 0) red[tid / 64] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float top = __uint_as_float(wave_max_u32(bits));
+    if constexpr (W == 4) {
+      if (tid % 64 == 0) red[wave] = top;
+      __syncthreads();
+      top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // the wave's rows, before other lanes read them
+    }
     const float s = fmaxf(had, top / 127.0f);
     const bool grown = old && s > had;
     // the reciprocal of a very small scale overflows: both sides times 2^64, exactly
     const float up = s < 0x1p-64f ? 0x1p64f : 1.0f, su = s * up, hu = had * up;
     const float inv = s > 0.0f ? 1.0f / su : 0.0f;  // scale 0: all numbers are 0, and so are their quotients
-    auto code = [&](bool held, unsigned was, float v) {
-      const float c = (float)((int)was - 128), m = c * hu;
-      return nearest_code(held ? m : v * up, held ? __builtin_fmaf(c, hu, -m) : 0.0f, su, inv);
+    // four codes: of new numbers v, or where `held` says so of the codes `was`
+    auto codes = [&](const bool (&held)[4], unsigned was, const float (&v)[4]) {
+      float p[4], e[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        p[k] = v[k] * up;
+        e[k] = 0.0f;
+        if (old) {
+          const float c = (float)((int)(was >> (8 * k) & 255) - 128), m = c * hu;
+          e[k] = held[k] ? __builtin_fmaf(c, hu, -m) : 0.0f;
+          p[k] = held[k] ? m : p[k];
+        }
+      }
+      return nearest_codes(p, e, su, inv);
     };
-    if (!values) {
+    if (W == 1 && old == 0 && end == (int)KV_BLOCK) {
+      // a whole new block, as most of a prompt are: the same without conditions
+      const int lane = tid, i = lane % 16, g = lane / 16;
+      const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (!values) {
+        const int full = hd / 64 * 16;  // numbers of a lane whose 16 consecutive ones all exist
+#pragma unroll 2
+        for (int n = 0; n < full; n += 8) {
+          const float* v = x + i * ldx + key_dim(a.g.chunks, n, g);
+          const f32x4 v0 = *(const f32x4*)v * up, v1 = *(const f32x4*)(v + 4) * up;
+          *(u32x2*)(region + key_at(a.g.chunks, n, blk.block, lane)) =
+              u32x2{nearest_codes({v0[0], v0[1], v0[2], v0[3]}, none, su, inv), nearest_codes({v1[0], v1[1], v1[2], v1[3]}, none, su, inv)};
+        }
+        for (int n = full; n < a.g.chunks * 8; n += 8) {
+          const int d = key_dim(a.g.chunks, n, g);
+          if (d >= hd) continue;
+          const float* v = x + i * ldx + d;
+          const f32x4 v0 = *(const f32x4*)v * up, v1 = *(const f32x4*)(v + 4) * up;
+          *(u32x2*)(region + key_at(a.g.chunks, n, blk.block, lane)) =
+              u32x2{nearest_codes({v0[0], v0[1], v0[2], v0[3]}, none, su, inv), nearest_codes({v1[0], v1[1], v1[2], v1[3]}, none, su, inv)};
+        }
+      } else {
+        const float* v = x + 4 * g * ldx + i;
+        unsigned* at = (unsigned*)(region + a.g.v_off + lane * 16 + 4 * blk.block);
+#pragma unroll 4
+        for (int n = 0; n < hd / 16; n++, v += 16, at += 256)
+          *at = nearest_codes({v[0] * up, v[ldx] * up, v[2 * ldx] * up, v[3 * ldx] * up}, none, su, inv);
+      }
+    } else if (!values) {
       // thread: position i, numbers d .. d + 7 (lane and piece as in kv_key_byte)
-      for (int e = tid; e < a.g.chunks * 64; e += 256) {
+      for (int e = tid; e < a.g.chunks * 64; e += N) {
         const int lane = e % 64, i = lane % 16, n = e / 64 * 8;
         const int d = key_dim(a.g.chunks, n, lane / 16);
         const bool held = i < old;
@@ -308,40 +379,49 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
           v[1] = *(const f32x4*)(x + i * ldx + d + 4);
         }
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          w[j] = 0;
-#pragma unroll
-          for (int k = 0; k < 4; k++) w[j] |= code(held, o[j] >> (8 * k) & 255, v[j][k]) << (8 * k);
-        }
+        for (int j = 0; j < 2; j++) w[j] = codes({held, held, held, held}, o[j], {v[j][0], v[j][1], v[j][2], v[j][3]});
         *at = w;
       }
     } else {
       // thread: number d = 16 n + i, positions 4 g .. 4 g + 3
 #pragma unroll 2
-      for (int e = tid; e < hd * 4; e += 256) {
+      for (int e = tid; e < hd * 4; e += N) {
         const int lane = e % 64, i = lane % 16, g = lane / 16, n = e / 64;
         if (4 * g >= end || !(grown || 4 * g + 3 >= old)) continue;
         unsigned* at = (unsigned*)(region + a.g.v_off + e * 16 + 4 * blk.block);
         const unsigned o = 4 * g < old ? *at : 0;
-        unsigned w = 0;
+        float v[4];
+        bool held[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
           const int t = 4 * g + r;
-          const float v = t >= old && t < end ? x[t * ldx + 16 * n + i] : 0.0f;
-          w |= code(t < old, o >> (8 * r) & 255, v) << (8 * r);
+          v[r] = t >= old && t < end ? x[t * ldx + 16 * n + i] : 0.0f;
+          held[r] = t < old;
         }
-        *at = w;
+        *at = codes(held, o, v);
       }
     }
     if (tid == 0) *scale = s;
-    __syncthreads();  // the next block's rows may overwrite these
+    if constexpr (W == 4) __syncthreads();  // the next block's rows may overwrite these
   }
+}
+
+// More than 64 KiB of LDS is asked for.
+template <typename K>
+static hipError_t allow_lds(K kernel, uint32_t lds) {
+  if (lds <= 65536) return hipSuccess;
+  return hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
 }
 
 template <typename T>
 static hipError_t append_typed(const KvAppendArgs& a, unsigned n, hipStream_t st) {
-  const dim3 grid(std::min(n, 1u << 20), (unsigned)a.g.kv_heads, 2);
-  return launch(k_kv_append<T>, grid, 256, (uint32_t)(KV_BLOCK * (a.g.hd + 4) * 4), st, a);
+  const uint32_t lds = (uint32_t)(KV_BLOCK * (a.g.hd + 4) * 4);
+  const unsigned most = 1u << 20;
+  if ((size_t)n * a.g.kv_heads * 2 <= 2048)  // as many work-groups as run at once
+    return launch(k_kv_append<T, 4>, dim3(n, (unsigned)a.g.kv_heads, 2), 256, lds, st, a);
+  const hipError_t e = allow_lds(k_kv_append<T, 1>, 4 * lds);
+  if (e != hipSuccess) return e;
+  return launch(k_kv_append<T, 1>, dim3(std::min((n + 3) / 4, most), (unsigned)a.g.kv_heads, 2), 256, 4 * lds, st, a);
 }
 
 hipError_t launch_kv_append(int dtype, const KvAppendArgs& a, unsigned grid, hipStream_t st) {
@@ -358,64 +438,60 @@ hipError_t launch_kv_append(int dtype, const KvAppendArgs& a, unsigned grid, hip
 // reading back
 // ---------------------------------------------------------------------------
 
-// A work-group per page, head, and keys or values; a lane reads 16 bytes as they
-// lie: 16 numbers of one position of the keys (four 16-byte stores, 64 bytes of
-// a row), 16 positions of one number of the values (16 stores, of which a wave's
-// make 64-byte pieces of four rows).
+// A work-group per page, head, and keys or values: 16 bytes a lane as they lie,
+// through LDS into whole rows.
 __global__ __launch_bounds__(256) void k_kv_read(KvGeom g, size_t layer, uint32_t row, size_t first, size_t count,
                                                  float* k, float* v) {
+  extern __shared__ float x[];  // [64][hd + 4]
   const size_t p = first / KV_PAGE + blockIdx.x;
-  const int head = blockIdx.y, hd = g.hd;
+  const int head = blockIdx.y, hd = g.hd, ldx = hd + 4, tid = threadIdx.x;
   const uint8_t* region = g.pool + g.table[(size_t)row * g.max_pages + p] * g.page_bytes + layer * g.layer_bytes +
                           (size_t)head * g.head_bytes;
-  const long long base = (long long)(p * KV_PAGE) - (long long)first;  // output row of the page's position 0
-  const size_t stride = (size_t)g.kv_heads * hd;
   const f32x4 s = *(const f32x4*)(region + g.s_off + (blockIdx.z ? 16 : 0));
-  auto row_of = [&](int t) { return base + t; };
-  auto wanted = [&](long long r) { return r >= 0 && r < (long long)count; };
+  auto value = [](unsigned w, int b, float scale) { return (float)((int)(w >> (8 * b) & 255) - 128) * scale; };
   if (blockIdx.z == 0) {
-    float* out = k + (size_t)head * hd;
     const int whole = g.chunks / 2 * 256;
-    for (int e = threadIdx.x; e < whole; e += 256) {
+    for (int e = tid; e < whole; e += 256) {
       const int lane = e % 64, mm = e / 64 % 4, d = e / 256 * 64 + lane / 16 * 16;
-      const long long r = row_of(16 * mm + lane % 16);
-      if (!wanted(r) || d >= hd) continue;
+      if (d >= hd) continue;
       const u32x4 w = *(const u32x4*)(region + e * 16);
+      float* at = x + (16 * mm + lane % 16) * ldx + d;
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        f32x4 x;
-#pragma unroll
-        for (int b = 0; b < 4; b++) x[b] = (float)((int)(w[j] >> (8 * b) & 255) - 128) * s[mm];
-        *(f32x4u*)(out + r * stride + d + 4 * j) = x;
-      }
+      for (int j = 0; j < 4; j++)
+        *(f32x4*)(at + 4 * j) = f32x4{value(w[j], 0, s[mm]), value(w[j], 1, s[mm]), value(w[j], 2, s[mm]), value(w[j], 3, s[mm])};
     }
     if (g.chunks & 1) {
-      const int lane = threadIdx.x % 64, mm = threadIdx.x / 64, d = g.chunks / 2 * 64 + lane / 16 * 8;
-      const long long r = row_of(16 * mm + lane % 16);
-      if (wanted(r) && d < hd) {
-        const u32x2 w = *(const u32x2*)(region + whole * 16 + threadIdx.x * 8);
+      const int lane = tid % 64, mm = tid / 64, d = g.chunks / 2 * 64 + lane / 16 * 8;
+      if (d < hd) {
+        const u32x2 w = *(const u32x2*)(region + whole * 16 + tid * 8);
+        float* at = x + (16 * mm + lane % 16) * ldx + d;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          f32x4 x;
-#pragma unroll
-          for (int b = 0; b < 4; b++) x[b] = (float)((int)(w[j] >> (8 * b) & 255) - 128) * s[mm];
-          *(f32x4u*)(out + r * stride + d + 4 * j) = x;
-        }
+        for (int j = 0; j < 2; j++)
+          *(f32x4*)(at + 4 * j) = f32x4{value(w[j], 0, s[mm]), value(w[j], 1, s[mm]), value(w[j], 2, s[mm]), value(w[j], 3, s[mm])};
       }
     }
   } else {
-    for (int e = threadIdx.x; e < hd * 4; e += 256) {
-      const int lane = e % 64, d = e / 64 * 16 + lane % 16;
+    for (int e = tid; e < hd * 4; e += 256) {
+      const int lane = e % 64;
       const u32x4 w = *(const u32x4*)(region + g.v_off + e * 16);
-      float* out = v + (size_t)head * hd + d;
+      float* at = x + lane / 16 * 4 * ldx + e / 64 * 16 + lane % 16;
 #pragma unroll
       for (int mm = 0; mm < 4; mm++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const long long r = row_of(16 * mm + lane / 16 * 4 + j);
-          if (wanted(r)) out[r * stride] = (float)((int)(w[mm] >> (8 * j) & 255) - 128) * s[mm];
-        }
+        for (int j = 0; j < 4; j++) at[(16 * mm + j) * ldx] = value(w[mm], j, s[mm]);
     }
+  }
+  __syncthreads();
+  // the page's positions that are asked for
+  const size_t pos0 = p * KV_PAGE;
+  const int t0 = first > pos0 ? (int)(first - pos0) : 0;
+  const int t1 = first + count - pos0 < KV_PAGE ? (int)(first + count - pos0) : (int)KV_PAGE;
+  float* out = (blockIdx.z ? v : k) + (size_t)head * hd;
+  const size_t stride = (size_t)g.kv_heads * hd;
+  const int quads = hd / 4, n = (t1 - t0) * quads;
+  for (int e = tid; e < n; e += 256) {
+    const int t = t0 + e / quads, d = e % quads * 4;
+    *(f32x4u*)(out + (pos0 + t - first) * stride + d) = *(const f32x4*)(x + t * ldx + d);
   }
 }
 
@@ -423,7 +499,10 @@ hipError_t launch_kv_read(const KvGeom& g, size_t layer, uint32_t row, size_t fi
                           hipStream_t st) {
   if (count == 0) return hipSuccess;
   const size_t pages = (first + count - 1) / KV_PAGE - first / KV_PAGE + 1;
-  return launch(k_kv_read, dim3((unsigned)pages, (unsigned)g.kv_heads, 2), 256, 0, st, g, layer, row, first, count, k, v);
+  const uint32_t lds = (uint32_t)(KV_PAGE * (g.hd + 4) * 4);
+  const hipError_t e = allow_lds(k_kv_read, lds);
+  if (e != hipSuccess) return e;
+  return launch(k_kv_read, dim3((unsigned)pages, (unsigned)g.kv_heads, 2), 256, lds, st, g, layer, row, first, count, k, v);
 }
 
 }  // namespace hale

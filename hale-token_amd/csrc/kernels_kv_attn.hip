@@ -697,7 +697,7 @@ __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a) {
 // Joins the partial results of one row: a work-group, whose threads take four
 // numbers each of every so many'th part; the slices are added in their order.
 __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a) {
-  constexpr int AHEAD = 8;
+  constexpr int AHEAD = 16;
   __shared__ float sw[JOIN_PARTS];
   __shared__ float red[8];
   __shared__ f32x4 sv[256];
