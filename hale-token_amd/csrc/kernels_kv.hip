@@ -103,14 +103,15 @@ __global__ __launch_bounds__(256) void k_rope(RopeArgs a) {
   }
 }
 
-constexpr size_t ROPE_VEC_PAIRS = 65536;
+constexpr size_t ROPE_VEC_PAIRS = 1u << 18;
 
 template <typename T>
 static hipError_t rope_typed(const RopeArgs& a, hipStream_t st) {
   size_t bits = 0;
   for (int i = 0; i < 2; i++)
     if (a.heads[i]) bits |= (uintptr_t)a.src[i] | (uintptr_t)a.dst[i] | (a.src_stride[i] | a.dst_stride[i]) * sizeof(T);
-  // few rows are a matter of latency, where a thread per pair is the shorter way
+  // few rows are a matter of latency, where a thread per pair is the shorter way (36
+  // bf16 heads of 128, per pair / in pieces: 16 rows 2.7 / 3.2 us, 112 3.4 / 3.4, 224 4.5 / 3.6)
   const size_t pairs = a.rows * (size_t)(a.heads[0] + a.heads[1]) * a.half;
   if (pairs >= ROPE_VEC_PAIRS && bits % 16 == 0 && a.hd % 8 == 0 && a.half % 8 == 0) {
     const int units = (a.heads[0] + a.heads[1]) * (a.half / 8 + (a.hd - 2 * a.half) / 8);
@@ -135,12 +136,32 @@ hipError_t launch_rope(int dtype, const RopeArgs& a, hipStream_t st) {
 }
 
 // ---------------------------------------------------------------------------
-// plan upload, page copies
+// plan upload and page copies
 // ---------------------------------------------------------------------------
 
-// A thread per 16 bytes, all of them read at once: the host's memory is a
-// microsecond away, once.
-__global__ __launch_bounds__(256) void k_kv_upload(KvUploadArgs a, unsigned n4) {
+// One launch for what a step or a page operation sends and moves: the first
+// work-groups take a thread per 16 bytes of the plan, all of them read at once
+// (the host's memory is a microsecond or two away, once), the others a piece of a
+// page each, whose place they read from the same buffer.
+constexpr unsigned COPY_BYTES = 16384;  // per work-group: four 16-byte pieces a thread
+
+__global__ __launch_bounds__(256) void k_kv_upload(KvUploadArgs a, unsigned n4, unsigned uploads, unsigned chunks) {
+  if (blockIdx.x >= uploads) {
+    const unsigned w = blockIdx.x - uploads;
+    const KvCopy c = a.copies[w / chunks];
+    const size_t at = (size_t)(w % chunks) * COPY_BYTES;
+    const u32x4* s = (const u32x4*)(a.pool + c.src * a.page_bytes + at);
+    u32x4* d = (u32x4*)(a.pool + c.dst * a.page_bytes + at);
+    const unsigned n = (unsigned)(a.page_bytes - at < COPY_BYTES ? a.page_bytes - at : COPY_BYTES) / 16;
+    u32x4 x[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (threadIdx.x + 256 * j < n) x[j] = s[threadIdx.x + 256 * j];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (threadIdx.x + 256 * j < n) d[threadIdx.x + 256 * j] = x[j];
+    return;
+  }
   const unsigned id = blockIdx.x * 256 + threadIdx.x;
   // that this kernel runs says that the one before it has ended
   if (id == 0) __hip_atomic_store(a.done, a.number, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
@@ -164,33 +185,16 @@ __global__ __launch_bounds__(256) void k_kv_upload(KvUploadArgs a, unsigned n4) 
 hipError_t launch_kv_upload(const KvUploadArgs& a, hipStream_t st) {
   unsigned n4 = 0;
   for (int p = 0; p < a.pieces; p++) n4 += a.words[p] / 4;
-  if (n4 + a.npairs == 0) return hipSuccess;
-  return launch(k_kv_upload, (n4 + a.npairs + 255) / 256, 256, 0, st, a, n4);
-}
-
-constexpr unsigned COPY_BYTES = 16384;  // per work-group: four 16-byte pieces a thread
-
-__global__ __launch_bounds__(256) void k_kv_copy_pages(uint8_t* pool, size_t page_bytes, const KvCopy* list) {
-  const KvCopy c = list[blockIdx.y];
-  const size_t at = (size_t)blockIdx.x * COPY_BYTES;
-  const u32x4* s = (const u32x4*)(pool + c.src * page_bytes + at);
-  u32x4* d = (u32x4*)(pool + c.dst * page_bytes + at);
-  const unsigned n = (unsigned)(page_bytes - at < COPY_BYTES ? page_bytes - at : COPY_BYTES) / 16;
-  u32x4 x[4];
-#pragma unroll
-  for (int j = 0; j < 4; j++)
-    if (threadIdx.x + 256 * j < n) x[j] = s[threadIdx.x + 256 * j];
-#pragma unroll
-  for (int j = 0; j < 4; j++)
-    if (threadIdx.x + 256 * j < n) d[threadIdx.x + 256 * j] = x[j];
-}
-
-hipError_t launch_kv_copy_pages(uint8_t* pool, size_t page_bytes, const KvCopy* list, unsigned n, hipStream_t st) {
-  const unsigned chunks = (unsigned)((page_bytes + COPY_BYTES - 1) / COPY_BYTES);
-  for (unsigned at = 0; at < n; at += 32768) {  // the grid's second dimension ends at 65535
-    const hipError_t e = launch(k_kv_copy_pages, dim3(chunks, std::min(n - at, 32768u)), 256, 0, st, pool, page_bytes,
-                                list + at);
+  const unsigned uploads = (n4 + a.npairs + 255) / 256 + (n4 + a.npairs == 0);
+  const size_t chunks = (a.page_bytes + COPY_BYTES - 1) / COPY_BYTES;
+  const size_t most = (0x7fffffffu - uploads) / chunks;  // a grid's work-groups
+  KvUploadArgs b = a;
+  for (bool first = true; first || b.ncopies; first = false) {
+    const unsigned n = (unsigned)std::min<size_t>(b.ncopies, most);
+    const hipError_t e = launch(k_kv_upload, uploads + n * (unsigned)chunks, 256, 0, st, b, n4, uploads, (unsigned)chunks);
     if (e != hipSuccess) return e;
+    b.copies += n;
+    b.ncopies -= n;
   }
   return hipSuccess;
 }
@@ -250,8 +254,9 @@ __device__ __forceinline__ unsigned key_at(int kc, int n, int block, int lane) {
 
 //
 // W: waves per block, 4 or 1.  Four where few blocks leave the chain to be shortened; one
-// where more blocks than the compute units hold work-groups would wait for each
-// other (a bf16 prompt of 4090 tokens, 8 heads of 128: 17.7 us with four, XX with one).
+// where there are many (bf16, 8 heads of 128, this kernel alone, four / one: 512 tokens
+// 5.7 / 7.6 us, 1024 7.2 / 8.0, 2048 12.0 / 10.3, 4090 17.3 / 12.4).  A prompt of 4090
+// reads 17 MB and writes 8: bound by about 900 vector instructions a wave.
 template <typename T, int W>
 __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
   extern __shared__ float lds[];  // [4 / W][16][hd + 4]
@@ -417,7 +422,7 @@ template <typename T>
 static hipError_t append_typed(const KvAppendArgs& a, unsigned n, hipStream_t st) {
   const uint32_t lds = (uint32_t)(KV_BLOCK * (a.g.hd + 4) * 4);
   const unsigned most = 1u << 20;
-  if ((size_t)n * a.g.kv_heads * 2 <= 2048)  // as many work-groups as run at once
+  if ((size_t)n * a.g.kv_heads * 2 <= 1024)
     return launch(k_kv_append<T, 4>, dim3(n, (unsigned)a.g.kv_heads, 2), 256, lds, st, a);
   const hipError_t e = allow_lds(k_kv_append<T, 1>, 4 * lds);
   if (e != hipSuccess) return e;

@@ -58,9 +58,10 @@ __host__ __device__ inline unsigned kv_value_byte(unsigned t, unsigned d) {
   return (d / 16 * 64 + t % 16 / 4 * 16 + d % 16) * 16 + t / 16 * 4 + t % 4;
 }
 
-// Plan and page table changes, read from host memory by the device: the
-// pieces of src, one behind the other (16-byte aligned, multiples of four
-// words), each to its own place, and npairs pairs (index, value) into table.
+// What the device reads from host memory: the plan's pieces in src, one behind
+// the other (16-byte aligned, multiples of four words), each to its own place;
+// npairs changes (index, value) of the page table; and ncopies pages to copy, none of
+// them written that is read.
 constexpr int KV_MAX_PIECES = 24;
 struct KvUploadArgs {
   const uint32_t* src;
@@ -70,13 +71,14 @@ struct KvUploadArgs {
   const uint32_t* pairs;
   unsigned npairs;
   uint32_t* table;
+  const KvCopy* copies;
+  unsigned ncopies;
+  uint8_t* pool;
+  size_t page_bytes;
   uint32_t* done;   // host memory: receives `number`, the last upload before this one
   uint32_t number;
 };
 hipError_t launch_kv_upload(const KvUploadArgs& a, hipStream_t st);
-
-// n pages, [n] (source, destination), from pool to pool.
-hipError_t launch_kv_copy_pages(uint8_t* pool, size_t page_bytes, const KvCopy* list, unsigned n, hipStream_t st);
 
 struct KvAppendArgs {
   KvGeom g;

@@ -175,7 +175,6 @@ constexpr int STAGINGS = 32;
 
 struct View {  // the plan of the current step under one window
   size_t window = 0;
-  bool built = false;
   KvPlan plan;
 };
 
@@ -201,7 +200,6 @@ struct hale_kv_cache {
   uint32_t* plan = nullptr;
   Sections at;
   size_t cap_tokens = 0;
-  KvCopy* list = nullptr;  // pages to copy, [pages of the pool]
   float* part_o = nullptr;
   float2* part_ml = nullptr;
   Staging staging[STAGINGS];
@@ -212,7 +210,7 @@ struct hale_kv_cache {
   size_t tokens = 0, blocks = 0;
   uint64_t step_shape = 0;
   std::vector<KvStepSeq> seqs;
-  std::vector<KvCopy> copies;
+  std::vector<KvCopy> copies;  // pages that the next upload copies
   View views[HALE_KV_MAX_WINDOWS];
   int nviews = 0;
 };
@@ -269,48 +267,48 @@ struct Upload {
   int end() {
     hale_ctx* c = kv->ctx;
     auto& dirty = kv->pages.dirty;
-    a.pairs = (const uint32_t*)(s->base + used);
-    a.npairs = (unsigned)dirty.size();
-    a.table = kv->table;
     uint32_t* pairs = (uint32_t*)(s->base + used);
     for (size_t i = 0; i < dirty.size(); i++) {
       pairs[2 * i] = dirty[i];
       pairs[2 * i + 1] = kv->pages.entry(dirty[i]);
     }
+    KvCopy* copies = (KvCopy*)(pairs + 2 * dirty.size());
+    if (!kv->copies.empty()) std::memcpy(copies, kv->copies.data(), kv->copies.size() * sizeof(KvCopy));
     a.src = (const uint32_t*)s->base;
+    a.pairs = pairs;
+    a.npairs = (unsigned)dirty.size();
+    a.table = kv->table;
+    a.copies = copies;
+    a.ncopies = (unsigned)kv->copies.size();
+    a.pool = kv->geom.pool;
+    a.page_bytes = kv->geom.page_bytes;
     a.done = kv->done;
     a.number = kv->uploads++;  // from the first one's 0 on: numbers count from 1
     KV_LAUNCH(c, K_KV_PAGES, launch_kv_upload(a, c->stream));
     s->number = kv->uploads;
     dirty.clear();
+    kv->copies.clear();
     return HALE_OK;
   }
 };
 
 }  // namespace
 
-// Bytes of an upload: its pieces, each rounded up, and the table's changes.
+// Bytes of an upload: its pieces, each rounded up, the table's changes and the copies.
 static size_t upload_bytes(const hale_kv_cache* kv, size_t piece_bytes) {
-  return piece_bytes + 16 * KV_MAX_PIECES + kv->pages.dirty.size() * 8;
+  return piece_bytes + 16 * KV_MAX_PIECES + kv->pages.dirty.size() * 8 + kv->copies.size() * sizeof(KvCopy);
 }
 
-// Sends the page table's changes, and with them the page copies of `copies`.
-static int send_pages(hale_kv_cache* kv, const std::vector<KvCopy>& copies) {
-  if (kv->pages.dirty.empty() && copies.empty()) return HALE_OK;
-  hale_ctx* c = kv->ctx;
+// Sends the page table's changes and makes the page copies of kv->copies.
+static int send_pages(hale_kv_cache* kv) {
+  if (kv->pages.dirty.empty() && kv->copies.empty()) return HALE_OK;
   Upload u(kv);
-  int rc = u.begin(upload_bytes(kv, copies.size() * sizeof(KvCopy)));
-  if (rc) return rc;
-  u.put(kv->list, copies.data(), copies.size() * sizeof(KvCopy));
-  rc = u.end();
-  if (rc) return rc;
-  if (!copies.empty())
-    KV_LAUNCH(c, K_KV_PAGES, launch_kv_copy_pages(kv->geom.pool, kv->geom.page_bytes, kv->list, (unsigned)copies.size(), c->stream));
-  return HALE_OK;
+  const int rc = u.begin(upload_bytes(kv, 0));
+  return rc ? rc : u.end();
 }
 
 static void free_device(hale_kv_cache* kv) {
-  for (void* p : {(void*)kv->geom.pool, (void*)kv->table, (void*)kv->plan, (void*)kv->list, (void*)kv->part_o, (void*)kv->part_ml})
+  for (void* p : {(void*)kv->geom.pool, (void*)kv->table, (void*)kv->plan, (void*)kv->part_o, (void*)kv->part_ml})
     (void)hipFree(p);
   for (Staging& s : kv->staging) {
     if (s.base) (void)hipHostFree(s.base);
@@ -421,7 +419,6 @@ extern "C" int hale_kv_create(hale_ctx* c, size_t layers, size_t heads, size_t k
   rc = make_pool(c, g.page_bytes * num_pages, &g.pool);
   const size_t part_rows = kv_part_rows(hd);
   if (!rc && (hipMalloc(&kv->table, row * max_seqs * 4) != hipSuccess ||
-              hipMalloc(&kv->list, num_pages * sizeof(KvCopy) + 16) != hipSuccess ||
               hipMalloc(&kv->part_o, part_rows * hd * 4) != hipSuccess ||
               hipMalloc(&kv->part_ml, part_rows * sizeof(float2)) != hipSuccess))
     rc = ctx_fail(c, HALE_ENOMEM, "kv_create: page table and workspace");
@@ -504,7 +501,7 @@ static int moves_allowed(hale_kv_cache* kv, const char* what) {
   const int rc = capturing(kv->ctx, &cap);
   if (rc) return rc;
   if (cap) return ctx_fail(kv->ctx, HALE_EINVAL, "%s while the stream is being captured", what);
-  return HALE_OK;
+  return kv->copies.empty() ? HALE_OK : send_pages(kv);  // copies that found no staging memory
 }
 
 extern "C" int hale_kv_seq_copy(hale_kv_cache* kv, uint32_t seq, uint32_t* out) {
@@ -514,9 +511,8 @@ extern "C" int hale_kv_seq_copy(hale_kv_cache* kv, uint32_t seq, uint32_t* out) 
   int rc = moves_allowed(kv, "kv_seq_copy");
   if (rc) return rc;
   std::string err;
-  kv->copies.clear();
   rc = status(kv, "kv_seq_copy", kv->pages.copy(seq, out, &kv->copies, &err), err);
-  return rc ? rc : send_pages(kv, kv->copies);
+  return rc ? rc : send_pages(kv);
   KV_CATCH(kv->ctx)
 }
 
@@ -554,10 +550,9 @@ extern "C" int hale_kv_compact(hale_kv_cache* kv, size_t* moved) {
   std::lock_guard<std::recursive_mutex> lk(kv->ctx->mu);
   int rc = moves_allowed(kv, "kv_compact");
   if (rc) return rc;
-  kv->copies.clear();
   kv->pages.compact(&kv->copies);
   if (moved) *moved = kv->copies.size();
-  return send_pages(kv, kv->copies);
+  return send_pages(kv);
   KV_CATCH(kv->ctx)
 }
 
@@ -575,11 +570,10 @@ extern "C" int hale_kv_resize(hale_kv_cache* kv, size_t num_pages) {
   rc = hale_kv_compact(kv, nullptr);
   if (rc) return rc;
   uint8_t* pool = nullptr;
-  KvCopy* list = nullptr;
   rc = make_pool(c, kv->geom.page_bytes * num_pages, &pool);
   if (rc) return rc;
-  hipError_t e = hipMalloc(&list, num_pages * sizeof(KvCopy) + 16);
-  if (e == hipSuccess && used) e = launch_copy(pool, kv->geom.pool, used * kv->geom.page_bytes / 16, c->stream);
+  hipError_t e = hipSuccess;
+  if (used) e = launch_copy(pool, kv->geom.pool, used * kv->geom.page_bytes / 16, c->stream);
   if (e == hipSuccess) e = hipStreamSynchronize(c->stream);
   if (e == hipSuccess) {
     try {
@@ -590,13 +584,10 @@ extern "C" int hale_kv_resize(hale_kv_cache* kv, size_t num_pages) {
   }
   if (e != hipSuccess) {
     (void)hipFree(pool);
-    (void)hipFree(list);
     return ctx_fail(c, HALE_ENOMEM, "kv_resize: %s", hipGetErrorString(e));
   }
   (void)hipFree(kv->geom.pool);
-  (void)hipFree(kv->list);
   kv->geom.pool = pool;
-  kv->list = list;
   kv->epoch++;
   return HALE_OK;
   KV_CATCH(c)
@@ -606,10 +597,6 @@ extern "C" int hale_kv_resize(hale_kv_cache* kv, size_t num_pages) {
 // steps
 // ---------------------------------------------------------------------------
 
-// Puts a view's plan together; its pieces follow in put_view().
-static void build_view(hale_kv_cache* kv, View& v) {
-  kv_plan(kv->shape, kv->seqs, v.window, &v.plan);
-}
 static size_t view_bytes(const View& v) {
   return (v.plan.few.size() + v.plan.many.size()) * sizeof(KvItem) + (v.plan.few_joins.size() + v.plan.many_joins.size()) * sizeof(KvJoin) + 32;
 }
@@ -622,7 +609,6 @@ static void put_view(hale_kv_cache* kv, Upload& u, int i) {
   u.put(kv->plan + kv->at.items[i] + kv->at.many, v.plan.many.data(), v.plan.many.size() * sizeof(KvItem));
   u.put(kv->plan + kv->at.joins[i], v.plan.few_joins.data(), v.plan.few_joins.size() * sizeof(KvJoin));
   u.put(kv->plan + kv->at.joins[i] + kv->at.many_joins, v.plan.many_joins.data(), v.plan.many_joins.size() * sizeof(KvJoin));
-  v.built = true;
 }
 
 extern "C" int hale_kv_reserve(hale_kv_cache* kv, size_t max_tokens) {
@@ -649,35 +635,33 @@ extern "C" int hale_kv_step(hale_kv_cache* kv, size_t nseq, const uint32_t* seqs
   for (size_t i = 0; i < nseq; i++) tokens += ntok[i];
   if (tokens > (size_t)0x7fffffff / kv->shape.heads)
     return ctx_fail(c, HALE_EINVAL, "kv_step: %zu tokens of %zu heads", tokens, kv->shape.heads);
-  // everything that may fail for want of memory, then the bookkeeping
+  std::string err;
+  rc = status(kv, "kv_step", kv->pages.check_step(nseq, seqs, ntok, &err), err);
+  if (rc) return rc;
+  // all that may want memory, then the bookkeeping
+  std::vector<KvStepSeq> next;
   std::vector<KvBlock> blocks;
   blocks.reserve(kv_max_blocks(tokens, nseq));
   std::vector<int32_t> positions(tokens);
-  std::string err;
-  rc = status(kv, "kv_step", kv->pages.check_step(nseq, seqs, ntok, &err), err);
-  if (!rc) rc = grow_plan(kv, tokens);
-  if (rc) return rc;
-  kv->copies.clear();
-  rc = status(kv, "kv_step", kv->pages.step(nseq, seqs, ntok, &kv->seqs, &kv->copies, &err), err);
-  if (rc) return rc;
-  kv->stepped = false;
-  kv->tokens = tokens;
+  kv->pages.preview(nseq, seqs, ntok, &next);
+  kv_blocks(next, kv->pages.max_pages(), &blocks);
   uint64_t shape = 1469598103934665603ull;  // FNV-1a over the tokens per sequence
   auto mix = [&](uint32_t v) {
     for (int b = 0; b < 4; b++) shape = (shape ^ (v >> (8 * b) & 255)) * 1099511628211ull;
   };
   mix((uint32_t)nseq);
-  for (uint32_t i = 0; i < nseq; i++) {
-    const KvStepSeq& s = kv->seqs[i];
+  for (const KvStepSeq& s : next) {
     mix(s.ntok);
     for (uint32_t t = 0; t < s.ntok; t++) positions[s.tok0 + t] = (int32_t)(s.len0 + t);
   }
-  kv_blocks(kv->seqs, kv->pages.max_pages(), &blocks);
-  kv->step_shape = shape;
-  kv->blocks = blocks.size();
-  size_t bytes = kv->copies.size() * sizeof(KvCopy) + tokens * 4 + blocks.size() * sizeof(KvBlock) + 64;
+  rc = grow_plan(kv, tokens);
+  if (rc) return rc;
+  kv->stepped = false;  // the views' plans become the next step's
+  kv->seqs.swap(next);
+  size_t bytes = tokens * 4 + blocks.size() * sizeof(KvBlock) + 64;
+  bytes += kv->pages.step_changes() * 8 + kv->pages.step_copies() * sizeof(KvCopy);
   for (int i = 0; i < kv->nviews; i++) {
-    build_view(kv, kv->views[i]);
+    kv_plan(kv->shape, kv->seqs, kv->views[i].window, &kv->views[i].plan);
     bytes += view_bytes(kv->views[i]);
   }
   Upload u(kv);
@@ -687,12 +671,13 @@ extern "C" int hale_kv_step(hale_kv_cache* kv, size_t nseq, const uint32_t* seqs
   u.put(kv->plan + kv->at.counts, n, sizeof n);
   u.put(kv->plan + kv->at.positions, positions.data(), tokens * 4);
   u.put(kv->plan + kv->at.blocks, blocks.data(), blocks.size() * sizeof(KvBlock));
-  u.put(kv->list, kv->copies.data(), kv->copies.size() * sizeof(KvCopy));
   for (int i = 0; i < kv->nviews; i++) put_view(kv, u, i);
-  rc = u.end();
+  rc = status(kv, "kv_step", kv->pages.step(nseq, seqs, ntok, nullptr, &kv->copies, &err), err);
+  if (!rc) rc = u.end();
   if (rc) return rc;
-  if (!kv->copies.empty())
-    KV_LAUNCH(c, K_KV_PAGES, launch_kv_copy_pages(kv->geom.pool, kv->geom.page_bytes, kv->list, (unsigned)kv->copies.size(), c->stream));
+  kv->tokens = tokens;
+  kv->step_shape = shape;
+  kv->blocks = blocks.size();
   kv->stepped = true;
   return HALE_OK;
   KV_CATCH(c)
@@ -716,7 +701,7 @@ static int layer_call(hale_kv_cache* kv, const char* what, size_t layer, int dty
   KVCHK(c, hipSetDevice(c->device));
   int rc = capturing(c, cap);
   if (rc) return rc;
-  if (!*cap) return send_pages(kv, {});  // table changes since the step
+  if (!*cap) return send_pages(kv);  // table changes since the step
   for (const KvUse& u : c->kv_uses) {
     if (u.kv != kv) continue;
     if (u.epoch != kv->epoch || u.shape != kv->step_shape)
@@ -736,7 +721,7 @@ int hale::kv_check_replay(hale_ctx* c, const std::vector<KvUse>& uses) {
       return ctx_fail(c, HALE_EINVAL, "graph_launch: its key/value cache's buffers grew since the capture");
     if (!u.kv->stepped || u.kv->step_shape != u.shape)
       return ctx_fail(c, HALE_EINVAL, "graph_launch: the key/value cache's step is not of the captured tokens per sequence");
-    const int rc = send_pages(u.kv, {});
+    const int rc = send_pages(u.kv);
     if (rc) return rc;
   }
   return HALE_OK;
@@ -783,7 +768,9 @@ extern "C" int hale_kv_attention_device(hale_kv_cache* kv, size_t layer, int dty
   hale_ctx* c = kv->ctx;
   KV_TRY
   std::lock_guard<std::recursive_mutex> lk(c->mu);
-  if (!(scale > 0.0f) || !std::isfinite(scale)) return ctx_fail(c, HALE_EINVAL, "kv_attention: scale %g is not positive", (double)scale);
+  // scores are in powers of two: scale log2(e) has to be finite as well
+  if (!(scale > 0.0f) || !std::isfinite(scale * 2.0f))
+    return ctx_fail(c, HALE_EINVAL, "kv_attention: scale %g is not positive and below 2^127", (double)scale);
   if (float_type(dtype) && ntok) {
     const size_t row = kv->shape.heads * kv->shape.head_dim;
     if (!q || !out) return ctx_fail(c, HALE_EINVAL, "kv_attention: NULL argument");
@@ -803,7 +790,7 @@ extern "C" int hale_kv_attention_device(hale_kv_cache* kv, size_t layer, int dty
     if (cap) return ctx_fail(c, HALE_EINVAL, "kv_attention: first call with window %zu in a capture; make it once before", window);
     View& v = kv->views[i];
     v.window = window;
-    build_view(kv, v);
+    kv_plan(kv->shape, kv->seqs, window, &v.plan);
     Upload u(kv);
     rc = u.begin(upload_bytes(kv, view_bytes(v)));
     if (rc) return rc;
@@ -873,7 +860,7 @@ extern "C" int hale_kv_read_device(hale_kv_cache* kv, size_t layer, uint32_t seq
     return ctx_fail(c, HALE_EINVAL, "kv_read: outputs are NULL or not aligned");
   rc = moves_allowed(kv, "kv_read");
   if (rc) return rc;
-  rc = send_pages(kv, {});
+  rc = send_pages(kv);
   if (rc) return rc;
   KV_LAUNCH(c, K_KV_READ, launch_kv_read(kv->geom, layer, seq, first, count, k, v, c->stream));
   return HALE_OK;

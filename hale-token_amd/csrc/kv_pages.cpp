@@ -170,22 +170,28 @@ KvPages::Status KvPages::check_step(size_t nseq, const uint32_t* seqs, const uin
   return OK;
 }
 
+void KvPages::preview(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, std::vector<KvStepSeq>* plan) const {
+  plan->resize(nseq);
+  uint32_t tok0 = 0;
+  for (size_t i = 0; i < nseq; i++) {
+    (*plan)[i] = {seqs[i], (uint32_t)seqs_[seqs[i]].len, ntok[i], tok0};
+    tok0 += ntok[i];
+  }
+}
+
 KvPages::Status KvPages::step(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, std::vector<KvStepSeq>* plan,
                               std::vector<KvCopy>* copies, std::string* err) {
   const Status st = check_step(nseq, seqs, ntok, err);
   if (st) return st;
-  plan->resize(nseq);
+  if (plan) preview(nseq, seqs, ntok, plan);
   copies->reserve(copies->size() + copies_);
   dirty.reserve(dirty.size() + need_);
   for (size_t i = 0; i < nseq; i++) {
     Seq& s = seqs_[seqs[i]];
     s.pages.reserve(ceil_div(s.len + ntok[i], KV_PAGE));
   }
-  uint32_t tok0 = 0;
   for (size_t i = 0; i < nseq; i++) {
     Seq& s = seqs_[seqs[i]];
-    (*plan)[i] = {seqs[i], (uint32_t)s.len, ntok[i], tok0};
-    tok0 += ntok[i];
     if (mark_[seqs[i]] == 0) {
       const uint32_t p = take();
       copies->push_back({s.pages.back(), p});

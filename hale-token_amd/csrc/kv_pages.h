@@ -123,8 +123,13 @@ class KvPages {
   Status len(uint32_t seq, size_t* len, std::string* err) const;
   // Whether step() would succeed, and a message if not.
   Status check_step(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, std::string* err);
+  // After check_step(): what the step would be, and the page table changes and
+  // page copies that it would make.
+  void preview(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, std::vector<KvStepSeq>* plan) const;
+  size_t step_changes() const { return need_; }
+  size_t step_copies() const { return copies_; }
   // Room for ntok[i] more positions of seqs[i]: new pages, and copies of
-  // shared, partly filled pages that the step writes to.
+  // shared, partly filled pages that the step writes to.  plan (may be null): as preview().
   Status step(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, std::vector<KvStepSeq>* plan,
               std::vector<KvCopy>* copies, std::string* err);
   // Moves the pages behind the first used() into the holes before.

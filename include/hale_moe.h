@@ -645,11 +645,14 @@ int hale_kv_append_device(hale_kv_cache *kv, size_t layer, int dtype,
  * d_q and d_out [ntok][num_heads][head_dim] of `dtype`; query head h reads
  * key/value head h / (num_heads / num_kv_heads).  A token at position p sees the
  * positions up to p, with window > 0 only those above p - window.  Scores are
- * scale (positive) times q . k.  At most HALE_KV_MAX_WINDOWS different windows
+ * scale (positive, below 2^127) times q . k.  At most HALE_KV_MAX_WINDOWS different windows
  * (0 among them) per cache.  Sums and the softmax's statistics are f32; queries
- * of f16 and bf16 enter exactly, of f32 to 2^-23 of the row's largest; probabilities
- * are rounded to 2^-11 of their value for f16 and bf16 and 2^-23 for f32.  The
- * order of all sums is fixed: equal calls give equal bits. */
+ * enter to 2^-28 (f16, bf16) or 2^-23 (f32) of their row's largest number;
+ * probabilities are rounded to 2^-11 of their value for f16 and bf16 and 2^-23 for
+ * f32 (no finer than 2^-31 and 2^-39 of the row's largest, each times 127 times the
+ * largest scale of the values that the row sees).  A query row that is not finite gives NaN in
+ * its own results only.  The order of all sums is fixed: equal calls give equal
+ * bits.  d_out may be d_q with the same stride. */
 int hale_kv_attention_device(hale_kv_cache *kv, size_t layer, int dtype,
                              size_t ntok, const void *d_q, size_t q_stride,
                              float scale, size_t window, void *d_out,

@@ -206,7 +206,7 @@ def test_attention_head_dims(rig, dtype, dim):
     r.check_attention(g, 0, dtype, seqs, [0, 2, 9], pad=3, offset=1)
 
 
-@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (7, 7), (16, 1), (17, 1), (33, 1), (64, 2), (40, 8), (12, 4)])
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (7, 7), (16, 1), (17, 1), (33, 1), (64, 2), (40, 8), (12, 4), (150, 1)])
 def test_attention_head_groups(rig, heads, kv_heads):
     r = rig(dim=64, heads=heads, kv_heads=kv_heads, pages=40)
     g = np.random.default_rng(heads)
@@ -286,26 +286,82 @@ def test_attention_zero_and_huge_scales(rig):
     r.kv.step([a], [n])
     r.append(0, "f32", [a], [n], k, v)
     r.check_attention(g, 0, "f32", [a], [n])
+    r.check_attention(g, 0, "bf16", [a], [n])
     q = np.zeros((n, 2, 64), np.float32)
     got = r.attend(0, "f32", q)
     want, mag, prod, total, vtop = r.model.attend(a, 0, q, 0.125)
     assert (np.abs(got - want) <= attention_bound("f32", mag, prod, total, vtop, 64)).all()
+    r.step(g, "f32", [a], [3])  # few rows
+    r.check_attention(g, 0, "f32", [a], [3])
+    r.check_attention(g, 0, "bf16", [a], [3])
 
 
-def test_a_query_that_is_not_finite_spoils_only_its_row(rig):
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [5, 60])
+def test_a_query_that_is_not_finite_spoils_only_its_row(rig, dtype, n):
     r = rig(dim=64, heads=4, kv_heads=2, pages=40)
     g = np.random.default_rng(7)
     a = r.create()
-    r.step(g, "f32", [a], [70])
-    r.step(g, "f32", [a], [5])
-    q = g.standard_normal((5, 4, 64)).astype(np.float32)
-    clean = r.attend(0, "f32", q)
-    q[2, 1, 3], q[4, 0, 0] = np.nan, np.inf
-    got = r.attend(0, "f32", q)
-    hit = np.zeros((5, 4), bool)
-    hit[2, 1] = hit[4, 0] = True
+    r.step(g, dtype, [a], [70])
+    r.step(g, dtype, [a], [n])
+    q = g.standard_normal((n, 4, 64)).astype(np.float32)
+    clean = r.attend(0, dtype, q)
+    q[2, 1, 3], q[4, 0, 0], q[n - 1, 3, 63] = np.nan, np.inf, -np.inf
+    got = r.attend(0, dtype, q)
+    hit = np.zeros((n, 4), bool)
+    hit[2, 1] = hit[4, 0] = hit[n - 1, 3] = True
     assert (got[~hit].view(np.uint32) == clean[~hit].view(np.uint32)).all()
     assert np.isnan(got[hit]).all()
+
+
+@pytest.mark.parametrize("n", [1, 50])
+def test_results_in_place_of_queries(rig, n):
+    r = rig(dim=64, heads=4, kv_heads=2, pages=40)
+    g = np.random.default_rng(8)
+    a = r.create()
+    r.step(g, "bf16", [a], [900])
+    r.step(g, "bf16", [a], [n])
+    q = g.standard_normal((n, 4, 64)).astype(np.float32)
+    want = r.attend(0, "bf16", q)
+    raw = encode(q, "bf16")[0].reshape(-1)
+    b = r.put(raw)
+    r.kv.attention_device(0, "bf16", n, b.address, b.address)
+    assert (decode(b.download(np.uint16, raw.size), "bf16").reshape(q.shape) == want).all()
+
+
+def test_later_tokens_of_any_size_do_not_reach_earlier_rows(rig):
+    """Keys and values behind a row's position, 10^20 times as large as those
+    before, in its page and its tile: its result is that of the tokens it sees."""
+    r = rig(dim=64, heads=2, kv_heads=1, pages=40)
+    g = np.random.default_rng(9)
+    for start in (16, 64, 80):  # blocks of their own
+        a, n = r.create(), start + 40
+        k, v = g.standard_normal((n, 1, 64)), g.standard_normal((n, 1, 64))
+        k[start:] *= 1e10
+        v[start:] *= 1e20
+        r.kv.step([a], [n])
+        r.append(0, "f32", [a], [n], k, v)
+        q = g.standard_normal((n, 2, 64)).astype(np.float32)
+        for dtype in ("f32", "bf16"):
+            qd = encode(q, dtype)[1]
+            got = r.attend(0, dtype, qd)[:start]
+            want, mag, prod, total, vtop = r.model.attend(a, 0, qd, 0.125)
+            bound = attention_bound(dtype, mag[:start], prod[:start], total, vtop[:start], 64)
+            assert vtop[:start].max() < 1e3 and (np.abs(got - want[:start]) <= bound).all(), (start, dtype)
+        r.free(a)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 127, 3e38, float("inf"), -1.0])
+def test_scales_out_of_range_are_refused(rig, ctx, scale):
+    r = rig(dim=64, pages=4)
+    a = r.create()
+    r.kv.step([a], [1])
+    x = np.zeros((1, 2, 64), np.float32)
+    r.append(0, "f32", [a], [1], x, x)
+    b = ctx.malloc(1 << 12)
+    with pytest.raises(ValueError, match="below 2\\^127"):
+        r.kv.attention_device(0, "f32", 1, b.address, b.address, scale=scale)
+    b.free()
 
 
 def test_what_lies_behind_a_sequence_does_not_matter(rig):
