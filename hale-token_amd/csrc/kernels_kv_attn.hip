@@ -813,9 +813,12 @@ hipError_t launch_kv_attend_many(const KvAttnArgs& a, unsigned grid, hipStream_t
   HALE_KV_SIZED(many_sized, Bf16, grid, st)
 }
 
-hipError_t launch_kv_join(const KvAttnArgs& a, unsigned grid, unsigned rows, hipStream_t st) {
+hipError_t launch_kv_join(const KvAttnArgs& a, unsigned grid, unsigned rows, unsigned parts, hipStream_t st) {
   if (grid == 0) return hipSuccess;
-  if (a.kind == 0) return launch(k_kv_join, dim3(grid, rows), 256, 0, st, a);
+  // (with the attention, by row / rows together: 16 sequences of 1000, 4 parts 13.3 / 11.9 us;
+  // of 6000, 8 parts 25.1 / 24.1; 4 of 3000, 12 parts 11.5 / 11.7; one of 131000, 512 parts
+  // 31.1 / 54.5.  Many rows are the more work-groups: 300 behind 8000 102 / 68.)
+  if (a.kind == 0 && parts > 8) return launch(k_kv_join, dim3(grid, rows), 256, 0, st, a);
   const unsigned per = a.g.hd <= 64 ? 16 : a.g.hd <= 128 ? 8 : 4;
   return launch(k_kv_join_rows, dim3(grid, (rows + per - 1) / per), 256, 0, st, a);
 }

@@ -62,7 +62,7 @@ __host__ __device__ inline unsigned kv_value_byte(unsigned t, unsigned d) {
 // the other (16-byte aligned, multiples of four words), each to its own place;
 // npairs changes (index, value) of the page table; and ncopies pages to copy, none of
 // them written that is read.
-constexpr int KV_MAX_PIECES = 24;
+constexpr int KV_MAX_PIECES = 40;
 struct KvUploadArgs {
   const uint32_t* src;
   int pieces;
@@ -122,7 +122,7 @@ hipError_t launch_kv_attend_few(const KvAttnArgs& a, int cols, unsigned grid, hi
 // Of many rows: kv_many_rows per work-group.
 hipError_t launch_kv_attend_many(const KvAttnArgs& a, unsigned grid, hipStream_t st);
 // Joins of one kind, of at most `rows` rows each.
-hipError_t launch_kv_join(const KvAttnArgs& a, unsigned grid, unsigned rows, hipStream_t st);
+hipError_t launch_kv_join(const KvAttnArgs& a, unsigned grid, unsigned rows, unsigned parts, hipStream_t st);
 
 // ---- rotary positions --------------------------------------------------------
 

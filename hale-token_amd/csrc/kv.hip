@@ -173,19 +173,21 @@ struct Staging {
 };
 constexpr int STAGINGS = 32;
 
-struct View {  // the plan of the current step under one window
+constexpr int MAX_VIEWS = 2 * HALE_KV_MAX_WINDOWS;
+struct View {  // the plan of the current step under one window, for f32 or the half types
   size_t window = 0;
+  bool f32 = false;
   KvPlan plan;
 };
 
 // Sections of the plan's device buffer, in 32-bit words (multiples of four).
 // Their places hold until the buffer grows, so captured kernels keep them.
 struct Sections {
-  size_t counts = 0, positions = 0, blocks = 0, items[HALE_KV_MAX_WINDOWS] = {},  // few, `many` words on many
-         many = 0, joins[HALE_KV_MAX_WINDOWS] = {},                         // likewise
+  size_t counts = 0, positions = 0, blocks = 0, items[MAX_VIEWS] = {},  // few, `many` words on many
+         many = 0, joins[MAX_VIEWS] = {},                         // likewise
          many_joins = 0, words = 0;
 };
-constexpr size_t COUNT_WORDS = 4 + 4 * HALE_KV_MAX_WINDOWS;  // blocks; then few, many and their joins per window
+constexpr size_t COUNT_WORDS = 4 + 4 * MAX_VIEWS;  // blocks; then few, many and their joins per view
 
 }  // namespace
 
@@ -211,7 +213,7 @@ struct hale_kv_cache {
   uint64_t step_shape = 0;
   std::vector<KvStepSeq> seqs;
   std::vector<KvCopy> copies;  // pages that the next upload copies
-  View views[HALE_KV_MAX_WINDOWS];
+  View views[MAX_VIEWS];
   int nviews = 0;
 };
 
@@ -324,7 +326,7 @@ static Sections sections(const hale_kv_cache* kv, size_t tokens) {
   size_t w = COUNT_WORDS;
   s.positions = w, w += round_up(tokens, 4);
   s.blocks = w, w += round_up(kv_max_blocks(tokens, n) * sizeof(KvBlock) / 4, 4);
-  for (int v = 0; v < HALE_KV_MAX_WINDOWS; v++) {
+  for (int v = 0; v < MAX_VIEWS; v++) {
     s.items[v] = w, w += 2 * s.many;
     s.joins[v] = w, w += 2 * s.many_joins;
   }
@@ -661,7 +663,7 @@ extern "C" int hale_kv_step(hale_kv_cache* kv, size_t nseq, const uint32_t* seqs
   size_t bytes = tokens * 4 + blocks.size() * sizeof(KvBlock) + 64;
   bytes += kv->pages.step_changes() * 8 + kv->pages.step_copies() * sizeof(KvCopy);
   for (int i = 0; i < kv->nviews; i++) {
-    kv_plan(kv->shape, kv->seqs, kv->views[i].window, &kv->views[i].plan);
+    kv_plan(kv->shape, kv->seqs, kv->views[i].window, kv->views[i].f32, &kv->views[i].plan);
     bytes += view_bytes(kv->views[i]);
   }
   Upload u(kv);
@@ -783,14 +785,22 @@ extern "C" int hale_kv_attention_device(hale_kv_cache* kv, size_t layer, int dty
   if (rc || ntok == 0) return rc;
   if (window >= kv->pages.max_len()) window = 0;  // sees everything
   int i = 0;
-  while (i < kv->nviews && kv->views[i].window != window) i++;
+  const bool f32 = dtype == HALE_F32;
+  while (i < kv->nviews && (kv->views[i].window != window || kv->views[i].f32 != f32)) i++;
   if (i == kv->nviews) {
-    if (i == HALE_KV_MAX_WINDOWS)
+    int windows = 0;  // others than this one
+    for (int k = 0; k < i; k++) {
+      bool counted = kv->views[k].window == window;
+      for (int j = 0; j < k; j++) counted |= kv->views[j].window == kv->views[k].window;
+      windows += !counted;
+    }
+    if (windows == HALE_KV_MAX_WINDOWS)
       return ctx_fail(c, HALE_EINVAL, "kv_attention: window %zu is a fifth one (at most %d)", window, HALE_KV_MAX_WINDOWS);
-    if (cap) return ctx_fail(c, HALE_EINVAL, "kv_attention: first call with window %zu in a capture; make it once before", window);
+    if (cap) return ctx_fail(c, HALE_EINVAL, "kv_attention: first call with window %zu and this type in a capture; make it once before", window);
     View& v = kv->views[i];
     v.window = window;
-    kv_plan(kv->shape, kv->seqs, window, &v.plan);
+    v.f32 = f32;
+    kv_plan(kv->shape, kv->seqs, window, f32, &v.plan);
     Upload u(kv);
     rc = u.begin(upload_bytes(kv, view_bytes(v)));
     if (rc) return rc;
@@ -823,8 +833,9 @@ extern "C" int hale_kv_attention_device(hale_kv_cache* kv, size_t layer, int dty
     return (unsigned)std::min<size_t>(cap && now ? std::max(now, std::min<size_t>(most, KV_FEW_GROUPS)) : now, 1u << 20);
   };
   const size_t tiles = kv_max_items(kv->shape, ntok, kv->seqs.size()) - KV_MAX_PARTS;
+  const size_t limit = kv_few_limit(kv->shape, kv->seqs, f32);
   bool few = false, many = false;
-  for (const KvStepSeq& s : kv->seqs) (s.ntok * kv->shape.group() <= kv_few_rows(kv->shape.head_dim) ? few : many) |= s.ntok > 0;
+  for (const KvStepSeq& s : kv->seqs) (s.ntok * kv->shape.group() <= limit ? few : many) |= s.ntok > 0;
   for (int kind = 0; kind < 2; kind++) {
     if (!(kind ? many : few)) continue;
     const size_t nitems = (kind ? v.plan.many : v.plan.few).size(), njoins = (kind ? v.plan.many_joins : v.plan.few_joins).size();
@@ -836,7 +847,9 @@ extern "C" int hale_kv_attention_device(hale_kv_cache* kv, size_t layer, int dty
     const unsigned gi = grid(nitems, tiles + KV_MAX_PARTS), gj = cap ? (unsigned)std::min<size_t>(tiles, 256) : grid(njoins, 0);
     const unsigned rows = kind ? (unsigned)kv_many_rows(kv->shape.head_dim) : 16u * v.plan.cols;
     KV_LAUNCH(c, K_KV_ATTENTION, kind ? launch_kv_attend_many(a, gi, c->stream) : launch_kv_attend_few(a, v.plan.cols, gi, c->stream));
-    KV_LAUNCH(c, K_KV_ATTENTION, launch_kv_join(a, gj, rows, c->stream));
+    unsigned parts = 0;  // of a row, now
+    for (const KvJoin& j : kind ? v.plan.many_joins : v.plan.few_joins) parts = std::max(parts, j.parts);
+    KV_LAUNCH(c, K_KV_ATTENTION, launch_kv_join(a, gj, rows, parts, c->stream));
   }
   return HALE_OK;
   KV_CATCH(c)

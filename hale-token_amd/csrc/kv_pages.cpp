@@ -278,7 +278,9 @@ size_t count_pages(const std::vector<Tile>& tiles) {
 // Most pages of an item of many rows.  The work-groups that run at once take the
 // items in rounds; with the longest tile cut into 1, 2, .. parts, the time is about
 // the rounds times an item's mean pages (at least the longest item), and a
-// part costs about four pages for its partial result.  The cut of the least time.
+// part costs about four pages for its partial result.  The cut of the least time
+// (4 heads of 128, bf16: 300 tokens behind 8000 67.6 us, uncut 214.6; 64 behind 16000 39.4,
+// uncut 404.9; 2048 behind 4000 are not cut).
 size_t many_each(const std::vector<Tile>& tiles) {
   const size_t total = count_pages(tiles), least = ceil_div(total, KV_MANY_GROUPS);
   size_t longest = 0, best = 0;
@@ -307,7 +309,8 @@ size_t many_each(const std::vector<Tile>& tiles) {
 
 // Work-group i runs on accelerator die i % 8, each of which has its own L2: the
 // items of one sequence and head, which read the same pages, go to one die (or
-// as few as keep all eight busy), the longest first.
+// as few as keep all eight busy), the longest first (bf16, 4 heads of 128: 2048 tokens
+// behind 4000 192 us, 225 in the order of the tiles; two prompts of 1000 36.5, 45.1).
 void spread(std::vector<KvItem>* items) {
   constexpr size_t DIES = 8;
   if (items->size() < 2 * DIES) return;
@@ -336,20 +339,40 @@ void spread(std::vector<KvItem>* items) {
 
 }  // namespace
 
-void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window, KvPlan* out) {
+// A work-group of few rows reads its pages for up to 32 rows, one of many for up to 128, of
+// which the missing ones cost as much; but few rows run on four times as many pages at
+// once.  So few rows while their tiles leave compute units idle (4 heads of 128, 8
+// rows a token, few / many: bf16 of 64 rows, 1 sequence of 8000 = 8 tiles 15.5 / 21.9 us,
+// 2 of 4000 15.8 / 16.9, 4 of 4000 = 32 tiles 27.2 / 20.4; 24 rows, 4 of 4000 16.3 / 19.0,
+// 8 of 4000 26.4 / 21.1, 32 of 2000 42.1 / 26.4).  In f32, whose products are doubled,
+// the missing rows cost more: 32 rows at any number (8 of 4000 33.2 / 39.5), 64 as
+// above (2 of 4000 17.4 / 22.3, 4 31.1 / 25.5).
+size_t kv_few_limit(const KvShape& s, const std::vector<KvStepSeq>& seqs, bool f32) {
+  const size_t group = s.group(), rows = kv_few_rows(s.head_dim);
+  if (rows == 16) return 16;
+  size_t tiles = 0;
+  for (const KvStepSeq& q : seqs)
+    if (q.ntok * group <= 64) tiles += ceil_div(q.ntok * group, rows) * s.kv_heads;
+  return tiles < 32 ? 64 : f32 ? 32 : 16;
+}
+
+void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window, bool f32, KvPlan* out) {
   out->few.clear();
   out->many.clear();
   out->few_joins.clear();
   out->many_joins.clear();
   out->part_rows = 0;
   const size_t group = s.group(), few_rows = kv_few_rows(s.head_dim), many_rows = kv_many_rows(s.head_dim);
+  const size_t limit = kv_few_limit(s, seqs, f32);
   size_t most = 0;
   for (const KvStepSeq& q : seqs)
-    if (q.ntok * group <= few_rows) most = std::max(most, q.ntok * group);
+    if (q.ntok * group <= limit) most = std::max(most, q.ntok * group);
+  // a second group of 16 rows costs though it be empty: 32 bf16 sequences of 4000, 8 rows
+  // each, 33.6 us with one, 44.0 with two
   out->cols = most <= 16 ? 1 : 2;
   std::vector<Tile> few, many;
   for (const KvStepSeq& q : seqs) {
-    const bool is_few = q.ntok * group <= few_rows;
+    const bool is_few = q.ntok * group <= limit;
     const size_t rows = is_few ? few_rows : many_rows;
     for (uint32_t h = 0; h < s.kv_heads; h++)
       // the rows with the most pages first, so that the last work-groups are short
@@ -360,7 +383,10 @@ void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window
         (is_few ? few : many).push_back({&q, h, (uint32_t)r, (uint32_t)n, (uint32_t)page0, (uint32_t)(high / KV_PAGE + 1)});
       }
   }
-  // few rows: a work-group's waves take a page each, fewer than four leave some idle
+  // few rows: a work-group's waves take a page each, fewer than four leave some idle; eight
+  // pages at least instead of four take longer (1 x 4096 f32 12.9 us for 11.2), as do
+  // 256 or 1024 groups for 512 (32 of 200 to 8000 40.7 and 41.5 us for 39.5, one of
+  // 131000 30.0 and 38.2 for 31.1)
   divide(few, std::max<size_t>(4, ceil_div(count_pages(few), KV_FEW_GROUPS)), 16 * (size_t)out->cols, &out->few, &out->few_joins,
          &out->part_rows);
   if (!many.empty()) divide(many, many_each(many), many_rows, &out->many, &out->many_joins, &out->part_rows);

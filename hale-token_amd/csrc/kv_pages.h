@@ -80,16 +80,21 @@ struct KvShape {
 constexpr size_t KV_FEW_GROUPS = 512, KV_MANY_GROUPS = 512;
 constexpr size_t KV_MAX_PARTS = 2 * (KV_FEW_GROUPS + KV_MANY_GROUPS);
 
-// Rows per work-group for sequences of few rows, at most, and of many.
+// Rows per work-group of the kernel of few rows, at most, and of that of many.
 inline size_t kv_few_rows(size_t head_dim) { return head_dim <= 128 ? 32 : 16; }
 inline size_t kv_many_rows(size_t head_dim) { return head_dim <= 128 ? 128 : 64; }
 inline size_t kv_part_rows(size_t head_dim) {
   return 2 * KV_FEW_GROUPS * kv_few_rows(head_dim) + 2 * KV_MANY_GROUPS * kv_many_rows(head_dim);
 }
 
+// Most rows of a sequence that the kernel of few rows takes in this step (f32: type of
+// queries and results).  Of tokens per sequence only, so that a captured launch
+// holds for all later steps of as many.
+size_t kv_few_limit(const KvShape& s, const std::vector<KvStepSeq>& seqs, bool f32);
+
 // Divides the attention of a step: tiles of rows, and few enough pages each
 // that all compute units take part.  Window 0 sees every earlier position.
-void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window, KvPlan* out);
+void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window, bool f32, KvPlan* out);
 
 // The blocks that a step's tokens touch.
 void kv_blocks(const std::vector<KvStepSeq>& seqs, size_t max_pages, std::vector<KvBlock>* out);

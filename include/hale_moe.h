@@ -717,8 +717,8 @@ const char *hale_kernel_name(int kind);
  *     not freed, until the last of those graphs is destroyed, so an older
  *     graph replays correctly after a larger call.
  *   - Matrices, layers and attention blocks a graph uses must outlive it.
- *   - hale_kv_append_device and hale_kv_attention_device may be captured (call
- *     each window once before).  A launch then works on the cache's step of
+ *   - hale_kv_append_device and hale_kv_attention_device may be captured (call each
+ *     window, for f32 or the half types, once before).  A launch works on the step of
  *     that moment, which must have the same tokens per sequence as the captured
  *     one (lengths and pages may differ); hale_graph_launch is refused
  *     (HALE_EINVAL) for another step, or once the cache's buffers grew or the

@@ -202,7 +202,10 @@ void plans() {
     }
     const size_t window = below(2) ? 0 : 1 + below(below(2) ? 100 : 5000);
     KvPlan plan;
-    kv_plan(s, seqs, window, &plan);
+    const bool f32 = below(2);
+    kv_plan(s, seqs, window, f32, &plan);
+    const size_t limit = kv_few_limit(s, seqs, f32);
+    CHECK(limit >= 16 && limit <= 64 && (s.head_dim <= 128 || limit == 16));
     CHECK(plan.cols >= 1 && 16 * (size_t)plan.cols <= kv_few_rows(s.head_dim));
     CHECK(plan.few.size() + plan.many.size() <= kv_max_items(s, tok, seqs.size()));
     CHECK(plan.few_joins.size() + plan.many_joins.size() + KV_MAX_PARTS <= kv_max_items(s, tok, seqs.size()));
@@ -230,7 +233,7 @@ void plans() {
       for (const KvItem& it : kind ? plan.many : plan.few) {
         CHECK(it.row < seqs.size() && it.len0 == seqs[it.row].len0 && it.tok0 == seqs[it.row].tok0);
         const size_t all = seqs[it.row].ntok * s.group(), tile = kind ? kv_many_rows(s.head_dim) : 16 * (size_t)plan.cols;
-        CHECK((all > kv_few_rows(s.head_dim)) == (kind == 1));
+        CHECK((all > limit) == (kind == 1));
         CHECK(it.head < s.kv_heads && it.rows >= 1 && it.rows <= tile);
         CHECK(it.row0 % tile == 0 && it.row0 + it.rows <= all && (it.rows == tile || it.row0 + it.rows == all));
         CHECK(it.page0 < it.page1);
@@ -238,7 +241,7 @@ void plans() {
       }
     size_t want = 0;
     for (auto& q : seqs) {
-      const size_t all = q.ntok * s.group(), tile = all > kv_few_rows(s.head_dim) ? kv_many_rows(s.head_dim) : kv_few_rows(s.head_dim);
+      const size_t all = q.ntok * s.group(), tile = all > limit ? kv_many_rows(s.head_dim) : kv_few_rows(s.head_dim);
       want += (all + tile - 1) / tile * s.kv_heads;
     }
     CHECK(tiles.size() == want);

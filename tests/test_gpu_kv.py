@@ -351,6 +351,71 @@ def test_later_tokens_of_any_size_do_not_reach_earlier_rows(rig):
         r.free(a)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nseq, ntok, dim, window", [
+    (1, 5, 64, 0), (1, 8, 128, 0), (2, 7, 96, 150), (3, 8, 80, 0),  # 33..64 rows, few tiles
+    (9, 3, 64, 0), (9, 4, 96, 200), (9, 8, 64, 0), (8, 5, 128, 70),  # and many
+    (2, 8, 160, 0), (1, 3, 256, 90)])
+def test_rows_between_few_and_many(rig, dtype, nseq, ntok, dim, window):
+    r = rig(dim=dim, heads=32, kv_heads=4, pages=200, seqs=12)
+    g = np.random.default_rng(11)
+    seqs = [r.create() for _ in range(nseq)]
+    r.step(g, dtype, seqs, [int(n) for n in g.integers(1, 700, nseq)])
+    r.step(g, dtype, seqs, [ntok] * nseq)
+    r.check_attention(g, 0, dtype, seqs, [ntok] * nseq, window=window)
+
+
+@pytest.mark.parametrize("first, second", [("f32", "bf16"), ("f16", "f32")])
+def test_types_in_turn_on_one_cache(rig, first, second):
+    """Both types' plans of one step, kept over the next; four windows each."""
+    r = rig(dim=64, heads=32, kv_heads=4, pages=200, seqs=12)
+    g = np.random.default_rng(12)
+    seqs = [r.create() for _ in range(9)]
+    for ntok in (100, 3, 4):
+        r.step(g, first, seqs, [ntok] * 9)
+        for window in (0, 33, 65, 120):
+            for dtype in (first, second):
+                r.check_attention(g, 0, dtype, seqs, [ntok] * 9, window=window)
+    b = r.ctx.malloc(36 * 32 * 64 * 4)
+    for dtype in (first, second):
+        with pytest.raises(ValueError, match="fifth"):
+            r.kv.attention_device(0, dtype, 36, b.address, b.address, window=7)
+    b.free()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_captured_join_meets_any_number_of_parts(rig, ctx, dtype):
+    """Captured with sequences of few parts, replayed on others of many, and the other
+    way round: one of the two joins is fixed by the capture, its parts are not."""
+    for lens in ((300, 7000, 300), (7000, 300, 7000)):
+        r = rig(dim=64, heads=8, kv_heads=1, pages=260, max_len=8000)
+        g = np.random.default_rng(13)
+        r.kv.reserve(8000)
+        q = ctx.malloc(8 * 64 * 4)
+        out = ctx.malloc(8 * 64 * 4)
+        graph = None
+        for n in lens:
+            a = r.create()
+            r.step(g, dtype, [a], [n])
+            r.step(g, dtype, [a], [1])
+            raw, x = encode(g.standard_normal((1, 8, 64)).astype(np.float32), dtype)
+            q.upload(raw.reshape(-1))
+            r.kv.attention_device(0, dtype, 1, q.address, out.address)
+            eager = out.download(raw.dtype, raw.size).copy()
+            if graph is None:
+                graph = ctx.capture(lambda: r.kv.attention_device(0, dtype, 1, q.address, out.address))
+            for _ in range(2):
+                graph.launch()
+                got = decode(out.download(raw.dtype, raw.size), dtype).reshape(1, 8, 64)
+                want, mag, prod, total, vtop = r.model.attend(a, 0, x, 0.125)
+                assert (np.abs(got - want) <= attention_bound(dtype, mag, prod, total, vtop, 64)).all(), (n, lens)
+            assert np.isfinite(decode(eager, dtype)).all()
+            r.free(a)
+        graph.close()
+        q.free()
+        out.free()
+
+
 @pytest.mark.parametrize("scale", [2.0 ** 127, 3e38, float("inf"), -1.0])
 def test_scales_out_of_range_are_refused(rig, ctx, scale):
     r = rig(dim=64, pages=4)
