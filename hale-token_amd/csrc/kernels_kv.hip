@@ -104,6 +104,8 @@ __global__ __launch_bounds__(256) void k_rope(RopeArgs a) {
 }
 
 constexpr size_t ROPE_VEC_PAIRS = 1u << 18;
+// Work-groups of 256 in a grid's dimension, whose threads are counted in 32 bits.
+constexpr unsigned MAX_GROUPS = (1u << 24) - 1;
 
 template <typename T>
 static hipError_t rope_typed(const RopeArgs& a, hipStream_t st) {
@@ -118,8 +120,21 @@ static hipError_t rope_typed(const RopeArgs& a, hipStream_t st) {
     // few rows: their heads spread over more work-groups (bf16, 40 heads of 128, split / not:
     // 700 rows 4.7 / 5.6 us, 1024 5.8 / 6.8, 2048 9.8 / 9.2)
     const unsigned split = a.rows > 1024 ? 1 : (unsigned)(units + 255) / 256;
-    const dim3 grid((unsigned)a.rows, split);
-    return a.interleaved ? launch(k_rope_vec<T, true>, grid, 256, 0, st, a) : launch(k_rope_vec<T, false>, grid, 256, 0, st, a);
+    RopeArgs b = a;
+    for (size_t row = 0; row < a.rows; row += b.rows) {
+      b.rows = std::min<size_t>(a.rows - row, MAX_GROUPS);
+      b.pos = a.pos + row;
+      for (int i = 0; i < 2; i++) {
+        if (!a.heads[i]) continue;
+        b.src[i] = (const T*)a.src[i] + row * a.src_stride[i];
+        b.dst[i] = (T*)a.dst[i] + row * a.dst_stride[i];
+      }
+      const dim3 grid((unsigned)b.rows, split);
+      const hipError_t e =
+          a.interleaved ? launch(k_rope_vec<T, true>, grid, 256, 0, st, b) : launch(k_rope_vec<T, false>, grid, 256, 0, st, b);
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
   }
   const size_t total = a.rows * (size_t)(a.heads[0] + a.heads[1]) * (a.hd - a.half);
   if (total == 0) return hipSuccess;
@@ -188,7 +203,7 @@ hipError_t launch_kv_upload(const KvUploadArgs& a, hipStream_t st) {
   for (int p = 0; p < a.pieces; p++) n4 += a.words[p] / 4;
   const unsigned uploads = (n4 + a.npairs + 255) / 256 + (n4 + a.npairs == 0);
   const size_t chunks = (a.page_bytes + COPY_BYTES - 1) / COPY_BYTES;
-  const size_t most = (0x7fffffffu - uploads) / chunks;  // a grid's work-groups
+  const size_t most = (MAX_GROUPS - uploads) / chunks;
   KvUploadArgs b = a;
   for (bool first = true; first || b.ncopies; first = false) {
     const unsigned n = (unsigned)std::min<size_t>(b.ncopies, most);
@@ -318,7 +333,7 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
       __syncthreads();
       top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     } else {
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // the wave's rows, before other lanes read them
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's rows, before other lanes read them
     }
     const float s = fmaxf(had, top / 127.0f);
     const bool grown = old && s > had;
@@ -408,7 +423,11 @@ __global__ __launch_bounds__(256) void k_kv_append(KvAppendArgs a) {
       }
     }
     if (tid == 0) *scale = s;
-    if constexpr (W == 4) __syncthreads();  // the next block's rows may overwrite these
+    // the next block's rows overwrite these
+    if constexpr (W == 4)
+      __syncthreads();
+    else
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 

@@ -357,7 +357,11 @@ static int grow_plan(hale_kv_cache* kv, size_t tokens) {
   return HALE_OK;
 }
 
-static int make_pool(hale_ctx* c, size_t bytes, uint8_t** out) {
+static int make_pool(hale_ctx* c, size_t page_bytes, size_t pages, uint8_t** out) {
+  *out = nullptr;
+  if (pages > (SIZE_MAX >> 8) / page_bytes)  // the product would wrap
+    return ctx_fail(c, HALE_ENOMEM, "kv: a pool of %zu pages of %zu bytes", pages, page_bytes);
+  const size_t bytes = page_bytes * pages;
   if (hipMalloc(out, bytes) != hipSuccess) {
     *out = nullptr;
     return ctx_fail(c, HALE_ENOMEM, "kv: a pool of %zu bytes", bytes);
@@ -418,7 +422,7 @@ extern "C" int hale_kv_create(hale_ctx* c, size_t layers, size_t heads, size_t k
   g.layer_bytes = (size_t)g.head_bytes * kv_heads;
   g.page_bytes = g.layer_bytes * layers;
   g.max_pages = (unsigned)row;
-  rc = make_pool(c, g.page_bytes * num_pages, &g.pool);
+  rc = make_pool(c, g.page_bytes, num_pages, &g.pool);
   const size_t part_rows = kv_part_rows(hd);
   if (!rc && (hipMalloc(&kv->table, row * max_seqs * 4) != hipSuccess ||
               hipMalloc(&kv->part_o, part_rows * hd * 4) != hipSuccess ||
@@ -572,7 +576,7 @@ extern "C" int hale_kv_resize(hale_kv_cache* kv, size_t num_pages) {
   rc = hale_kv_compact(kv, nullptr);
   if (rc) return rc;
   uint8_t* pool = nullptr;
-  rc = make_pool(c, kv->geom.page_bytes * num_pages, &pool);
+  rc = make_pool(c, kv->geom.page_bytes, num_pages, &pool);
   if (rc) return rc;
   hipError_t e = hipSuccess;
   if (used) e = launch_copy(pool, kv->geom.pool, used * kv->geom.page_bytes / 16, c->stream);

@@ -80,6 +80,11 @@ KvPages::Status KvPages::fork(uint32_t seq, size_t n, uint32_t* out, std::string
   const size_t np = seqs_[seq].pages.size();
   dirty.reserve(dirty.size() + n * np);
   for (size_t i = 0; i < n; i++) seqs_[free_seqs_[free_seqs_.size() - 1 - i]].pages.reserve(np);
+  if (dirty.size() > settled_) {  // forks without a step between: each entry once
+    std::sort(dirty.begin(), dirty.end());
+    dirty.erase(std::unique(dirty.begin(), dirty.end()), dirty.end());
+    settled_ = 2 * dirty.size() + 65536;
+  }
   for (size_t i = 0; i < n; i++) {
     uint32_t id = 0;
     (void)create(&id, err);

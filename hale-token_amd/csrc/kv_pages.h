@@ -172,6 +172,7 @@ class KvPages {
   std::vector<uint32_t> free_seqs_;
   // check_step(): what it saw of each sequence in its last call, and its counts
   std::vector<uint32_t> mark_;
+  size_t settled_ = 65536;  // changes from which on fork() looks for repeated ones
   uint32_t stamp_ = 0;
   size_t need_ = 0, copies_ = 0;
   size_t max_len_ = 0, max_pages_ = 0;

@@ -716,7 +716,7 @@ const char *hale_kernel_name(int kind);
  *     later call outgrows while any graph of the context exists is kept,
  *     not freed, until the last of those graphs is destroyed, so an older
  *     graph replays correctly after a larger call.
- *   - Matrices, layers and attention blocks a graph uses must outlive it.
+ *   - Matrices, layers, attention blocks and rotary tables a graph uses must outlive it.
  *   - hale_kv_append_device and hale_kv_attention_device may be captured (call each
  *     window, for f32 or the half types, once before).  A launch works on the step of
  *     that moment, which must have the same tokens per sequence as the captured

@@ -308,9 +308,30 @@ void refusals() {
 
 }  // namespace
 
+// Forks that are freed again without a step between do not pile up changes.
+void forks_without_steps() {
+  KvPages p;
+  p.init(64, 8, 64 * KV_PAGE);
+  std::string err;
+  std::vector<KvCopy> copies;
+  uint32_t a = 0, f = 0;
+  CHECK(p.create(&a, &err) == KvPages::OK);
+  const uint32_t n = 60 * KV_PAGE;
+  CHECK(p.step(1, &a, &n, nullptr, &copies, &err) == KvPages::OK);
+  for (int k = 0; k < 20000; k++) {
+    CHECK(p.fork(a, 1, &f, &err) == KvPages::OK);
+    if (k < 19999) CHECK(p.free(f, &err) == KvPages::OK);
+    CHECK(p.dirty.size() <= 200000);
+  }
+  std::vector<char> said(8 * 64, 0);  // every entry that holds a page is among the changes
+  for (uint32_t d : p.dirty) said[d] = 1;
+  for (uint32_t j = 0; j < 60; j++) CHECK(said[a * 64 + j] && said[f * 64 + j]);
+}
+
 int main() {
   long ops = 0, refused = 0;
   refusals();
+  forks_without_steps();
   plans();
   random_walk(12, 6, 300, 6000, &ops, &refused);
   random_walk(40, 9, 1000, 6000, &ops, &refused);

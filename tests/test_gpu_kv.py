@@ -416,6 +416,39 @@ def test_a_captured_join_meets_any_number_of_parts(rig, ctx, dtype):
         out.free()
 
 
+@pytest.mark.parametrize("ntok", [1, 40])
+def test_pages_past_4_gib(rig, ntok):
+    """Pages of 8.5 MB, the sequence's all behind byte 2^32 of the pool."""
+    r = rig(layers=64, dim=128, heads=8, kv_heads=8, pages=560, seqs=3, max_len=40000)
+    page = 64 * 8 * (64 * 128 * 2 + 128)
+    g = np.random.default_rng(14)
+    a, b = r.create(), r.create()
+    r.kv.step([a], [64 * 515])  # takes the lower pages, stores nothing
+    assert 515 * page > 1 << 32
+    n = 200
+    r.kv.step([b], [n])
+    for layer in (0, 63):
+        k, v = (g.standard_normal((n, 8, 128)) for _ in range(2))
+        r.append(layer, "bf16", [b], [n], k, v)
+    r.kv.step([b], [ntok])
+    for layer in (0, 63):
+        k, v = (g.standard_normal((ntok, 8, 128)) for _ in range(2))
+        r.append(layer, "bf16", [b], [ntok], k, v)
+        r.check_attention(g, layer, "bf16", [b], [ntok])
+    c = r.copy(b)
+    r.kv.step([c], [ntok])
+    for layer in (0, 63):
+        k, v = (g.standard_normal((ntok, 8, 128)) for _ in range(2))
+        r.append(layer, "bf16", [c], [ntok], k, v)
+        r.check_attention(g, layer, "bf16", [c], [ntok])
+
+
+def test_a_pool_past_64_bits_is_refused(ctx):
+    # 2^39 and a little bytes a page, 2^25 pages: the product wraps to little
+    with pytest.raises(MemoryError, match="pages of"):
+        H.KvCache(ctx, 4096, 4096, 4096, 256, 1 << 25, 1, 64)
+
+
 @pytest.mark.parametrize("scale", [2.0 ** 127, 3e38, float("inf"), -1.0])
 def test_scales_out_of_range_are_refused(rig, ctx, scale):
     r = rig(dim=64, pages=4)

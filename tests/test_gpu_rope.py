@@ -118,6 +118,32 @@ def test_rope_against_64_bits(ctx, case):
     rope.close()
 
 
+def test_rope_rows_past_a_grid(ctx):
+    """More rows than a grid has work-groups: rows about the edge against 64 bits."""
+    n, hd, edge = (1 << 24) + 70, 16, (1 << 24) - 1
+    rope = H.Rope(ctx, hd, 10000.0)
+    freq = np.asarray(rope.frequencies())
+    b, pos = ctx.malloc(n * hd * 2), ctx.malloc(n * 4)
+    b.upload(np.zeros(n * hd, np.uint16))
+    pos.upload(np.arange(n, dtype=np.int32))
+    x = {}
+    g = np.random.default_rng(5)
+    for first in (0, edge - 20, n - 20):
+        raw, x[first] = encode(g.standard_normal((20, hd)).astype(np.float32), "bf16")
+        b.upload(np.ascontiguousarray(raw.reshape(-1)), first * hd * 2)
+    rope.apply_device("bf16", n, pos.address, b.address, 1, b.address, 0, 0, 0)
+    for first, v in x.items():
+        v = np.asarray(v, np.float64).reshape(20, hd)
+        t = (first + np.arange(20))[:, None] * freq
+        want = np.concatenate([v[:, :8] * np.cos(t) - v[:, 8:] * np.sin(t), v[:, 8:] * np.cos(t) + v[:, :8] * np.sin(t)], 1)
+        got = decode(b.download(np.uint16, 20 * hd, first * hd * 2), "bf16").reshape(20, hd)
+        size = np.hypot(np.abs(v[:, :8]), np.abs(v[:, 8:]))
+        # result rounded by 2^-8 of it, products and cosines by a few 2^-24
+        assert (np.abs(got - want) <= np.abs(want) * 2.0 ** -8 + np.tile(size, 2) * 2.0 ** -20).all(), first
+    b.free()
+    pos.free()
+
+
 def test_rope_one_side_and_gradient(ctx):
     """Keys alone; and turning back with negative positions: the transpose, so
     <turn(x), y> = <x, turn back(y)>, and back after forth is the identity."""
