@@ -193,6 +193,14 @@ __device__ __forceinline__ void split_rows(const T (&raw)[KC][8], bool valid, in
     }
 }
 
+// A work-group's four waves take every fourth page each, for the same rows, and join
+// their results in LDS; a sequence whose pages are many is divided over work-groups too,
+// whose results the joins below put together.  The codes go from memory to registers as
+// the operands lie, a page ahead of their use.  Bound by memory: each code is read
+// once, for up to 32 rows.  bf16, heads of 128: 32 sequences of 200 to 8000 30.4 us for
+// 148 MB (4.9 TB/s), one of 131000 25.1 us for 135 MB (5.4 TB/s; a large copy, half of
+// it writes, reaches 4.85).  One of 4096 in f32 is 7.0 us for 4.3 MB, a chain of latencies: plan,
+// table, page, products, the waves' join.
 // T: type of queries and results; KC: padded head dimension / 32; C: groups of
 // 16 query rows.
 template <typename T, int KC, int C>
@@ -430,6 +438,9 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_kv_attend_few(KvAttnArgs a) 
 // registers of both for one, dimension 256 the LDS).  For f16 and bf16 the reference m
 // follows the maximum only where this is more than 2^8 above it (probabilities are then
 // up to 2^15 from 2^7), so that the sums are seldom rescaled.
+// Bound by the vector instructions beside the matrix ones: 2048 bf16 tokens behind 4000, 32
+// heads of 128 on 4, take 191 us for 169 GFLOP (882 TFLOP/s, where a large matrix
+// product reaches 1140); by the counters, at 2.4 GHz, the matrix units work for 67 of them.
 constexpr int many_waves(size_t size, int kc) { return (size == 4 ? kc == 2 || kc == 6 : kc <= 6) ? 2 : 1; }
 
 template <typename T, int KC, int C>
@@ -662,8 +673,9 @@ __global__ __launch_bounds__(256, many_waves(sizeof(T), KC)) void k_kv_attend_ma
 // Parts of one row: all of a step's at most.
 constexpr unsigned JOIN_PARTS = 2 * (KV_FEW_GROUPS > KV_MANY_GROUPS ? KV_FEW_GROUPS : KV_MANY_GROUPS);
 
-// Joins of many rows, most of few parts: a work-group takes as many rows as its
-// threads hold at four numbers each, the parts one behind the other.
+// Joins of few parts, or of many rows: a work-group takes as many rows as its
+// threads hold at four numbers each, the parts one behind the other.  A chain of three
+// reads: 5.0 us for 32 sequences of up to 7 parts, 4 rows of 128 each.
 __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a) {
   const int t = threadIdx.x;
   const int quads = a.g.hd / 4, lanes = quads <= 16 ? 16 : quads <= 32 ? 32 : 64, x = t % lanes;
@@ -695,7 +707,8 @@ __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a) {
 }
 
 // Joins the partial results of one row: a work-group, whose threads take four
-// numbers each of every so many'th part; the slices are added in their order.
+// numbers each of every so many'th part; the slices are added in their order.  16 parts
+// a slice are read while the weights are found.  5.3 us for 128 parts of 32 rows of 128.
 __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a) {
   constexpr int AHEAD = 16;
   __shared__ float sw[JOIN_PARTS];

@@ -449,6 +449,37 @@ def test_a_pool_past_64_bits_is_refused(ctx):
         H.KvCache(ctx, 4096, 4096, 4096, 256, 1 << 25, 1, 64)
 
 
+@pytest.mark.parametrize("dtype, ntok", [("bf16", [1, 40, 8]), ("f32", [3, 3, 3]), ("f16", [2] * 9), ("bf16", [3] * 9)])
+def test_captured_steps_of_every_kind_of_row(rig, ctx, dtype, ntok):
+    """Captured once, replayed over longer sequences, others beside them, twice each."""
+    r = rig(dim=64, heads=16, kv_heads=2, pages=260, seqs=12, max_len=8000)
+    g = np.random.default_rng(15)
+    r.kv.reserve(20000)
+    seqs, total = [r.create() for _ in ntok], sum(ntok)
+    q, out = ctx.malloc(total * 16 * 64 * 4), ctx.malloc(total * 16 * 64 * 4)
+    graph = None
+    for grow in (5, 700, 60):
+        r.step(g, dtype, seqs, [grow + 3 * i for i in range(len(seqs))])
+        r.step(g, dtype, seqs, ntok)
+        raw, x = encode(g.standard_normal((total, 16, 64)).astype(np.float32), dtype)
+        q.upload(raw.reshape(-1))
+        call = lambda: r.kv.attention_device(0, dtype, total, q.address, out.address, window=300)
+        call()
+        graph = graph or ctx.capture(call)
+        for _ in range(2):
+            out.upload(np.full(raw.size, 9, raw.dtype))
+            graph.launch()
+            got = decode(out.download(raw.dtype, raw.size), dtype).reshape(total, 16, 64)
+            at = 0
+            for s, m in zip(seqs, ntok):
+                want, mag, prod, tot, vtop = r.model.attend(s, 0, x[at:at + m], 0.125, 300)
+                assert (np.abs(got[at:at + m] - want) <= attention_bound(dtype, mag, prod, tot, vtop, 64)).all(), (grow, s)
+                at += m
+    graph.close()
+    q.free()
+    out.free()
+
+
 @pytest.mark.parametrize("scale", [2.0 ** 127, 3e38, float("inf"), -1.0])
 def test_scales_out_of_range_are_refused(rig, ctx, scale):
     r = rig(dim=64, pages=4)
