@@ -62,7 +62,6 @@ __host__ __device__ inline unsigned kv_value_byte(unsigned t, unsigned d) {
 // the other (16-byte aligned, multiples of four words), each to its own place;
 // npairs changes (index, value) of the page table; and ncopies pages to copy, none of
 // them written that is read.
-constexpr int KV_MAX_PIECES = 40;
 struct KvUploadArgs {
   const uint32_t* src;
   int pieces;

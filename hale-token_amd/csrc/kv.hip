@@ -173,7 +173,6 @@ struct Staging {
 };
 constexpr int STAGINGS = 32;
 
-constexpr int MAX_VIEWS = 2 * HALE_KV_MAX_WINDOWS;
 struct View {  // the plan of the current step under one window, for f32 or the half types
   size_t window = 0;
   bool f32 = false;
@@ -183,11 +182,11 @@ struct View {  // the plan of the current step under one window, for f32 or the 
 // Sections of the plan's device buffer, in 32-bit words (multiples of four).
 // Their places hold until the buffer grows, so captured kernels keep them.
 struct Sections {
-  size_t counts = 0, positions = 0, blocks = 0, items[MAX_VIEWS] = {},  // few, `many` words on many
-         many = 0, joins[MAX_VIEWS] = {},                         // likewise
+  size_t counts = 0, positions = 0, blocks = 0, items[KV_MAX_VIEWS] = {},  // few, `many` words on many
+         many = 0, joins[KV_MAX_VIEWS] = {},                         // likewise
          many_joins = 0, words = 0;
 };
-constexpr size_t COUNT_WORDS = 4 + 4 * MAX_VIEWS;  // blocks; then few, many and their joins per view
+constexpr size_t COUNT_WORDS = 4 + 4 * KV_MAX_VIEWS;  // blocks; then few, many and their joins per view
 
 }  // namespace
 
@@ -213,7 +212,7 @@ struct hale_kv_cache {
   uint64_t step_shape = 0;
   std::vector<KvStepSeq> seqs;
   std::vector<KvCopy> copies;  // pages that the next upload copies
-  View views[MAX_VIEWS];
+  View views[KV_MAX_VIEWS];
   int nviews = 0;
 };
 
@@ -229,6 +228,7 @@ struct Upload {
   Staging* s = nullptr;
   KvUploadArgs a{};
   size_t used = 0;
+  bool refused = false;  // a piece that there is no room for
   explicit Upload(hale_kv_cache* k) : kv(k) {}
 
   int begin(size_t bytes) {
@@ -250,25 +250,25 @@ struct Upload {
     }
     return HALE_OK;
   }
-  // room for `words` words (a multiple of four) that go to dst
-  uint32_t* piece(void* dst, size_t words) {
-    uint32_t* p = (uint32_t*)(s->base + used);
-    if (words) {
-      a.dst[a.pieces] = (uint32_t*)dst;
-      a.words[a.pieces++] = (unsigned)words;
-      used += words * 4;
-    }
-    return p;
-  }
+  // bytes that go to dst, as a piece of whole quads of words
   void put(void* dst, const void* src, size_t bytes) {
     const size_t words = round_up(bytes, 16) / 4;
-    uint32_t* p = piece(dst, words);
-    if (bytes) std::memcpy(p, src, bytes);
-    if (words * 4 > bytes) std::memset((char*)p + bytes, 0, words * 4 - bytes);
+    if (!words) return;
+    if (a.pieces == KV_MAX_PIECES || used + words * 4 > s->bytes) {
+      refused = true;
+      return;
+    }
+    char* p = s->base + used;
+    std::memcpy(p, src, bytes);
+    std::memset(p + bytes, 0, words * 4 - bytes);
+    a.dst[a.pieces] = (uint32_t*)dst;
+    a.words[a.pieces++] = (unsigned)words;
+    used += words * 4;
   }
   int end() {
     hale_ctx* c = kv->ctx;
     auto& dirty = kv->pages.dirty;
+    if (refused) return ctx_fail(c, HALE_EHIP, "kv: a plan of more than %d pieces", KV_MAX_PIECES);
     uint32_t* pairs = (uint32_t*)(s->base + used);
     for (size_t i = 0; i < dirty.size(); i++) {
       pairs[2 * i] = dirty[i];
@@ -326,7 +326,7 @@ static Sections sections(const hale_kv_cache* kv, size_t tokens) {
   size_t w = COUNT_WORDS;
   s.positions = w, w += round_up(tokens, 4);
   s.blocks = w, w += round_up(kv_max_blocks(tokens, n) * sizeof(KvBlock) / 4, 4);
-  for (int v = 0; v < MAX_VIEWS; v++) {
+  for (int v = 0; v < KV_MAX_VIEWS; v++) {
     s.items[v] = w, w += 2 * s.many;
     s.joins[v] = w, w += 2 * s.many_joins;
   }

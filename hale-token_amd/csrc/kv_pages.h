@@ -10,6 +10,8 @@
 #include <string>
 #include <vector>
 
+#include "../../include/hale_moe.h"
+
 namespace hale {
 
 constexpr size_t KV_PAGE = 64;   // positions per page (HALE_KV_PAGE)
@@ -68,6 +70,13 @@ struct KvPlan {
 struct KvCopy {
   uint32_t src, dst;
 };
+
+// The plans that a cache keeps: of each window, for f32 and for the half types.
+constexpr int KV_MAX_VIEWS = 2 * HALE_KV_MAX_WINDOWS;
+// Pieces that a step's upload is put together from, at most: its counts, positions and
+// blocks, and the counts, items and joins (of few and of many rows) of each view.
+constexpr int KV_STEP_PIECES = 3, KV_VIEW_PIECES = 5;
+constexpr int KV_MAX_PIECES = KV_STEP_PIECES + KV_MAX_VIEWS * KV_VIEW_PIECES;
 
 struct KvShape {
   size_t heads, kv_heads, head_dim;

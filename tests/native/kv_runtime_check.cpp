@@ -1,0 +1,95 @@
+// Runs the key/value cache's host side (hale-token_amd/csrc/kv.hip) over a HIP
+// runtime in host memory (kv_fake_hip.h), under AddressSanitizer and
+// UndefinedBehaviorSanitizer.  The argument names the check; exits 1 with a
+// message where it fails.
+#include "kv_fake_hip.h"
+
+using namespace hale;
+
+namespace {
+
+struct Cache {
+  hale_ctx c;
+  hale_kv_cache* kv = nullptr;
+  explicit Cache(size_t layers = 1, size_t heads = 4, size_t kv_heads = 2, size_t dim = 16, size_t pages = 64, size_t seqs = 8,
+                 size_t max_len = 1024) {
+    CHECK(hale_kv_create(&c, layers, heads, kv_heads, dim, pages, seqs, max_len, &kv) == HALE_OK);
+  }
+  ~Cache() { hale_kv_destroy(kv); }
+  uint32_t seq() {
+    uint32_t s = 0;
+    CHECK(hale_kv_seq_create(kv, &s) == HALE_OK);
+    return s;
+  }
+  int step(std::vector<uint32_t> seqs, std::vector<uint32_t> n) { return hale_kv_step(kv, seqs.size(), seqs.data(), n.data()); }
+  int append(size_t ntok) {
+    static float x[4];
+    return hale_kv_append_device(kv, 0, HALE_F32, ntok, x, 1 << 20, x, 1 << 20);
+  }
+  int attend(size_t ntok, int dtype = HALE_F32, size_t window = 0) {
+    static float x[4];
+    return hale_kv_attention_device(kv, 0, dtype, ntok, x, 1 << 20, 1.0f, window, x, 1 << 20);
+  }
+  size_t len(uint32_t s) {
+    size_t n = 0;
+    CHECK(hale_kv_seq_len(kv, s, &n) == HALE_OK);
+    return n;
+  }
+  size_t used() {
+    size_t n = 0;
+    CHECK(hale_kv_pages(kv, nullptr, &n) == HALE_OK);
+    return n;
+  }
+};
+
+// A step of one token and of a prompt's chunk, both behind long contexts, after
+// four windows were attended over in both kinds of type: every list of
+// every view has entries, and each arrives where the kernels read it.
+void every_view() {
+  const KvShape shape{32, 4, 128};
+  const size_t windows[4] = {0, 1024, 2048, 4096}, lens[2] = {9000, 8000};
+  const uint32_t ntok[2] = {1, 300};
+  Cache w(1, 32, 4, 128, 300, 2, 12000);
+  const uint32_t a = w.seq(), b = w.seq();
+  CHECK(w.step({a, b}, {(uint32_t)lens[0], (uint32_t)lens[1]}) == HALE_OK);
+  const size_t total = lens[0] + lens[1];
+  for (int dtype : {HALE_F32, HALE_BF16})
+    for (size_t window : windows) CHECK(w.attend(total, dtype, window) == HALE_OK);
+  CHECK(w.step({a, b}, {ntok[0], ntok[1]}) == HALE_OK);
+  CHECK(w.append(301) == HALE_OK);
+  const std::vector<KvStepSeq> seqs = {{a, (uint32_t)lens[0], ntok[0], 0}, {b, (uint32_t)lens[1], ntok[1], 1}};
+  int full = 0;
+  for (int dtype : {HALE_F32, HALE_BF16})
+    for (size_t window : windows) {
+      fake.attends.clear();
+      const int uploads = fake.uploads;
+      CHECK(w.attend(301, dtype, window) == HALE_OK);
+      CHECK(fake.uploads == uploads && fake.attends.size() == 2);
+      KvPlan plan;
+      kv_plan(shape, seqs, window, dtype == HALE_F32, &plan);
+      full += !plan.few.empty() && !plan.many.empty() && !plan.few_joins.empty() && !plan.many_joins.empty();
+      const uint32_t counts[4] = {(uint32_t)plan.few.size(), (uint32_t)plan.many.size(), (uint32_t)plan.few_joins.size(),
+                                  (uint32_t)plan.many_joins.size()};
+      for (int kind = 0; kind < 2; kind++) {
+        const KvAttnArgs& at = fake.attends[kind];
+        const auto& items = kind ? plan.many : plan.few;
+        const auto& joins = kind ? plan.many_joins : plan.few_joins;
+        CHECK(at.kind == kind && !memcmp(at.counts, counts, sizeof counts));
+        CHECK(!memcmp(at.items, items.data(), items.size() * sizeof(KvItem)));
+        CHECK(!memcmp(at.joins, joins.data(), joins.size() * sizeof(KvJoin)));
+      }
+    }
+  CHECK(full == 8);
+}
+
+}  // namespace
+
+int main(int argc, char** argv) {
+  const std::string what = argc > 1 ? argv[1] : "";
+  if (what == "every_view")
+    every_view();
+  else
+    return 2;
+  CHECK(fake.device.empty() && fake.host.empty());
+  return 0;
+}
