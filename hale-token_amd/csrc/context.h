@@ -78,6 +78,24 @@ struct hale_ctx {
   std::vector<hale::KvUse> kv_uses;
 };
 
+namespace hale {
+
+// Device memory that a call has outgrown: freed at once, or kept until the last
+// graph of the context is destroyed when a graph may still use it.
+inline void ctx_release(hale_ctx* c, void* p) {
+  if (!p) return;
+  if (c->live_graphs == 0) {
+    (void)hipFree(p);
+    return;
+  }
+  try {
+    c->retired.push_back(p);
+  } catch (...) {  // no room to remember it: it stays for good
+  }
+}
+
+}  // namespace hale
+
 struct hale_graph {
   hale_ctx* ctx = nullptr;
   hipGraph_t graph = nullptr;

@@ -310,8 +310,8 @@ static int send_pages(hale_kv_cache* kv) {
 }
 
 static void free_device(hale_kv_cache* kv) {
-  for (void* p : {(void*)kv->geom.pool, (void*)kv->table, (void*)kv->plan, (void*)kv->part_o, (void*)kv->part_ml})
-    (void)hipFree(p);
+  for (void* p : {(void*)kv->geom.pool, (void*)kv->table, (void*)kv->part_o, (void*)kv->part_ml}) (void)hipFree(p);
+  ctx_release(kv->ctx, kv->plan);
   for (Staging& s : kv->staging) {
     if (s.base) (void)hipHostFree(s.base);
   }
@@ -348,7 +348,7 @@ static int grow_plan(hale_kv_cache* kv, size_t tokens) {
   KVCHK(c, hipStreamSynchronize(c->stream));
   if (hipMalloc(&p, s.words * 4) != hipSuccess)
     return ctx_fail(c, HALE_ENOMEM, "kv: plan buffers of %zu bytes", s.words * 4);
-  (void)hipFree(kv->plan);
+  ctx_release(c, kv->plan);  // a graph's rotation may read the positions in it
   kv->plan = p;
   kv->at = s;
   kv->cap_tokens = tokens;

@@ -215,16 +215,6 @@ extern "C" int hale_ctx_synchronize(hale_ctx* c) {
   return HALE_OK;
 }
 
-// Device memory a call has outgrown: freed at once, or kept until the last
-// graph of the context is destroyed when a graph may still use it.
-static void scratch_release(hale_ctx* c, void* p) {
-  if (!p) return;
-  if (c->live_graphs > 0)
-    c->retired.push_back(p);
-  else
-    (void)hipFree(p);
-}
-
 // Scratch may only grow outside graph capture: growing synchronizes the
 // stream and allocates, which a capture cannot record.
 static int growth_allowed(hale_ctx* c, const char* what, size_t bytes) {
@@ -244,7 +234,7 @@ static int ctx_scratch(hale_ctx* c, size_t bytes, void** p) {
     int rc = growth_allowed(c, "context scratch", bytes);
     if (rc) return rc;
     HIPCHK(c, hipStreamSynchronize(c->stream));
-    scratch_release(c, c->scratch);
+    ctx_release(c, c->scratch);
     c->scratch = nullptr;
     c->scratch_bytes = 0;
     if (hipMalloc(&c->scratch, bytes) != hipSuccess)
@@ -1102,7 +1092,7 @@ static int moe_reserve(hale_moe* m, size_t ntok, TokScratch* out) {
     int rc = growth_allowed(c, "MoE layer scratch", bytes);
     if (rc) return rc;
     HIPCHK(c, hipStreamSynchronize(c->stream));
-    scratch_release(c, m->tok_base);
+    ctx_release(c, m->tok_base);
     m->tok_base = nullptr;
     m->cap_tok = 0;
     hipError_t e = hipMalloc(&m->tok_base, bytes);
@@ -1125,7 +1115,7 @@ static int moe_ws(hale_moe* m, size_t need, void** out) {
     int rc = growth_allowed(c, "MoE layer workspace", need);
     if (rc) return rc;
     HIPCHK(c, hipStreamSynchronize(c->stream));
-    scratch_release(c, m->pw.base);
+    ctx_release(c, m->pw.base);
     m->pw.base = nullptr;
     m->pw.bytes = 0;
     if (hipMalloc(&m->pw.base, need) != hipSuccess)

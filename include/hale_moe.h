@@ -629,7 +629,8 @@ int hale_kv_resize(hale_kv_cache *kv, size_t num_pages);
 int hale_kv_step(hale_kv_cache *kv, size_t nseq, const uint32_t *seqs,
                  const uint32_t *ntok);
 /* Room for steps of up to max_tokens tokens, so that none grows the plan's
- * buffers (which graphs hold: growing them makes older graphs unusable). */
+ * buffers (which graphs hold: growing them makes older graphs unusable).  Growing
+ * them ends the current step. */
 int hale_kv_reserve(hale_kv_cache *kv, size_t max_tokens);
 /* Device address of the positions of the step's tokens, [tokens] int32, for
  * hale_rope_device.  The same for every step until the buffers grow. */

@@ -82,12 +82,43 @@ void every_view() {
   CHECK(full == 8);
 }
 
+// Graphs keep the addresses that they were captured with: what a graph may still
+// read stays until the context's last graph is gone.
+void plan_behind_a_graph() {
+  hale_ctx c;
+  hale_kv_cache* kv = nullptr;
+  const int32_t *old = nullptr, *grown = nullptr;
+  CHECK(hale_kv_create(&c, 1, 4, 2, 16, 64, 8, 1024, &kv) == HALE_OK);
+  CHECK(hale_kv_positions(kv, &old) == HALE_OK);
+  const size_t before = fake.device.size();
+  c.live_graphs = 1;
+  CHECK(hale_kv_reserve(kv, 5000) == HALE_OK);
+  CHECK(hale_kv_positions(kv, &grown) == HALE_OK && grown != old);
+  CHECK(fake.device.size() == before + 1 && c.retired.size() == 1);
+  volatile int32_t at = old[0];  // as a replay reads it
+  (void)at;
+  hale_kv_destroy(kv);
+  at = old[0];
+  at = grown[0];
+  CHECK(c.retired.size() == 2 && fake.device.size() == 2);
+  for (void* p : c.retired) (void)hipFree(p);  // as the last graph's end does
+  // without a graph nothing is kept
+  c.live_graphs = 0;
+  c.retired.clear();
+  CHECK(hale_kv_create(&c, 1, 4, 2, 16, 64, 8, 1024, &kv) == HALE_OK);
+  CHECK(hale_kv_reserve(kv, 5000) == HALE_OK);
+  CHECK(c.retired.empty() && fake.device.size() == before);
+  hale_kv_destroy(kv);
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
   const std::string what = argc > 1 ? argv[1] : "";
   if (what == "every_view")
     every_view();
+  else if (what == "plan_behind_a_graph")
+    plan_behind_a_graph();
   else
     return 2;
   CHECK(fake.device.empty() && fake.host.empty());

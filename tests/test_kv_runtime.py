@@ -39,3 +39,7 @@ def check(tmp_path_factory):
 
 def test_every_list_of_every_view_in_one_step(check):
     check("every_view")
+
+
+def test_a_plan_that_was_outgrown_stays_while_graphs_exist(check):
+    check("plan_behind_a_graph")
