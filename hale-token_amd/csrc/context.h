@@ -17,14 +17,16 @@ using hale::K_KINDS;
 
 namespace hale {
 
-// One key/value cache that a captured graph stores to or attends over.  A
-// replay runs on the cache's step of that moment: it has to be a step of the
-// same tokens per sequence, and of buffers that have not moved since.
+// One key/value cache that a captured graph stores to or attends over, or whose
+// positions it rotates by.  A replay runs on the cache's step of that moment: its
+// buffers must not have moved since, and for stores and attention it has to be a step
+// of the same tokens per sequence.
 struct KvUse {
   hale_kv_cache* kv;
   uint64_t serial;  // of the cache: its address may be another's by now
-  uint64_t shape;  // what the calls' sizes follow from: tokens per sequence
   uint64_t epoch;  // counts moves of the cache's buffers
+  bool step;  // stores or attends
+  uint64_t shape;  // what those calls' sizes follow from: tokens per sequence
 };
 // HALE_OK, or why the graph cannot be replayed now (kv.hip).
 int kv_check_replay(hale_ctx* c, const std::vector<KvUse>& uses);

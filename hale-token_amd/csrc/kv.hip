@@ -114,6 +114,9 @@ extern "C" int hale_rope_frequencies(const hale_rope* r, double* freq, size_t n)
   return HALE_OK;
 }
 
+// Notes a captured rotation whose positions are those of a cache's step.
+static int note_positions(hale_ctx* c, const int32_t* pos);
+
 extern "C" int hale_rope_device(hale_rope* r, int dtype, size_t rows, const int32_t* pos, const void* q,
                                 size_t q_heads, size_t q_stride, void* q_out, size_t q_out_stride, const void* k,
                                 size_t k_heads, size_t k_stride, void* k_out, size_t k_out_stride) {
@@ -150,10 +153,14 @@ extern "C" int hale_rope_device(hale_rope* r, int dtype, size_t rows, const int3
   a.half = (int)(r->config.rotary_dim / 2);
   a.interleaved = r->config.layout == HALE_ROPE_INTERLEAVED;
   a.factor = (float)r->config.attention_factor;
+  KV_TRY
   std::lock_guard<std::recursive_mutex> lk(c->mu);
   KVCHK(c, hipSetDevice(c->device));
+  const int rc = note_positions(c, pos);
+  if (rc) return rc;
   KV_LAUNCH(c, K_ROPE, launch_rope(dtype, a, c->stream));
   return HALE_OK;
+  KV_CATCH(c)
 }
 
 // ---------------------------------------------------------------------------
@@ -708,13 +715,30 @@ static int layer_call(hale_kv_cache* kv, const char* what, size_t layer, int dty
   int rc = capturing(c, cap);
   if (rc) return rc;
   if (!*cap) return send_pages(kv);  // table changes since the step
-  for (const KvUse& u : c->kv_uses) {
+  for (KvUse& u : c->kv_uses) {
     if (u.kv != kv) continue;
-    if (u.epoch != kv->epoch || u.shape != kv->step_shape)
+    if (u.epoch != kv->epoch || (u.step && u.shape != kv->step_shape))
       return ctx_fail(c, HALE_EINVAL, "%s: the graph holds calls for another step of this cache", what);
+    u.step = true;
+    u.shape = kv->step_shape;
     return HALE_OK;
   }
-  c->kv_uses.push_back({kv, kv->serial, kv->step_shape, kv->epoch});
+  c->kv_uses.push_back({kv, kv->serial, kv->epoch, true, kv->step_shape});
+  return HALE_OK;
+}
+
+static int note_positions(hale_ctx* c, const int32_t* pos) {
+  for (hale_kv_cache* kv : c->kvs) {
+    const uintptr_t at = (uintptr_t)pos, first = (uintptr_t)(kv->plan + kv->at.positions);
+    if (at < first || at >= first + 4 * kv->cap_tokens) continue;
+    bool cap = false;
+    const int rc = capturing(c, &cap);
+    if (rc || !cap) return rc;
+    for (const KvUse& u : c->kv_uses)
+      if (u.kv == kv) return HALE_OK;
+    c->kv_uses.push_back({kv, kv->serial, kv->epoch, false, 0});
+    return HALE_OK;
+  }
   return HALE_OK;
 }
 
@@ -725,6 +749,7 @@ int hale::kv_check_replay(hale_ctx* c, const std::vector<KvUse>& uses) {
       return ctx_fail(c, HALE_EINVAL, "graph_launch: its key/value cache is gone");
     if (u.kv->epoch != u.epoch)
       return ctx_fail(c, HALE_EINVAL, "graph_launch: its key/value cache's buffers grew since the capture");
+    if (!u.step) continue;
     if (!u.kv->stepped || u.kv->step_shape != u.shape)
       return ctx_fail(c, HALE_EINVAL, "graph_launch: the key/value cache's step is not of the captured tokens per sequence");
     const int rc = send_pages(u.kv);

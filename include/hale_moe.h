@@ -633,7 +633,8 @@ int hale_kv_step(hale_kv_cache *kv, size_t nseq, const uint32_t *seqs,
  * them ends the current step. */
 int hale_kv_reserve(hale_kv_cache *kv, size_t max_tokens);
 /* Device address of the positions of the step's tokens, [tokens] int32, for
- * hale_rope_device.  The same for every step until the buffers grow. */
+ * hale_rope_device.  The same for every step until the buffers grow: from then on
+ * a graph that rotates by them is refused. */
 int hale_kv_positions(const hale_kv_cache *kv, const int32_t **d_positions);
 
 /* Stores the step's keys and values into a layer: d_k and d_v
@@ -723,7 +724,8 @@ const char *hale_kernel_name(int kind);
  *     that moment, which must have the same tokens per sequence as the captured
  *     one (lengths and pages may differ); hale_graph_launch is refused
  *     (HALE_EINVAL) for another step, or once the cache's buffers grew or the
- *     cache is gone. */
+ *     cache is gone.  A graph with hale_rope_device by hale_kv_positions and neither
+ *     of the two may be launched for any step, and is refused for the last two reasons. */
 typedef struct hale_graph hale_graph;
 int hale_graph_begin(hale_ctx *ctx);
 int hale_graph_end(hale_ctx *ctx, hale_graph **out);

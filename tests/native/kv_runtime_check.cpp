@@ -111,6 +111,55 @@ void plan_behind_a_graph() {
   hale_kv_destroy(kv);
 }
 
+// A captured rotation of the step's positions: replayed for any step, refused
+// once the positions lie elsewhere.
+void rotation_in_a_graph() {
+  Cache w;
+  const uint32_t a = w.seq();
+  hale_rope_config config{};
+  config.head_dim = config.rotary_dim = 16;
+  config.base = 1e4;
+  config.attention_factor = 1.0;
+  hale_rope* rope = nullptr;
+  CHECK(hale_rope_create(&w.c, &config, &rope) == HALE_OK);
+  const int32_t* pos = nullptr;
+  int32_t other[4] = {};
+  float x[64];
+  auto turn = [&](const int32_t* p) { return hale_rope_device(rope, HALE_F32, 2, p, x, 1, 16, x, 16, nullptr, 0, 0, nullptr, 0); };
+  CHECK(hale_kv_positions(w.kv, &pos) == HALE_OK);
+  CHECK(w.step({a}, {3}) == HALE_OK && turn(pos) == HALE_OK && w.c.kv_uses.empty());
+  fake.capturing = true;
+  CHECK(turn(other) == HALE_OK && w.c.kv_uses.empty());
+  CHECK(turn(pos) == HALE_OK && turn(pos + 1) == HALE_OK && w.c.kv_uses.size() == 1);
+  fake.capturing = false;
+  std::vector<KvUse> uses = w.c.kv_uses;
+  w.c.kv_uses.clear();
+  CHECK(kv_check_replay(&w.c, uses) == HALE_OK);
+  CHECK(w.step({a}, {5}) == HALE_OK && kv_check_replay(&w.c, uses) == HALE_OK);
+  // with a store in the same graph, in either order, the step has to be of the same tokens
+  for (int first = 0; first < 2; first++) {
+    fake.capturing = true;
+    CHECK((first ? turn(pos) : w.append(5)) == HALE_OK && (first ? w.append(5) : turn(pos)) == HALE_OK);
+    fake.capturing = false;
+    std::vector<KvUse> both;
+    both.swap(w.c.kv_uses);
+    CHECK(kv_check_replay(&w.c, both) == HALE_OK);
+    CHECK(w.step({a}, {4}) == HALE_OK && kv_check_replay(&w.c, both) == HALE_EINVAL);
+    CHECK(w.step({a}, {5}) == HALE_OK && kv_check_replay(&w.c, both) == HALE_OK);
+  }
+  CHECK(hale_kv_reserve(w.kv, 5000) == HALE_OK);
+  CHECK(kv_check_replay(&w.c, uses) == HALE_EINVAL && w.c.err.find("grew") != std::string::npos);
+  fake.capturing = true;
+  CHECK(hale_kv_positions(w.kv, &pos) == HALE_OK && turn(pos) == HALE_OK);
+  fake.capturing = false;
+  uses.swap(w.c.kv_uses);
+  CHECK(kv_check_replay(&w.c, uses) == HALE_OK);
+  hale_kv_destroy(w.kv);
+  w.kv = nullptr;
+  CHECK(kv_check_replay(&w.c, uses) == HALE_EINVAL && w.c.err.find("gone") != std::string::npos);
+  hale_rope_destroy(rope);
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -119,6 +168,8 @@ int main(int argc, char** argv) {
     every_view();
   else if (what == "plan_behind_a_graph")
     plan_behind_a_graph();
+  else if (what == "rotation_in_a_graph")
+    rotation_in_a_graph();
   else
     return 2;
   CHECK(fake.device.empty() && fake.host.empty());

@@ -43,3 +43,7 @@ def test_every_list_of_every_view_in_one_step(check):
 
 def test_a_plan_that_was_outgrown_stays_while_graphs_exist(check):
     check("plan_behind_a_graph")
+
+
+def test_a_captured_rotation_of_positions_that_moved_is_refused(check):
+    check("rotation_in_a_graph")
