@@ -30,8 +30,9 @@ template <> __device__ __forceinline__ _Float16 from_f32<_Float16>(float v) {
   return (_Float16)v;
 }
 template <> __device__ __forceinline__ Bf16 from_f32<Bf16>(float v) {
+  // by its bits: the attention's unit is compiled without comparisons of NaNs
   const unsigned u = __float_as_uint(v);
-  if (v != v) return {(uint16_t)((u >> 16) | 0x40)};
+  if ((u & 0x7fffffffu) > 0x7f800000u) return {(uint16_t)((u >> 16) | 0x40)};
   return {(uint16_t)((u + 0x7fffu + ((u >> 16) & 1)) >> 16)};
 }
 

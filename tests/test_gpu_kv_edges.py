@@ -1,9 +1,11 @@
 """Edges of the paged 8-bit key/value cache on the GPU (hale_kv_*): steps that
-fill every list of the plan, graphs around a cache whose buffers grow."""
+fill every list of the plan, graphs around a cache whose buffers grow, queries
+that are not finite."""
 import numpy as np
 import pytest
 
 import hale_moe as H
+from kv_model import NP, decode, encode
 from test_gpu_kv import rig  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -59,3 +61,45 @@ def test_a_captured_rotation_of_the_steps_positions(rig, ctx):
     graph.close()
     rope.close()
     out.free()
+
+
+def set_number(raw, dtype, at, value):
+    """A number of an encoded array, given as its bits."""
+    raw.view({"f32": np.uint32, "f16": np.uint16, "bf16": np.uint16}[dtype])[at] = value
+
+
+INF = {"f32": 0x7F800000, "f16": 0x7C00, "bf16": 0x7F80}
+SIGN = {"f32": 1 << 31, "f16": 1 << 15, "bf16": 1 << 15}
+
+
+def attend_raw(r, dtype, raw):
+    """Results of queries given as encoded numbers [n][heads][dim]."""
+    q, out = r.put(raw.reshape(-1)), r.ctx.malloc(raw.nbytes)
+    r.kv.attention_device(0, dtype, raw.shape[0], q.address, out.address)
+    got = decode(out.download(NP[dtype], raw.size), dtype).reshape(raw.shape)
+    out.free()
+    return got
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 60])
+def test_every_kind_of_nan_in_a_query(rig, dtype, n):
+    """Quiet and signalling, of both signs, with the smallest and largest payloads."""
+    r = rig(dim=64, heads=4, kv_heads=2, pages=40)
+    g = np.random.default_rng(34)
+    a = r.create()
+    r.step(g, dtype, [a], [70])
+    r.step(g, dtype, [a], [n])
+    low = INF[dtype]
+    quiet = {"f32": 1 << 22, "f16": 1 << 9, "bf16": 1 << 6}[dtype]
+    full = SIGN[dtype] - 1 - low
+    clean = encode(g.standard_normal((n, 4, 64)), dtype)[0]
+    want = attend_raw(r, dtype, clean)
+    for payload in (1, quiet, full - quiet, full):
+        for sign in (0, SIGN[dtype]):
+            raw = clean.copy()
+            set_number(raw, dtype, (n - 1, 2, 33), sign | low | payload)
+            got = attend_raw(r, dtype, raw)
+            assert np.isnan(got[n - 1, 2]).all(), (hex(payload), sign)
+            got[n - 1, 2] = want[n - 1, 2]
+            assert (got.view(np.uint32) == want.view(np.uint32)).all()
