@@ -18,6 +18,11 @@
 // high part and rest, good to 2^-23 of its largest, in two products.  The
 // probabilities are up to 2^15 (relative to m), rounded to f16 (2^-11 of each)
 // for f16 and bf16 results, or kept as two f16 parts (2^-23) for f32 results.
+//
+// Every row sees its own position, so its sum, relative to a score that it has seen, is 1
+// at least and the division needs no guard.  The sum is 0 only where all scores are -inf (an infinite number in the query
+// and codes of one sign in that dimension): 0 / 0 makes the row NaN, as any
+// other score that is not finite does.
 #include <hip/hip_runtime.h>
 
 #include "hale_device.h"
@@ -406,7 +411,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_kv_attend_few(KvAttnArgs a) 
         }
         const unsigned tok = (item.row0 + row) / (unsigned)a.g.group;
         const unsigned h = item.head * a.g.group + (item.row0 + row) % (unsigned)a.g.group;
-        const float inv = total > 0.0f ? 1.0f / total : 0.0f;  // nothing visible: zeros
+        const float inv = 1.0f / total;
         const size_t prow = (size_t)item.part + row;
         for (int d = threadIdx.x % 16 * 4; d < a.g.hd; d += 64) {
           f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -655,7 +660,7 @@ __global__ __launch_bounds__(256, many_waves(sizeof(T), KC)) void k_kv_attend_ma
       const float total = row_sum(l[c]), up = pow2(vk[c] - SHIFT);
       if (r >= item.rows) continue;
       const unsigned tok = (item.row0 + r) / group, h = item.head * group + (item.row0 + r) % group;
-      const float inv = total > 0.0f ? up / total : 0.0f;
+      const float inv = up / total;
 #pragma unroll
       for (int n = 0; n < ND; n++)
         if (n < NDMIN || n < nd) {
@@ -701,7 +706,7 @@ __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a) {
     }
     const unsigned tok = (join.row0 + row) / (unsigned)a.g.group;
     const unsigned h = join.head * a.g.group + (join.row0 + row) % (unsigned)a.g.group;
-    const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+    const float inv = 1.0f / total;
     store4(a.dtype, a.out, (size_t)(join.tok0 + tok) * a.out_stride + (size_t)h * a.g.hd + 4 * x, a.vec, v * inv);
   }
 }
@@ -775,7 +780,7 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a) {
       for (int k = 1; k < slices; k++) v = v + sv[x + lanes * k];
       const unsigned tok = (join.row0 + row) / (unsigned)a.g.group;
       const unsigned h = join.head * a.g.group + (join.row0 + row) % (unsigned)a.g.group;
-      const float inv = total > 0.0f ? 1.0f / total : 0.0f;
+      const float inv = 1.0f / total;
       store4(a.dtype, a.out, (size_t)(join.tok0 + tok) * a.out_stride + (size_t)h * a.g.hd + 4 * x, a.vec, v * inv);
     }
   }

@@ -103,3 +103,27 @@ def test_every_kind_of_nan_in_a_query(rig, dtype, n):
             assert np.isnan(got[n - 1, 2]).all(), (hex(payload), sign)
             got[n - 1, 2] = want[n - 1, 2]
             assert (got.view(np.uint32) == want.view(np.uint32)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("old, n", [(0, 1), (0, 5), (70, 1), (70, 60), (3000, 1), (3000, 20)])
+def test_infinite_queries_over_keys_of_one_sign(rig, dtype, old, n):
+    """All scores of a row infinite, of one sign: NaN in the row, and in no other."""
+    r = rig(dim=64, heads=4, kv_heads=2, pages=60)
+    g = np.random.default_rng(33)
+    a = r.create()
+    for m in (old, n):
+        if m:
+            r.kv.step([a], [m])
+            k = g.standard_normal((m, 2, 64)).astype(np.float32)
+            k[:, :, 7] = 3.0 + np.abs(k[:, :, 7])  # codes of one sign, none 0
+            r.append(0, dtype, [a], [m], k, g.standard_normal((m, 2, 64)))
+    raw = encode(g.standard_normal((n, 4, 64)), dtype)[0]
+    clean = attend_raw(r, dtype, raw)
+    hit = np.zeros((n, 4), bool)
+    for t, h, bits in ((0, 1, INF[dtype]), (0, 2, INF[dtype] | SIGN[dtype]), (n - 1, 3, INF[dtype] | SIGN[dtype])):
+        set_number(raw, dtype, (t, h, 7), bits)
+        hit[t, h] = True
+    got = attend_raw(r, dtype, raw)
+    assert np.isnan(got[hit]).all()
+    assert (got[~hit].view(np.uint32) == clean[~hit].view(np.uint32)).all()
