@@ -85,6 +85,15 @@ __device__ __forceinline__ float row_sum(float v) {
 // 2^k for k up to 127; 0 below 2^-126.
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float((unsigned)(k < -127 ? 0 : k + 127) << 23); }
 
+// A k for which 2^k is above v, v >= 0.  Sums of p_j v_j are kept times 2^-above(sum of p_j), which is
+// exact: they are as large as values then, and finite where those are.
+__device__ __forceinline__ int above(float v) { return (int)(__float_as_uint(v) >> 23) - 126; }
+
+// v 2^k.
+__device__ __forceinline__ f32x4 scaled(f32x4 v, int k) {
+  return f32x4{__builtin_ldexpf(v[0], k), __builtin_ldexpf(v[1], k), __builtin_ldexpf(v[2], k), __builtin_ldexpf(v[3], k)};
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The pages first, first + step, .. below end of a page table's row, 64 of them
@@ -328,7 +337,7 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_kv_attend_few(KvAttnArgs a) 
             vr[mm] = pos0 + 16 * mm <= hi[c] && pos0 + 16 * mm + 15 > lo[c] ? vr[mm] : 0.0f;
         }
         const float vtop = fmaxf(fmaxf(vr[0], vr[1]), fmaxf(vr[2], vr[3]));
-        const int k_now = (int)(__float_as_uint(vtop) >> 23) - 126, k_new = k_now > vk[c] ? k_now : vk[c];
+        const int k_now = above(vtop), k_new = k_now > vk[c] ? k_now : vk[c];
         const float shrink = pow2(vk[c] - k_new);
         vk[c] = k_new;
         vr = vr * pow2(P_SHIFT - k_new);
@@ -391,11 +400,12 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_kv_attend_few(KvAttnArgs a) 
 #pragma unroll
     for (int c = 0; c < C; c++) {
       const float sum = row_sum(l[c]);
+      const int scale = vk[c] - P_SHIFT - above(sum);
       __syncthreads();  // the rows before, or the item before, are read
       if (g == 0) sml[wave][i] = float2{m[c], sum};
 #pragma unroll
       for (int n = 0; n < ND; n++)
-        if (n < NDMIN || n < nd) *(f32x4*)&so[wave][i][16 * n + 4 * g] = o[c][n] * pow2(vk[c] - P_SHIFT);
+        if (n < NDMIN || n < nd) *(f32x4*)&so[wave][i][16 * n + 4 * g] = scaled(o[c][n], scale);
       __syncthreads();
       const unsigned r = threadIdx.x / 16, row = 16 * c + r;
       if (row < item.rows) {
@@ -403,15 +413,19 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_kv_attend_few(KvAttnArgs a) 
 #pragma unroll
         for (int w = 0; w < ATT_WAVES; w++) top = fmaxf(top, sml[w][r].x);
         const float base2 = top == -__builtin_inff() ? 0.0f : top;
-        float f[ATT_WAVES], total = 0.0f;
+        float f[ATT_WAVES], sums[ATT_WAVES], total = 0.0f;
 #pragma unroll
         for (int w = 0; w < ATT_WAVES; w++) {
           f[w] = exp2_fast(sml[w][r].x - base2);
-          total += f[w] * sml[w][r].y;
+          sums[w] = sml[w][r].y;
+          total += f[w] * sums[w];
         }
+        const int e = above(total);
+#pragma unroll
+        for (int w = 0; w < ATT_WAVES; w++) f[w] = __builtin_ldexpf(f[w], above(sums[w]) - e);
         const unsigned tok = (item.row0 + row) / (unsigned)a.g.group;
         const unsigned h = item.head * a.g.group + (item.row0 + row) % (unsigned)a.g.group;
-        const float inv = 1.0f / total;
+        const float inv = pow2(e) / total;
         const size_t prow = (size_t)item.part + row;
         for (int d = threadIdx.x % 16 * 4; d < a.g.hd; d += 64) {
           f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -602,7 +616,7 @@ __global__ __launch_bounds__(256, many_waves(sizeof(T), KC)) void k_kv_attend_ma
           for (int mm = 0; mm < 4; mm++)
             top = fmaxf(top, f[mm] * fmaxf(fmaxf(s[c][mm][0], s[c][mm][1]), fmaxf(s[c][mm][2], s[c][mm][3])));
           top = row_max(top);
-          const int k_now = (int)(__float_as_uint(vtop) >> 23) - 126, k_new = k_now > vk[c] ? k_now : vk[c];
+          const int k_now = above(vtop), k_new = k_now > vk[c] ? k_now : vk[c];
           const float mnew = top > m[c] + (float)SLACK ? top : m[c];
           const float ref = mnew == -__builtin_inff() ? 0.0f : mnew;
           const float alpha = exp2_fast(m[c] - ref), scale = alpha * pow2(vk[c] - k_new);
@@ -658,6 +672,7 @@ __global__ __launch_bounds__(256, many_waves(sizeof(T), KC)) void k_kv_attend_ma
     for (int c = 0; c < C; c++) {
       const unsigned r = wrow + 16 * c + i;
       const float total = row_sum(l[c]), up = pow2(vk[c] - SHIFT);
+      const int scale = vk[c] - SHIFT - above(total);
       if (r >= item.rows) continue;
       const unsigned tok = (item.row0 + r) / group, h = item.head * group + (item.row0 + r) % group;
       const float inv = up / total;
@@ -668,7 +683,7 @@ __global__ __launch_bounds__(256, many_waves(sizeof(T), KC)) void k_kv_attend_ma
           if (item.part == KV_WHOLE)
             store4(a.dtype, a.out, (size_t)(item.tok0 + tok) * a.out_stride + (size_t)h * a.g.hd + d, a.vec, o[c][n] * inv);
           else
-            *(f32x4*)(a.part_o + ((size_t)item.part + r) * a.g.hd + d) = o[c][n] * up;
+            *(f32x4*)(a.part_o + ((size_t)item.part + r) * a.g.hd + d) = scaled(o[c][n], scale);
         }
       if (item.part != KV_WHOLE && g == 0) a.part_ml[(size_t)item.part + r] = float2{m[c], total};
     }
@@ -677,6 +692,8 @@ __global__ __launch_bounds__(256, many_waves(sizeof(T), KC)) void k_kv_attend_ma
 
 // Parts of one row: all of a step's at most.
 constexpr unsigned JOIN_PARTS = 2 * (KV_FEW_GROUPS > KV_MANY_GROUPS ? KV_FEW_GROUPS : KV_MANY_GROUPS);
+constexpr int JOIN_BITS = 10;
+static_assert(JOIN_PARTS <= 1u << JOIN_BITS, "the sum of a row's parts");
 
 // Joins of few parts, or of many rows: a work-group takes as many rows as its
 // threads hold at four numbers each, the parts one behind the other.  A chain of three
@@ -692,9 +709,14 @@ __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a) {
     const float2* ml = a.part_ml + (size_t)join.part0 + row;
     const float* po = a.part_o + ((size_t)join.part0 + row) * a.g.hd + 4 * x;
     const size_t step = (size_t)join.step * a.g.hd;
-    float top = -__builtin_inff(), total = 0.0f;
+    float top = -__builtin_inff(), most = 0.0f, total = 0.0f;
 #pragma unroll 4
-    for (unsigned k = 0; k < join.parts; k++) top = fmaxf(top, ml[(size_t)k * join.step].x);
+    for (unsigned k = 0; k < join.parts; k++) {
+      const float2 part = ml[(size_t)k * join.step];
+      top = fmaxf(top, part.x);
+      most = fmaxf(most, part.y);
+    }
+    const int e = above(most) + JOIN_BITS;  // 2^e is above the row's sum
     const float base2 = top == -__builtin_inff() ? 0.0f : top;
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
@@ -702,11 +724,11 @@ __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a) {
       const float2 part = ml[(size_t)k * join.step];
       const float w = exp2_fast(part.x - base2);
       total += w * part.y;
-      v = v + *(const f32x4*)(po + k * step) * w;
+      v = v + *(const f32x4*)(po + k * step) * (w * pow2(above(part.y) - e));
     }
     const unsigned tok = (join.row0 + row) / (unsigned)a.g.group;
     const unsigned h = join.head * a.g.group + (join.row0 + row) % (unsigned)a.g.group;
-    const float inv = 1.0f / total;
+    const float inv = pow2(e) / total;
     store4(a.dtype, a.out, (size_t)(join.tok0 + tok) * a.out_stride + (size_t)h * a.g.hd + 4 * x, a.vec, v * inv);
   }
 }
@@ -756,7 +778,7 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a) {
     for (int k = 0; k < (int)JOIN_PARTS / 256; k++) {
       const unsigned part = t + 256 * k;
       const float w = exp2_fast(mine[k].x - base2);
-      if (part < join.parts) sw[part] = w;
+      if (part < join.parts) sw[part] = w * pow2(above(mine[k].y));
       total += w * mine[k].y;
     }
 #pragma unroll
@@ -764,15 +786,17 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a) {
     if (t % 64 == 0) red[4 + wave] = total;
     __syncthreads();
     total = (red[4] + red[5]) + (red[6] + red[7]);
+    const int e = above(total);
+    const float down = pow2(-e);
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     if (x < quads) {
 #pragma unroll
       for (int k = 0; k < AHEAD; k++) {
         const unsigned part = slice + slices * k;
-        if (part < join.parts) v = v + early[k] * sw[part];
+        if (part < join.parts) v = v + early[k] * (sw[part] * down);
       }
 #pragma unroll 8
-      for (unsigned k = slice + slices * AHEAD; k < join.parts; k += slices) v = v + *(const f32x4*)(po + k * step) * sw[k];
+      for (unsigned k = slice + slices * AHEAD; k < join.parts; k += slices) v = v + *(const f32x4*)(po + k * step) * (sw[k] * down);
     }
     sv[t] = v;
     __syncthreads();
@@ -780,7 +804,7 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a) {
       for (int k = 1; k < slices; k++) v = v + sv[x + lanes * k];
       const unsigned tok = (join.row0 + row) / (unsigned)a.g.group;
       const unsigned h = join.head * a.g.group + (join.row0 + row) % (unsigned)a.g.group;
-      const float inv = 1.0f / total;
+      const float inv = pow2(e) / total;
       store4(a.dtype, a.out, (size_t)(join.tok0 + tok) * a.out_stride + (size_t)h * a.g.hd + 4 * x, a.vec, v * inv);
     }
   }

@@ -111,7 +111,7 @@ struct KvAttnArgs {
   const uint32_t* counts;      // {few, many, joins of few, of many} of the plan, on the device
   unsigned nitems, njoins;     // the same, or 0xffffffff: read counts (captured calls)
   int kind;                    // 0: items and joins of few rows, 1: of many
-  float* part_o;               // [row][hd]
+  float* part_o;               // [row][hd], times a power of two that follows from the sum
   float2* part_ml;             // [row] running maximum (base 2) and sum
   bool vec;                    // q and out rows start at multiples of four elements
 };

@@ -1,11 +1,11 @@
 """Edges of the paged 8-bit key/value cache on the GPU (hale_kv_*): steps that
 fill every list of the plan, graphs around a cache whose buffers grow, queries
-that are not finite."""
+that are not finite, values next to the largest number."""
 import numpy as np
 import pytest
 
 import hale_moe as H
-from kv_model import NP, decode, encode
+from kv_model import NP, attention_bound, decode, encode
 from test_gpu_kv import rig  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -127,3 +127,22 @@ def test_infinite_queries_over_keys_of_one_sign(rig, dtype, old, n):
     got = attend_raw(r, dtype, raw)
     assert np.isnan(got[hit]).all()
     assert (got[~hit].view(np.uint32) == clean[~hit].view(np.uint32)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("old, n", [(0, 40), (200, 1), (5000, 1), (200, 60), (5000, 40)])
+def test_values_next_to_the_largest_number(rig, dtype, old, n):
+    """Values up to 3.38e38: sums of them are not finite, their means are."""
+    r = rig(dim=64, heads=8, kv_heads=1, pages=100, max_len=6000)
+    g = np.random.default_rng(35)
+    a = r.create()
+    for m in (old, n):
+        if m:
+            r.kv.step([a], [m])
+            v = g.uniform(0.2, 1.0, (m, 1, 64)) * 3.38e38
+            r.append(0, dtype, [a], [m], g.standard_normal((m, 1, 64)), v)
+    q = encode(g.standard_normal((n, 8, 64)), dtype)[1]
+    got = r.attend(0, dtype, q)
+    want, mag, prod, total, vtop = r.model.attend(a, 0, q, 0.125)
+    assert np.isfinite(got).all()
+    assert (np.abs(got.astype(np.float64) - want) <= attention_bound(dtype, mag, prod, total, vtop, 64)).all()
