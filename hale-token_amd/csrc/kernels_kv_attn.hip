@@ -671,8 +671,7 @@ __global__ __launch_bounds__(256, many_waves(sizeof(T), KC)) void k_kv_attend_ma
 #pragma unroll
     for (int c = 0; c < C; c++) {
       const unsigned r = wrow + 16 * c + i;
-      const float total = row_sum(l[c]), up = pow2(vk[c] - SHIFT);
-      const int scale = vk[c] - SHIFT - above(total);
+      const float total = row_sum(l[c]), up = pow2(vk[c] - SHIFT), down = pow2(-above(total));
       if (r >= item.rows) continue;
       const unsigned tok = (item.row0 + r) / group, h = item.head * group + (item.row0 + r) % group;
       const float inv = up / total;
@@ -683,7 +682,7 @@ __global__ __launch_bounds__(256, many_waves(sizeof(T), KC)) void k_kv_attend_ma
           if (item.part == KV_WHOLE)
             store4(a.dtype, a.out, (size_t)(item.tok0 + tok) * a.out_stride + (size_t)h * a.g.hd + d, a.vec, o[c][n] * inv);
           else
-            *(f32x4*)(a.part_o + ((size_t)item.part + r) * a.g.hd + d) = scaled(o[c][n], scale);
+            *(f32x4*)(a.part_o + ((size_t)item.part + r) * a.g.hd + d) = o[c][n] * down * up;
         }
       if (item.part != KV_WHOLE && g == 0) a.part_ml[(size_t)item.part + r] = float2{m[c], total};
     }
