@@ -184,6 +184,7 @@ struct View {  // the plan of the current step under one window, for f32 or the 
   size_t window = 0;
   bool f32 = false;
   KvPlan plan;
+  KvPlan next;  // of the step that is being put together
 };
 
 // Sections of the plan's device buffer, in 32-bit words (multiples of four).
@@ -610,8 +611,8 @@ extern "C" int hale_kv_resize(hale_kv_cache* kv, size_t num_pages) {
 // steps
 // ---------------------------------------------------------------------------
 
-static size_t view_bytes(const View& v) {
-  return (v.plan.few.size() + v.plan.many.size()) * sizeof(KvItem) + (v.plan.few_joins.size() + v.plan.many_joins.size()) * sizeof(KvJoin) + 32;
+static size_t plan_bytes(const KvPlan& p) {
+  return (p.few.size() + p.many.size()) * sizeof(KvItem) + (p.few_joins.size() + p.many_joins.size()) * sizeof(KvJoin) + 32;
 }
 static void put_view(hale_kv_cache* kv, Upload& u, int i) {
   View& v = kv->views[i];
@@ -651,7 +652,7 @@ extern "C" int hale_kv_step(hale_kv_cache* kv, size_t nseq, const uint32_t* seqs
   std::string err;
   rc = status(kv, "kv_step", kv->pages.check_step(nseq, seqs, ntok, &err), err);
   if (rc) return rc;
-  // all that may want memory, then the bookkeeping
+  // all that may run out of memory first: until then the current step stands
   std::vector<KvStepSeq> next;
   std::vector<KvBlock> blocks;
   blocks.reserve(kv_max_blocks(tokens, nseq));
@@ -667,19 +668,20 @@ extern "C" int hale_kv_step(hale_kv_cache* kv, size_t nseq, const uint32_t* seqs
     mix(s.ntok);
     for (uint32_t t = 0; t < s.ntok; t++) positions[s.tok0 + t] = (int32_t)(s.len0 + t);
   }
-  rc = grow_plan(kv, tokens);
-  if (rc) return rc;
-  kv->stepped = false;  // the views' plans become the next step's
-  kv->seqs.swap(next);
+  kv->pages.reserve_step(nseq, seqs, ntok, &kv->copies);
   size_t bytes = tokens * 4 + blocks.size() * sizeof(KvBlock) + 64;
   bytes += kv->pages.step_changes() * 8 + kv->pages.step_copies() * sizeof(KvCopy);
   for (int i = 0; i < kv->nviews; i++) {
-    kv_plan(kv->shape, kv->seqs, kv->views[i].window, kv->views[i].f32, &kv->views[i].plan);
-    bytes += view_bytes(kv->views[i]);
+    kv_plan(kv->shape, next, kv->views[i].window, kv->views[i].f32, &kv->views[i].next);
+    bytes += plan_bytes(kv->views[i].next);
   }
   Upload u(kv);
   rc = u.begin(upload_bytes(kv, bytes));
+  if (!rc) rc = grow_plan(kv, tokens);
   if (rc) return rc;
+  kv->stepped = false;
+  kv->seqs.swap(next);
+  for (int i = 0; i < kv->nviews; i++) std::swap(kv->views[i].plan, kv->views[i].next);
   const uint32_t n[4] = {(uint32_t)blocks.size(), (uint32_t)tokens, 0, 0};
   u.put(kv->plan + kv->at.counts, n, sizeof n);
   u.put(kv->plan + kv->at.positions, positions.data(), tokens * 4);
@@ -831,7 +833,7 @@ extern "C" int hale_kv_attention_device(hale_kv_cache* kv, size_t layer, int dty
     v.f32 = f32;
     kv_plan(kv->shape, kv->seqs, window, f32, &v.plan);
     Upload u(kv);
-    rc = u.begin(upload_bytes(kv, view_bytes(v)));
+    rc = u.begin(upload_bytes(kv, plan_bytes(v.plan)));
     if (rc) return rc;
     put_view(kv, u, i);
     rc = u.end();

@@ -184,17 +184,21 @@ void KvPages::preview(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, s
   }
 }
 
-KvPages::Status KvPages::step(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, std::vector<KvStepSeq>* plan,
-                              std::vector<KvCopy>* copies, std::string* err) {
-  const Status st = check_step(nseq, seqs, ntok, err);
-  if (st) return st;
-  if (plan) preview(nseq, seqs, ntok, plan);
+void KvPages::reserve_step(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, std::vector<KvCopy>* copies) {
   copies->reserve(copies->size() + copies_);
   dirty.reserve(dirty.size() + need_);
   for (size_t i = 0; i < nseq; i++) {
     Seq& s = seqs_[seqs[i]];
     s.pages.reserve(ceil_div(s.len + ntok[i], KV_PAGE));
   }
+}
+
+KvPages::Status KvPages::step(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, std::vector<KvStepSeq>* plan,
+                              std::vector<KvCopy>* copies, std::string* err) {
+  const Status st = check_step(nseq, seqs, ntok, err);
+  if (st) return st;
+  if (plan) preview(nseq, seqs, ntok, plan);
+  reserve_step(nseq, seqs, ntok, copies);
   for (size_t i = 0; i < nseq; i++) {
     Seq& s = seqs_[seqs[i]];
     if (mark_[seqs[i]] == 0) {

@@ -140,6 +140,8 @@ class KvPages {
   // After check_step(): what the step would be, and the page table changes and
   // page copies that it would make.
   void preview(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, std::vector<KvStepSeq>* plan) const;
+  // and room for what step() adds, so that it throws nothing.  Throws std::bad_alloc.
+  void reserve_step(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, std::vector<KvCopy>* copies);
   size_t step_changes() const { return need_; }
   size_t step_copies() const { return copies_; }
   // Room for ntok[i] more positions of seqs[i]: new pages, and copies of

@@ -9,6 +9,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <new>
 #include <set>
 #include <string>
 #include <vector>
@@ -27,8 +28,7 @@
 // What the fake runtime is told and what it saw.
 struct Fake {
   bool capturing = false;
-  int host_allocs_until_failure = -1;    // -1: none fails
-  int device_allocs_until_failure = -1;
+  int allocs_until_failure = -1;         // of any kind; -1: none fails
   std::set<void*> device, host;          // allocated now
   int uploads = 0;
   std::vector<hale::KvAttnArgs> attends;  // in the order of the calls
@@ -38,13 +38,25 @@ struct Fake {
 };
 static Fake fake;
 
-static bool fails(int* n) { return *n >= 0 && (*n)-- == 0; }
+static bool fails() { return fake.allocs_until_failure >= 0 && fake.allocs_until_failure-- == 0; }
+
+void* operator new(size_t n) {
+  void* p = fails() ? nullptr : malloc(n);
+  if (!p) throw std::bad_alloc();
+  return p;
+}
+void* operator new(size_t n, const std::nothrow_t&) noexcept { return fails() ? nullptr : malloc(n); }
+void operator delete(void* p) noexcept { free(p); }
+void operator delete(void* p, size_t) noexcept { free(p); }
 
 extern "C" {
 hipError_t hipMalloc(void** p, size_t n) {
-  if (fails(&fake.device_allocs_until_failure)) return hipErrorOutOfMemory;
+  if (fails()) return hipErrorOutOfMemory;
   *p = malloc(n);
+  const int left = fake.allocs_until_failure;  // the fake's own books never fail
+  fake.allocs_until_failure = -1;
   fake.device.insert(*p);
+  fake.allocs_until_failure = left;
   return *p ? hipSuccess : hipErrorOutOfMemory;
 }
 hipError_t hipFree(void* p) {
@@ -54,9 +66,12 @@ hipError_t hipFree(void* p) {
   return hipSuccess;
 }
 hipError_t hipHostMalloc(void** p, size_t n, unsigned) {
-  if (fails(&fake.host_allocs_until_failure)) return hipErrorOutOfMemory;
+  if (fails()) return hipErrorOutOfMemory;
   *p = malloc(n);
+  const int left = fake.allocs_until_failure;
+  fake.allocs_until_failure = -1;
   fake.host.insert(*p);
+  fake.allocs_until_failure = left;
   return *p ? hipSuccess : hipErrorOutOfMemory;
 }
 hipError_t hipHostFree(void* p) {
@@ -89,6 +104,7 @@ int ctx_fail(hale_ctx* c, int code, const char* fmt, ...) {
   va_start(ap, fmt);
   vsnprintf(buf, sizeof buf, fmt, ap);
   va_end(ap);
+  fake.allocs_until_failure = -1;
   if (c) c->err = buf;
   return code;
 }
@@ -112,6 +128,7 @@ hipError_t launch_kv_upload(const KvUploadArgs& a, hipStream_t) {
   return hipSuccess;
 }
 hipError_t launch_kv_append(int, const KvAppendArgs& a, unsigned, hipStream_t) {
+  fake.allocs_until_failure = -1;
   fake.appends.push_back(a);
   return hipSuccess;
 }
@@ -120,10 +137,12 @@ hipError_t launch_kv_read(const KvGeom&, size_t, uint32_t, size_t, size_t count,
   return hipSuccess;
 }
 hipError_t launch_kv_attend_few(const KvAttnArgs& a, int, unsigned, hipStream_t) {
+  fake.allocs_until_failure = -1;
   fake.attends.push_back(a);
   return hipSuccess;
 }
 hipError_t launch_kv_attend_many(const KvAttnArgs& a, unsigned, hipStream_t) {
+  fake.allocs_until_failure = -1;
   fake.attends.push_back(a);
   return hipSuccess;
 }

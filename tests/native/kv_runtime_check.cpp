@@ -160,6 +160,90 @@ void rotation_in_a_graph() {
   hale_rope_destroy(rope);
 }
 
+// What a caller can see of a cache: sequences, pages, the current step's plan as the
+// kernels read it, and every position's page through the page table.
+struct Seen {
+  std::vector<size_t> lens;
+  size_t used = 0;
+  std::vector<std::vector<uint8_t>> plan;
+  std::vector<uint8_t> contents;
+  bool operator==(const Seen& o) const {
+    return lens == o.lens && used == o.used && plan == o.plan && contents == o.contents;
+  }
+};
+Seen look(Cache& w, const std::vector<uint32_t>& seqs, size_t tokens) {
+  fake.allocs_until_failure = -1;
+  Seen s;
+  for (uint32_t q : seqs) s.lens.push_back(w.len(q));
+  s.used = w.used();
+  fake.attends.clear();
+  fake.appends.clear();
+  if (tokens) {
+    CHECK(w.append(tokens) == HALE_OK);  // sends what the page table lacks
+    for (size_t window : {0, 20}) CHECK(w.attend(tokens, HALE_F32, window) == HALE_OK);
+    const KvAppendArgs& p = fake.appends[0];
+    auto keep = [&](const void* at, size_t n) { s.plan.emplace_back((const uint8_t*)at, (const uint8_t*)at + n); };
+    keep(&p.nblocks, 4);
+    keep(p.blocks, p.nblocks * sizeof(KvBlock));
+    for (const KvAttnArgs& a : fake.attends) {
+      keep(a.counts, 16);
+      keep(a.items, a.nitems * sizeof(KvItem));
+      keep(a.joins, a.njoins * sizeof(KvJoin));
+    }
+    for (size_t i = 0; i < seqs.size(); i++)
+      for (size_t j = 0; j * KV_PAGE < s.lens[i]; j++)
+        s.contents.push_back(p.g.pool[p.g.table[seqs[i] * p.g.max_pages + j] * p.g.page_bytes]);
+  }
+  return s;
+}
+// A byte of each page, by which its copies are known.
+void mark_pages(Cache& w) {
+  fake.appends.clear();
+  CHECK(w.append(430) == HALE_OK);
+  const KvGeom& g = fake.appends[0].g;
+  for (size_t p = 0; p < 64; p++) g.pool[p * g.page_bytes] = (uint8_t)(p + 1);
+}
+
+// Runs `call` with the first, second, .. allocation failing until none does: after
+// each failure all that can be seen is as before.  Returns the failures.
+template <typename F>
+int without_memory(Cache& w, const std::vector<uint32_t>& seqs, size_t tokens, F call) {
+  const Seen before = look(w, seqs, tokens);
+  for (int k = 0;; k++) {
+    CHECK(k < 1000);
+    fake.allocs_until_failure = k;
+    const int rc = call();
+    fake.allocs_until_failure = -1;
+    if (rc == HALE_OK) return k;
+    CHECK(rc == HALE_ENOMEM);
+    CHECK(look(w, seqs, tokens) == before);
+  }
+}
+
+// Sequences of 300, 120 and 10 positions, the second's pages shared with a fork, and
+// a hole in the pool; the step in progress has 430 tokens.
+std::vector<uint32_t> furnish(Cache& w) {
+  const uint32_t hole = w.seq(), a = w.seq(), b = w.seq(), c = w.seq();
+  CHECK(w.step({hole}, {200}) == HALE_OK && w.attend(200) == HALE_OK && w.attend(200, HALE_F32, 20) == HALE_OK);
+  CHECK(w.step({a, b, c}, {300, 120, 10}) == HALE_OK);
+  CHECK(hale_kv_seq_free(w.kv, hole) == HALE_OK);
+  uint32_t f = 0;
+  CHECK(hale_kv_seq_fork(w.kv, b, 1, &f) == HALE_OK);
+  mark_pages(w);
+  return {a, b, c, f};
+}
+
+void step_without_memory() {
+  for (uint32_t n : {1u, 3000u}) {  // within the plan's buffers, and growing them
+    Cache w(1, 4, 2, 16, 64, 8, 4000);
+    const std::vector<uint32_t> s = furnish(w);
+    const uint32_t seqs[2] = {s[1], s[2]}, ntok[2] = {n, 70};
+    CHECK(without_memory(w, s, 430, [&] { return hale_kv_step(w.kv, 2, seqs, ntok); }) > 0);
+    const Seen after = look(w, s, n + 70);
+    CHECK((after.lens == std::vector<size_t>{300, 120 + n, 80, 120}));
+  }
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -170,6 +254,8 @@ int main(int argc, char** argv) {
     plan_behind_a_graph();
   else if (what == "rotation_in_a_graph")
     rotation_in_a_graph();
+  else if (what == "step_without_memory")
+    step_without_memory();
   else
     return 2;
   CHECK(fake.device.empty() && fake.host.empty());

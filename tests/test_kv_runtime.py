@@ -47,3 +47,7 @@ def test_a_plan_that_was_outgrown_stays_while_graphs_exist(check):
 
 def test_a_captured_rotation_of_positions_that_moved_is_refused(check):
     check("rotation_in_a_graph")
+
+
+def test_a_step_that_finds_no_memory_changes_nothing(check):
+    check("step_without_memory")
