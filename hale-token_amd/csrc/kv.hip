@@ -525,8 +525,13 @@ extern "C" int hale_kv_seq_copy(hale_kv_cache* kv, uint32_t seq, uint32_t* out) 
   int rc = moves_allowed(kv, "kv_seq_copy");
   if (rc) return rc;
   std::string err;
-  rc = status(kv, "kv_seq_copy", kv->pages.copy(seq, out, &kv->copies, &err), err);
-  return rc ? rc : send_pages(kv);
+  size_t len = 0;
+  rc = status(kv, "kv_seq_copy", kv->pages.len(seq, &len, &err), err);
+  if (rc) return rc;
+  Upload u(kv);  // its memory before the sequence
+  rc = u.begin(upload_bytes(kv, (len + KV_PAGE - 1) / KV_PAGE * (8 + sizeof(KvCopy))));
+  if (!rc) rc = status(kv, "kv_seq_copy", kv->pages.copy(seq, out, &kv->copies, &err), err);
+  return rc ? rc : u.end();
   KV_CATCH(kv->ctx)
 }
 

@@ -244,6 +244,28 @@ void step_without_memory() {
   }
 }
 
+// Sequences that can still be made (and are given back).
+size_t free_sequences(Cache& w) {
+  std::vector<uint32_t> made;
+  uint32_t s = 0;
+  while (hale_kv_seq_create(w.kv, &s) == HALE_OK) made.push_back(s);
+  for (uint32_t m : made) CHECK(hale_kv_seq_free(w.kv, m) == HALE_OK);
+  return made.size();
+}
+
+void copy_without_memory() {
+  Cache w(1, 4, 2, 16, 64, 8, 4000);
+  const std::vector<uint32_t> s = furnish(w);
+  const size_t left = free_sequences(w);
+  uint32_t out = 0;
+  CHECK(without_memory(w, s, 430, [&] { return hale_kv_seq_copy(w.kv, s[0], &out); }) > 0);
+  CHECK(free_sequences(w) == left - 1 && w.len(out) == 300);
+  const uint32_t one[1] = {1}, both[2] = {s[0], out};
+  CHECK(hale_kv_step(w.kv, 1, both + 1, one) == HALE_OK);  // sends the page table
+  const Seen a = look(w, {s[0]}, 1), b = look(w, {out}, 1);
+  CHECK(a.contents == b.contents && b.contents.size() == 5);
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -256,6 +278,8 @@ int main(int argc, char** argv) {
     rotation_in_a_graph();
   else if (what == "step_without_memory")
     step_without_memory();
+  else if (what == "copy_without_memory")
+    copy_without_memory();
   else
     return 2;
   CHECK(fake.device.empty() && fake.host.empty());

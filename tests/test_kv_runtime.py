@@ -51,3 +51,7 @@ def test_a_captured_rotation_of_positions_that_moved_is_refused(check):
 
 def test_a_step_that_finds_no_memory_changes_nothing(check):
     check("step_without_memory")
+
+
+def test_a_copy_that_finds_no_memory_makes_no_sequence(check):
+    check("copy_without_memory")
