@@ -515,7 +515,7 @@ static int moves_allowed(hale_kv_cache* kv, const char* what) {
   const int rc = capturing(kv->ctx, &cap);
   if (rc) return rc;
   if (cap) return ctx_fail(kv->ctx, HALE_EINVAL, "%s while the stream is being captured", what);
-  return kv->copies.empty() ? HALE_OK : send_pages(kv);  // copies that found no staging memory
+  return kv->copies.empty() ? HALE_OK : send_pages(kv);  // copies whose launch failed
 }
 
 extern "C" int hale_kv_seq_copy(hale_kv_cache* kv, uint32_t seq, uint32_t* out) {
@@ -569,9 +569,14 @@ extern "C" int hale_kv_compact(hale_kv_cache* kv, size_t* moved) {
   std::lock_guard<std::recursive_mutex> lk(kv->ctx->mu);
   int rc = moves_allowed(kv, "kv_compact");
   if (rc) return rc;
+  size_t pages = 0, entries = 0;
+  kv->pages.compact_size(&pages, &entries);
+  Upload u(kv);  // its memory before the moves
+  rc = u.begin(upload_bytes(kv, pages * sizeof(KvCopy) + entries * 8));
+  if (rc) return rc;
   kv->pages.compact(&kv->copies);
-  if (moved) *moved = kv->copies.size();
-  return send_pages(kv);
+  if (moved) *moved = pages;
+  return pages || !kv->pages.dirty.empty() ? u.end() : HALE_OK;
   KV_CATCH(kv->ctx)
 }
 

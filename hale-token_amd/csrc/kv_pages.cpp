@@ -217,15 +217,21 @@ KvPages::Status KvPages::step(size_t nseq, const uint32_t* seqs, const uint32_t*
   return OK;
 }
 
+void KvPages::compact_size(size_t* moved, size_t* entries) const {
+  const size_t n = used();
+  *moved = *entries = 0;
+  for (size_t p = n; p < refs_.size(); p++) *moved += refs_[p] != 0;
+  if (*moved == 0) return;
+  for (const Seq& s : seqs_)
+    for (uint32_t p : s.pages) *entries += p >= n;
+}
+
 void KvPages::compact(std::vector<KvCopy>* copies) {
   const size_t n = used();
   std::vector<uint32_t> to(refs_.size());
-  size_t hole = 0, moved = 0;
-  for (size_t p = n; p < refs_.size(); p++) moved += refs_[p] != 0;
+  size_t hole = 0, moved = 0, entries = 0;
+  compact_size(&moved, &entries);
   copies->reserve(copies->size() + moved);
-  size_t entries = 0;
-  for (const Seq& s : seqs_)
-    for (uint32_t p : s.pages) entries += p >= n;
   dirty.reserve(dirty.size() + entries);
   for (size_t p = n; p < refs_.size(); p++) {
     if (!refs_[p]) continue;

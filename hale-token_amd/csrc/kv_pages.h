@@ -148,6 +148,8 @@ class KvPages {
   // shared, partly filled pages that the step writes to.  plan (may be null): as preview().
   Status step(size_t nseq, const uint32_t* seqs, const uint32_t* ntok, std::vector<KvStepSeq>* plan,
               std::vector<KvCopy>* copies, std::string* err);
+  // What compact() would move: pages, and page table entries that change.
+  void compact_size(size_t* moved, size_t* entries) const;
   // Moves the pages behind the first used() into the holes before.
   void compact(std::vector<KvCopy>* copies);
   // Another number of pages, at least used(), of a compacted pool.  Throws

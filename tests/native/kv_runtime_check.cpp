@@ -266,6 +266,17 @@ void copy_without_memory() {
   CHECK(a.contents == b.contents && b.contents.size() == 5);
 }
 
+void compact_without_memory() {
+  Cache w(1, 4, 2, 16, 64, 8, 4000);
+  const std::vector<uint32_t> s = furnish(w);  // the first pages are free
+  size_t moved = 99;
+  CHECK(without_memory(w, s, 430, [&] { return hale_kv_compact(w.kv, &moved); }) > 0);
+  CHECK(moved == 4);  // all of them by the call that succeeded
+  CHECK(hale_kv_compact(w.kv, &moved) == HALE_OK && moved == 0);
+  const Seen after = look(w, s, 430);
+  CHECK(after.used == 8 && after.contents.size() == 10);
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -280,6 +291,8 @@ int main(int argc, char** argv) {
     step_without_memory();
   else if (what == "copy_without_memory")
     copy_without_memory();
+  else if (what == "compact_without_memory")
+    compact_without_memory();
   else
     return 2;
   CHECK(fake.device.empty() && fake.host.empty());

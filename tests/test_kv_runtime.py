@@ -55,3 +55,7 @@ def test_a_step_that_finds_no_memory_changes_nothing(check):
 
 def test_a_copy_that_finds_no_memory_makes_no_sequence(check):
     check("copy_without_memory")
+
+
+def test_a_compaction_that_finds_no_memory_moves_nothing(check):
+    check("compact_without_memory")
