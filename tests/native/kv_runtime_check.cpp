@@ -277,6 +277,58 @@ void compact_without_memory() {
   CHECK(after.used == 8 && after.contents.size() == 10);
 }
 
+void others_without_memory() {
+  Cache w(1, 4, 2, 16, 64, 8, 4000);
+  const std::vector<uint32_t> s = furnish(w);
+  const size_t left = free_sequences(w);
+  static float x[4];
+  for (size_t window : {40, 60}) {  // the third and the fourth one
+    CHECK(without_memory(w, s, 430, [&] {
+            return hale_kv_attention_device(w.kv, 0, HALE_F32, 430, x, 1 << 20, 1.0f, window, x, 1 << 20);
+          }) > 0);
+  }
+  CHECK(w.attend(430, HALE_F32, 80) == HALE_EINVAL);
+  uint32_t out[2] = {};
+  CHECK(without_memory(w, s, 430, [&] { return hale_kv_seq_fork(w.kv, s[0], 2, out); }) > 0);
+  CHECK(free_sequences(w) == left - 2 && w.len(out[0]) == 300 && w.len(out[1]) == 300);
+  CHECK(without_memory(w, s, 430, [&] { return hale_kv_seq_truncate(w.kv, out[0], 70); }) >= 0);
+  CHECK(without_memory(w, s, 430, [&] { return hale_kv_seq_free(w.kv, out[0]); }) >= 0);
+  CHECK(without_memory(w, s, 430, [&] { return hale_kv_seq_create(w.kv, out); }) >= 0);
+  CHECK(without_memory(w, s, 430, [&] { return hale_kv_resize(w.kv, 30); }) > 0);
+  CHECK(without_memory(w, s, 430, [&] { return hale_kv_resize(w.kv, 50); }) > 0);
+  const Seen resized = look(w, s, 430);
+  CHECK(resized.contents.size() == 10);
+  hale_rope_config config{};
+  config.head_dim = config.rotary_dim = 16;
+  config.base = 1e4;
+  config.attention_factor = 1.0;
+  hale_rope* rope = nullptr;
+  const size_t device = fake.device.size();
+  CHECK(without_memory(w, s, 430, [&] { return hale_rope_create(&w.c, &config, &rope); }) > 0);
+  CHECK(fake.device.size() == device + 1);
+  hale_rope_destroy(rope);
+  hale_kv_cache* more = nullptr;
+  const size_t host = fake.host.size();
+  CHECK(without_memory(w, s, 430, [&] {
+          const int rc = hale_kv_create(&w.c, 1, 4, 2, 16, 64, 8, 4000, &more);
+          CHECK(rc == HALE_OK || (!more && fake.device.size() == device && w.c.kvs.size() == 1));
+          return rc;
+        }) > 0);
+  CHECK(fake.host.size() == host + 1);
+  hale_kv_destroy(more);
+  // a graph's notes
+  fake.capturing = true;
+  for (int k = 0;; k++) {
+    fake.allocs_until_failure = k;
+    const int rc = hale_kv_append_device(w.kv, 0, HALE_F32, 430, x, 1 << 20, x, 1 << 20);
+    fake.allocs_until_failure = -1;
+    if (rc == HALE_OK) break;
+    CHECK(rc == HALE_ENOMEM && w.c.kv_uses.empty());
+  }
+  fake.capturing = false;
+  CHECK(w.c.kv_uses.size() == 1);
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -293,6 +345,8 @@ int main(int argc, char** argv) {
     copy_without_memory();
   else if (what == "compact_without_memory")
     compact_without_memory();
+  else if (what == "others_without_memory")
+    others_without_memory();
   else
     return 2;
   CHECK(fake.device.empty() && fake.host.empty());

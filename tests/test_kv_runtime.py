@@ -59,3 +59,7 @@ def test_a_copy_that_finds_no_memory_makes_no_sequence(check):
 
 def test_a_compaction_that_finds_no_memory_moves_nothing(check):
     check("compact_without_memory")
+
+
+def test_other_calls_that_find_no_memory_change_nothing(check):
+    check("others_without_memory")
