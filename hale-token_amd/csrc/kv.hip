@@ -756,6 +756,10 @@ static int note_positions(hale_ctx* c, const int32_t* pos) {
 
 int hale::kv_check_replay(hale_ctx* c, const std::vector<KvUse>& uses) {
   KVCHK(c, hipSetDevice(c->device));
+  bool cap = false;
+  int rc = capturing(c, &cap);
+  if (rc) return rc;
+  if (cap) return ctx_fail(c, HALE_EINVAL, "graph_launch of a key/value cache's graph while the stream is being captured");
   for (const KvUse& u : uses) {
     if (std::find(c->kvs.begin(), c->kvs.end(), u.kv) == c->kvs.end() || u.kv->serial != u.serial)
       return ctx_fail(c, HALE_EINVAL, "graph_launch: its key/value cache is gone");
@@ -764,7 +768,7 @@ int hale::kv_check_replay(hale_ctx* c, const std::vector<KvUse>& uses) {
     if (!u.step) continue;
     if (!u.kv->stepped || u.kv->step_shape != u.shape)
       return ctx_fail(c, HALE_EINVAL, "graph_launch: the key/value cache's step is not of the captured tokens per sequence");
-    const int rc = send_pages(u.kv);
+    rc = send_pages(u.kv);
     if (rc) return rc;
   }
   return HALE_OK;

@@ -724,8 +724,8 @@ const char *hale_kernel_name(int kind);
  *     that moment, which must have the same tokens per sequence as the captured
  *     one (lengths and pages may differ); hale_graph_launch is refused
  *     (HALE_EINVAL) for another step, or once the cache's buffers grew or the
- *     cache is gone.  A graph with hale_rope_device by hale_kv_positions and neither
- *     of the two may be launched for any step, and is refused for the last two reasons. */
+ *     cache is gone, and within another capture.  A graph with hale_rope_device by hale_kv_positions and neither
+ *     of the two may be launched for any step, and is refused for the other reasons. */
 typedef struct hale_graph hale_graph;
 int hale_graph_begin(hale_ctx *ctx);
 int hale_graph_end(hale_ctx *ctx, hale_graph **out);

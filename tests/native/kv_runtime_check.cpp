@@ -329,6 +329,23 @@ void others_without_memory() {
   CHECK(w.c.kv_uses.size() == 1);
 }
 
+// A launch works on the step of its moment, which a graph inside another one
+// would not see: refused while a capture goes on.
+void launch_in_a_capture() {
+  Cache w;
+  const uint32_t a = w.seq();
+  CHECK(w.step({a}, {3}) == HALE_OK && w.attend(3) == HALE_OK);
+  fake.capturing = true;
+  CHECK(w.attend(3) == HALE_OK);
+  std::vector<KvUse> uses;
+  uses.swap(w.c.kv_uses);
+  uint32_t f = 0;
+  CHECK(hale_kv_seq_fork(w.kv, a, 1, &f) == HALE_OK);  // a page table change to be sent
+  CHECK(kv_check_replay(&w.c, uses) == HALE_EINVAL && w.c.err.find("captur") != std::string::npos);
+  fake.capturing = false;
+  CHECK(kv_check_replay(&w.c, uses) == HALE_OK);
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -347,6 +364,8 @@ int main(int argc, char** argv) {
     compact_without_memory();
   else if (what == "others_without_memory")
     others_without_memory();
+  else if (what == "launch_in_a_capture")
+    launch_in_a_capture();
   else
     return 2;
   CHECK(fake.device.empty() && fake.host.empty());

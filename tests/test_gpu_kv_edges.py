@@ -146,3 +146,22 @@ def test_values_next_to_the_largest_number(rig, dtype, old, n):
     want, mag, prod, total, vtop = r.model.attend(a, 0, q, 0.125)
     assert np.isfinite(got).all()
     assert (np.abs(got.astype(np.float64) - want) <= attention_bound(dtype, mag, prod, total, vtop, 64)).all()
+
+
+def test_a_graph_is_not_launched_inside_a_capture(rig, ctx):
+    r = rig(dim=64)
+    g = np.random.default_rng(36)
+    a = r.create()
+    r.step(g, "f32", [a], [3])
+    q, out = r.put(g.standard_normal((3, 4, 64)).astype(np.float32)), ctx.malloc(3 * 4 * 64 * 4)
+    call = lambda: r.kv.attention_device(0, "f32", 3, q.address, out.address)
+    call()
+    want = out.download(np.float32, 3 * 4 * 64).copy()
+    graph = ctx.capture(call)
+    with pytest.raises(ValueError, match="captur"):
+        ctx.capture(graph.launch)
+    out.upload(np.zeros(3 * 4 * 64, np.float32))
+    graph.launch()
+    assert (out.download(np.float32, 3 * 4 * 64) == want).all()
+    graph.close()
+    out.free()

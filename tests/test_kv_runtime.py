@@ -63,3 +63,7 @@ def test_a_compaction_that_finds_no_memory_moves_nothing(check):
 
 def test_other_calls_that_find_no_memory_change_nothing(check):
     check("others_without_memory")
+
+
+def test_a_graph_of_a_cache_is_not_launched_inside_a_capture(check):
+    check("launch_in_a_capture")
