@@ -1,11 +1,13 @@
 """Edges of the paged 8-bit key/value cache on the GPU (hale_kv_*): steps that
 fill every list of the plan, graphs around a cache whose buffers grow, queries
 that are not finite, values next to the largest number."""
+import os
+
 import numpy as np
 import pytest
 
 import hale_moe as H
-from kv_model import NP, attention_bound, decode, encode
+from kv_model import NP, Model, attention_bound, decode, encode
 from test_gpu_kv import rig  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -165,3 +167,35 @@ def test_a_graph_is_not_launched_inside_a_capture(rig, ctx):
     assert (out.download(np.float32, 3 * 4 * 64) == want).all()
     graph.close()
     out.free()
+
+
+def test_the_documented_step_runs(ctx):
+    """README.md's example of several sequences, as it stands there."""
+    with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "README.md")) as f:
+        blocks = f.read().split("```python\n")[1:]
+    code = next(b.split("```")[0] for b in blocks if "H.KvCache(" in b)
+    g = np.random.default_rng(37)
+    heads, kv_heads, dim, n = 8, 2, 64, 6
+    x = {name: encode(g.standard_normal((n, h, dim)), "bf16") for name, h in (("q", heads), ("k", kv_heads), ("v", kv_heads))}
+    bufs = {name: ctx.malloc(raw.nbytes) for name, (raw, _) in x.items()}
+    for name, (raw, _) in x.items():
+        bufs[name].upload(raw)
+    bufs["out"] = ctx.malloc(x["q"][0].nbytes)
+    space = dict(H=H, ctx=ctx, layers=1, layer=0, heads=heads, kv_heads=kv_heads, head_dim=dim, num_pages=8, max_seqs=4,
+                 max_len=256, **{name: b.address for name, b in bufs.items()})
+    exec(code, space)
+    # one token and five, each from position 0: the rotation of both sides and causal attention
+    got = decode(bufs["out"].download(np.uint16, x["q"][0].size), "bf16").reshape(n, heads, dim)
+    q = decode(bufs["q"].download(np.uint16, x["q"][0].size), "bf16").reshape(n, heads, dim)  # turned in place
+    k = decode(bufs["k"].download(np.uint16, x["k"][0].size), "bf16").reshape(n, kv_heads, dim)
+    assert (q[0] == x["q"][1][0]).all() and (q[2] != x["q"][1][2]).any()
+    model = Model(1, heads, kv_heads, dim)
+    for s, at, m in ((0, 0, 1), (1, 1, 5)):
+        model.create(s)
+        model.append(s, 0, k[at:at + m], x["v"][1][at:at + m])
+        want, mag, prod, total, vtop = model.attend(s, 0, q[at:at + m], dim ** -0.5)
+        assert (np.abs(got[at:at + m] - want) <= attention_bound("bf16", mag, prod, total, vtop, dim)).all()
+    for name in ("rope", "kv"):
+        space[name].close()
+    for b in bufs.values():
+        b.free()
