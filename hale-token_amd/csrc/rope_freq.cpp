@@ -15,7 +15,8 @@ bool rope_frequencies(const hale_rope_config& c, std::vector<double>* freq, std:
   if (c.head_dim == 0 || c.head_dim > 1024) return no("head_dim outside 1..1024");
   if (r == 0 || r % 2 || r > c.head_dim) return no("rotary_dim must be even, from 2 to head_dim");
   if (!(c.base > 1.0) || !std::isfinite(c.base)) return no("base must be a finite number above 1");
-  if (!std::isfinite(c.attention_factor) || c.attention_factor <= 0.0) return no("attention_factor must be positive");
+  const float factor = (float)c.attention_factor;  // as the kernels take it
+  if (!(factor > 0.0f) || !std::isfinite(factor)) return no("attention_factor must be positive, and a finite f32 number");
   if (c.scaling < HALE_ROPE_NONE || c.scaling > HALE_ROPE_PARTS) return no("unknown scaling");
   if (c.scaling != HALE_ROPE_NONE && (!(c.factor >= 1.0) || !std::isfinite(c.factor)))
     return no("factor must be a finite number from 1 on");

@@ -531,7 +531,7 @@ typedef struct {
   double factor;           /* from 1 on (unless HALE_ROPE_NONE)              */
   double original_len;     /* HALE_ROPE_PARTS                                */
   double low, high;        /* HALE_ROPE_PARTS: 0 <= low < high               */
-  double attention_factor; /* multiplies cos and sin; 1 for none             */
+  double attention_factor; /* multiplies cos and sin, as f32; 1 for none     */
 } hale_rope_config;
 
 int hale_rope_create(hale_ctx *ctx, const hale_rope_config *config,
