@@ -28,6 +28,7 @@ bool rope_frequencies(const hale_rope_config& c, std::vector<double>* freq, std:
   }
   const double n = (double)r;
   const double base = c.scaling == HALE_ROPE_NTK ? c.base * std::pow(c.factor, n / (n - 2.0)) : c.base;
+  if (!std::isfinite(base)) return no("base times its scaling is not finite");
   freq->resize(r / 2);
   for (size_t i = 0; i < r / 2; i++) {
     double f = std::pow(base, -2.0 * (double)i / n);
