@@ -920,7 +920,12 @@ extern "C" int hale_kv_read_device(hale_kv_cache* kv, size_t layer, uint32_t seq
   if (rc) return rc;
   rc = send_pages(kv);
   if (rc) return rc;
-  KV_LAUNCH(c, K_KV_READ, launch_kv_read(kv->geom, layer, seq, first, count, k, v, c->stream));
+  const size_t row = kv->shape.kv_heads * kv->shape.head_dim;
+  for (size_t done = 0; done < count;) {
+    const size_t n = kv_read_part(first + done, count - done);
+    KV_LAUNCH(c, K_KV_READ, launch_kv_read(kv->geom, layer, seq, first + done, n, k + done * row, v + done * row, c->stream));
+    done += n;
+  }
   return HALE_OK;
   KV_CATCH(c)
 }

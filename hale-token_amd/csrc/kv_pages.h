@@ -105,6 +105,14 @@ size_t kv_few_limit(const KvShape& s, const std::vector<KvStepSeq>& seqs, bool f
 // that all compute units take part.  Window 0 sees every earlier position.
 void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window, bool f32, KvPlan* out);
 
+// Positions that one launch of the reading kernel takes of those first .. first + count - 1: its
+// grid has a work-group of 256 threads per page, and counts threads in 32 bits.
+inline size_t kv_read_part(size_t first, size_t count) {
+  constexpr size_t pages = (1u << 24) - 1;
+  const size_t most = (first / KV_PAGE + pages) * KV_PAGE - first;
+  return count < most ? count : most;
+}
+
 // The blocks that a step's tokens touch.
 void kv_blocks(const std::vector<KvStepSeq>& seqs, size_t max_pages, std::vector<KvBlock>* out);
 

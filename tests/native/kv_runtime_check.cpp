@@ -346,6 +346,30 @@ void launch_in_a_capture() {
   CHECK(kv_check_replay(&w.c, uses) == HALE_OK);
 }
 
+// Reading goes in launches whose threads, 256 for each page, a grid's dimension can
+// count, and whose positions lie one behind the other.
+void long_reads() {
+  const size_t most = (1u << 30);
+  for (size_t first : {(size_t)0, (size_t)1, (size_t)63, (size_t)64, (size_t)5000})
+    for (size_t count : {(size_t)1, (size_t)64, (size_t)1000, most - 64 - first, most - 63 - first, most - first}) {
+      size_t at = first, launches = 0;
+      while (at < first + count) {
+        const size_t n = kv_read_part(at, first + count - at);
+        CHECK(n >= 1 && at + n <= first + count);
+        CHECK(((at + n - 1) / KV_PAGE - at / KV_PAGE + 1) * 256 < (size_t)1 << 32);
+        at += n;
+        launches++;
+      }
+      CHECK(at == first + count && launches <= 2);
+    }
+  Cache w;
+  const uint32_t a = w.seq();
+  CHECK(w.step({a}, {300}) == HALE_OK);
+  float x[4];
+  CHECK(hale_kv_read_device(w.kv, 0, a, 70, 200, x, x) == HALE_OK);
+  CHECK(fake.read_counts == std::vector<size_t>{200});
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -366,6 +390,8 @@ int main(int argc, char** argv) {
     others_without_memory();
   else if (what == "launch_in_a_capture")
     launch_in_a_capture();
+  else if (what == "long_reads")
+    long_reads();
   else
     return 2;
   CHECK(fake.device.empty() && fake.host.empty());

@@ -67,3 +67,7 @@ def test_other_calls_that_find_no_memory_change_nothing(check):
 
 def test_a_graph_of_a_cache_is_not_launched_inside_a_capture(check):
     check("launch_in_a_capture")
+
+
+def test_reads_of_any_length_fit_their_launches(check):
+    check("long_reads")
