@@ -211,9 +211,10 @@ __device__ __forceinline__ void split_rows(const T (&raw)[KC][8], bool valid, in
 // their results in LDS; a sequence whose pages are many is divided over work-groups too,
 // whose results the joins below put together.  The codes go from memory to registers as
 // the operands lie, a page ahead of their use.  Bound by memory: each code is read
-// once, for up to 32 rows.  bf16, heads of 128: 32 sequences of 200 to 8000 30.4 us for
-// 148 MB (4.9 TB/s), one of 131000 25.1 us for 135 MB (5.4 TB/s; a large copy, half of
-// it writes, reaches 4.85).  One of 4096 in f32 is 7.0 us for 4.3 MB, a chain of latencies: plan,
+// once, for up to 32 rows.  bf16, heads of 128: 32 sequences of 200 to 8000 36.7 us for
+// 145 MB (4.0 TB/s), one of 131000 30.4 us for 135 MB (4.4 TB/s; a large copy, half of
+// it writes, reaches 4.85).  Read pass after pass they stay in the last-level cache of 256
+// MB and take 30.3 and 25.6 us.  One of 4096 in f32 is 7.0 us for 4.3 MB, a chain of latencies: plan,
 // table, page, products, the waves' join.
 // T: type of queries and results; KC: padded head dimension / 32; C: groups of
 // 16 query rows.
@@ -452,14 +453,19 @@ __global__ __launch_bounds__(64 * ATT_WAVES) void k_kv_attend_few(KvAttnArgs a) 
 // other: no bank conflicts).  Two buffers, so one barrier a page; the next
 // page's codes are read from memory while this one is computed.  Per page of 64
 // positions and 16 rows at head dimension 128 the matrix instructions take 512
-// cycles and the softmax about 500, so two work-groups on a compute unit, whose
-// waves are in different phases, keep both busy (f32 at dimensions 96 and 128 needs the
-// registers of both for one, dimension 256 the LDS).  For f16 and bf16 the reference m
+// cycles and the softmax about 500, so two work-groups share a compute unit, for
+// one's products beside the other's softmax (f32 at dimensions 96 and 128 needs the
+// registers of both for one, dimensions above 128 the LDS).  For f16 and bf16 the reference m
 // follows the maximum only where this is more than 2^8 above it (probabilities are then
 // up to 2^15 from 2^7), so that the sums are seldom rescaled.
-// Bound by the vector instructions beside the matrix ones: 2048 bf16 tokens behind 4000, 32
-// heads of 128 on 4, take 191 us for 169 GFLOP (882 TFLOP/s, where a large matrix
-// product reaches 1140); by the counters, at 2.4 GHz, the matrix units work for 67 of them.
+// 2048 bf16 tokens behind 4000, 32 heads of 128 on 4, take 191 us for 169 GFLOP (882
+// TFLOP/s, where a large matrix product reaches 1140).  By the counters, at 2.4 GHz, the vector
+// units work for 102 of them and the matrix units for 67, most of that one after the
+// other: scores, softmax and values are phases of a wave, which meets the other waves at a
+// barrier each page.  Bound by that missing overlap.
+// Waves per SIMD that the registers are divided among.  At padded dimension 192 LDS holds one
+// work-group, yet half of the registers do, and the whole of them are slower (2048 behind
+// 4000: bf16 477 us, 527; f32 612, 693).
 constexpr int many_waves(size_t size, int kc) { return (size == 4 ? kc == 2 || kc == 6 : kc <= 6) ? 2 : 1; }
 
 template <typename T, int KC, int C>
@@ -696,7 +702,7 @@ static_assert(JOIN_PARTS <= 1u << JOIN_BITS, "the sum of a row's parts");
 
 // Joins of few parts, or of many rows: a work-group takes as many rows as its
 // threads hold at four numbers each, the parts one behind the other.  A chain of three
-// reads: 5.0 us for 32 sequences of up to 7 parts, 4 rows of 128 each.
+// reads: 5.1 us for 32 sequences of up to 7 parts, 4 rows of 128 each.
 __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a) {
   const int t = threadIdx.x;
   const int quads = a.g.hd / 4, lanes = quads <= 16 ? 16 : quads <= 32 ? 32 : 64, x = t % lanes;
@@ -734,7 +740,7 @@ __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a) {
 
 // Joins the partial results of one row: a work-group, whose threads take four
 // numbers each of every so many'th part; the slices are added in their order.  16 parts
-// a slice are read while the weights are found.  5.3 us for 128 parts of 32 rows of 128.
+// a slice are read while the weights are found.  5.5 us for 128 parts of 32 rows of 128.
 __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a) {
   constexpr int AHEAD = 16;
   __shared__ float sw[JOIN_PARTS];

@@ -324,7 +324,10 @@ size_t many_each(const std::vector<Tile>& tiles) {
 
 // Work-group i runs on accelerator die i % 8, each of which has its own L2: the
 // items of one sequence and head, which read the same pages, go to one die (or
-// as few as keep all eight busy), the longest first (bf16, 4 heads of 128: 2048 tokens
+// as few as keep all eight busy), the longest first.  That holds while all eight lists have
+// items: for 1, 2, 4 or a multiple of 8 streams of as many items.  Where lists are empty or
+// run out, the rest of the others goes over all dies, still the longest first, which keeps
+// the dies equally busy (bf16, 4 heads of 128: 2048 tokens
 // behind 4000 192 us, 225 in the order of the tiles; two prompts of 1000 36.5, 45.1).
 void spread(std::vector<KvItem>* items) {
   constexpr size_t DIES = 8;

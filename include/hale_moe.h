@@ -580,8 +580,12 @@ int hale_rope_device(hale_rope *rope, int dtype, size_t rows,
  * stored, and the positions of a step that was followed by another without it,
  * read what the page held before.
  *
+ * hale_kv_seq_free and hale_kv_seq_truncate of one of its sequences end the current
+ * step, even where no position goes away: stores and attention need a new one.
+ *
  * Calls return HALE_EINVAL for arguments they refuse and HALE_ENOMEM where
- * pages, sequences or memory run out; either way nothing has changed. */
+ * pages, sequences or memory run out; either way nothing has changed that a
+ * caller can see. */
 
 #define HALE_KV_PAGE 64
 #define HALE_KV_BLOCK 16
@@ -652,7 +656,9 @@ int hale_kv_append_device(hale_kv_cache *kv, size_t layer, int dtype,
  * enter to 2^-28 (f16, bf16) or 2^-23 (f32) of their row's largest number;
  * probabilities are rounded to 2^-11 of their value for f16 and bf16 and 2^-23 for
  * f32 (no finer than 2^-31 and 2^-39 of the row's largest, each times 127 times the
- * largest scale of the values that the row sees).  A query row that is not finite gives NaN in
+ * largest scale of the values that the row sees, or 2^-100 if that is larger).  Each window
+ * and kind of type (f32, the half types) that was ever attended with is planned in every later
+ * step of the cache.  A query row that is not finite gives NaN in
  * its own results only.  The order of all sums is fixed: equal calls give equal
  * bits.  d_out may be d_q with the same stride. */
 int hale_kv_attention_device(hale_kv_cache *kv, size_t layer, int dtype,

@@ -199,3 +199,26 @@ def test_the_documented_step_runs(ctx):
         space[name].close()
     for b in bufs.values():
         b.free()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [1e-27, 1e-33, 1e-38])
+@pytest.mark.parametrize("old, n", [(0, 40), (200, 1), (5000, 1), (5000, 40)])
+def test_values_next_to_zero(rig, dtype, size, old, n):
+    """The smallest values: probabilities are no finer than the documented floor, in which
+    scales below 2^-100 count as that."""
+    r = rig(dim=64, heads=8, kv_heads=1, pages=100, max_len=6000)
+    g = np.random.default_rng(38)
+    a = r.create()
+    for m in (old, n):
+        if m:
+            r.kv.step([a], [m])
+            r.append(0, dtype, [a], [m], g.standard_normal((m, 1, 64)), g.standard_normal((m, 1, 64)) * size)
+    q = encode(g.standard_normal((n, 8, 64)), dtype)[1]
+    got = r.attend(0, dtype, q)
+    want, mag, prod, total, vtop = r.model.attend(a, 0, q, 0.125)
+    bound = attention_bound(dtype, mag, prod, total, np.maximum(vtop, 127 * 2.0 ** -100), 64)
+    # numbers below 2^-126 are multiples of 2^-149 (bf16: 2^-133): half a step of the result's rounding,
+    # and of each partial sum's, which is held times 2^-10 or less of it
+    bound = bound + (2.0 ** -134 if dtype == "bf16" else 2.0 ** -150) + 1024 * 2.0 ** -149
+    assert (np.abs(got.astype(np.float64) - want) <= bound).all()
