@@ -612,7 +612,8 @@ int hale_kv_seq_free(hale_kv_cache *kv, uint32_t seq);
  * which the step then copies first. */
 int hale_kv_seq_fork(hale_kv_cache *kv, uint32_t seq, size_t n, uint32_t *out);
 /* One new sequence with seq's contents in pages of its own (copied on the
- * context's stream). */
+ * context's stream: what a current step has not stored yet is stored to seq only,
+ * where a fork shares it). */
 int hale_kv_seq_copy(hale_kv_cache *kv, uint32_t seq, uint32_t *out);
 /* Drops the positions from len on (drafted tokens that were not accepted). */
 int hale_kv_seq_truncate(hale_kv_cache *kv, uint32_t seq, size_t len);
