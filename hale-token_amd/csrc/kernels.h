@@ -310,6 +310,9 @@ enum KernelKind : int {
   K_KV_READ,
   K_KV_PAGES,
   K_KV_ATTENTION,
+  K_NORM_Q8,
+  K_Q4G,
+  K_LOGITS,
   K_KINDS
 };
 

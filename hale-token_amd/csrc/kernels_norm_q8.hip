@@ -1,0 +1,224 @@
+// kernels_norm_q8.hip -- the residual's addition and RMS norm of rows, handing
+// on 8 bits with a scale per block.
+//
+// s = x + delta (in f32, rounded to the type), u = s w, r = 1 / sqrt(sum(s^2) / n
+// + eps), y = r u; a block's scale is r max|u| / 127 and its codes are 127 u /
+// max|u| to the nearest whole number, ties to even.  r is no part of the codes:
+// they follow from u alone, which 64 bits hold exactly (24 bits times 24), so that
+// every code is the nearest one.  The squares are summed in 64 bits too, where no f32
+// number's square leaves the range.
+#include <hip/hip_runtime.h>
+
+#include "hale_device.h"
+#include "kernels.h"
+#include "kv_device.h"
+#include "step_ops.h"
+
+namespace hale {
+
+// Eight numbers of a row as f32.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const void* base, size_t at, float (&v)[8]) {
+  const T* p = (const T*)base + at;
+  T raw[8];
+  if constexpr (VEC) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 16 / (int)sizeof(T)) *(u32x4*)&raw[j] = *(const u32x4*)(p + j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) raw[j] = p[j];
+  }
+#pragma unroll
+  for (int j = 0; j < 8; j++) v[j] = to_f32(raw[j]);
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(void* base, size_t at, const float (&v)[8]) {
+  T* p = (T*)base + at;
+  T raw[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) raw[j] = from_f32<T>(v[j]);
+  if constexpr (VEC) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 16 / (int)sizeof(T)) *(u32x4*)(p + j) = *(u32x4*)&raw[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) p[j] = raw[j];
+  }
+}
+
+__device__ __forceinline__ double from_words(unsigned lo, unsigned hi) {
+  return __longlong_as_double((long long)((unsigned long long)hi << 32 | lo));
+}
+template <int CTRL> __device__ __forceinline__ double dpp64(double v) {
+  const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+  return from_words((unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)b, CTRL, 0xF, 0xF, false),
+                    (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), CTRL, 0xF, 0xF, false));
+}
+// Over the whole wave, from within rows of 16 lanes outward.
+template <typename Op> __device__ __forceinline__ double over_rows(double v, Op op) {
+  unsigned long long b = (unsigned long long)__double_as_longlong(v);
+  auto lo = __builtin_amdgcn_permlane16_swap((unsigned)b, (unsigned)b, false, false);
+  auto hi = __builtin_amdgcn_permlane16_swap((unsigned)(b >> 32), (unsigned)(b >> 32), false, false);
+  v = op(from_words(lo[0], hi[0]), from_words(lo[1], hi[1]));
+  b = (unsigned long long)__double_as_longlong(v);
+  lo = __builtin_amdgcn_permlane32_swap((unsigned)b, (unsigned)b, false, false);
+  hi = __builtin_amdgcn_permlane32_swap((unsigned)(b >> 32), (unsigned)(b >> 32), false, false);
+  return op(from_words(lo[0], hi[0]), from_words(lo[1], hi[1]));
+}
+struct Add64 { __device__ double operator()(double a, double b) const { return a + b; } };
+struct Max64 { __device__ double operator()(double a, double b) const { return fmax(a, b); } };
+
+// The code of u, inv = 127 / top: the nearest whole number to 127 u / top.  The
+// product is good to 2^-51 of at most 127; where it lies that near to a border, both
+// sides of 254 |u| <> (2 k + 1) top are compared exactly (each product and its rounding).
+__device__ __forceinline__ int code_of(double u, double top, double inv) {
+  const double t = u * inv, q = rint(t);
+  if (fabs(fabs(t - q) - 0.5) < 1e-12) {
+    const double k = floor(fabs(t)), a = fabs(u), odd = 2 * k + 1;
+    const double p = 254 * a, pe = __builtin_fma(254.0, a, -p), r = odd * top, re = __builtin_fma(odd, top, -r);
+    const double d = (p - r) + (pe - re);
+    const int m = (int)k, c = d > 0 ? m + 1 : d < 0 ? m : m + (m & 1);
+    return u < 0 ? -c : c;
+  }
+  return (int)q;
+}
+
+// A work-group of NT threads per row, C groups of eight numbers a thread, all of them
+// read before anything is written.  Blocks of 32, 64 and 128 numbers lie in 4, 8 and 16
+// neighbouring lanes.
+template <typename T, int NT, int C, bool VEC>
+__global__ __launch_bounds__(NT) void k_norm_q8(NormQ8Args a) {
+  constexpr int W = NT / 64;
+  __shared__ double red[2][W];
+  const int t = threadIdx.x, wave = t >> 6;
+  const size_t row = blockIdx.x;
+  const unsigned groups = a.n / 8;
+  float s[C][8], w[C][8];
+#pragma unroll
+  for (int c = 0; c < C; c++) {
+    const unsigned at = (unsigned)(t + NT * c);
+    if (at < groups) {
+      load8<T, VEC>(a.x, row * a.x_stride + 8 * at, s[c]);
+      load8<float, VEC>(a.w, 8 * at, w[c]);
+      if (a.delta) {
+        float d[8];
+        load8<T, VEC>(a.delta, row * a.delta_stride + 8 * at, d);
+#pragma unroll
+        for (int j = 0; j < 8; j++) s[c][j] = to_f32(from_f32<T>(s[c][j] + d[j]));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) s[c][j] = w[c][j] = 0.0f;
+    }
+  }
+  double sum = 0, top[C];
+#pragma unroll
+  for (int c = 0; c < C; c++) {
+    double most = 0, odd = 0;  // odd: not a number where some u is not finite
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const double v = s[c][j], u = v * (double)w[c][j];
+      sum = __builtin_fma(v, v, sum);
+      most = fmax(most, fabs(u));
+      odd = __builtin_fma(u, 0.0, odd);
+    }
+    top[c] = odd == 0 ? most : __builtin_inf();
+  }
+  sum = sum + dpp64<0xB1>(sum);
+  sum = sum + dpp64<0x4E>(sum);
+  sum = sum + dpp64<0x141>(sum);
+  sum = sum + dpp64<0x140>(sum);
+  sum = over_rows(sum, Add64());
+  if (a.block == 0) {
+    double most = top[0];
+#pragma unroll
+    for (int c = 1; c < C; c++) most = fmax(most, top[c]);
+    most = fmax(most, dpp64<0xB1>(most));
+    most = fmax(most, dpp64<0x4E>(most));
+    most = fmax(most, dpp64<0x141>(most));
+    most = fmax(most, dpp64<0x140>(most));
+    most = over_rows(most, Max64());
+    if (W > 1 && t % 64 == 0) red[1][wave] = most;
+    top[0] = most;
+  }
+  if constexpr (W > 1) {
+    if (t % 64 == 0) red[0][wave] = sum;
+    __syncthreads();
+    sum = red[0][0];
+#pragma unroll
+    for (int k = 1; k < W; k++) sum += red[0][k];
+    if (a.block == 0) {
+      top[0] = red[1][0];
+#pragma unroll
+      for (int k = 1; k < W; k++) top[0] = fmax(top[0], red[1][k]);
+    }
+  }
+  // a row with a number that is not finite: nothing of it is
+  const double r = sum < __builtin_inf() ? 1.0 / sqrt(sum / (double)a.n + (double)a.eps) : __builtin_nan("");
+#pragma unroll
+  for (int c = 0; c < C; c++) {
+    const unsigned at = (unsigned)(t + NT * c);
+    double m = a.block == 0 ? top[0] : top[c];
+    if (a.block) {
+      m = fmax(m, dpp64<0xB1>(m));
+      m = fmax(m, dpp64<0x4E>(m));
+      if (a.block > 32) m = fmax(m, dpp64<0x141>(m));
+      if (a.block > 64) m = fmax(m, dpp64<0x140>(m));
+    }
+    const bool finite = m < __builtin_inf() && r < __builtin_inf();
+    const double inv = finite && m > 0 ? 127.0 / m : 0.0;
+    if (at >= groups) continue;
+    unsigned q[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      q[h] = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int i = 4 * h + j;
+        // (m and not inv: 0 times a number that is not finite)
+        const int code = finite ? code_of((double)s[c][i] * (double)w[c][i], m, inv) : 0;
+        q[h] |= (unsigned)(code & 255) << (8 * j);
+      }
+    }
+    int8_t* pq = a.q + row * a.n + 8 * at;
+    if constexpr (VEC) {
+      *(u32x2*)pq = u32x2{q[0], q[1]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) pq[j] = (int8_t)(q[j / 4] >> (8 * (j % 4)));
+    }
+    const float scale = finite ? (float)(r * m / 127.0) : __builtin_nanf("");
+    if (a.block == 0) {
+      if (at == 0) a.scales[row] = scale;
+    } else if (8 * at % a.block == 0) {
+      a.scales[row * (a.n / a.block) + 8 * at / a.block] = scale;
+    }
+    if (a.sum) store8<T, VEC>(a.sum, row * a.sum_stride + 8 * at, s[c]);
+    if (a.y) {
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) y[j] = (float)((double)s[c][j] * (double)w[c][j] * r);
+      store8<T, VEC>(a.y, row * a.y_stride + 8 * at, y);
+    }
+  }
+}
+
+template <typename T, bool VEC>
+static hipError_t norm_sized(const NormQ8Args& a, size_t rows, hipStream_t st) {
+  const unsigned groups = a.n / 8, grid = (unsigned)rows;
+  if (groups <= 64) return launch(k_norm_q8<T, 64, 1, VEC>, grid, 64, 0, st, a);
+  if (groups <= 256) return launch(k_norm_q8<T, 256, 1, VEC>, grid, 256, 0, st, a);
+  if (groups <= 512) return launch(k_norm_q8<T, 256, 2, VEC>, grid, 256, 0, st, a);
+  if (groups <= 1024) return launch(k_norm_q8<T, 512, 2, VEC>, grid, 512, 0, st, a);
+  return launch(k_norm_q8<T, 1024, 2, VEC>, grid, 1024, 0, st, a);
+}
+
+hipError_t launch_norm_q8(int dtype, const NormQ8Args& a, size_t rows, hipStream_t st) {
+  if (rows == 0) return hipSuccess;
+  if (dtype == F32) return a.vec ? norm_sized<float, true>(a, rows, st) : norm_sized<float, false>(a, rows, st);
+  if (dtype == F16) return a.vec ? norm_sized<_Float16, true>(a, rows, st) : norm_sized<_Float16, false>(a, rows, st);
+  return a.vec ? norm_sized<Bf16, true>(a, rows, st) : norm_sized<Bf16, false>(a, rows, st);
+}
+
+}  // namespace hale

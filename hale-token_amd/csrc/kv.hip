@@ -12,46 +12,12 @@
 
 #include "context.h"
 #include "hale_device.h"
+#include "host_call.h"
 #include "kernels.h"
 #include "kv.h"
 #include "rope_freq.h"
 
 using namespace hale;
-
-#define KVCHK(ctx, call)                                                                       \
-  do {                                                                                         \
-    hipError_t e_ = (call);                                                                    \
-    if (e_ != hipSuccess)                                                                      \
-      return ctx_fail((ctx), HALE_EHIP, "%s failed: %s", #call, hipGetErrorString(e_));        \
-  } while (0)
-
-// Launches `call` (returning hipError_t) bracketed for the profiler.
-#define KV_LAUNCH(ctx, kind, call)  \
-  do {                              \
-    ctx_prof_begin((ctx), (kind));  \
-    hipError_t le_ = (call);        \
-    ctx_prof_end((ctx));            \
-    KVCHK((ctx), le_);              \
-  } while (0)
-
-// No C++ exception leaves a C entry point.
-#define KV_TRY try {
-#define KV_CATCH(ctx)                                                                  \
-  }                                                                                    \
-  catch (const std::bad_alloc&) { return ctx_fail((ctx), HALE_ENOMEM, "out of host memory"); } \
-  catch (...) { return ctx_fail((ctx), HALE_EHIP, "unexpected failure"); }
-
-static bool float_type(int dtype) { return dtype == HALE_F32 || dtype == HALE_F16 || dtype == HALE_BF16; }
-static size_t type_bytes(int dtype) { return dtype == HALE_F32 ? 4 : 2; }
-static size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
-static bool aligned(const void* p, int dtype) { return (uintptr_t)p % type_bytes(dtype) == 0; }
-
-static int capturing(hale_ctx* c, bool* yes) {
-  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-  KVCHK(c, hipStreamIsCapturing(c->stream, &st));
-  *yes = st != hipStreamCaptureStatusNone;
-  return HALE_OK;
-}
 
 // ---------------------------------------------------------------------------
 // rotary positions
@@ -67,7 +33,7 @@ struct hale_rope {
 extern "C" int hale_rope_create(hale_ctx* c, const hale_rope_config* config, hale_rope** out) {
   if (!c || !config || !out) return ctx_fail(c, HALE_EINVAL, "rope_create: NULL argument");
   *out = nullptr;
-  KV_TRY
+  CALL_TRY
   std::vector<double> freq;
   std::string err;
   if (!rope_frequencies(*config, &freq, &err)) return ctx_fail(c, HALE_EINVAL, "rope: %s", err.c_str());
@@ -75,7 +41,7 @@ extern "C" int hale_rope_create(hale_ctx* c, const hale_rope_config* config, hal
   for (size_t i = 0; i < freq.size(); i++) turns[i] = freq[i] / (2.0 * M_PI);
   std::lock_guard<std::recursive_mutex> lk(c->mu);
   bool cap = false;
-  KVCHK(c, hipSetDevice(c->device));
+  CALL_CHK(c, hipSetDevice(c->device));
   const int rc = capturing(c, &cap);
   if (rc) return rc;
   if (cap) return ctx_fail(c, HALE_EINVAL, "rope_create while the stream is being captured");
@@ -93,7 +59,7 @@ extern "C" int hale_rope_create(hale_ctx* c, const hale_rope_config* config, hal
   }
   *out = r;
   return HALE_OK;
-  KV_CATCH(c)
+  CALL_CATCH(c)
 }
 
 extern "C" void hale_rope_destroy(hale_rope* r) {
@@ -153,14 +119,14 @@ extern "C" int hale_rope_device(hale_rope* r, int dtype, size_t rows, const int3
   a.half = (int)(r->config.rotary_dim / 2);
   a.interleaved = r->config.layout == HALE_ROPE_INTERLEAVED;
   a.factor = (float)r->config.attention_factor;
-  KV_TRY
+  CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(c->mu);
-  KVCHK(c, hipSetDevice(c->device));
+  CALL_CHK(c, hipSetDevice(c->device));
   const int rc = note_positions(c, pos);
   if (rc) return rc;
-  KV_LAUNCH(c, K_ROPE, launch_rope(dtype, a, c->stream));
+  CALL_LAUNCH(c, K_ROPE, launch_rope(dtype, a, c->stream));
   return HALE_OK;
-  KV_CATCH(c)
+  CALL_CATCH(c)
 }
 
 // ---------------------------------------------------------------------------
@@ -243,7 +209,7 @@ struct Upload {
     hale_ctx* c = kv->ctx;
     s = &kv->staging[kv->uploads % STAGINGS];
     if (s->number && (int32_t)(__atomic_load_n(kv->done, __ATOMIC_ACQUIRE) - s->number) < 0)
-      KVCHK(c, hipStreamSynchronize(c->stream));
+      CALL_CHK(c, hipStreamSynchronize(c->stream));
     s->number = 0;
     if (s->bytes < bytes) {
       if (s->base) (void)hipHostFree(s->base);
@@ -294,7 +260,7 @@ struct Upload {
     a.page_bytes = kv->geom.page_bytes;
     a.done = kv->done;
     a.number = kv->uploads++;  // from the first one's 0 on: numbers count from 1
-    KV_LAUNCH(c, K_KV_PAGES, launch_kv_upload(a, c->stream));
+    CALL_LAUNCH(c, K_KV_PAGES, launch_kv_upload(a, c->stream));
     s->number = kv->uploads;
     dirty.clear();
     kv->copies.clear();
@@ -353,7 +319,7 @@ static int grow_plan(hale_kv_cache* kv, size_t tokens) {
   tokens = round_up(std::max(tokens, kv->cap_tokens * 2), 256);
   const Sections s = sections(kv, tokens);
   uint32_t* p = nullptr;
-  KVCHK(c, hipStreamSynchronize(c->stream));
+  CALL_CHK(c, hipStreamSynchronize(c->stream));
   if (hipMalloc(&p, s.words * 4) != hipSuccess)
     return ctx_fail(c, HALE_ENOMEM, "kv: plan buffers of %zu bytes", s.words * 4);
   ctx_release(c, kv->plan);  // a graph's rotation may read the positions in it
@@ -401,9 +367,9 @@ extern "C" int hale_kv_create(hale_ctx* c, size_t layers, size_t heads, size_t k
   if (row * max_seqs > (1u << 30))
     return ctx_fail(c, HALE_EINVAL, "kv_create: a page table of %zu sequences x %zu pages", max_seqs, row);
   hale_kv_cache* kv = nullptr;
-  KV_TRY
+  CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(c->mu);
-  KVCHK(c, hipSetDevice(c->device));
+  CALL_CHK(c, hipSetDevice(c->device));
   bool cap = false;
   int rc = capturing(c, &cap);
   if (rc) return rc;
@@ -453,7 +419,7 @@ extern "C" int hale_kv_create(hale_ctx* c, size_t layers, size_t heads, size_t k
   c->kvs.push_back(kv);
   *out = own.release();
   return HALE_OK;
-  KV_CATCH(c)
+  CALL_CATCH(c)
 }
 
 extern "C" void hale_kv_destroy(hale_kv_cache* kv) {
@@ -480,37 +446,37 @@ static void leaves_step(hale_kv_cache* kv, uint32_t seq) {
 
 extern "C" int hale_kv_seq_create(hale_kv_cache* kv, uint32_t* seq) {
   if (!kv || !seq) return ctx_fail(kv ? kv->ctx : nullptr, HALE_EINVAL, "kv_seq_create: NULL argument");
-  KV_TRY
+  CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(kv->ctx->mu);
   std::string err;
   return status(kv, "kv_seq_create", kv->pages.create(seq, &err), err);
-  KV_CATCH(kv->ctx)
+  CALL_CATCH(kv->ctx)
 }
 
 extern "C" int hale_kv_seq_free(hale_kv_cache* kv, uint32_t seq) {
   if (!kv) return ctx_fail(nullptr, HALE_EINVAL, "kv_seq_free: NULL argument");
-  KV_TRY
+  CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(kv->ctx->mu);
   std::string err;
   const int rc = status(kv, "kv_seq_free", kv->pages.free(seq, &err), err);
   if (!rc) leaves_step(kv, seq);
   return rc;
-  KV_CATCH(kv->ctx)
+  CALL_CATCH(kv->ctx)
 }
 
 extern "C" int hale_kv_seq_fork(hale_kv_cache* kv, uint32_t seq, size_t n, uint32_t* out) {
   if (!kv || (n && !out)) return ctx_fail(kv ? kv->ctx : nullptr, HALE_EINVAL, "kv_seq_fork: NULL argument");
-  KV_TRY
+  CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(kv->ctx->mu);
   std::string err;
   return status(kv, "kv_seq_fork", kv->pages.fork(seq, n, out, &err), err);
-  KV_CATCH(kv->ctx)
+  CALL_CATCH(kv->ctx)
 }
 
 // Page moves are enqueued at once, in the order of the calls: not while the
 // stream is being captured, where they would run at the replay.
 static int moves_allowed(hale_kv_cache* kv, const char* what) {
-  KVCHK(kv->ctx, hipSetDevice(kv->ctx->device));
+  CALL_CHK(kv->ctx, hipSetDevice(kv->ctx->device));
   bool cap = false;
   const int rc = capturing(kv->ctx, &cap);
   if (rc) return rc;
@@ -520,7 +486,7 @@ static int moves_allowed(hale_kv_cache* kv, const char* what) {
 
 extern "C" int hale_kv_seq_copy(hale_kv_cache* kv, uint32_t seq, uint32_t* out) {
   if (!kv || !out) return ctx_fail(kv ? kv->ctx : nullptr, HALE_EINVAL, "kv_seq_copy: NULL argument");
-  KV_TRY
+  CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(kv->ctx->mu);
   int rc = moves_allowed(kv, "kv_seq_copy");
   if (rc) return rc;
@@ -532,27 +498,27 @@ extern "C" int hale_kv_seq_copy(hale_kv_cache* kv, uint32_t seq, uint32_t* out) 
   rc = u.begin(upload_bytes(kv, (len + KV_PAGE - 1) / KV_PAGE * (8 + sizeof(KvCopy))));
   if (!rc) rc = status(kv, "kv_seq_copy", kv->pages.copy(seq, out, &kv->copies, &err), err);
   return rc ? rc : u.end();
-  KV_CATCH(kv->ctx)
+  CALL_CATCH(kv->ctx)
 }
 
 extern "C" int hale_kv_seq_truncate(hale_kv_cache* kv, uint32_t seq, size_t len) {
   if (!kv) return ctx_fail(nullptr, HALE_EINVAL, "kv_seq_truncate: NULL argument");
-  KV_TRY
+  CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(kv->ctx->mu);
   std::string err;
   const int rc = status(kv, "kv_seq_truncate", kv->pages.truncate(seq, len, &err), err);
   if (!rc) leaves_step(kv, seq);
   return rc;
-  KV_CATCH(kv->ctx)
+  CALL_CATCH(kv->ctx)
 }
 
 extern "C" int hale_kv_seq_len(const hale_kv_cache* kv, uint32_t seq, size_t* len) {
   if (!kv || !len) return ctx_fail(kv ? kv->ctx : nullptr, HALE_EINVAL, "kv_seq_len: NULL argument");
-  KV_TRY
+  CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(kv->ctx->mu);
   std::string err;
   return status(const_cast<hale_kv_cache*>(kv), "kv_seq_len", kv->pages.len(seq, len, &err), err);
-  KV_CATCH(kv->ctx)
+  CALL_CATCH(kv->ctx)
 }
 
 extern "C" int hale_kv_pages(const hale_kv_cache* kv, size_t* total, size_t* used) {
@@ -565,7 +531,7 @@ extern "C" int hale_kv_pages(const hale_kv_cache* kv, size_t* total, size_t* use
 
 extern "C" int hale_kv_compact(hale_kv_cache* kv, size_t* moved) {
   if (!kv) return ctx_fail(nullptr, HALE_EINVAL, "kv_compact: NULL argument");
-  KV_TRY
+  CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(kv->ctx->mu);
   int rc = moves_allowed(kv, "kv_compact");
   if (rc) return rc;
@@ -577,13 +543,13 @@ extern "C" int hale_kv_compact(hale_kv_cache* kv, size_t* moved) {
   kv->pages.compact(&kv->copies);
   if (moved) *moved = pages;
   return pages || !kv->pages.dirty.empty() ? u.end() : HALE_OK;
-  KV_CATCH(kv->ctx)
+  CALL_CATCH(kv->ctx)
 }
 
 extern "C" int hale_kv_resize(hale_kv_cache* kv, size_t num_pages) {
   if (!kv) return ctx_fail(nullptr, HALE_EINVAL, "kv_resize: NULL argument");
   hale_ctx* c = kv->ctx;
-  KV_TRY
+  CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(c->mu);
   int rc = moves_allowed(kv, "kv_resize");
   if (rc) return rc;
@@ -614,7 +580,7 @@ extern "C" int hale_kv_resize(hale_kv_cache* kv, size_t num_pages) {
   kv->geom.pool = pool;
   kv->epoch++;
   return HALE_OK;
-  KV_CATCH(c)
+  CALL_CATCH(c)
 }
 
 // ---------------------------------------------------------------------------
@@ -638,19 +604,19 @@ static void put_view(hale_kv_cache* kv, Upload& u, int i) {
 extern "C" int hale_kv_reserve(hale_kv_cache* kv, size_t max_tokens) {
   if (!kv) return ctx_fail(nullptr, HALE_EINVAL, "kv_reserve: NULL argument");
   hale_ctx* c = kv->ctx;
-  KV_TRY
+  CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(c->mu);
-  KVCHK(c, hipSetDevice(c->device));
+  CALL_CHK(c, hipSetDevice(c->device));
   if (max_tokens > (size_t)0x7fffffff / kv->shape.heads)
     return ctx_fail(c, HALE_EINVAL, "kv_reserve: %zu tokens of %zu heads", max_tokens, kv->shape.heads);
   return grow_plan(kv, max_tokens);
-  KV_CATCH(c)
+  CALL_CATCH(c)
 }
 
 extern "C" int hale_kv_step(hale_kv_cache* kv, size_t nseq, const uint32_t* seqs, const uint32_t* ntok) {
   if (!kv || (nseq && (!seqs || !ntok))) return ctx_fail(kv ? kv->ctx : nullptr, HALE_EINVAL, "kv_step: NULL argument");
   hale_ctx* c = kv->ctx;
-  KV_TRY
+  CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(c->mu);
   int rc = moves_allowed(kv, "kv_step");
   if (rc) return rc;
@@ -705,7 +671,7 @@ extern "C" int hale_kv_step(hale_kv_cache* kv, size_t nseq, const uint32_t* seqs
   kv->blocks = blocks.size();
   kv->stepped = true;
   return HALE_OK;
-  KV_CATCH(c)
+  CALL_CATCH(c)
 }
 
 extern "C" int hale_kv_positions(const hale_kv_cache* kv, const int32_t** out) {
@@ -723,7 +689,7 @@ static int layer_call(hale_kv_cache* kv, const char* what, size_t layer, int dty
   if (!float_type(dtype)) return ctx_fail(c, HALE_EINVAL, "%s: dtype %d is not f32, f16 or bf16", what, dtype);
   if (!kv->stepped) return ctx_fail(c, HALE_EINVAL, "%s without a current step", what);
   if (ntok != kv->tokens) return ctx_fail(c, HALE_EINVAL, "%s: %zu tokens, but the step has %zu", what, ntok, kv->tokens);
-  KVCHK(c, hipSetDevice(c->device));
+  CALL_CHK(c, hipSetDevice(c->device));
   int rc = capturing(c, cap);
   if (rc) return rc;
   if (!*cap) return send_pages(kv);  // table changes since the step
@@ -755,7 +721,7 @@ static int note_positions(hale_ctx* c, const int32_t* pos) {
 }
 
 int hale::kv_check_replay(hale_ctx* c, const std::vector<KvUse>& uses) {
-  KVCHK(c, hipSetDevice(c->device));
+  CALL_CHK(c, hipSetDevice(c->device));
   bool cap = false;
   int rc = capturing(c, &cap);
   if (rc) return rc;
@@ -778,7 +744,7 @@ extern "C" int hale_kv_append_device(hale_kv_cache* kv, size_t layer, int dtype,
                                      size_t k_stride, const void* v, size_t v_stride) {
   if (!kv) return ctx_fail(nullptr, HALE_EINVAL, "kv_append: NULL argument");
   hale_ctx* c = kv->ctx;
-  KV_TRY
+  CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(c->mu);
   if (float_type(dtype) && ntok) {
     const size_t row = kv->shape.kv_heads * kv->shape.head_dim;
@@ -804,16 +770,16 @@ extern "C" int hale_kv_append_device(hale_kv_cache* kv, size_t layer, int dtype,
   a.vec = both % 16 == 0;  // head_dim is a multiple of 16
   // later steps of these tokens may touch one block more per sequence
   const size_t grid = cap ? kv_max_blocks(ntok, kv->seqs.size()) : kv->blocks;
-  KV_LAUNCH(c, K_KV_STORE, launch_kv_append(dtype, a, (unsigned)grid, c->stream));
+  CALL_LAUNCH(c, K_KV_STORE, launch_kv_append(dtype, a, (unsigned)grid, c->stream));
   return HALE_OK;
-  KV_CATCH(c)
+  CALL_CATCH(c)
 }
 
 extern "C" int hale_kv_attention_device(hale_kv_cache* kv, size_t layer, int dtype, size_t ntok, const void* q,
                                         size_t q_stride, float scale, size_t window, void* out, size_t out_stride) {
   if (!kv) return ctx_fail(nullptr, HALE_EINVAL, "kv_attention: NULL argument");
   hale_ctx* c = kv->ctx;
-  KV_TRY
+  CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(c->mu);
   // scores are in powers of two: scale log2(e) has to be finite as well
   if (!(scale > 0.0f) || !std::isfinite(scale * 2.0f))
@@ -891,20 +857,20 @@ extern "C" int hale_kv_attention_device(hale_kv_cache* kv, size_t layer, int dty
     a.njoins = cap ? 0xffffffffu : (unsigned)njoins;
     const unsigned gi = grid(nitems, tiles + KV_MAX_PARTS), gj = cap ? (unsigned)std::min<size_t>(tiles, 256) : grid(njoins, 0);
     const unsigned rows = kind ? (unsigned)kv_many_rows(kv->shape.head_dim) : 16u * v.plan.cols;
-    KV_LAUNCH(c, K_KV_ATTENTION, kind ? launch_kv_attend_many(a, gi, c->stream) : launch_kv_attend_few(a, v.plan.cols, gi, c->stream));
+    CALL_LAUNCH(c, K_KV_ATTENTION, kind ? launch_kv_attend_many(a, gi, c->stream) : launch_kv_attend_few(a, v.plan.cols, gi, c->stream));
     unsigned parts = 0;  // of a row, now
     for (const KvJoin& j : kind ? v.plan.many_joins : v.plan.few_joins) parts = std::max(parts, j.parts);
-    KV_LAUNCH(c, K_KV_ATTENTION, launch_kv_join(a, gj, rows, parts, c->stream));
+    CALL_LAUNCH(c, K_KV_ATTENTION, launch_kv_join(a, gj, rows, parts, c->stream));
   }
   return HALE_OK;
-  KV_CATCH(c)
+  CALL_CATCH(c)
 }
 
 extern "C" int hale_kv_read_device(hale_kv_cache* kv, size_t layer, uint32_t seq, size_t first, size_t count, float* k,
                                    float* v) {
   if (!kv) return ctx_fail(nullptr, HALE_EINVAL, "kv_read: NULL argument");
   hale_ctx* c = kv->ctx;
-  KV_TRY
+  CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(c->mu);
   if (layer >= kv->layers) return ctx_fail(c, HALE_EINVAL, "kv_read: layer %zu of %zu", layer, kv->layers);
   size_t len = 0;
@@ -923,9 +889,9 @@ extern "C" int hale_kv_read_device(hale_kv_cache* kv, size_t layer, uint32_t seq
   const size_t row = kv->shape.kv_heads * kv->shape.head_dim;
   for (size_t done = 0; done < count;) {
     const size_t n = kv_read_part(first + done, count - done);
-    KV_LAUNCH(c, K_KV_READ, launch_kv_read(kv->geom, layer, seq, first + done, n, k + done * row, v + done * row, c->stream));
+    CALL_LAUNCH(c, K_KV_READ, launch_kv_read(kv->geom, layer, seq, first + done, n, k + done * row, v + done * row, c->stream));
     done += n;
   }
   return HALE_OK;
-  KV_CATCH(c)
+  CALL_CATCH(c)
 }

@@ -2518,7 +2518,8 @@ extern "C" const char* hale_kernel_name(int kind) {
                                        "repack", "fill", "group", "grouped_gate_up",
                                        "grouped_down", "combine", "copy", "rms_norm",
                                        "attention", "gather", "decode", "stream_read",
-                                       "rope", "kv_store", "kv_read", "kv_pages", "kv_attention"};
+                                       "rope", "kv_store", "kv_read", "kv_pages", "kv_attention",
+                                       "rms_norm_q8", "q4g", "logits"};
   return kind >= 0 && kind < K_KINDS ? names[kind] : "";
 }
 

@@ -1,0 +1,84 @@
+// step_ops.h -- launch interface of the operators around a serving step's
+// layers: norms that hand on 8 bits, products of 4-bit weights with group
+// scales, and the rules on logits (host side: step_ops.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "../../include/hale_moe.h"
+
+namespace hale {
+
+// ---- norms ---------------------------------------------------------------------
+
+struct NormQ8Args {
+  const void *x, *delta;  // [rows][n], a stride of so many elements per row; delta may be null
+  const float* w;
+  void *sum, *y;          // may be null
+  int8_t* q;              // [rows][n]
+  float* scales;          // [rows][n / block]
+  size_t x_stride, delta_stride, sum_stride, y_stride;
+  unsigned n, block;      // block 0: one a row
+  float eps;
+  bool vec;               // all rows (and w) start at multiples of 16 bytes, codes of 8
+};
+constexpr size_t NORM_Q8_MAX = 16384;  // numbers per row
+hipError_t launch_norm_q8(int dtype, const NormQ8Args& a, size_t rows, hipStream_t st);
+
+// ---- 4-bit weights with group scales ---------------------------------------------
+//
+// Tiles of 16 rows, along them chunks of 128 numbers:
+//   codes   16 rows x 128 numbers, lane 16 g + i of a wave 16 bytes: row i,
+//           word j holds numbers 32 j + 8 g .. + 7, number b (b < 4) in bits 8 b ..
+//           8 b + 3 and number 4 + b in bits 8 b + 4 .. 8 b + 7;
+//   scales  [128 / group][16 rows], 16 bits;
+//   zeros   [128 / group][16 rows], a byte; only where the matrix has them.
+// Numbers and rows that pad the last chunk and tile are code 8 (zero 8), scale 0.
+// The matrix instructions take operands of 16 rows x 32 numbers whose lane 16 g + i holds
+// row i, numbers 8 g .. 8 g + 7: a word of codes.
+constexpr unsigned Q4G_CHUNK = 128, Q4G_ROWS = 16;
+
+struct Q4gGeom {
+  uint8_t* data;
+  size_t rows, cols;
+  unsigned group, chunks;       // chunks of 128 numbers per row
+  unsigned per;                 // groups per chunk
+  unsigned chunk_bytes;
+  size_t tile_bytes;
+  bool zeros, bf16;             // bf16: type of the scales (else f16)
+};
+
+hipError_t launch_q4g_pack(const Q4gGeom& g, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros,
+                           hipStream_t st);
+hipError_t launch_q4g_unpack(const Q4gGeom& g, uint8_t* codes, uint16_t* scales, uint8_t* zeros, hipStream_t st);
+
+struct Q4gArgs {
+  Q4gGeom g;
+  const void* x;             // [ntok][cols] of a float type with a stride, or codes
+  const float* x_scales;     // [ntok][cols / x_block] of codes
+  size_t x_stride;           // elements
+  unsigned x_block;          // numbers per scale of codes; cols: one a token
+  size_t ntok;
+  int out_dtype;
+  void* out;                 // [ntok][rows]
+  size_t out_stride;
+  bool vec;                  // x: all rows start at multiples of 16 bytes
+};
+enum Q4gInput : int { Q4G_F32 = 0, Q4G_F16 = 1, Q4G_BF16 = 2, Q4G_I8 = 3 };
+hipError_t launch_q4g(Q4gInput in, const Q4gArgs& a, hipStream_t st);
+
+// ---- logits ------------------------------------------------------------------------
+
+struct LogitsArgs {
+  const void* in;
+  void* out;
+  size_t in_stride, out_stride;
+  size_t vocab;
+  hale_logits_rules r;
+  bool vec;                  // rows of in and out start at multiples of 16 bytes
+};
+hipError_t launch_logits(int dtype, const LogitsArgs& a, size_t rows, hipStream_t st);
+
+}  // namespace hale

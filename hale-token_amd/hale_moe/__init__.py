@@ -17,6 +17,9 @@ names and argument meaning:
 ``KvCache``            keys and values of many sequences in 8 bits, in pages, and
                        their attention (beyond ``LayerCache``,
                        src/model/kv_cache.rs)
+``GroupQ4Matrix``      4-bit weights with a scale (and zero) per group, times one to
+                       many tokens, floats or 8-bit
+``LogitsRules``        penalties, biases and masks of ``logits_device``
 =====================  ==========================================================
 
 Errors follow the reference: shape and length violations (which panic in
@@ -140,6 +143,17 @@ SIGNATURES = {
     "hale_kv_append_device": (C.c_int, [_vp, _sz, C.c_int, _sz, _vp, _sz, _vp, _sz]),
     "hale_kv_attention_device": (C.c_int, [_vp, _sz, C.c_int, _sz, _vp, _sz, C.c_float, _sz, _vp, _sz]),
     "hale_kv_read_device": (C.c_int, [_vp, _sz, C.c_uint32, _sz, _sz, _vp, _vp]),
+    "hale_rms_norm_q8_device": (C.c_int, [_vp, C.c_int, _sz, _sz, _vp, _sz, _vp, _sz, _vp, C.c_float, _sz, _vp, _sz,
+                                          _vp, _sz, _vp, _vp]),
+    "hale_q4g_upload": (C.c_int, [_vp, _sz, _sz, _sz, C.c_int, _vp, _vp, _vp, C.POINTER(_vp)]),
+    "hale_q4g_upload_device": (C.c_int, [_vp, _sz, _sz, _sz, C.c_int, _vp, _vp, _vp, C.POINTER(_vp)]),
+    "hale_q4g_destroy": (None, [_vp]),
+    "hale_q4g_shape": (C.c_int, [_vp, C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz), C.POINTER(C.c_int),
+                                 C.POINTER(C.c_int)]),
+    "hale_q4g_download": (C.c_int, [_vp, _vp, _vp, _vp]),
+    "hale_q4g_matmul_device": (C.c_int, [_vp, C.c_int, _sz, _vp, _sz, _vp, _sz]),
+    "hale_q4g_matmul_q8_device": (C.c_int, [_vp, _sz, _sz, _vp, _vp, C.c_int, _vp, _sz]),
+    "hale_logits_device": (C.c_int, [_vp, C.c_int, _sz, _sz, _vp, _sz, _vp, _vp, _sz]),
     "hale_device_malloc": (C.c_int, [_vp, _sz, C.POINTER(_vp)]),
     "hale_device_free": (C.c_int, [_vp, _vp]),
     "hale_memcpy_htod": (C.c_int, [_vp, _vp, _vp, _sz]),
@@ -983,6 +997,97 @@ class KvCache:
             self.close()
         except Exception:
             pass
+
+
+def rms_norm_q8_device(ctx: "Context", dtype, rows: int, n: int, d_x: int, d_weight: int, eps: float, d_quants: int,
+                       d_scales: int, *, block: int = 32, d_delta: int = 0, d_sum: int = 0, d_y: int = 0,
+                       x_stride: int = 0, delta_stride: int = 0, sum_stride: int = 0, y_stride: int = 0):
+    """Rows x (+ delta) normed and handed on as 8-bit codes with a scale per
+    block (device addresses; strides 0: without gaps)."""
+    ctx.check(lib().hale_rms_norm_q8_device(ctx.handle, parse_dtype(dtype), rows, n, _vp(d_x), x_stride or n,
+                                            _vp(d_delta), delta_stride or n, _vp(d_weight), eps, block, _vp(d_sum),
+                                            sum_stride or n, _vp(d_y), y_stride or n, _vp(d_quants), _vp(d_scales)),
+              "rms_norm_q8")
+
+
+class GroupQ4Matrix:
+    """4-bit weights scale * (code - zero) with a scale, and perhaps a zero, per
+    group of 32, 64 or 128 numbers of a row."""
+
+    def __init__(self, ctx: "Context", handle, rows: int, cols: int, group: int):
+        self.ctx, self.handle = ctx, handle
+        self.rows, self.cols, self.group = rows, cols, group
+        ctx.adopt(self)
+
+    @classmethod
+    def new(cls, ctx: "Context", rows: int, cols: int, group: int, codes, scales, zeros=None,
+            scale_dtype="f16") -> "GroupQ4Matrix":
+        """codes [rows][cols / 2] bytes (the first number in the low half), scales
+        [rows][cols / group] of 16 bits, zeros [rows][cols / group] bytes or None (8)."""
+        c = np.ascontiguousarray(codes, dtype=np.uint8).reshape(-1)
+        s = np.ascontiguousarray(scales)
+        s = s.view(np.uint16).reshape(-1)
+        z = None if zeros is None else np.ascontiguousarray(zeros, dtype=np.uint8).reshape(-1)
+        groups = rows * (cols // group) if group else 0
+        if c.size != rows * (cols // 2) or s.size != groups or (z is not None and z.size != groups):
+            raise ValueError("GroupQ4Matrix: codes, scales or zeros of another size")
+        h = _vp()
+        ctx.check(lib().hale_q4g_upload(ctx.handle, rows, cols, group, parse_dtype(scale_dtype), c.ctypes.data,
+                                        s.ctypes.data, z.ctypes.data if z is not None else None, C.byref(h)), "q4g")
+        return cls(ctx, h, rows, cols, group)
+
+    @classmethod
+    def from_device(cls, ctx: "Context", rows: int, cols: int, group: int, d_codes: int, d_scales: int,
+                    d_zeros: int = 0, scale_dtype="f16") -> "GroupQ4Matrix":
+        h = _vp()
+        ctx.check(lib().hale_q4g_upload_device(ctx.handle, rows, cols, group, parse_dtype(scale_dtype), _vp(d_codes),
+                                               _vp(d_scales), _vp(d_zeros), C.byref(h)), "q4g")
+        return cls(ctx, h, rows, cols, group)
+
+    def download(self) -> tuple:
+        """(codes, scales as 16 bits, zeros) as they were given (zeros 8 where none were)."""
+        groups = self.cols // self.group
+        c = np.empty((self.rows, self.cols // 2), np.uint8)
+        s, z = np.empty((self.rows, groups), np.uint16), np.empty((self.rows, groups), np.uint8)
+        self.ctx.check(lib().hale_q4g_download(self.handle, c.ctypes.data, s.ctypes.data, z.ctypes.data), "q4g")
+        return c, s, z
+
+    def matmul_device(self, dtype, ntok: int, d_x: int, d_out: int, *, x_stride: int = 0, out_stride: int = 0):
+        """d_out [ntok][rows] = d_x [ntok][cols] times the weights, both of dtype."""
+        self.ctx.check(lib().hale_q4g_matmul_device(self.handle, parse_dtype(dtype), ntok, _vp(d_x),
+                                                    x_stride or self.cols, _vp(d_out), out_stride or self.rows), "q4g")
+
+    def matmul_q8_device(self, dtype, ntok: int, d_quants: int, d_scales: int, d_out: int, *, block: int = 32,
+                         out_stride: int = 0):
+        """The same for 8-bit codes with a scale per block; dtype: of d_out."""
+        self.ctx.check(lib().hale_q4g_matmul_q8_device(self.handle, ntok, block, _vp(d_quants), _vp(d_scales),
+                                                       parse_dtype(dtype), _vp(d_out), out_stride or self.rows), "q4g")
+
+    def close(self):
+        if getattr(self, "handle", None) and self.ctx.alive:
+            lib().hale_q4g_destroy(self.handle)
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class LogitsRules(C.Structure):
+    """hale_logits_rules: device addresses (0: that part is left out) and counts."""
+
+    _fields_ = [("tokens", _vp), ("token_start", _vp), ("ntokens", _sz), ("prompt_len", _vp), ("repetition", _vp),
+                ("frequency", _vp), ("presence", _vp), ("bias_tokens", _vp), ("bias", _vp), ("bias_start", _vp),
+                ("nbiases", _sz), ("mask", _vp), ("mask_rows", _sz), ("mask_stride", _sz), ("mask_row", _vp)]
+
+
+def logits_device(ctx: "Context", dtype, rows: int, vocab: int, d_logits: int, rules: LogitsRules, d_out: int, *,
+                  stride: int = 0, out_stride: int = 0):
+    """Penalties, biases and masks on rows of logits (d_out may be d_logits)."""
+    ctx.check(lib().hale_logits_device(ctx.handle, parse_dtype(dtype), rows, vocab, _vp(d_logits), stride or vocab,
+                                       C.byref(rules), _vp(d_out), out_stride or vocab), "logits")
 
 
 @dataclass(frozen=True)

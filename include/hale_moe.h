@@ -554,6 +554,119 @@ int hale_rope_device(hale_rope *rope, int dtype, size_t rows,
                      size_t q_out_stride, const void *d_k, size_t k_heads,
                      size_t k_stride, void *d_k_out, size_t k_out_stride);
 
+/* ---- norms that hand on 8 bits ----------------------------------------------
+ * No counterpart in the reference, which quantizes activations apart from their
+ * norm (Q8Activations::quantize); for callers that hand rows to 8-bit products. */
+
+/* For each of `rows` rows of n numbers (dtype HALE_F32, HALE_F16 or HALE_BF16):
+ *   s = x + delta, in f32, rounded to dtype (x where d_delta is NULL);
+ *   u = s * weight;  r = 1 / sqrt(sum(s^2) / n + eps);
+ *   scale = r * max |u| / 127 over each block of `block` numbers, rounded to f32;
+ *   code  = 127 u / max |u|, rounded to the nearest whole number (ties to even);
+ *   y     = r * u, rounded to dtype.
+ * Sums and products are 64 bits.  d_sum (NULL: not wanted) receives s, d_y (NULL: not
+ * wanted) y, d_quants [rows][n] the codes, d_scales [rows][n / block] the scales: the
+ * form of hale_quantize_q8_act for blocks of 32 (whose codes round ties away from 0).
+ * block: 32, 64, 128 or n; n a multiple of block and of 32, at most 16384.  Strides count
+ * elements from row to row, at least n.  A block of zeros has scale 0 and codes 0.  A
+ * row with a number that is not finite (or of zeros with eps 0) has scales NaN, codes 0
+ * and y NaN; a block whose weights are not finite has scale NaN and codes 0.
+ * d_sum and d_y may each be d_x or d_delta with that one's stride (not both the same);
+ * otherwise no output may overlap an input or another output.  eps: not negative.
+ * Enqueued on the context's stream. */
+int hale_rms_norm_q8_device(hale_ctx *ctx, int dtype, size_t rows, size_t n,
+                            const void *d_x, size_t x_stride,
+                            const void *d_delta, size_t delta_stride,
+                            const float *d_weight, float eps, size_t block,
+                            void *d_sum, size_t sum_stride, void *d_y,
+                            size_t y_stride, int8_t *d_quants, float *d_scales);
+
+/* ---- products of 4-bit weights with group scales -----------------------------
+ * No counterpart in the reference, whose 4-bit rows (HALE_Q4_0) have blocks of 32
+ * without zeros and take one f32 activation at a time; for checkpoints whose
+ * weights come with a scale, and perhaps a zero, per group. */
+
+typedef struct hale_q4g hale_q4g;
+
+/* A matrix of rows x cols weights scale * (code - zero): codes [rows][cols / 2], two to
+ * a byte, the first in the low half; scales [rows][cols / group] of scale_dtype
+ * (HALE_F16 or HALE_BF16); zeros [rows][cols / group], a byte of 0..15 each, or NULL
+ * where all are 8.  group: 32, 64 or 128; cols a multiple of it.  The bytes are laid
+ * out anew in device memory; both forms return when they have been read. */
+int hale_q4g_upload(hale_ctx *ctx, size_t rows, size_t cols, size_t group,
+                    int scale_dtype, const uint8_t *codes, const void *scales,
+                    const uint8_t *zeros, hale_q4g **out);
+/* Same from device memory (of zeros above 15 the low four bits count). */
+int hale_q4g_upload_device(hale_ctx *ctx, size_t rows, size_t cols,
+                           size_t group, int scale_dtype,
+                           const uint8_t *d_codes, const void *d_scales,
+                           const uint8_t *d_zeros, hale_q4g **out);
+void hale_q4g_destroy(hale_q4g *m);
+/* Any output may be NULL.  has_zeros: whether it was given zeros. */
+int hale_q4g_shape(const hale_q4g *m, size_t *rows, size_t *cols, size_t *group,
+                   int *scale_dtype, int *has_zeros);
+/* The matrix back as it was given, into host memory (zeros may be NULL; 8 where
+ * it has none). */
+int hale_q4g_download(hale_q4g *m, uint8_t *codes, void *scales, uint8_t *zeros);
+
+/* out[t][r] = sum_k weight[r][k] * x[t][k] for ntok tokens: d_x [ntok][cols] and d_out
+ * [ntok][rows] of dtype (HALE_F32, HALE_F16, HALE_BF16), strides in elements from token
+ * to token.  Each group's sum of products, and of x, is formed of exact products in
+ * f32, and the groups' sums in f32; results are rounded once.  Equal calls give equal
+ * bits; a token's results do not depend on what the others hold (on how many they are,
+ * in their last bits).  A token with a number that is not finite gives results that are
+ * not finite (NaN where the formula has an infinity).  d_out may not overlap d_x.
+ * Enqueued on the context's stream. */
+int hale_q4g_matmul_device(hale_q4g *m, int dtype, size_t ntok, const void *d_x,
+                           size_t x_stride, void *d_out, size_t out_stride);
+/* Same for tokens of 8-bit codes with a scale per `block` numbers (32, 64, 128 or cols),
+ * as hale_rms_norm_q8_device and hale_quantize_q8_act give them: d_quants [ntok][cols]
+ * (at a multiple of 8 bytes), d_scales [ntok][cols / block].  Sums within a group and
+ * block are whole numbers, between them f32.  dtype: of d_out. */
+int hale_q4g_matmul_q8_device(hale_q4g *m, size_t ntok, size_t block,
+                              const int8_t *d_quants, const float *d_scales,
+                              int dtype, void *d_out, size_t out_stride);
+
+/* ---- rules on logits -----------------------------------------------------------
+ * No counterpart in the reference, whose sampler takes the logits as they are. */
+
+/* All pointers are device memory; a part whose first pointer is NULL is left out.
+ * Ranges [start[r], start[r + 1]) are taken within 0 .. the count. */
+typedef struct {
+  /* row r's tokens: its prompt_len[r] first ones are the prompt (NULL: none), the
+   * others were generated */
+  const int32_t *tokens;
+  const int64_t *token_start; /* [rows + 1]                                       */
+  size_t ntokens;
+  const int64_t *prompt_len;  /* [rows]                                           */
+  const float *repetition;    /* [rows], NULL: 1                                  */
+  const float *frequency;     /* [rows], NULL: 0                                  */
+  const float *presence;      /* [rows], NULL: 0                                  */
+  /* row r's biases; of several for one token the last counts                     */
+  const int32_t *bias_tokens;
+  const float *bias;
+  const int64_t *bias_start;  /* [rows + 1]                                       */
+  size_t nbiases;
+  /* masks of vocab bits, token t bit t % 32 of word t / 32                       */
+  const uint32_t *mask;
+  size_t mask_rows, mask_stride; /* strides in words                              */
+  const int32_t *mask_row;    /* [rows] the row's mask, outside 0 .. mask_rows - 1
+                                 for none; NULL: row r has mask r                 */
+} hale_logits_rules;
+
+/* For each of `rows` rows of logits (dtype HALE_F32, HALE_F16, HALE_BF16; strides in
+ * elements), in f32, rounded once: a token that the row's tokens hold becomes x /
+ * repetition, or x * repetition where x is not positive; one that occurs g > 0
+ * times among the generated ones loses frequency * g, then presence; a bias is added;
+ * and a token whose mask bit is 0 becomes -inf.  Tokens outside the vocabulary are passed
+ * over.  A logit that no rule names keeps its bits.  vocab at most 2^26, ntokens and
+ * nbiases below 2^31.  d_out may be d_logits with the same stride, and may not overlap
+ * anything else.  Enqueued on the context's stream. */
+int hale_logits_device(hale_ctx *ctx, int dtype, size_t rows, size_t vocab,
+                       const void *d_logits, size_t stride,
+                       const hale_logits_rules *rules, void *d_out,
+                       size_t out_stride);
+
 /* ---- paged 8-bit key/value cache and its attention ----------------------
  * No counterpart in the reference, whose LayerCache (src/model/kv_cache.rs)
  * holds one sequence's f32 keys and values; for callers that serve many
