@@ -815,6 +815,82 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a) {
   }
 }
 
+// Joins a row's partial results over its own pages with those over shared ones: SLICES
+// groups of threads take every so many'th part of the series laid end to end, four numbers of
+// the head dimension a thread, and put theirs together in LDS in the slices' order.
+constexpr int SHARE_SLICES = 4;
+static_assert(KV_SHARE_PARTS <= 1u << JOIN_BITS, "the sum of a row's parts");
+
+__global__ __launch_bounds__(256) void k_kv_join_shared(KvAttnArgs a) {
+  constexpr int S = SHARE_SLICES;
+  __shared__ f32x4 sv[256];
+  __shared__ float2 sml[256];
+  const int t = threadIdx.x;
+  const int quads = a.g.hd / 4, lanes = quads <= 16 ? 16 : quads <= 32 ? 32 : 64, x = t % lanes;
+  const int slice = t / lanes % S, per = 256 / lanes / S;
+  const unsigned njoins = a.njoins != 0xffffffffu ? a.njoins : a.counts[2];
+  for (unsigned it = blockIdx.x; it < njoins; it += gridDim.x) {
+    const KvShareJoin join = a.share_joins[it];
+    const unsigned row = blockIdx.y * per + t / lanes / S;
+    const bool mine = row < join.rows && x < quads;
+    float top = -__builtin_inff(), most = 0.0f, total = 0.0f;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    int e = 0;
+    if (mine) {
+      auto each = [&](auto&& f) {
+        unsigned from = slice;
+#pragma unroll
+        for (int s = 0; s <= KV_SHARE_LEVELS; s++) {
+          if (s >= (int)join.n) break;
+          const KvSeries& r = join.of[s];
+#pragma unroll 4
+          for (; from < r.parts; from += S) f((size_t)r.part0 + row + (size_t)from * r.step);
+          from -= r.parts;
+        }
+      };
+      each([&](size_t at) {
+        const float2 part = a.part_ml[at];
+        top = fmaxf(top, part.x);
+        most = fmaxf(most, part.y);
+      });
+      e = above(most) + JOIN_BITS;  // 2^e is above the sum
+      const float base2 = top == -__builtin_inff() ? 0.0f : top;
+      each([&](size_t at) {
+        const float2 part = a.part_ml[at];
+        const float w = exp2_fast(part.x - base2);
+        total += w * part.y;
+        v = v + *(const f32x4*)(a.part_o + at * a.g.hd + 4 * x) * (w * pow2(above(part.y) - e));
+      });
+      // as large as values, times 2^-above(total)
+      v = scaled(v, e - above(total));
+    }
+    __syncthreads();  // the join before is read
+    sv[t] = v;
+    sml[t] = float2{top, total};
+    __syncthreads();
+    if (!mine || slice) continue;
+    float f[S], sums[S];
+    top = -__builtin_inff();
+    total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < S; k++) top = fmaxf(top, sml[t + k * lanes].x);
+    const float base2 = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+    for (int k = 0; k < S; k++) {
+      f[k] = exp2_fast(sml[t + k * lanes].x - base2);
+      sums[k] = sml[t + k * lanes].y;
+      total += f[k] * sums[k];
+    }
+    e = above(total);
+    v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < S; k++) v = v + sv[t + k * lanes] * __builtin_ldexpf(f[k], above(sums[k]) - e);
+    const unsigned tok = (join.row0 + row) / (unsigned)a.g.group;
+    const unsigned h = join.head * a.g.group + (join.row0 + row) % (unsigned)a.g.group;
+    store4(a.dtype, a.out, (size_t)(join.tok0 + tok) * a.out_stride + (size_t)h * a.g.hd + 4 * x, a.vec, v * (pow2(e) / total));
+  }
+}
+
 template <typename T, int KC>
 static hipError_t few_sized(const KvAttnArgs& a, int cols, unsigned grid, hipStream_t st) {
   if (cols == 1) return launch(k_kv_attend_few<T, KC, 1>, grid, 64 * ATT_WAVES, 0, st, a);
@@ -862,6 +938,10 @@ hipError_t launch_kv_attend_many(const KvAttnArgs& a, unsigned grid, hipStream_t
 
 hipError_t launch_kv_join(const KvAttnArgs& a, unsigned grid, unsigned rows, unsigned parts, hipStream_t st) {
   if (grid == 0) return hipSuccess;
+  if (a.kind == 2) {
+    const unsigned lanes = a.g.hd <= 64 ? 16 : a.g.hd <= 128 ? 32 : 64, per = 256 / lanes / SHARE_SLICES;
+    return launch(k_kv_join_shared, dim3(grid, (rows + per - 1) / per), 256, 0, st, a);
+  }
   // (with the attention, by row / rows together: 16 sequences of 1000, 4 parts 13.3 / 11.9 us;
   // of 6000, 8 parts 25.1 / 24.1; 4 of 3000, 12 parts 11.5 / 11.7; one of 131000, 512 parts
   // 31.1 / 54.5.  Many rows are the more work-groups: 300 behind 8000 102 / 68.)

@@ -108,9 +108,10 @@ struct KvAttnArgs {
   int window;                  // 0: none
   const KvItem* items;         // of one kind
   const KvJoin* joins;
-  const uint32_t* counts;      // {few, many, joins of few, of many} of the plan, on the device
+  const KvShareJoin* share_joins;  // of kind 2
+  const uint32_t* counts;      // {few, many, joins of few (or all, of kind 2), of many} of the plan, on the device
   unsigned nitems, njoins;     // the same, or 0xffffffff: read counts (captured calls)
-  int kind;                    // 0: items and joins of few rows, 1: of many
+  int kind;                    // 0: items and joins of few rows, 1: of many; 2: joins of shared pages
   float* part_o;               // [row][hd], times a power of two that follows from the sum
   float2* part_ml;             // [row] running maximum (base 2) and sum
   bool vec;                    // q and out rows start at multiples of four elements
@@ -120,7 +121,7 @@ struct KvAttnArgs {
 hipError_t launch_kv_attend_few(const KvAttnArgs& a, int cols, unsigned grid, hipStream_t st);
 // Of many rows: kv_many_rows per work-group.
 hipError_t launch_kv_attend_many(const KvAttnArgs& a, unsigned grid, hipStream_t st);
-// Joins of one kind, of at most `rows` rows each.
+// Joins of one kind, of at most `rows` rows each; parts: of a row, at most (kinds 0 and 1).
 hipError_t launch_kv_join(const KvAttnArgs& a, unsigned grid, unsigned rows, unsigned parts, hipStream_t st);
 
 // ---- rotary positions --------------------------------------------------------

@@ -175,6 +175,7 @@ struct hale_kv_cache {
   uint32_t* plan = nullptr;
   Sections at;
   size_t cap_tokens = 0;
+  size_t share = 0;  // least pages that sequences have to have in common, 0: never shared
   float* part_o = nullptr;
   float2* part_ml = nullptr;
   Staging staging[STAGINGS];
@@ -587,18 +588,46 @@ extern "C" int hale_kv_resize(hale_kv_cache* kv, size_t num_pages) {
 // steps
 // ---------------------------------------------------------------------------
 
+// A step's attention in one of the views.
+static void make_plan(const hale_kv_cache* kv, const std::vector<KvStepSeq>& seqs, const View& v, KvPlan* out) {
+  if (kv->share && v.window == 0) kv_plan_shared(kv->shape, seqs, kv->pages, kv->share, v.f32, out);
+  else kv_plan(kv->shape, seqs, v.window, v.f32, out);
+}
 static size_t plan_bytes(const KvPlan& p) {
-  return (p.few.size() + p.many.size()) * sizeof(KvItem) + (p.few_joins.size() + p.many_joins.size()) * sizeof(KvJoin) + 32;
+  return (p.few.size() + p.many.size()) * sizeof(KvItem) + (p.few_joins.size() + p.many_joins.size()) * sizeof(KvJoin) +
+         p.share_joins.size() * sizeof(KvShareJoin) + 32;
 }
 static void put_view(hale_kv_cache* kv, Upload& u, int i) {
   View& v = kv->views[i];
-  const uint32_t n[4] = {(uint32_t)v.plan.few.size(), (uint32_t)v.plan.many.size(), (uint32_t)v.plan.few_joins.size(),
-                         (uint32_t)v.plan.many_joins.size()};
+  const uint32_t n[4] = {(uint32_t)v.plan.few.size(), (uint32_t)v.plan.many.size(),
+                         (uint32_t)(v.plan.shared ? v.plan.share_joins.size() : v.plan.few_joins.size()), (uint32_t)v.plan.many_joins.size()};
   u.put(kv->plan + kv->at.counts + 4 + 4 * i, n, sizeof n);
   u.put(kv->plan + kv->at.items[i], v.plan.few.data(), v.plan.few.size() * sizeof(KvItem));
   u.put(kv->plan + kv->at.items[i] + kv->at.many, v.plan.many.data(), v.plan.many.size() * sizeof(KvItem));
+  // in the place of both kinds of joins: as many of these as there are of those take twice one kind's room
+  static_assert(sizeof(KvShareJoin) == 2 * sizeof(KvJoin), "the sections' sizes");
+  u.put(kv->plan + kv->at.joins[i], v.plan.share_joins.data(), v.plan.share_joins.size() * sizeof(KvShareJoin));
   u.put(kv->plan + kv->at.joins[i], v.plan.few_joins.data(), v.plan.few_joins.size() * sizeof(KvJoin));
   u.put(kv->plan + kv->at.joins[i] + kv->at.many_joins, v.plan.many_joins.data(), v.plan.many_joins.size() * sizeof(KvJoin));
+}
+
+extern "C" int hale_kv_share_prefixes(hale_kv_cache* kv, size_t min_len) {
+  if (!kv) return ctx_fail(nullptr, HALE_EINVAL, "kv_share_prefixes: NULL argument");
+  hale_ctx* c = kv->ctx;
+  CALL_TRY
+  std::lock_guard<std::recursive_mutex> lk(c->mu);
+  CALL_CHK(c, hipSetDevice(c->device));
+  bool cap = false;
+  const int rc = capturing(c, &cap);
+  if (rc) return rc;
+  if (cap) return ctx_fail(c, HALE_EINVAL, "kv_share_prefixes while the stream is being captured");
+  const size_t pages = std::min(min_len, kv->pages.max_len() + KV_PAGE) / KV_PAGE + (min_len % KV_PAGE != 0);
+  if (pages == kv->share) return HALE_OK;
+  kv->share = pages;
+  kv->stepped = false;
+  kv->epoch++;  // plans are laid out otherwise: graphs hold the launches of the former ones
+  return HALE_OK;
+  CALL_CATCH(c)
 }
 
 extern "C" int hale_kv_reserve(hale_kv_cache* kv, size_t max_tokens) {
@@ -648,7 +677,7 @@ extern "C" int hale_kv_step(hale_kv_cache* kv, size_t nseq, const uint32_t* seqs
   size_t bytes = tokens * 4 + blocks.size() * sizeof(KvBlock) + 64;
   bytes += kv->pages.step_changes() * 8 + kv->pages.step_copies() * sizeof(KvCopy);
   for (int i = 0; i < kv->nviews; i++) {
-    kv_plan(kv->shape, next, kv->views[i].window, kv->views[i].f32, &kv->views[i].next);
+    make_plan(kv, next, kv->views[i], &kv->views[i].next);
     bytes += plan_bytes(kv->views[i].next);
   }
   Upload u(kv);
@@ -730,7 +759,7 @@ int hale::kv_check_replay(hale_ctx* c, const std::vector<KvUse>& uses) {
     if (std::find(c->kvs.begin(), c->kvs.end(), u.kv) == c->kvs.end() || u.kv->serial != u.serial)
       return ctx_fail(c, HALE_EINVAL, "graph_launch: its key/value cache is gone");
     if (u.kv->epoch != u.epoch)
-      return ctx_fail(c, HALE_EINVAL, "graph_launch: its key/value cache's buffers grew since the capture");
+      return ctx_fail(c, HALE_EINVAL, "graph_launch: its key/value cache's buffers grew, or its sharing changed, since the capture");
     if (!u.step) continue;
     if (!u.kv->stepped || u.kv->step_shape != u.shape)
       return ctx_fail(c, HALE_EINVAL, "graph_launch: the key/value cache's step is not of the captured tokens per sequence");
@@ -811,7 +840,7 @@ extern "C" int hale_kv_attention_device(hale_kv_cache* kv, size_t layer, int dty
     View& v = kv->views[i];
     v.window = window;
     v.f32 = f32;
-    kv_plan(kv->shape, kv->seqs, window, f32, &v.plan);
+    make_plan(kv, kv->seqs, v, &v.plan);
     Upload u(kv);
     rc = u.begin(upload_bytes(kv, plan_bytes(v.plan)));
     if (rc) return rc;
@@ -847,6 +876,28 @@ extern "C" int hale_kv_attention_device(hale_kv_cache* kv, size_t layer, int dty
   const size_t limit = kv_few_limit(kv->shape, kv->seqs, f32);
   bool few = false, many = false;
   for (const KvStepSeq& s : kv->seqs) (s.ntok * kv->shape.group() <= limit ? few : many) |= s.ntok > 0;
+  if (v.plan.shared) {
+    // captured: later steps of these tokens may share otherwise, so both kinds and their joins
+    a.nitems = a.njoins = 0xffffffffu;
+    unsigned rows = 0;
+    for (const KvStepSeq& q : kv->seqs) rows = std::max(rows, std::min<unsigned>(q.ntok * kv->shape.group(), kv_many_rows(kv->shape.head_dim)));
+    for (int kind = 0; kind < 2; kind++) {
+      const size_t n = (kind ? v.plan.many : v.plan.few).size();
+      if (!n && !cap) continue;
+      a.kind = kind;
+      a.items = kind ? items + kv->at.many * 4 / sizeof(KvItem) : items;
+      if (!cap) a.nitems = (unsigned)n;
+      const unsigned gi = grid(cap ? std::max<size_t>(n, 1) : n, tiles + KV_MAX_PARTS);
+      CALL_LAUNCH(c, K_KV_ATTENTION, kind ? launch_kv_attend_many(a, gi, c->stream) : launch_kv_attend_few(a, v.plan.cols, gi, c->stream));
+    }
+    a.kind = 2;
+    a.share_joins = (const KvShareJoin*)joins;
+    const size_t n = v.plan.share_joins.size();
+    if (!cap) a.njoins = (unsigned)n;
+    if (n || cap)
+      CALL_LAUNCH(c, K_KV_ATTENTION, launch_kv_join(a, (unsigned)(cap ? std::min<size_t>(tiles, 256) : std::min<size_t>(n, 1u << 20)), rows, 0, c->stream));
+    return HALE_OK;
+  }
   for (int kind = 0; kind < 2; kind++) {
     if (!(kind ? many : few)) continue;
     const size_t nitems = (kind ? v.plan.many : v.plan.few).size(), njoins = (kind ? v.plan.many_joins : v.plan.few_joins).size();

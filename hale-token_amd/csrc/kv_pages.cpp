@@ -217,6 +217,20 @@ KvPages::Status KvPages::step(size_t nseq, const uint32_t* seqs, const uint32_t*
   return OK;
 }
 
+// A page that two sequences hold came to them by a fork, and all pages before it did,
+// since only last pages are ever exchanged, added or dropped: so the common ones are found
+// by halving.
+size_t KvPages::common(uint32_t a, uint32_t b, size_t most) const {
+  const auto &p = seqs_[a].pages, &q = seqs_[b].pages;
+  size_t lo = 0, hi = std::min(most, std::min(p.size(), q.size()));
+  while (lo < hi) {
+    const size_t mid = (lo + hi + 1) / 2;
+    if (p[mid - 1] == q[mid - 1]) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
 void KvPages::compact_size(size_t* moved, size_t* entries) const {
   const size_t n = used();
   *moved = *entries = 0;
@@ -379,6 +393,8 @@ void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window
   out->many.clear();
   out->few_joins.clear();
   out->many_joins.clear();
+  out->share_joins.clear();
+  out->shared = false;
   out->part_rows = 0;
   const size_t group = s.group(), few_rows = kv_few_rows(s.head_dim), many_rows = kv_many_rows(s.head_dim);
   const size_t limit = kv_few_limit(s, seqs, f32);
@@ -408,6 +424,155 @@ void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window
   divide(few, std::max<size_t>(4, ceil_div(count_pages(few), KV_FEW_GROUPS)), 16 * (size_t)out->cols, &out->few, &out->few_joins,
          &out->part_rows);
   if (!many.empty()) divide(many, many_each(many), many_rows, &out->many, &out->many_joins, &out->part_rows);
+  spread(&out->many);
+}
+
+namespace {
+
+// Pages page0 .. page1 - 1, which sequences first .. last - 1 of the step (of those with
+// tokens) all hold.
+struct Shared {
+  size_t first, last;
+  uint32_t page0, page1;
+  uint32_t rows = 0, part = 0, parts = 0;  // of a head; `part` of head 0
+  bool few = false;
+};
+
+// Which sequences share which pages, from the whole step downward: a run of sequences
+// shares what its least similar neighbours have in common, and falls into the runs
+// between those.
+void find_shared(const std::vector<const KvStepSeq*>& seqs, const KvPages& pages, size_t min_pages, std::vector<Shared>* out) {
+  const size_t n = seqs.size();
+  out->clear();
+  if (n < 2 || n > KV_SHARE_SEQS) return;
+  std::vector<size_t> common(n - 1);
+  for (size_t i = 0; i + 1 < n; i++)  // whole pages that neither writes to in this step
+    common[i] = pages.common(seqs[i]->row, seqs[i + 1]->row, std::min(seqs[i]->len0, seqs[i + 1]->len0) / KV_PAGE);
+  struct Run {
+    size_t first, last, page0;
+    int level;
+  };
+  std::vector<Run> todo{{0, n, 0, 0}};
+  while (!todo.empty()) {
+    Run r = todo.back();
+    todo.pop_back();
+    const size_t least = *std::min_element(common.begin() + r.first, common.begin() + r.last - 1);
+    if (least >= r.page0 + min_pages) {
+      out->push_back({r.first, r.last, (uint32_t)r.page0, (uint32_t)least});
+      r.page0 = least;
+      if (++r.level == KV_SHARE_LEVELS) continue;
+    }
+    for (size_t i = r.first, from = r.first; i < r.last; i++)
+      if (i + 1 == r.last || common[i] == least) {
+        if (i > from) todo.push_back({from, i + 1, r.page0, r.level});
+        from = i + 1;
+      }
+  }
+}
+
+}  // namespace
+
+void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const KvPages& pages, size_t min_pages, bool f32,
+                    KvPlan* out) {
+  const size_t group = s.group(), few_rows = kv_few_rows(s.head_dim), many_rows = kv_many_rows(s.head_dim);
+  const size_t limit = kv_few_limit(s, seqs, f32);
+  std::vector<const KvStepSeq*> with;  // tokens: theirs lie one behind the other
+  size_t most = 0, tokens = 0;
+  for (const KvStepSeq& q : seqs) {
+    if (q.ntok) with.push_back(&q);
+    if (q.ntok * group <= limit) most = std::max(most, q.ntok * group);
+    tokens += q.ntok;
+  }
+  const size_t room = kv_max_items(s, tokens, seqs.size());
+  std::vector<Shared> shared;
+  find_shared(with, pages, min_pages, &shared);
+  for (;;) {  // without sharing where its partial results or lists exceed what there is room for
+    out->few.clear();
+    out->many.clear();
+    out->few_joins.clear();
+    out->many_joins.clear();
+    out->share_joins.clear();
+    out->shared = true;
+    out->cols = most <= 16 ? 1 : 2;
+    std::vector<Tile> few, many;
+    // each sequence's shared pages, from the whole down, and the tiles of the rest
+    std::vector<std::vector<const Shared*>> over(with.size());
+    for (Shared& d : shared) {
+      const KvStepSeq &a = *with[d.first], &b = *with[d.last - 1];
+      d.rows = (uint32_t)((b.tok0 + b.ntok - a.tok0) * group);
+      d.few = d.rows <= 16 * (size_t)out->cols;
+      const size_t rows = d.few ? 16 * (size_t)out->cols : many_rows;
+      for (uint32_t h = 0; h < s.kv_heads; h++)
+        for (size_t r = 0; r < d.rows; r += rows)
+          (d.few ? few : many).push_back({&a, h, (uint32_t)r, (uint32_t)std::min(rows, d.rows - r), d.page0, d.page1});
+      for (size_t i = d.first; i < d.last; i++) over[i].push_back(&d);
+    }
+    const size_t few_shared = few.size(), many_shared = many.size();
+    std::vector<size_t> few_seq, many_seq;  // whose tiles these are
+    for (size_t i = 0; i < with.size(); i++) {
+      const KvStepSeq& q = *with[i];
+      const bool is_few = q.ntok * group <= limit;
+      const size_t rows = is_few ? few_rows : many_rows;
+      for (uint32_t h = 0; h < s.kv_heads; h++)
+        for (size_t t = ceil_div(q.ntok * group, rows); t-- > 0;) {
+          const size_t r = t * rows, n = std::min(rows, q.ntok * group - r);
+          (is_few ? few : many).push_back({&q, h, (uint32_t)r, (uint32_t)n, over[i].empty() ? 0 : over[i].back()->page1,
+                                           (uint32_t)((q.len0 + (r + n - 1) / group) / KV_PAGE + 1)});
+          (is_few ? few_seq : many_seq).push_back(i);
+        }
+    }
+    const size_t each[2] = {std::max<size_t>(4, ceil_div(count_pages(few), KV_FEW_GROUPS)), many.empty() ? 1 : many_each(many)};
+    size_t rows = 0, longest = 0;
+    for (Shared& d : shared) {
+      d.parts = (uint32_t)ceil_div(d.page1 - d.page0, each[!d.few]);
+      d.part = (uint32_t)rows;
+      rows += (size_t)d.rows * d.parts * s.kv_heads;
+      for (uint32_t h = 0; h < s.kv_heads; h++)
+        for (uint32_t p = 0; p < d.parts; p++) {
+          const size_t n = d.page1 - d.page0, tile = d.few ? 16 * (size_t)out->cols : many_rows;
+          const KvStepSeq& a = *with[d.first];
+          // positions behind the shared ones: every row sees all of these
+          for (size_t r = 0; r < d.rows; r += tile)
+            (d.few ? out->few : out->many)
+                .push_back({a.row, d.page1 * (uint32_t)KV_PAGE, a.tok0, (uint16_t)h, (uint16_t)std::min(tile, d.rows - r), (uint32_t)r,
+                            (uint32_t)(d.page0 + n * p / d.parts), (uint32_t)(d.page0 + n * (p + 1) / d.parts),
+                            (uint32_t)(d.part + ((size_t)h * d.parts + p) * d.rows + r)});
+        }
+      if (rows > kv_part_rows(s.head_dim)) break;
+    }
+    for (int kind = 0; kind < 2 && rows <= kv_part_rows(s.head_dim); kind++) {
+      const auto& tiles = kind ? many : few;
+      for (size_t k = kind ? many_shared : few_shared; k < tiles.size(); k++) {
+        const Tile& t = tiles[k];
+        const size_t i = (kind ? many_seq : few_seq)[k - (kind ? many_shared : few_shared)];
+        const size_t n = t.page1 - t.page0, parts = ceil_div(n, each[kind]);
+        const bool joined = parts > 1 || !over[i].empty();
+        if (joined) {
+          KvShareJoin j{t.q->tok0, (uint16_t)t.head, (uint16_t)t.rows, t.row0, 0, {}};
+          size_t sum = parts;
+          for (const Shared* d : over[i]) {
+            const size_t row = (t.q->tok0 - with[d->first]->tok0) * group + t.row0;
+            j.of[j.n++] = {(uint32_t)(d->part + (size_t)t.head * d->parts * d->rows + row), d->parts, d->rows};
+            sum += d->parts;
+          }
+          j.of[j.n++] = {(uint32_t)rows, (uint32_t)parts, t.rows};
+          longest = std::max(longest, sum);
+          out->share_joins.push_back(j);
+        }
+        for (size_t p = 0; p < parts; p++) {
+          (kind ? out->many : out->few)
+              .push_back({t.q->row, t.q->len0, t.q->tok0, (uint16_t)t.head, (uint16_t)t.rows, t.row0, (uint32_t)(t.page0 + n * p / parts),
+                          (uint32_t)(t.page0 + n * (p + 1) / parts), joined ? (uint32_t)rows : KV_WHOLE});
+          if (joined) rows += t.rows;
+        }
+        if (rows > kv_part_rows(s.head_dim)) break;
+      }
+    }
+    out->part_rows = (uint32_t)rows;
+    if (shared.empty() || (rows <= kv_part_rows(s.head_dim) && longest <= KV_SHARE_PARTS && out->few.size() <= room && out->many.size() <= room))
+      break;
+    shared.clear();
+  }
   spread(&out->many);
 }
 

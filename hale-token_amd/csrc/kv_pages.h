@@ -58,12 +58,28 @@ struct KvJoin {
   uint32_t pad[2];
 };
 
+// The join of a row's partial results over its own pages and over those that its
+// sequence shares with its neighbours in the step, on up to so many levels.
+constexpr int KV_SHARE_LEVELS = 3;
+struct KvSeries {
+  uint32_t part0, parts, step;  // as in KvJoin
+};
+struct KvShareJoin {
+  uint32_t tok0;
+  uint16_t head, rows;
+  uint32_t row0;
+  uint32_t n;  // series
+  KvSeries of[KV_SHARE_LEVELS + 1];
+};
+
 // The attention of a step under one window: sequences of few rows (the waves of
 // a work-group share their pages) and of many (the waves share their rows).
 struct KvPlan {
   int cols = 1;  // few: groups of 16 rows per work-group, 1 or 2
   std::vector<KvItem> few, many;
   std::vector<KvJoin> few_joins, many_joins;
+  bool shared = false;  // made by kv_plan_shared: all joins are these
+  std::vector<KvShareJoin> share_joins;
   uint32_t part_rows = 0;
 };
 
@@ -101,9 +117,21 @@ inline size_t kv_part_rows(size_t head_dim) {
 // holds for all later steps of as many.
 size_t kv_few_limit(const KvShape& s, const std::vector<KvStepSeq>& seqs, bool f32);
 
+class KvPages;
+
 // Divides the attention of a step: tiles of rows, and few enough pages each
 // that all compute units take part.  Window 0 sees every earlier position.
 void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window, bool f32, KvPlan* out);
+
+// The same for window 0 where sequences that stand side by side in the step hold the same
+// first pages, at least min_pages of them: the pages are attended over once for all of
+// the sequences' rows, and again so among those that share more behind them.
+void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const KvPages& pages, size_t min_pages,
+                    bool f32, KvPlan* out);
+// Sequences with new tokens in a step up to which pages are shared: finding out who
+// shares what takes up to the square of their number.
+constexpr size_t KV_SHARE_SEQS = 1024;
+constexpr size_t KV_SHARE_PARTS = 1024;  // of a row, over all its series
 
 // Positions that one launch of the reading kernel takes of those first .. first + count - 1: its
 // grid has a work-group of 256 threads per page, and counts threads in 32 bits.
@@ -164,6 +192,8 @@ class KvPages {
   // std::bad_alloc, leaving everything as it was.
   void resize(size_t pages);
 
+  // How many first pages two sequences have in common, of the first `most` of both.
+  size_t common(uint32_t a, uint32_t b, size_t most) const;
   // The page that holds a sequence's position (which it holds).
   uint32_t page_of(uint32_t seq, size_t pos) const { return seqs_[seq].pages[pos / KV_PAGE]; }
   bool live(uint32_t seq) const { return seq < seqs_.size() && seqs_[seq].live; }

@@ -138,6 +138,7 @@ SIGNATURES = {
     "hale_kv_compact": (C.c_int, [_vp, C.POINTER(_sz)]),
     "hale_kv_resize": (C.c_int, [_vp, _sz]),
     "hale_kv_step": (C.c_int, [_vp, _sz, _u32p, _u32p]),
+    "hale_kv_share_prefixes": (C.c_int, [_vp, _sz]),
     "hale_kv_reserve": (C.c_int, [_vp, _sz]),
     "hale_kv_positions": (C.c_int, [_vp, C.POINTER(_vp)]),
     "hale_kv_append_device": (C.c_int, [_vp, _sz, C.c_int, _sz, _vp, _sz, _vp, _sz]),
@@ -939,6 +940,11 @@ class KvCache:
 
     def reserve(self, max_tokens: int):
         self._check(lib().hale_kv_reserve(self.handle, max_tokens), "reserve")
+
+    def share_prefixes(self, min_len: int):
+        """Attention over pages that neighbours in a step have in common, min_len
+        positions or more, is computed once for all of them (0: never)."""
+        self._check(lib().hale_kv_share_prefixes(self.handle, min_len), "share_prefixes")
 
     def step(self, seqs, ntok):
         """Begins a step: ntok[i] new tokens for sequence seqs[i]."""

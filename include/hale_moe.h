@@ -742,6 +742,17 @@ int hale_kv_compact(hale_kv_cache *kv, size_t *moved);
  * graph of the context exists, since graphs keep the pool's address. */
 int hale_kv_resize(hale_kv_cache *kv, size_t num_pages);
 
+/* From the next step on, attention without a window computes over pages that sequences
+ * have in common once for all of them: where sequences that stand side by side in a step
+ * (those without new tokens aside) hold the same whole pages from their start, min_len
+ * positions of them or more, the pages are read for all of their rows together, and those
+ * that some of them share behind these likewise (on up to three levels, each of min_len
+ * positions more; in steps of up to 1024 sequences with tokens).  Forks
+ * (hale_kv_seq_fork) share so what their origin held.  Results are the same but for the order
+ * of sums, so for their last bits.  0, the default: never.  A changed setting ends the current
+ * step, and graphs that use the cache have to be captured anew. */
+int hale_kv_share_prefixes(hale_kv_cache *kv, size_t min_len);
+
 /* Begins a step: ntok[i] new tokens (0 allowed) for sequence seqs[i], all
  * different.  Refused while the context's stream is being captured. */
 int hale_kv_step(hale_kv_cache *kv, size_t nseq, const uint32_t *seqs,
@@ -838,13 +849,13 @@ const char *hale_kernel_name(int kind);
  *     later call outgrows while any graph of the context exists is kept,
  *     not freed, until the last of those graphs is destroyed, so an older
  *     graph replays correctly after a larger call.
- *   - Matrices, layers, attention blocks and rotary tables a graph uses must outlive it.
+ *   - Matrices (4-bit ones too), layers, attention blocks and rotary tables a graph uses must outlive it.
  *   - hale_kv_append_device and hale_kv_attention_device may be captured (call each
  *     window, for f32 or the half types, once before).  A launch works on the step of
  *     that moment, which must have the same tokens per sequence as the captured
- *     one (lengths and pages may differ); hale_graph_launch is refused
- *     (HALE_EINVAL) for another step, or once the cache's buffers grew or the
- *     cache is gone, and within another capture.  A graph with hale_rope_device by hale_kv_positions and neither
+ *     one (lengths, pages and what is shared may differ); hale_graph_launch is refused
+ *     (HALE_EINVAL) for another step, or once the cache's buffers grew, its
+ *     prefixes are shared otherwise or it is gone, and within another capture.  A graph with hale_rope_device by hale_kv_positions and neither
  *     of the two may be launched for any step, and is refused for the other reasons. */
 typedef struct hale_graph hale_graph;
 int hale_graph_begin(hale_ctx *ctx);
