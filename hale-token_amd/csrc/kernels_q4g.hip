@@ -2,38 +2,42 @@
 // many tokens.
 //
 // out[t][r] = sum over groups of scale[r][group] (sum_k q[r][k] x[t][k] - zero[r][group]
-// sum_k x[t][k]).  Within a group both sums are matrix products of whole numbers 0..15
-// (and of ones) with x: of f16 and bf16 exactly, of f32 as three bf16 parts that add up
-// to it, of 8-bit codes in whole numbers.  Their accumulators and the sum over
-// groups are f32 (i32 within a unit of 8-bit codes).  Layout of the weights: step_ops.h.
+// sum_k x[t][k]).  Within a group both sums are matrix products of whole numbers (16 + q, and
+// ones; the 16 goes with the zero) with x: of f16 and bf16 exactly, of f32 as three
+// bf16 parts that add up to it, of 8-bit codes in whole numbers.  Their accumulators and
+// the sum over groups are f32 (i32 within a unit of 8-bit codes).  Layout of the weights:
+// step_ops.h.
 #include <hip/hip_runtime.h>
 
 #include "hale_device.h"
 #include "kernels.h"
 #include "kv_device.h"
 #include "step_ops.h"
+#include <cstdlib>
 
 namespace hale {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // ---- laying out and back ---------------------------------------------------------
 
-// The word of codes at `word` of a tile's chunk holds numbers k0 .. k0 + 7 of row i.
+// The word of codes at `word` of a tile's chunk holds numbers k0 .. k0 + 7 of row i,
+// number b in bits code_bit(b) ..
 __device__ __forceinline__ void q4g_word(unsigned word, unsigned* i, unsigned* k0) {
   const unsigned lane = word / 4, j = word % 4;
   *i = lane % 16;
   *k0 = 32 * j + 8 * (lane / 16);
 }
+__device__ __forceinline__ constexpr int code_bit(int b) { return 4 * (b / 2) + 16 * (b % 2); }
 
 __global__ __launch_bounds__(256) void k_q4g_pack(Q4gGeom g, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros) {
   const size_t tile = blockIdx.x;
   for (unsigned c = blockIdx.y; c < g.chunks; c += gridDim.y) {
-    uint8_t* to = g.data + tile * g.tile_bytes + (size_t)c * g.chunk_bytes;
+    uint8_t* to = g.data + tile * g.tile_bytes + (size_t)c * 1024;
     unsigned i, k0;
     q4g_word(threadIdx.x, &i, &k0);
     const size_t row = tile * Q4G_ROWS + i, k = (size_t)c * Q4G_CHUNK + k0;
@@ -42,16 +46,17 @@ __global__ __launch_bounds__(256) void k_q4g_pack(Q4gGeom g, const uint8_t* code
       const uint8_t* p = codes + row * (g.cols / 2) + k / 2;
       w = 0;
 #pragma unroll
-      for (int b = 0; b < 8; b++) w |= (unsigned)(p[b / 2] >> (4 * (b % 2)) & 15) << (b < 4 ? 8 * b : 8 * (b - 4) + 4);
+      for (int b = 0; b < 8; b++) w |= (unsigned)(p[b / 2] >> (4 * (b % 2)) & 15) << code_bit(b);
     }
     ((uint32_t*)to)[threadIdx.x] = w;
     if (threadIdx.x < 16 * g.per) {
-      const unsigned r = threadIdx.x % 16, s = threadIdx.x / 16;
+      const unsigned r = threadIdx.x % 4 + threadIdx.x / (4 * g.per) * 4, s = threadIdx.x / 4 % g.per;
       const size_t at = tile * Q4G_ROWS + r, group = (size_t)c * g.per + s;
       const bool in = at < g.rows && group * g.group < g.cols;
       const size_t from = at * (g.cols / g.group) + group;
-      ((uint16_t*)(to + 1024))[threadIdx.x] = in ? scales[from] : 0;
-      if (g.zeros) (to + 1024 + 32 * g.per)[threadIdx.x] = in ? zeros[from] & 15 : 8;
+      ((uint16_t*)(g.data + tile * g.tile_bytes + g.scales_at))[c * 16 * g.per + threadIdx.x] = in ? scales[from] : 0;
+      if (g.zeros)
+        (const_cast<uint8_t*>(g.zero_data) + tile * g.zero_tile)[c * g.zero_chunk + threadIdx.x] = Q4G_OFFSET + (in ? zeros[from] & 15 : 8);
     }
   }
 }
@@ -59,7 +64,7 @@ __global__ __launch_bounds__(256) void k_q4g_pack(Q4gGeom g, const uint8_t* code
 __global__ __launch_bounds__(256) void k_q4g_unpack(Q4gGeom g, uint8_t* codes, uint16_t* scales, uint8_t* zeros) {
   const size_t tile = blockIdx.x;
   for (unsigned c = blockIdx.y; c < g.chunks; c += gridDim.y) {
-    const uint8_t* from = g.data + tile * g.tile_bytes + (size_t)c * g.chunk_bytes;
+    const uint8_t* from = g.data + tile * g.tile_bytes + (size_t)c * 1024;
     unsigned i, k0;
     q4g_word(threadIdx.x, &i, &k0);
     const size_t row = tile * Q4G_ROWS + i, k = (size_t)c * Q4G_CHUNK + k0;
@@ -67,18 +72,15 @@ __global__ __launch_bounds__(256) void k_q4g_unpack(Q4gGeom g, uint8_t* codes, u
     if (row < g.rows && k < g.cols) {
       uint8_t* p = codes + row * (g.cols / 2) + k / 2;
 #pragma unroll
-      for (int b = 0; b < 8; b += 2) {
-        const unsigned lo = w >> (b < 4 ? 8 * b : 8 * (b - 4) + 4) & 15, hi = w >> (b < 4 ? 8 * b + 8 : 8 * (b - 4) + 12) & 15;
-        p[b / 2] = (uint8_t)(lo | hi << 4);
-      }
+      for (int b = 0; b < 8; b += 2) p[b / 2] = (uint8_t)((w >> code_bit(b) & 15) | (w >> code_bit(b + 1) & 15) << 4);
     }
     if (threadIdx.x < 16 * g.per) {
-      const unsigned r = threadIdx.x % 16, s = threadIdx.x / 16;
+      const unsigned r = threadIdx.x % 4 + threadIdx.x / (4 * g.per) * 4, s = threadIdx.x / 4 % g.per;
       const size_t at = tile * Q4G_ROWS + r, group = (size_t)c * g.per + s;
       if (at < g.rows && group * g.group < g.cols) {
         const size_t to = at * (g.cols / g.group) + group;
-        scales[to] = ((const uint16_t*)(from + 1024))[threadIdx.x];
-        if (zeros) zeros[to] = g.zeros ? (from + 1024 + 32 * g.per)[threadIdx.x] : 8;
+        scales[to] = ((const uint16_t*)(g.data + tile * g.tile_bytes + g.scales_at))[c * 16 * g.per + threadIdx.x];
+        if (zeros) zeros[to] = g.zeros ? (g.zero_data + tile * g.zero_tile)[c * g.zero_chunk + threadIdx.x] - Q4G_OFFSET : 8;
       }
     }
   }
@@ -87,54 +89,45 @@ __global__ __launch_bounds__(256) void k_q4g_unpack(Q4gGeom g, uint8_t* codes, u
 // ---- operands ----------------------------------------------------------------------
 
 // Input types: what a lane holds of eight numbers of a token, and of the weights.
-template <int IN> struct Q4gType;
+template <int IN> struct Q4gType {  // Q4G_F32, Q4G_BF16
+  static constexpr int PARTS = IN == Q4G_F32 ? 3 : 1, SIZE = IN == Q4G_F32 ? 4 : 2;
+  typedef bf16x8 Frag;
+  typedef f32x4 Acc;
+  typedef float Sum;
+};
 template <> struct Q4gType<Q4G_F16> {
-  static constexpr int PARTS = 1;
+  static constexpr int PARTS = 1, SIZE = 2;
   typedef f16x8 Frag;
   typedef f32x4 Acc;
-};
-template <> struct Q4gType<Q4G_BF16> {
-  static constexpr int PARTS = 1;
-  typedef bf16x8 Frag;
-  typedef f32x4 Acc;
-};
-template <> struct Q4gType<Q4G_F32> {
-  static constexpr int PARTS = 3;
-  typedef bf16x8 Frag;
-  typedef f32x4 Acc;
+  typedef float Sum;
 };
 template <> struct Q4gType<Q4G_I8> {
-  static constexpr int PARTS = 1;
+  static constexpr int PARTS = 1, SIZE = 1;
   typedef u32x2 Frag;
   typedef i32x4 Acc;
+  typedef int Sum;
 };
 
-// A word's eight codes.  A byte 0 .. 15 is the 8-bit float (4 exponent bits, 3 of
-// mantissa, whose smallest numbers step by 2^-9) that stands for that many 2^-9, so
-// the conversion with the scale 2^9 gives the whole number.
+// A word's eight codes, each 16 + q.  16 .. 31 are consecutive steps of a float's mantissa:
+// the four bits of a code go into it below the pattern of 16.  (A conversion
+// instruction takes four times as long as one of these: a vocabulary's product 41 us with
+// conversions, 28 so.)
 template <int IN> __device__ __forceinline__ typename Q4gType<IN>::Frag codes8(unsigned w) {
-  const unsigned lo = w & 0x0f0f0f0fu, hi = w >> 4 & 0x0f0f0f0fu;
   if constexpr (IN == Q4G_I8) {
-    return u32x2{lo, hi};
-  } else if constexpr (IN == Q4G_F16) {
-    union {
-      f16x2 h[4];
-      f16x8 v;
-    } r;
-    r.h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, false);
-    r.h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, true);
-    r.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, false);
-    r.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, true);
-    return r.v;
+    return u32x2{(w & 0x0f0f0f0fu) | 0x10101010u, (w >> 4 & 0x0f0f0f0fu) | 0x10101010u};
   } else {
+    constexpr int AT = IN == Q4G_F16 ? 6 : 3;  // of a code in the mantissa
+    unsigned base = IN == Q4G_F16 ? 0x4c004c00u : 0x41804180u, mask = 0x000f000fu << AT;
+    asm("" : "+v"(base), "+s"(mask));  // in registers, as the instruction of both operations takes them
     union {
-      bf16x2 h[4];
-      bf16x8 v;
+      unsigned u[4];
+      typename Q4gType<IN>::Frag v;
     } r;
-    r.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, false);
-    r.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, true);
-    r.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, false);
-    r.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, true);
+#pragma unroll
+    for (int p = 0; p < 4; p++) {
+      const unsigned m = 4 * p <= AT ? w << (AT - 4 * p) : w >> (4 * p - AT);
+      r.u[p] = (m & mask) | base;
+    }
     return r.v;
   }
 }
@@ -178,21 +171,21 @@ __device__ __forceinline__ typename Q4gType<IN>::Acc products(const typename Q4g
   return acc;
 }
 
-// Eight numbers of a token's row as operands; `in`: whether the row has them.
+typedef unsigned u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));  // at any 16-bit number's address
+
+// Eight numbers of a token's row from 32 j + 8 g of a chunk on as operands.  Those behind the row's
+// end are some of the row: their groups have scale 0.
 template <int IN>
-__device__ __forceinline__ void load_x(const Q4gArgs& a, const void* row, size_t k, bool in, typename Q4gType<IN>::Frag (&x)[Q4gType<IN>::PARTS]) {
+__device__ __forceinline__ void load_x(const Q4gArgs& a, const void* row, unsigned chunk, unsigned j, unsigned g,
+                                       typename Q4gType<IN>::Frag (&x)[Q4gType<IN>::PARTS]) {
+  const size_t from = (size_t)chunk * Q4G_CHUNK + 32 * j, k = (from < a.g.cols ? from : 0) + 8 * g;
   if constexpr (IN == Q4G_I8) {
-    x[0] = in ? *(const u32x2*)((const int8_t*)row + k) : u32x2{0, 0};
+    const u32x2 v = *(const u32x2*)((const int8_t*)row + k);
+    // in the order of the codes' bytes: 0 4 1 5, 2 6 3 7 of a word's numbers lie at 0 1 2 3, 4 5 6 7
+    x[0] = u32x2{__builtin_amdgcn_perm(v[1], v[0], 0x05010400u), __builtin_amdgcn_perm(v[1], v[0], 0x07030602u)};
   } else if constexpr (IN == Q4G_F32) {
-    float v[8];
     const float* p = (const float*)row + k;
-    if (a.vec) {
-      *(u32x4*)&v[0] = in ? *(const u32x4*)p : u32x4{0, 0, 0, 0};
-      *(u32x4*)&v[4] = in ? *(const u32x4*)(p + 4) : u32x4{0, 0, 0, 0};
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; j++) v[j] = in ? p[j] : 0.0f;
-    }
+    const f32x4 lo = *(const f32x4u*)p, hi = *(const f32x4u*)(p + 4);
     // the upper 8 bits of the mantissa, of what is left, and the rest: each a bf16, their sum
     // the number (a rest below bf16's range is lost: 2^-133)
     union {
@@ -200,11 +193,11 @@ __device__ __forceinline__ void load_x(const Q4gArgs& a, const void* row, size_t
       bf16x8 v[3];
     } r;
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
+    for (int e = 0; e < 8; e += 2) {
       unsigned part[3][2];
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const float f = v[j + h];
+        const float f = e < 4 ? lo[e + h] : hi[e + h - 4];
         const unsigned b0 = __float_as_uint(f) & 0xffff0000u;
         const float f1 = f - __uint_as_float(b0);
         const unsigned b1 = __float_as_uint(f1) & 0xffff0000u;
@@ -212,163 +205,481 @@ __device__ __forceinline__ void load_x(const Q4gArgs& a, const void* row, size_t
         part[0][h] = b0, part[1][h] = b1, part[2][h] = __float_as_uint(f2);
       }
 #pragma unroll
-      for (int p3 = 0; p3 < 3; p3++) r.u[p3][j / 2] = __builtin_amdgcn_perm(part[p3][1], part[p3][0], 0x07060302u);
+      for (int p3 = 0; p3 < 3; p3++) r.u[p3][e / 2] = __builtin_amdgcn_perm(part[p3][1], part[p3][0], 0x07060302u);
     }
 #pragma unroll
     for (int p3 = 0; p3 < 3; p3++) x[p3] = r.v[p3];
   } else {
-    union {
-      u32x4 u;
-      uint16_t h[8];
-      typename Q4gType<IN>::Frag v;
-    } r;
-    const uint16_t* p = (const uint16_t*)row + k;
-    if (a.vec) {
-      r.u = in ? *(const u32x4*)p : u32x4{0, 0, 0, 0};
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; j++) r.h[j] = in ? p[j] : (uint16_t)0;
-    }
-    x[0] = r.v;
+    x[0] = __builtin_bit_cast(typename Q4gType<IN>::Frag, (u32x4)(*(const u32x4a2*)((const uint16_t*)row + k)));
   }
 }
 
 // Four scales of 16 bits.
-__device__ __forceinline__ f32x4 scales4(u32x2 s, bool bf16) {
-  if (bf16)
+template <bool BF> __device__ __forceinline__ f32x4 scales4(const float (&f)[2]) {
+  if constexpr (BF) {
+    const unsigned s[2] = {__float_as_uint(f[0]), __float_as_uint(f[1])};
     return f32x4{__uint_as_float(s[0] << 16), __uint_as_float(s[0] & 0xffff0000u), __uint_as_float(s[1] << 16),
                  __uint_as_float(s[1] & 0xffff0000u)};
-  union {
-    u32x2 u;
-    _Float16 h[4];
-  } r;
-  r.u = s;
-  return f32x4{(float)r.h[0], (float)r.h[1], (float)r.h[2], (float)r.h[3]};
-}
-
-// Rows row .. row + 3 of a token's results.
-__device__ __forceinline__ void store_rows(const Q4gArgs& a, size_t token, size_t row, f32x4 v) {
-  const size_t at = token * a.out_stride + row;
-#pragma unroll
-  for (int r = 0; r < 4; r++) {
-    if (row + r >= a.g.rows) break;
-    if (a.out_dtype == F32)
-      ((float*)a.out)[at + r] = v[r];
-    else if (a.out_dtype == F16)
-      ((_Float16*)a.out)[at + r] = from_f32<_Float16>(v[r]);
-    else
-      ((Bf16*)a.out)[at + r] = from_f32<Bf16>(v[r]);
+  } else {
+    const f16x2 a = __builtin_bit_cast(f16x2, f[0]), b = __builtin_bit_cast(f16x2, f[1]);
+    return f32x4{(float)a[0], (float)a[1], (float)b[0], (float)b[1]};
   }
 }
 
-// A work-group of W waves computes RT tiles of 16 rows for NT groups of 16 tokens; its
-// waves take every W'th chunk of 128 numbers each and join their sums in LDS, in the waves'
-// order.  UNITS: units per chunk, within which scales (of weights and of 8-bit codes) are the same.
-template <int IN, int UNITS, int RT, int NT, int W>
-__global__ __launch_bounds__(64 * W) void k_q4g_few(Q4gArgs a) {
+// Rows row .. row + 3 of a token's results, whose type is that of float tokens.
+template <int IN> __device__ __forceinline__ void store_rows(const Q4gArgs& a, size_t token, unsigned row, f32x4 v) {
+  const int type = IN == Q4G_F32 ? F32 : IN == Q4G_F16 ? F16 : IN == Q4G_BF16 ? BF16 : a.out_dtype;
+  const size_t at = token * a.out_stride + row;
+  const unsigned n = (unsigned)a.g.rows - row;  // (rows that pad the last tile: more than there are)
+  if (row >= a.g.rows) return;
+  if (type == F32) {
+    float* p = (float*)a.out + at;
+    if (a.out_vec && n >= 4) {
+      *(f32x4*)p = v;
+      return;
+    }
+#pragma unroll
+    for (unsigned r = 0; r < 4; r++)
+      if (r < n) p[r] = v[r];
+    return;
+  }
+  union {
+    uint16_t h[4];
+    _Float16 f[4];
+    u32x2 u;
+  } h;
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    if (type == F16) h.f[r] = from_f32<_Float16>(v[r]);
+    else h.h[r] = from_f32<Bf16>(v[r]).bits;
+  }
+  uint16_t* p = (uint16_t*)a.out + at;
+  if (a.out_vec && n >= 4) {
+    *(u32x2*)p = h.u;
+    return;
+  }
+#pragma unroll
+  for (unsigned r = 0; r < 4; r++)
+    if (r < n) p[r] = h.h[r];
+}
+
+// What a lane holds of a tile's chunk: its word of codes of each operand, and of each
+// group the scales and zeros of its four result rows.
+template <int PER> struct Q4gChunk {
+  u32x4 w;
+  float s[PER][2];  // two of 16 bits each: as whole numbers the compiler takes them apart where they arrive,
+  unsigned z[PER];  // which waits for loads that are meant to be ahead
+  // What is computed of them is computed where they are used.
+  __device__ __forceinline__ void arrive() {
+#pragma unroll
+    for (int u = 0; u < PER; u++) asm volatile("" : "+v"(s[u][0]), "+v"(s[u][1]), "+v"(z[u]));
+  }
+};
+
+// A tile's chunks: places of a wave, and within them of a lane.  In as few loads as 16
+// bytes each allow.
+template <int PER> struct Q4gTile {
+  const uint8_t *p, *ps, *pz;
+  unsigned zstep, lw, ls, lz;
+  __device__ __forceinline__ Q4gTile(const Q4gGeom& g, unsigned tile, unsigned lane)
+      : p(g.data + (size_t)tile * g.tile_bytes),
+        ps(p + g.scales_at),
+        pz(g.zero_data + (size_t)tile * g.zero_tile),
+        zstep(g.zero_chunk),
+        lw(lane * 16),
+        ls((lane >> 4) * 8 * PER),
+        lz((lane >> 4) * 4 * PER) {}
+  __device__ __forceinline__ void next(const Q4gGeom& g) {
+    p += g.tile_bytes, ps += g.tile_bytes, pz += g.zero_tile;
+  }
+  __device__ __forceinline__ void load(unsigned chunk, Q4gChunk<PER>& c) const {
+    const uint8_t *b = p + (size_t)chunk * 1024, *bs = ps + (size_t)chunk * 32 * PER, *bz = pz + (size_t)chunk * zstep;
+    c.w = __builtin_nontemporal_load((const u32x4*)(b + lw));
+    if constexpr (PER == 1) {
+      const f32x2 v = *(const f32x2*)(bs + ls);
+      c.s[0][0] = v[0], c.s[0][1] = v[1];
+      c.z[0] = *(const unsigned*)(bz + lz);
+    } else {
+#pragma unroll
+      for (int u = 0; u < PER; u += 2) {
+        const f32x4 v = *(const f32x4*)(bs + ls + 8 * u);
+        c.s[u][0] = v[0], c.s[u][1] = v[1], c.s[u + 1][0] = v[2], c.s[u + 1][1] = v[3];
+      }
+      if constexpr (PER == 2) {
+        const u32x2 z = *(const u32x2*)(bz + lz);
+        c.z[0] = z[0], c.z[1] = z[1];
+      } else {
+        const u32x4 z = *(const u32x4*)(bz + lz);
+#pragma unroll
+        for (int u = 0; u < 4; u++) c.z[u] = z[u];
+      }
+    }
+  }
+};
+
+// Adds a unit's products to four rows' sums.  xs: the unit's scale of 8-bit codes.
+template <int IN>
+__device__ __forceinline__ f32x4 add_unit(f32x4 sum, typename Q4gType<IN>::Acc acc, typename Q4gType<IN>::Sum total, f32x4 s,
+                                          unsigned z, float xs) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const unsigned zero = z >> (8 * e) & 255;
+    if constexpr (IN == Q4G_I8)
+      sum[e] = __builtin_fmaf((float)(acc[e] - __mul24((int)zero, total)), s[e] * xs, sum[e]);
+    else
+      sum[e] = __builtin_fmaf(__builtin_fmaf(-(float)zero, total, acc[e]), s[e], sum[e]);
+  }
+  return sum;
+}
+
+// ---- few tokens ----------------------------------------------------------------------
+
+// Partial sums, written and read past the caches of one die, so that another die's
+// work-group sees them without either cache being emptied (a fence there takes some 15 us).
+__device__ __forceinline__ void put_part(float* p, f32x4 v) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) __hip_atomic_store(p + e, v[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x4 get_part(const float* p) {
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = __hip_atomic_load(p + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return v;
+}
+
+// Up to 16 tokens.  A work-group of W waves computes a tile of 16 rows; its waves take CH
+// chunks of 128 numbers at a time, all of them on their way before the first is used,
+// and join their sums in LDS, in the waves' order.  Long rows of few tiles are divided over
+// gridDim.y work-groups: the last of a tile's to finish adds their sums up in the splits' order.
+// UNITS: units per chunk, within which the scales (of weights and of 8-bit codes) are the
+// same.
+template <int IN, int PER, int UNITS, bool BF, int CH, int W>
+__global__ __launch_bounds__(64 * W) void k_q4g_few(Q4gArgs a, unsigned per_split) {
   typedef Q4gType<IN> Ty;
   typedef typename Ty::Frag Frag;
   constexpr int STEPS = 4 / UNITS;  // operands of 32 numbers per unit
-  __shared__ f32x4 red[W][RT][NT][64];
+  __shared__ f32x4 red[W][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned i = lane & 15, g = lane >> 4;
-  const size_t tile0 = (size_t)blockIdx.x * RT, tok0 = (size_t)blockIdx.y * (16 * NT);
-  const size_t tiles = (a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS;
-  const uint8_t* base[RT];
-#pragma unroll
-  for (int r = 0; r < RT; r++) base[r] = a.g.data + (tile0 + r < tiles ? tile0 + r : tiles - 1) * a.g.tile_bytes;
-  const void* row[NT];
-  const float* xscale[NT];
-  constexpr int SIZE = IN == Q4G_I8 ? 1 : IN == Q4G_F32 ? 4 : 2;
-#pragma unroll
-  for (int n = 0; n < NT; n++) {  // tokens that are missing read the last one
-    size_t t = tok0 + 16 * n + i;
-    t = t < a.ntok ? t : a.ntok - 1;
-    row[n] = (const char*)a.x + t * a.x_stride * SIZE;
-    xscale[n] = IN == Q4G_I8 ? a.x_scales + t * (a.g.cols / a.x_block) : nullptr;
-  }
+  const unsigned i = lane & 15, g = lane >> 4, tile = blockIdx.x;
+  const unsigned c0 = blockIdx.y * per_split, c1 = min(c0 + per_split, a.g.chunks);
+  const unsigned t = i < a.ntok ? i : (unsigned)a.ntok - 1;  // tokens that are missing read the last one
+  const void* row = (const char*)a.x + t * a.x_stride * Ty::SIZE;
+  const float* xscale = IN == Q4G_I8 ? a.x_scales + t * (a.g.cols / a.x_block) : nullptr;
   const unsigned xlast = IN == Q4G_I8 ? (unsigned)(a.g.cols / a.x_block) - 1 : 0;
+  const Q4gTile<PER> weights(a.g, tile, lane);
+
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (unsigned from = c0 + wave; from < c1; from += CH * W) {
+    Frag x[CH][4][Ty::PARTS];
+    float xs[CH][UNITS];
+    Q4gChunk<PER> q[CH];
+#pragma unroll
+    for (int k = 0; k < CH; k++)
+      if (from + W * k < c1) weights.load(from + W * k, q[k]);
+#pragma unroll
+    for (int k = 0; k < CH; k++) {
+      const unsigned c = from + W * k;
+      if (c >= c1) continue;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        load_x<IN>(a, row, c, j, g, x[k][j]);
+      if constexpr (IN == Q4G_I8) {
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) {
+          const unsigned at = (c * Q4G_CHUNK + u * (128 / UNITS)) / a.x_block;
+          xs[k][u] = xscale[at < xlast ? at : xlast];
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < CH; k++) {
+      if (from + W * k >= c1) continue;
+      q[k].arrive();
+#pragma unroll
+      for (int u = 0; u < UNITS; u++) {
+        Frag w[STEPS], ones[STEPS];
+#pragma unroll
+        for (int e = 0; e < STEPS; e++) w[e] = codes8<IN>(q[k].w[u * STEPS + e]), ones[e] = ones8<IN>();
+        const typename Ty::Sum total = products<IN, STEPS>(ones, &x[k][u * STEPS])[0];
+        sum = add_unit<IN>(sum, products<IN, STEPS>(w, &x[k][u * STEPS]), total, scales4<BF>(q[k].s[u * PER / UNITS]),
+                           q[k].z[u * PER / UNITS], xs[k][u]);
+      }
+    }
+  }
+  red[wave][lane] = sum;
+  __syncthreads();
+  if (wave) return;
+  f32x4 v = red[0][lane];
+#pragma unroll
+  for (int o = 1; o < W; o++) v = v + red[o][lane];
+  if (gridDim.y > 1) {
+    const size_t step = (size_t)gridDim.x * 256;
+    float* part = a.g.parts + ((size_t)tile * 64 + lane) * 4;
+    put_part(part + blockIdx.y * step, v);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the sums are where the others look before they are counted
+    unsigned before = 0;
+    if (lane == 0) before = atomicAdd(&a.g.done[tile], 1u);
+    if (__builtin_amdgcn_readfirstlane(before) != gridDim.y - 1) return;
+    v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (unsigned o = 0; o < gridDim.y; o++) v = v + get_part(part + o * step);
+    if (lane == 0) a.g.done[tile] = 0;
+  }
+  if (i < a.ntok) store_rows<IN>(a, i, tile * Q4G_ROWS + 4 * g, v);
+}
+
+// The tokens in LDS: [chunk][token] operands [j][part][g] and then a gap that puts 16 tokens'
+// equal operands into different banks, and [chunk][token][unit] sums and scales.
+template <int IN, int UNITS> struct Q4gTokens {
+  typedef typename Q4gType<IN>::Frag Frag;
+  static constexpr unsigned ROW = 16 * Q4gType<IN>::PARTS + 1;  // operands
+  static constexpr unsigned BYTES = ROW * sizeof(Frag) + 8 * UNITS;  // of a chunk and token
+};
+
+// Up to 16 tokens and many tiles.  The tokens' numbers are laid out in LDS as the operands
+// lie, with their sums; then each wave streams through tiles of its own, one behind the
+// other in memory, AHEAD chunks of weights on their way, and meets no other wave.
+template <int IN, int PER, int UNITS, bool BF, int AHEAD>
+__global__ __launch_bounds__(1024) void k_q4g_stream(Q4gArgs a) {
+  typedef Q4gType<IN> Ty;
+  typedef typename Ty::Frag Frag;
+  typedef Q4gTokens<IN, UNITS> Tok;
+  constexpr int STEPS = 4 / UNITS, P = Ty::PARTS;
+  extern __shared__ char lds[];
+  const unsigned ntok = (unsigned)a.ntok, chunks = a.g.chunks;
+  Frag* xl = (Frag*)lds;
+  typename Ty::Sum* totals = (typename Ty::Sum*)(xl + (size_t)chunks * ntok * Tok::ROW);
+  float* xsl = (float*)(totals + chunks * ntok * UNITS);
+  const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned i = lane & 15, g = lane >> 4, tok = i < ntok ? i : ntok - 1;
+  const unsigned tiles = (unsigned)((a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS);
+  const unsigned waves = blockDim.x / 64 * gridDim.x, me = blockIdx.x * (blockDim.x / 64) + wave;
+  const unsigned first = (unsigned)((size_t)tiles * me / waves), end = (unsigned)((size_t)tiles * (me + 1) / waves);
+  const unsigned n = (end - first) * chunks;  // chunks of the wave
+  Q4gTile<PER> weights(a.g, first, lane);  // of the next chunk to be read
+  unsigned ahead = 0, left = n;            // which chunk of its tile that is, and how many there are from it on
+  Q4gChunk<PER> q[AHEAD];
+  // (the last one again at the end: from a cache, without a branch around the loads)
+  auto load_next = [&](Q4gChunk<PER>& to) {
+    weights.load(ahead, to);
+    if (left > 1) {
+      left--;
+      if (++ahead == chunks) ahead = 0, weights.next(a.g);
+    }
+  };
+  if (n)
+#pragma unroll
+    for (int d = 0; d < AHEAD; d++) load_next(q[d]);
+
+  const unsigned pieces = chunks * 16;
+  for (unsigned k = threadIdx.x; k < pieces * ntok; k += blockDim.x) {  // along a token's row
+    const unsigned part = k % pieces, t = k / pieces, c = part / 16, j = part / 4 % 4, gg = part % 4;
+    Frag x[P];
+    load_x<IN>(a, (const char*)a.x + t * a.x_stride * Ty::SIZE, c, j, gg, x);
+#pragma unroll
+    for (int p = 0; p < P; p++) xl[(c * ntok + t) * Tok::ROW + (j * P + p) * 4 + gg] = x[p];
+  }
+  __syncthreads();
+  for (unsigned k = threadIdx.x; k < chunks * ntok * UNITS; k += blockDim.x) {
+    const unsigned u = k % UNITS, t = k / UNITS % ntok, c = k / UNITS / ntok;
+    typename Ty::Sum sum = 0;
+    for (int e = 0; e < STEPS * P * 4; e++) {
+      const Frag f = xl[(c * ntok + t) * Tok::ROW + u * STEPS * P * 4 + e];
+#pragma unroll
+      for (int b = 0; b < 8; b++) {
+        if constexpr (IN == Q4G_I8) sum += (int)(int8_t)(f[b / 4] >> (8 * (b % 4)));
+        else sum += (float)f[b];
+      }
+    }
+    totals[k] = sum;
+    if constexpr (IN == Q4G_I8) {
+      const unsigned xlast = (unsigned)(a.g.cols / a.x_block) - 1, at = (c * Q4G_CHUNK + u * (128 / UNITS)) / a.x_block;
+      xsl[k] = a.x_scales[t * (xlast + 1) + (at < xlast ? at : xlast)];
+    }
+  }
+  __syncthreads();
+
+  if (n == 0) return;
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  unsigned c = 0, tile = first;
+  const Frag* px = xl + tok * Tok::ROW + g;
+  unsigned pt = tok * UNITS;
+  for (unsigned from = 0; from < n; from += AHEAD) {
+#pragma unroll
+    for (int d = 0; d < AHEAD; d++) {
+      if (from + d >= n) return;
+      Frag x[4][P];
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int p = 0; p < P; p++) x[j][p] = px[(j * P + p) * 4];
+      q[d].arrive();
+#pragma unroll
+      for (int u = 0; u < UNITS; u++) {
+        Frag w[STEPS];
+#pragma unroll
+        for (int e = 0; e < STEPS; e++) w[e] = codes8<IN>(q[d].w[u * STEPS + e]);
+        sum = add_unit<IN>(sum, products<IN, STEPS>(w, &x[u * STEPS]), totals[pt + u], scales4<BF>(q[d].s[u * PER / UNITS]),
+                           q[d].z[u * PER / UNITS], IN == Q4G_I8 ? xsl[pt + u] : 0.0f);
+      }
+      load_next(q[d]);
+      px += ntok * Tok::ROW;
+      pt += ntok * UNITS;
+      if (++c == chunks) {
+        if (i < ntok) store_rows<IN>(a, i, tile * Q4G_ROWS + 4 * g, sum);
+        sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        c = 0;
+        tile++;
+        px = xl + tok * Tok::ROW + g;
+        pt = tok * UNITS;
+      }
+    }
+  }
+}
+
+// ---- many tokens -----------------------------------------------------------------------
+
+// A work-group computes 4 RT tiles of 16 rows for 64 tokens; its waves divide the rows, and
+// (WK) the chunks of 128 numbers.  For each chunk the tokens' numbers go through LDS as the
+// operands lie (wave k of four brings tokens 16 k .. and their sums); they are read from
+// memory two chunks ahead, and so are the weights, to registers.
+template <int IN, int PER, int UNITS, bool BF, int RT, int WK>
+__global__ __launch_bounds__(256 * WK) void k_q4g_many(Q4gArgs a, unsigned token_tiles) {
+  typedef Q4gType<IN> Ty;
+  typedef typename Ty::Frag Frag;
+  constexpr int STEPS = 4 / UNITS, WR = 4, NT = 4, P = Ty::PARTS;
+  struct Stage {
+    Frag x[NT][4][P][64];
+    typename Ty::Sum total[UNITS][NT * 16];
+    float xs[UNITS][NT * 16];
+  };
+  extern __shared__ char lds[];  // [WK][2] stages; then the second half's sums
+  const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned wr = wave % WR, wk = wave / WR;
+  Stage* stage = (Stage*)lds + 2 * wk;
+  const unsigned i = lane & 15, g = lane >> 4;
+  const unsigned tiles = (unsigned)((a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS);
+  // work-group b runs on die b % 8: all tokens of a row block on one, whose cache holds its weights
+  const unsigned b = blockIdx.x, block = (b / 8 / token_tiles) * 8 + b % 8;
+  const size_t tok0 = (size_t)(b / 8 % token_tiles) * (16 * NT);
+  const unsigned tile0 = (block * WR + wr) * RT;
+  if (block * WR * RT >= tiles) return;  // the whole work-group
+
+  const size_t t = min(tok0 + 16 * wr + i, a.ntok - 1);  // the token that this lane brings
+  const void* row = (const char*)a.x + t * a.x_stride * Ty::SIZE;
+  const float* xscale = IN == Q4G_I8 ? a.x_scales + t * (a.g.cols / a.x_block) : nullptr;
+  const unsigned xlast = IN == Q4G_I8 ? (unsigned)(a.g.cols / a.x_block) - 1 : 0;
+
+  struct Tokens {
+    Frag x[4][P];
+    float s[UNITS];
+  } in[2];
+  Q4gChunk<PER> q[4][RT];
+  // turn k of this half is chunk k WK + wk (the last again where there are no more)
+  auto load = [&](unsigned turn, Tokens& x, Q4gChunk<PER> (&to)[RT]) {
+    const unsigned c = min(turn * WK + wk, a.g.chunks - 1);
+#pragma unroll
+    for (int r = 0; r < RT; r++) Q4gTile<PER>(a.g, min(tile0 + r, tiles - 1), lane).load(c, to[r]);
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      load_x<IN>(a, row, c, j, g, x.x[j]);
+    if constexpr (IN == Q4G_I8) {
+#pragma unroll
+      for (int u = 0; u < UNITS; u++) {
+        const unsigned at = (c * Q4G_CHUNK + u * (128 / UNITS)) / a.x_block;
+        x.s[u] = xscale[at < xlast ? at : xlast];
+      }
+    }
+  };
+  auto bring = [&](Stage& s, const Tokens& x) {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int p = 0; p < P; p++) s.x[wr][j][p][lane] = x.x[j][p];
+#pragma unroll
+    for (int u = 0; u < UNITS; u++) {
+      Frag ones[STEPS];
+#pragma unroll
+      for (int e = 0; e < STEPS; e++) ones[e] = ones8<IN>();
+      const typename Ty::Acc total = products<IN, STEPS>(ones, &x.x[u * STEPS]);
+      if (g == 0) {
+        s.total[u][16 * wr + i] = total[0];
+        if constexpr (IN == Q4G_I8) s.xs[u][16 * wr + i] = x.s[u];
+      }
+    }
+  };
 
   f32x4 sum[RT][NT];
 #pragma unroll
   for (int r = 0; r < RT; r++)
 #pragma unroll
     for (int n = 0; n < NT; n++) sum[r][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-  for (unsigned c = wave; c < a.g.chunks; c += W) {
-    u32x4 w[RT];
-    u32x2 sc[RT][UNITS];
-    unsigned z[RT][UNITS];
-    Frag x[NT][4][Ty::PARTS];
-    float xs[NT][UNITS];
+  auto compute = [&](const Stage& s, Q4gChunk<PER> (&w)[RT]) {
 #pragma unroll
-    for (int r = 0; r < RT; r++) {
-      const uint8_t* p = base[r] + (size_t)c * a.g.chunk_bytes;
-      w[r] = *(const u32x4*)(p + lane * 16);
-#pragma unroll
-      for (int u = 0; u < UNITS; u++) {
-        const unsigned s = u * (128 / UNITS) / a.g.group;
-        sc[r][u] = *(const u32x2*)(p + 1024 + 32 * s + 8 * g);
-        z[r][u] = a.g.zeros ? *(const unsigned*)(p + 1024 + 32 * a.g.per + 16 * s + 4 * g) : 0x08080808u;
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const size_t k = (size_t)c * Q4G_CHUNK + 32 * j + 8 * g;
-        load_x<IN>(a, row[n], k, (size_t)c * Q4G_CHUNK + 32 * j < a.g.cols, x[n][j]);
-      }
-      if constexpr (IN == Q4G_I8) {
-#pragma unroll
-        for (int u = 0; u < UNITS; u++) {
-          const unsigned at = (c * Q4G_CHUNK + u * (128 / UNITS)) / a.x_block;
-          xs[n][u] = xscale[n][at < xlast ? at : xlast];
-        }
-      }
-    }
+    for (int r = 0; r < RT; r++) w[r].arrive();
 #pragma unroll
     for (int u = 0; u < UNITS; u++) {
-      Frag ones[STEPS];
-      typename Ty::Acc total[NT];
-#pragma unroll
-      for (int k = 0; k < STEPS; k++) ones[k] = ones8<IN>();
-#pragma unroll
-      for (int n = 0; n < NT; n++) total[n] = products<IN, STEPS>(ones, &x[n][u * STEPS]);
+      Frag k8[RT][STEPS];
+      f32x4 sc[RT];
 #pragma unroll
       for (int r = 0; r < RT; r++) {
-        Frag q[STEPS];
 #pragma unroll
-        for (int k = 0; k < STEPS; k++) q[k] = codes8<IN>(w[r][u * STEPS + k]);
-        const f32x4 s = scales4(sc[r][u], a.g.bf16);
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-          const typename Ty::Acc acc = products<IN, STEPS>(q, &x[n][u * STEPS]);
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const unsigned zero = z[r][u] >> (8 * e) & 255;
-            if constexpr (IN == Q4G_I8)
-              sum[r][n][e] = __builtin_fmaf((float)(acc[e] - (int)zero * total[n][0]), s[e] * xs[n][u], sum[r][n][e]);
-            else
-              sum[r][n][e] = __builtin_fmaf(__builtin_fmaf(-(float)zero, total[n][0], acc[e]), s[e], sum[r][n][e]);
-          }
-        }
+        for (int e = 0; e < STEPS; e++) k8[r][e] = codes8<IN>(w[r].w[u * STEPS + e]);
+        sc[r] = scales4<BF>(w[r].s[u * PER / UNITS]);
       }
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        Frag x[STEPS][P];
+#pragma unroll
+        for (int e = 0; e < STEPS; e++)
+#pragma unroll
+          for (int p = 0; p < P; p++) x[e][p] = s.x[n][u * STEPS + e][p][lane];
+        const typename Ty::Sum total = s.total[u][16 * n + i];
+        const float xs = IN == Q4G_I8 ? s.xs[u][16 * n + i] : 0.0f;
+#pragma unroll
+        for (int r = 0; r < RT; r++) sum[r][n] = add_unit<IN>(sum[r][n], products<IN, STEPS>(k8[r], x), total, sc[r], w[r].z[u * PER / UNITS], xs);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // the next unit's operands wait for this one's registers
     }
+  };
+  // the halves make as many turns; a chunk that is missing is not computed
+  const unsigned turns = (a.g.chunks + WK - 1) / WK;
+  load(0, in[0], q[0]);
+  load(1, in[1], q[1]);
+  bring(stage[0], in[0]);
+  __syncthreads();
+  for (unsigned from = 0; from < turns; from += 4) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      if (from + k >= turns) break;
+      load(from + k + 2, in[k % 2], q[(k + 2) % 4]);
+      __builtin_amdgcn_sched_barrier(0);  // on their way first
+      if ((from + k) * WK + wk < a.g.chunks) compute(stage[k % 2], q[k]);
+      bring(stage[(k + 1) % 2], in[(k + 1) % 2]);
+      __syncthreads();
+    }
+  }
+  if constexpr (WK == 2) {  // the second half's sums to the first
+    f32x4(*part)[RT][NT][64] = (f32x4(*)[RT][NT][64])lds;
+    if (wk == 1) {
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+#pragma unroll
+        for (int n = 0; n < NT; n++) part[wr][r][n][lane] = sum[r][n];
+    }
+    __syncthreads();
+    if (wk == 1) return;
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+      for (int n = 0; n < NT; n++) sum[r][n] = sum[r][n] + part[wr][r][n][lane];
   }
 #pragma unroll
   for (int r = 0; r < RT; r++)
 #pragma unroll
-    for (int n = 0; n < NT; n++) red[wave][r][n][lane] = sum[r][n];
-  __syncthreads();
-  for (int k = threadIdx.x; k < RT * NT * 64; k += 64 * W) {
-    f32x4 v = ((const f32x4*)red[0])[k];
-#pragma unroll
-    for (int o = 1; o < W; o++) v = v + ((const f32x4*)red[o])[k];
-    const int l = k % 64, n = k / 64 % NT, r = k / 64 / NT;
-    const size_t token = tok0 + 16 * n + l % 16;
-    if (token < a.ntok) store_rows(a, token, (tile0 + r) * Q4G_ROWS + 4 * (l / 16), v);
-  }
+    for (int n = 0; n < NT; n++) {
+      const size_t token = tok0 + 16 * n + i;
+      if (token < a.ntok) store_rows<IN>(a, token, (tile0 + r) * Q4G_ROWS + 4 * g, sum[r][n]);
+    }
 }
 
 hipError_t launch_q4g_pack(const Q4gGeom& g, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, hipStream_t st) {
@@ -380,31 +691,91 @@ hipError_t launch_q4g_unpack(const Q4gGeom& g, uint8_t* codes, uint16_t* scales,
   return launch(k_q4g_unpack, dim3(tiles, g.chunks < 1024 ? g.chunks : 1024), 256, 0, st, g, codes, scales, zeros);
 }
 
-template <int IN, int UNITS>
-static hipError_t q4g_sized(const Q4gArgs& a, hipStream_t st) {
-  const size_t tiles = (a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS;
-  if (a.ntok <= 16) return launch(k_q4g_few<IN, UNITS, 1, 1, 8>, dim3((unsigned)tiles, 1), 512, 0, st, a);
-  return launch(k_q4g_few<IN, UNITS, 2, 2, 4>, dim3((unsigned)((tiles + 1) / 2), (unsigned)((a.ntok + 31) / 32)), 256, 0, st, a);
+template <int IN, int PER, int UNITS, bool BF, int CH, int W>
+static hipError_t q4g_few(const Q4gArgs& a, hipStream_t st) {
+  const unsigned tiles = (unsigned)((a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS);
+  // as many work-groups as there are compute units, each with a chunk a wave at least
+  unsigned splits = 256 / tiles, most = (a.g.chunks + W - 1) / W;
+  splits = splits < 1 ? 1 : splits;
+  splits = splits > most ? most : splits;
+  splits = splits > Q4G_SPLITS ? Q4G_SPLITS : splits;
+  const unsigned per = (a.g.chunks + splits - 1) / splits;
+  splits = (a.g.chunks + per - 1) / per;
+  return launch(k_q4g_few<IN, PER, UNITS, BF, CH, W>, dim3(tiles, splits), 64 * W, 0, st, a, per);
 }
 
-template <int IN>
-static hipError_t q4g_units(const Q4gArgs& a, hipStream_t st) {
-  const unsigned unit = IN == Q4G_I8 && a.x_block < a.g.group ? a.x_block : a.g.group;
-  switch (unit) {
-    case 32: return q4g_sized<IN, 4>(a, st);
-    case 64: return q4g_sized<IN, 2>(a, st);
-    case 128: return q4g_sized<IN, 1>(a, st);
-    default: return hipErrorInvalidValue;
+template <int IN, int PER, int UNITS, bool BF, int AHEAD>
+static hipError_t q4g_stream(const Q4gArgs& a, uint32_t lds, hipStream_t st) {
+  const unsigned tiles = (unsigned)((a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS);
+  if (lds > 65536) {  // more than a kernel has unasked
+    const hipError_t e = hipFuncSetAttribute((const void*)k_q4g_stream<IN, PER, UNITS, BF, AHEAD>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
   }
+  static const char* env = getenv("Q4W");
+  unsigned waves = 16, best = ~0u;
+  for (unsigned w = 16; w >= 8; w--) {
+    const unsigned longest = (tiles + 256 * w - 1) / (256 * w) * w;  // tiles that the waves' time is that of
+    if (longest < best) best = longest, waves = w;
+  }
+  if (env) waves = atoi(env);
+  return launch(k_q4g_stream<IN, PER, UNITS, BF, AHEAD>, 256, 64 * waves, lds, st, a);
+}
+
+template <int IN, int PER, int UNITS, bool BF, int RT, int WK>
+static hipError_t q4g_many(const Q4gArgs& a, hipStream_t st) {
+  const unsigned tiles = (unsigned)((a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS);
+  const unsigned blocks = (tiles + 4 * RT - 1) / (4 * RT), token_tiles = (unsigned)((a.ntok + 63) / 64);
+  constexpr uint32_t stage = 4 * 4 * 64 * Q4gType<IN>::PARTS * sizeof(typename Q4gType<IN>::Frag) + 2 * UNITS * 64 * 4;
+  constexpr uint32_t sums = WK == 2 ? 4 * RT * 4 * 1024 : 0, lds = 2 * WK * stage > sums ? 2 * WK * stage : sums;
+  static_assert(lds <= 163840, "LDS of a compute unit");
+  if (lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute((const void*)k_q4g_many<IN, PER, UNITS, BF, RT, WK>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  const size_t grid = (size_t)(blocks + 7) / 8 * 8 * token_tiles;
+  if (grid > 0x7fffffffu) return hipErrorInvalidValue;
+  return launch(k_q4g_many<IN, PER, UNITS, BF, RT, WK>, dim3((unsigned)grid), 256 * WK, lds, st, a, token_tiles);
+}
+
+template <int IN, int PER, int UNITS, bool BF>
+static hipError_t q4g_sized(const Q4gArgs& a, hipStream_t st) {
+  if (a.ntok <= 16) {
+    const size_t tiles = (a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS, lds = (size_t)a.g.chunks * a.ntok * Q4gTokens<IN, UNITS>::BYTES;
+    if (tiles * a.g.chunks >= 65536 && lds <= 65536) return q4g_stream<IN, PER, UNITS, BF, UNITS == 4 ? 4 : 6>(a, (uint32_t)lds, st);
+    return q4g_few<IN, PER, UNITS, BF, IN == Q4G_F32 ? 1 : 2, 8>(a, st);
+  }
+  return q4g_many<IN, PER, UNITS, BF, 2, IN == Q4G_F32 ? 1 : 2>(a, st);
+}
+
+template <int IN, bool BF>
+static hipError_t q4g_units(const Q4gArgs& a, hipStream_t st) {
+  if constexpr (IN == Q4G_I8) {
+    const unsigned unit = a.x_block < a.g.group ? a.x_block : a.g.group;
+    switch (a.g.per * 8 + 128 / unit) {
+      case 9: return q4g_sized<IN, 1, 1, BF>(a, st);
+      case 10: return q4g_sized<IN, 1, 2, BF>(a, st);
+      case 12: return q4g_sized<IN, 1, 4, BF>(a, st);
+      case 18: return q4g_sized<IN, 2, 2, BF>(a, st);
+      case 20: return q4g_sized<IN, 2, 4, BF>(a, st);
+      case 36: return q4g_sized<IN, 4, 4, BF>(a, st);
+    }
+  } else {
+    switch (a.g.per) {
+      case 1: return q4g_sized<IN, 1, 1, BF>(a, st);
+      case 2: return q4g_sized<IN, 2, 2, BF>(a, st);
+      case 4: return q4g_sized<IN, 4, 4, BF>(a, st);
+    }
+  }
+  return hipErrorInvalidValue;
 }
 
 hipError_t launch_q4g(Q4gInput in, const Q4gArgs& a, hipStream_t st) {
   if (a.ntok == 0 || a.g.rows == 0) return hipSuccess;
   switch (in) {
-    case Q4G_F32: return q4g_units<Q4G_F32>(a, st);
-    case Q4G_F16: return q4g_units<Q4G_F16>(a, st);
-    case Q4G_BF16: return q4g_units<Q4G_BF16>(a, st);
-    case Q4G_I8: return q4g_units<Q4G_I8>(a, st);
+    case Q4G_F32: return a.g.bf16 ? q4g_units<Q4G_F32, true>(a, st) : q4g_units<Q4G_F32, false>(a, st);
+    case Q4G_F16: return a.g.bf16 ? q4g_units<Q4G_F16, true>(a, st) : q4g_units<Q4G_F16, false>(a, st);
+    case Q4G_BF16: return a.g.bf16 ? q4g_units<Q4G_BF16, true>(a, st) : q4g_units<Q4G_BF16, false>(a, st);
+    case Q4G_I8: return a.g.bf16 ? q4g_units<Q4G_I8, true>(a, st) : q4g_units<Q4G_I8, false>(a, st);
   }
   return hipErrorInvalidValue;
 }

@@ -29,26 +29,39 @@ hipError_t launch_norm_q8(int dtype, const NormQ8Args& a, size_t rows, hipStream
 
 // ---- 4-bit weights with group scales ---------------------------------------------
 //
-// Tiles of 16 rows, along them chunks of 128 numbers:
+// Tiles of 16 rows, along them chunks of 128 numbers.  In a tile, from a multiple of 128 bytes
+// on, first the codes of all chunks, then their scales, then their zeros:
 //   codes   16 rows x 128 numbers, lane 16 g + i of a wave 16 bytes: row i,
-//           word j holds numbers 32 j + 8 g .. + 7, number b (b < 4) in bits 8 b ..
-//           8 b + 3 and number 4 + b in bits 8 b + 4 .. 8 b + 7;
-//   scales  [128 / group][16 rows], 16 bits;
-//   zeros   [128 / group][16 rows], a byte; only where the matrix has them.
+//           word j holds numbers 32 j + 8 g .. + 7, number b in the four bits from
+//           4 (b / 2) + 16 (b % 2) on;
+//   scales  [4][128 / group][4 rows], 16 bits;
+//   zeros   [4][128 / group][4 rows], a byte, plus 16; only where the matrix has them.
 // Numbers and rows that pad the last chunk and tile are code 8 (zero 8), scale 0.
 // The matrix instructions take operands of 16 rows x 32 numbers whose lane 16 g + i holds
-// row i, numbers 8 g .. 8 g + 7: a word of codes.
-constexpr unsigned Q4G_CHUNK = 128, Q4G_ROWS = 16;
+// row i, numbers 8 g .. 8 g + 7: a word of codes; the results' lane 16 g + i holds rows 4 g ..
+// 4 g + 3 of token i, whose scales and zeros lie side by side.
+constexpr unsigned Q4G_CHUNK = 128, Q4G_ROWS = 16, Q4G_OFFSET = 16;
 
 struct Q4gGeom {
   uint8_t* data;
   size_t rows, cols;
   unsigned group, chunks;       // chunks of 128 numbers per row
   unsigned per;                 // groups per chunk
-  unsigned chunk_bytes;
-  size_t tile_bytes;
+  size_t tile_bytes, scales_at;  // scales_at: of a tile's first chunk
   bool zeros, bf16;             // bf16: type of the scales (else f16)
+  // where the first tile's zeros are read, and how far apart chunks' and tiles' are: in the data,
+  // or, for a matrix without zeros, 64 bytes of 16 + 8 for all (no branch, and no bytes from
+  // memory)
+  const uint8_t* zero_data;
+  unsigned zero_chunk;
+  size_t zero_tile;
+  // sums of tiles whose rows are divided over work-groups, [split][tile][64][4], and how many
+  // of a tile's work-groups are done (0 between calls)
+  float* parts;
+  unsigned* done;
 };
+// Most work-groups that a tile's row is divided over.
+constexpr unsigned Q4G_SPLITS = 8;
 
 hipError_t launch_q4g_pack(const Q4gGeom& g, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros,
                            hipStream_t st);
@@ -64,7 +77,7 @@ struct Q4gArgs {
   int out_dtype;
   void* out;                 // [ntok][rows]
   size_t out_stride;
-  bool vec;                  // x: all rows start at multiples of 16 bytes
+  bool out_vec;              // out: all rows start at multiples of four numbers
 };
 enum Q4gInput : int { Q4G_F32 = 0, Q4G_F16 = 1, Q4G_BF16 = 2, Q4G_I8 = 3 };
 hipError_t launch_q4g(Q4gInput in, const Q4gArgs& a, hipStream_t st);

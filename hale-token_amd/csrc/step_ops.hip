@@ -108,20 +108,28 @@ static int q4g_make(hale_ctx* c, size_t rows, size_t cols, size_t group, int sca
   g.per = (unsigned)(Q4G_CHUNK / group);
   g.zeros = zeros != nullptr;
   g.bf16 = scale_dtype == HALE_BF16;
-  g.chunk_bytes = 1024 + (g.zeros ? 48 : 32) * g.per;
-  g.tile_bytes = (size_t)g.chunks * g.chunk_bytes;
+  g.scales_at = (size_t)g.chunks * 1024;
+  const size_t zeros_at = g.scales_at + (size_t)g.chunks * 32 * g.per;
+  g.tile_bytes = round_up(zeros_at + (g.zeros ? (size_t)g.chunks * 16 * g.per : 0), 128);
   const size_t tiles = (rows + Q4G_ROWS - 1) / Q4G_ROWS, bytes = tiles * g.tile_bytes;
-  if (hipMalloc(&g.data, bytes) != hipSuccess)
-    return ctx_fail(c, HALE_ENOMEM, "q4g_upload: %zu bytes of weights", bytes);
+  const size_t parts = Q4G_SPLITS * tiles * 1024, done = round_up(tiles * 4, 256);
+  if (hipMalloc(&g.data, bytes + parts + done + 64) != hipSuccess)
+    return ctx_fail(c, HALE_ENOMEM, "q4g_upload: %zu bytes of weights and workspace", bytes + parts + done + 64);
+  g.parts = (float*)(g.data + bytes);
+  g.done = (unsigned*)(g.data + bytes + parts);
+  g.zero_data = g.zeros ? g.data + zeros_at : g.data + bytes + parts + done;
+  g.zero_chunk = g.zeros ? 16 * g.per : 0;
+  g.zero_tile = g.zeros ? g.tile_bytes : 0;
   uint8_t* sent = nullptr;
-  hipError_t e = hipSuccess;
+  hipError_t e = hipMemsetAsync(g.done, 0, done, c->stream);
+  if (e == hipSuccess) e = hipMemsetAsync(g.data + bytes + parts + done, Q4G_OFFSET + 8, 64, c->stream);
   if (host) {
     const size_t cb = round_up(rows * (cols / 2), 256), sb = round_up(groups * 2, 256);
     if (hipMalloc(&sent, cb + sb + groups) != hipSuccess) {
       (void)hipFree(g.data);
       return ctx_fail(c, HALE_ENOMEM, "q4g_upload: %zu bytes on the way", cb + sb + groups);
     }
-    e = hipMemcpyAsync(sent, codes, rows * (cols / 2), hipMemcpyHostToDevice, c->stream);
+    if (e == hipSuccess) e = hipMemcpyAsync(sent, codes, rows * (cols / 2), hipMemcpyHostToDevice, c->stream);
     if (e == hipSuccess) e = hipMemcpyAsync(sent + cb, scales, groups * 2, hipMemcpyHostToDevice, c->stream);
     if (e == hipSuccess && zeros) e = hipMemcpyAsync(sent + cb + sb, zeros, groups, hipMemcpyHostToDevice, c->stream);
     codes = sent;
@@ -218,6 +226,7 @@ static int q4g_run(hale_q4g* m, Q4gInput in, Q4gArgs& a, int dtype, size_t ntok,
   a.out_dtype = dtype;
   a.out = out;
   a.out_stride = out_stride;
+  a.out_vec = ((uintptr_t)out | out_stride * type_bytes(dtype)) % (4 * type_bytes(dtype)) == 0;
   CALL_TRY
   std::lock_guard<std::recursive_mutex> lk(c->mu);
   CALL_CHK(c, hipSetDevice(c->device));
@@ -232,7 +241,6 @@ extern "C" int hale_q4g_matmul_device(hale_q4g* m, int dtype, size_t ntok, const
   Q4gArgs a{};
   a.x = x;
   a.x_stride = x_stride;
-  a.vec = ((uintptr_t)x | x_stride * type_bytes(dtype)) % 16 == 0;
   const Q4gInput in = dtype == HALE_F32 ? Q4G_F32 : dtype == HALE_F16 ? Q4G_F16 : Q4G_BF16;
   return q4g_run(m, in, a, dtype, ntok, out, out_stride);
 }

@@ -25,7 +25,7 @@ hipError_t launch_q4g_pack(const Q4gGeom& g, const uint8_t* codes, const uint16_
   for (size_t i = 0; i < g.rows * (g.cols / 2); i++) sum = sum + codes[i];
   for (size_t i = 0; i < g.rows * (g.cols / g.group); i++) sum = sum + (uint8_t)scales[i] + (zeros ? zeros[i] : 0);
   memset(g.data, sum, (g.rows + Q4G_ROWS - 1) / Q4G_ROWS * g.tile_bytes);
-  CHECK(g.chunk_bytes == 1024 + g.per * (g.zeros ? 48 : 32) && g.tile_bytes == (size_t)g.chunks * g.chunk_bytes);
+  CHECK(g.scales_at == g.chunks * 1024 && g.tile_bytes % 128 == 0 && g.tile_bytes >= g.scales_at + g.chunks * g.per * (g.zeros ? 48 : 32));
   return hipSuccess;
 }
 hipError_t launch_q4g_unpack(const Q4gGeom& g, uint8_t* codes, uint16_t* scales, uint8_t* zeros, hipStream_t) {
@@ -134,9 +134,9 @@ void matrices() {
   CHECK(hale_q4g_download(m, codes.data(), scales.data(), nullptr) == HALE_OK);
   // products
   auto f = [&](int dtype, size_t n, const void* x, size_t xs, void* o, size_t os) { return hale_q4g_matmul_device(m, dtype, n, x, xs, o, os); };
-  CHECK(f(HALE_F32, 2, mem, 96, mem + 4096, 33) == HALE_OK && products == 1 && last_q4g.vec && last_q4g.ntok == 2);
-  CHECK(f(HALE_F32, 2, mem, 97, mem + 4096, 33) == HALE_OK && !last_q4g.vec);
-  CHECK(f(HALE_BF16, 2, mem, 104, mem + 4096, 40) == HALE_OK && last_q4g.vec);
+  CHECK(f(HALE_F32, 2, mem, 96, mem + 4096, 33) == HALE_OK && products == 1 && !last_q4g.out_vec && last_q4g.ntok == 2);
+  CHECK(f(HALE_F32, 2, mem, 97, mem + 4096, 36) == HALE_OK && last_q4g.out_vec);
+  CHECK(f(HALE_BF16, 2, mem, 104, mem + 4098, 40) == HALE_OK && !last_q4g.out_vec);
   auto q = [&](size_t block, const void* x, const void* s, size_t os) {
     return hale_q4g_matmul_q8_device(m, 2, block, (const int8_t*)x, (const float*)s, HALE_BF16, mem + 4096, os);
   };

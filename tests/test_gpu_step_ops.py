@@ -209,18 +209,18 @@ def q4_weights(rng, rows, cols, group, zeros, scale_dtype):
 
 
 def q4_model(codes, scales, z, group, x):
-    """The product, and sum scale (q + zero) |x|, in 64 bits."""
+    """The product, and sum scale (16 + q + 16 + zero) |x|, in 64 bits."""
     q = np.stack((codes & 15, codes >> 4), -1).reshape(len(codes), -1).astype(np.float64)
     zz = np.full(scales.shape, 8.0) if z is None else z.astype(np.float64)
     s, zz = np.repeat(scales, group, 1), np.repeat(zz, group, 1)
     x = x.astype(np.float64)
-    return x @ (s * (q - zz)).T, np.abs(x) @ (np.abs(s) * (q + zz)).T
+    return x @ (s * (q - zz)).T, np.abs(x) @ (np.abs(s) * (q + zz + 32)).T
 
 
 def q4_bound(dtype, want, mag, cols, group):
-    """Products are exact (4 bits times at most 11, or three parts of 8).  A group's sums are
-    at most 3 * 128 products, each addition off by 2^-23 of the partial sums at most (however the
-    matrix unit rounds), zero times the second sum and the difference by 2^-24 each: against
+    """Products are exact (16 + q, 5 bits, times at most 11, or three parts of 8).  A group's sums
+    are at most 3 * 128 products, each addition off by 2^-23 of the partial sums at most (however the
+    matrix unit rounds), 16 + zero times the second sum and the difference by 2^-24 each: against
     `mag`, (3 * 128 + 2) 2^-23.  Between groups a product and a sum each, and the joins of up to 16
     parts: (cols / group + 18) 2^-24.  Then the result's own rounding."""
     rel = (3 * 128 + 2) * 2.0 ** -23 + (cols / group + 18) * 2.0 ** -24
@@ -286,7 +286,7 @@ def test_q4_weights_from_device_memory(ctx, bufs):
     (130, 300, 896, 128, 896, False, "f32"), (64, 128, 256, 32, 128, True, "bf16"),
 ])
 def test_q4_products_of_8_bit_tokens(ctx, bufs, ntok, rows, cols, group, block, zeros, dtype):
-    """Whole numbers up to 128 * 127 * 15 < 2^24 within a unit of 32 to 128 numbers; per unit the
+    """Whole numbers up to 128 * 127 * 31 < 2^24 within a unit of 32 to 128 numbers; per unit the
     product of the scales, and a fused product and sum, round by 2^-24 of partial sums of the units'
     magnitudes; then the joins (up to 16 parts) and the result's own rounding."""
     rng = np.random.default_rng(rows + cols + ntok)
