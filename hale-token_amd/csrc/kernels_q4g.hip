@@ -214,6 +214,9 @@ __device__ __forceinline__ void load_x(const Q4gArgs& a, const void* row, unsign
   }
 }
 
+// Which of a token's scales is that of its number k (the last one's behind the row's end).
+__device__ __forceinline__ unsigned x_scale_at(const Q4gArgs& a, unsigned k) { return min(k >> a.x_shift, a.x_per - 1); }
+
 // Four scales of 16 bits.
 template <bool BF> __device__ __forceinline__ f32x4 scales4(const float (&f)[2]) {
   if constexpr (BF) {
@@ -364,8 +367,7 @@ __global__ __launch_bounds__(64 * W) void k_q4g_few(Q4gArgs a, unsigned per_spli
   const unsigned c0 = blockIdx.y * per_split, c1 = min(c0 + per_split, a.g.chunks);
   const unsigned t = i < a.ntok ? i : (unsigned)a.ntok - 1;  // tokens that are missing read the last one
   const void* row = (const char*)a.x + t * a.x_stride * Ty::SIZE;
-  const float* xscale = IN == Q4G_I8 ? a.x_scales + t * (a.g.cols / a.x_block) : nullptr;
-  const unsigned xlast = IN == Q4G_I8 ? (unsigned)(a.g.cols / a.x_block) - 1 : 0;
+  const float* xscale = IN == Q4G_I8 ? a.x_scales + t * a.x_per : nullptr;
   const Q4gTile<PER> weights(a.g, tile, lane);
 
   f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -386,8 +388,7 @@ __global__ __launch_bounds__(64 * W) void k_q4g_few(Q4gArgs a, unsigned per_spli
       if constexpr (IN == Q4G_I8) {
 #pragma unroll
         for (int u = 0; u < UNITS; u++) {
-          const unsigned at = (c * Q4G_CHUNK + u * (128 / UNITS)) / a.x_block;
-          xs[k][u] = xscale[at < xlast ? at : xlast];
+          xs[k][u] = xscale[x_scale_at(a, c * Q4G_CHUNK + u * (128 / UNITS))];
         }
       }
     }
@@ -492,8 +493,7 @@ __global__ __launch_bounds__(1024) void k_q4g_stream(Q4gArgs a) {
     }
     totals[k] = sum;
     if constexpr (IN == Q4G_I8) {
-      const unsigned xlast = (unsigned)(a.g.cols / a.x_block) - 1, at = (c * Q4G_CHUNK + u * (128 / UNITS)) / a.x_block;
-      xsl[k] = a.x_scales[t * (xlast + 1) + (at < xlast ? at : xlast)];
+      xsl[k] = a.x_scales[(size_t)t * a.x_per + x_scale_at(a, c * Q4G_CHUNK + u * (128 / UNITS))];
     }
   }
   __syncthreads();
@@ -566,8 +566,7 @@ __global__ __launch_bounds__(256 * WK) void k_q4g_many(Q4gArgs a, unsigned token
 
   const size_t t = min(tok0 + 16 * wr + i, a.ntok - 1);  // the token that this lane brings
   const void* row = (const char*)a.x + t * a.x_stride * Ty::SIZE;
-  const float* xscale = IN == Q4G_I8 ? a.x_scales + t * (a.g.cols / a.x_block) : nullptr;
-  const unsigned xlast = IN == Q4G_I8 ? (unsigned)(a.g.cols / a.x_block) - 1 : 0;
+  const float* xscale = IN == Q4G_I8 ? a.x_scales + t * a.x_per : nullptr;
 
   struct Tokens {
     Frag x[4][P];
@@ -585,8 +584,7 @@ __global__ __launch_bounds__(256 * WK) void k_q4g_many(Q4gArgs a, unsigned token
     if constexpr (IN == Q4G_I8) {
 #pragma unroll
       for (int u = 0; u < UNITS; u++) {
-        const unsigned at = (c * Q4G_CHUNK + u * (128 / UNITS)) / a.x_block;
-        x.s[u] = xscale[at < xlast ? at : xlast];
+        x.s[u] = xscale[x_scale_at(a, c * Q4G_CHUNK + u * (128 / UNITS))];
       }
     }
   };
@@ -750,7 +748,7 @@ static hipError_t q4g_sized(const Q4gArgs& a, hipStream_t st) {
 template <int IN, bool BF>
 static hipError_t q4g_units(const Q4gArgs& a, hipStream_t st) {
   if constexpr (IN == Q4G_I8) {
-    const unsigned unit = a.x_block < a.g.group ? a.x_block : a.g.group;
+    const unsigned unit = a.x_shift < 7 && (1u << a.x_shift) < a.g.group ? 1u << a.x_shift : a.g.group;
     switch (a.g.per * 8 + 128 / unit) {
       case 9: return q4g_sized<IN, 1, 1, BF>(a, st);
       case 10: return q4g_sized<IN, 1, 2, BF>(a, st);

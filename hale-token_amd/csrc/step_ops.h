@@ -70,9 +70,9 @@ hipError_t launch_q4g_unpack(const Q4gGeom& g, uint8_t* codes, uint16_t* scales,
 struct Q4gArgs {
   Q4gGeom g;
   const void* x;             // [ntok][cols] of a float type with a stride, or codes
-  const float* x_scales;     // [ntok][cols / x_block] of codes
+  const float* x_scales;     // [ntok][x_per] of codes
   size_t x_stride;           // elements
-  unsigned x_block;          // numbers per scale of codes; cols: one a token
+  unsigned x_shift, x_per;   // numbers per scale of codes, as a power of two (31: one a token), and a token's scales
   size_t ntok;
   int out_dtype;
   void* out;                 // [ntok][rows]

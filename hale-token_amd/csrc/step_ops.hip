@@ -254,7 +254,8 @@ extern "C" int hale_q4g_matmul_q8_device(hale_q4g* m, size_t ntok, size_t block,
   a.x = quants;
   a.x_scales = scales;
   a.x_stride = m->g.cols;
-  a.x_block = (unsigned)block;
+  a.x_shift = block == 32 ? 5 : block == 64 ? 6 : block == 128 ? 7 : 31;
+  a.x_per = (unsigned)(m->g.cols / block);
   return q4g_run(m, Q4G_I8, a, dtype, ntok, out, out_stride);
 }
 

@@ -140,7 +140,7 @@ void matrices() {
   auto q = [&](size_t block, const void* x, const void* s, size_t os) {
     return hale_q4g_matmul_q8_device(m, 2, block, (const int8_t*)x, (const float*)s, HALE_BF16, mem + 4096, os);
   };
-  CHECK(q(32, mem, mem, 33) == HALE_OK && q(96, mem, mem, 33) == HALE_OK && last_q4g.x_block == 96);
+  CHECK(q(32, mem, mem, 33) == HALE_OK && q(96, mem, mem, 33) == HALE_OK && last_q4g.x_shift == 31 && last_q4g.x_per == 1);
   const int before = products;
   CHECK(f(HALE_Q8_0, 2, mem, 96, mem, 33) == HALE_EINVAL && f(HALE_F32, 2, nullptr, 96, mem, 33) == HALE_EINVAL);
   CHECK(f(HALE_F32, 2, mem, 95, mem, 33) == HALE_EINVAL && f(HALE_F32, 2, mem, 96, mem, 32) == HALE_EINVAL);
