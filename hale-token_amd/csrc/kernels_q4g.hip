@@ -13,7 +13,6 @@
 #include "kernels.h"
 #include "kv_device.h"
 #include "step_ops.h"
-#include <cstdlib>
 
 namespace hale {
 
@@ -171,6 +170,7 @@ __device__ __forceinline__ typename Q4gType<IN>::Acc products(const typename Q4g
   return acc;
 }
 
+typedef float f32x2u __attribute__((ext_vector_type(2), aligned(4)));
 typedef unsigned u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));  // at any 16-bit number's address
 
 // Eight numbers of a token's row from 32 j + 8 g of a chunk on as operands.  Those behind the row's
@@ -214,8 +214,25 @@ __device__ __forceinline__ void load_x(const Q4gArgs& a, const void* row, unsign
   }
 }
 
-// Which of a token's scales is that of its number k (the last one's behind the row's end).
-__device__ __forceinline__ unsigned x_scale_at(const Q4gArgs& a, unsigned k) { return min(k >> a.x_shift, a.x_per - 1); }
+// A chunk's M scales of a token's 8-bit codes, in one load.  Behind the row's end they are the last
+// ones' (and the groups' scales are 0).
+template <int M> __device__ __forceinline__ void load_x_scales(const Q4gArgs& a, const float* row, unsigned chunk, float (&s)[M]) {
+  const unsigned at = a.x_per == 1 ? 0 : chunk * M;
+  if constexpr (M == 1) {
+    s[0] = row[at];
+  } else if (at + M <= a.x_per) {
+    if constexpr (M == 4) {
+      const f32x4 v = *(const f32x4u*)(row + at);
+      s[0] = v[0], s[1] = v[1], s[2] = v[2], s[3] = v[3];
+    } else {
+      const f32x2u v = *(const f32x2u*)(row + at);
+      s[0] = v[0], s[1] = v[1];
+    }
+  } else {
+#pragma unroll
+    for (int m = 0; m < M; m++) s[m] = row[min(at + m, a.x_per - 1)];
+  }
+}
 
 // Four scales of 16 bits.
 template <bool BF> __device__ __forceinline__ f32x4 scales4(const float (&f)[2]) {
@@ -350,30 +367,41 @@ __device__ __forceinline__ f32x4 get_part(const float* p) {
   return v;
 }
 
+// Tokens in LDS: a row per token and chunk of operands of eight numbers [part][16], and a gap that
+// puts the same operand of 16 tokens into different banks.
+template <int IN> struct Q4gRow {
+  typedef typename Q4gType<IN>::Frag Frag;
+  static constexpr int P = Q4gType<IN>::PARTS, SIZE = 16 * P + 1;
+  Frag f[SIZE];
+};
+
 // Up to 16 tokens.  A work-group of W waves computes a tile of 16 rows; its waves take CH
 // chunks of 128 numbers at a time, all of them on their way before the first is used,
-// and join their sums in LDS, in the waves' order.  Long rows of few tiles are divided over
-// gridDim.y work-groups: the last of a tile's to finish adds their sums up in the splits' order.
-// UNITS: units per chunk, within which the scales (of weights and of 8-bit codes) are the
+// and join their sums in LDS, in the waves' order.  A token's numbers of a chunk are read by 16
+// neighbouring lanes and change lanes through LDS (16 tokens of 4096, 8-bit: 11.0 us where each
+// lane read its operands itself).  Long rows of few tiles are divided over gridDim.y
+// work-groups: the last of a tile's to finish adds their sums up in the splits' order.
+// UNITS: units per chunk, within which the scales (PER of the weights, M of 8-bit codes) are the
 // same.
-template <int IN, int PER, int UNITS, bool BF, int CH, int W>
+template <int IN, int PER, int M, bool BF, int CH, int W>
 __global__ __launch_bounds__(64 * W) void k_q4g_few(Q4gArgs a, unsigned per_split) {
   typedef Q4gType<IN> Ty;
   typedef typename Ty::Frag Frag;
-  constexpr int STEPS = 4 / UNITS;  // operands of 32 numbers per unit
-  __shared__ f32x4 red[W][64];
+  constexpr int UNITS = PER > M ? PER : M, STEPS = 4 / UNITS;  // operands of 32 numbers per unit
+  extern __shared__ char lds[];  // [W][CH][ntok] rows; then [W][64] sums
+  f32x4(*red)[64] = (f32x4(*)[64])lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned i = lane & 15, g = lane >> 4, tile = blockIdx.x;
+  const unsigned i = lane & 15, g = lane >> 4, tile = blockIdx.x, ntok = (unsigned)a.ntok;
   const unsigned c0 = blockIdx.y * per_split, c1 = min(c0 + per_split, a.g.chunks);
-  const unsigned t = i < a.ntok ? i : (unsigned)a.ntok - 1;  // tokens that are missing read the last one
-  const void* row = (const char*)a.x + t * a.x_stride * Ty::SIZE;
+  const unsigned t = min(i, ntok - 1);  // tokens that are missing are the last one
   const float* xscale = IN == Q4G_I8 ? a.x_scales + t * a.x_per : nullptr;
   const Q4gTile<PER> weights(a.g, tile, lane);
+  Q4gRow<IN>* rows = (Q4gRow<IN>*)lds + wave * CH * ntok;
 
   f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
   for (unsigned from = c0 + wave; from < c1; from += CH * W) {
-    Frag x[CH][4][Ty::PARTS];
-    float xs[CH][UNITS];
+    Frag in[CH][4][Ty::PARTS];
+    float xs[CH][M];
     Q4gChunk<PER> q[CH];
 #pragma unroll
     for (int k = 0; k < CH; k++)
@@ -383,30 +411,45 @@ __global__ __launch_bounds__(64 * W) void k_q4g_few(Q4gArgs a, unsigned per_spli
       const unsigned c = from + W * k;
       if (c >= c1) continue;
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-        load_x<IN>(a, row, c, j, g, x[k][j]);
-      if constexpr (IN == Q4G_I8) {
+      for (int n = 0; n < 4; n++) {  // four tokens at a time
+        if (4 * n >= (int)ntok) break;
+        load_x<IN>(a, (const char*)a.x + min(4 * n + g, ntok - 1) * a.x_stride * Ty::SIZE, c, i / 4, i % 4, in[k][n]);
+      }
+      if constexpr (IN == Q4G_I8) load_x_scales<M>(a, xscale, c, xs[k]);
+    }
 #pragma unroll
-        for (int u = 0; u < UNITS; u++) {
-          xs[k][u] = xscale[x_scale_at(a, c * Q4G_CHUNK + u * (128 / UNITS))];
+    for (int k = 0; k < CH; k++) {
+      if (from + W * k >= c1) continue;
+#pragma unroll
+      for (int n = 0; n < 4; n++) {
+        if (4 * n >= (int)ntok) break;
+        if (4 * n + g < ntok) {
+#pragma unroll
+          for (int p = 0; p < Ty::PARTS; p++) rows[k * ntok + 4 * n + g].f[16 * p + i] = in[k][n][p];
         }
       }
     }
 #pragma unroll
     for (int k = 0; k < CH; k++) {
       if (from + W * k >= c1) continue;
+      Frag x[4][Ty::PARTS];
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int p = 0; p < Ty::PARTS; p++) x[j][p] = rows[k * ntok + t].f[16 * p + 4 * j + g];
       q[k].arrive();
 #pragma unroll
       for (int u = 0; u < UNITS; u++) {
         Frag w[STEPS], ones[STEPS];
 #pragma unroll
         for (int e = 0; e < STEPS; e++) w[e] = codes8<IN>(q[k].w[u * STEPS + e]), ones[e] = ones8<IN>();
-        const typename Ty::Sum total = products<IN, STEPS>(ones, &x[k][u * STEPS])[0];
-        sum = add_unit<IN>(sum, products<IN, STEPS>(w, &x[k][u * STEPS]), total, scales4<BF>(q[k].s[u * PER / UNITS]),
-                           q[k].z[u * PER / UNITS], xs[k][u]);
+        const typename Ty::Sum total = products<IN, STEPS>(ones, &x[u * STEPS])[0];
+        sum = add_unit<IN>(sum, products<IN, STEPS>(w, &x[u * STEPS]), total, scales4<BF>(q[k].s[u * PER / UNITS]),
+                           q[k].z[u * PER / UNITS], IN == Q4G_I8 ? xs[k][u * M / UNITS] : 0.0f);
       }
     }
   }
+  __syncthreads();  // the rows are read
   red[wave][lane] = sum;
   __syncthreads();
   if (wave) return;
@@ -439,12 +482,12 @@ template <int IN, int UNITS> struct Q4gTokens {
 // Up to 16 tokens and many tiles.  The tokens' numbers are laid out in LDS as the operands
 // lie, with their sums; then each wave streams through tiles of its own, one behind the
 // other in memory, AHEAD chunks of weights on their way, and meets no other wave.
-template <int IN, int PER, int UNITS, bool BF, int AHEAD>
+template <int IN, int PER, int M, bool BF, int AHEAD>
 __global__ __launch_bounds__(1024) void k_q4g_stream(Q4gArgs a) {
   typedef Q4gType<IN> Ty;
   typedef typename Ty::Frag Frag;
+  constexpr int UNITS = PER > M ? PER : M, STEPS = 4 / UNITS, P = Ty::PARTS;
   typedef Q4gTokens<IN, UNITS> Tok;
-  constexpr int STEPS = 4 / UNITS, P = Ty::PARTS;
   extern __shared__ char lds[];
   const unsigned ntok = (unsigned)a.ntok, chunks = a.g.chunks;
   Frag* xl = (Frag*)lds;
@@ -493,7 +536,7 @@ __global__ __launch_bounds__(1024) void k_q4g_stream(Q4gArgs a) {
     }
     totals[k] = sum;
     if constexpr (IN == Q4G_I8) {
-      xsl[k] = a.x_scales[(size_t)t * a.x_per + x_scale_at(a, c * Q4G_CHUNK + u * (128 / UNITS))];
+      xsl[k] = a.x_scales[(size_t)t * a.x_per + (a.x_per == 1 ? 0 : min(c * M + u * M / UNITS, a.x_per - 1))];
     }
   }
   __syncthreads();
@@ -538,20 +581,22 @@ __global__ __launch_bounds__(1024) void k_q4g_stream(Q4gArgs a) {
 
 // ---- many tokens -----------------------------------------------------------------------
 
+template <int IN, int UNITS> struct Q4gStage {
+  Q4gRow<IN> row[64];
+  typename Q4gType<IN>::Sum total[UNITS][64];
+  float xs[UNITS][64];
+};
+
 // A work-group computes 4 RT tiles of 16 rows for 64 tokens; its waves divide the rows, and
-// (WK) the chunks of 128 numbers.  For each chunk the tokens' numbers go through LDS as the
-// operands lie (wave k of four brings tokens 16 k .. and their sums); they are read from
-// memory two chunks ahead, and so are the weights, to registers.
-template <int IN, int PER, int UNITS, bool BF, int RT, int WK>
+// (WK) the chunks of 128 numbers.  For each chunk the tokens' numbers go through LDS (wave k of
+// four brings tokens 16 k .., each by 16 neighbouring lanes, and their sums); they are read
+// from memory two chunks ahead, and so are the weights, to registers.
+template <int IN, int PER, int M, bool BF, int RT, int WK>
 __global__ __launch_bounds__(256 * WK) void k_q4g_many(Q4gArgs a, unsigned token_tiles) {
   typedef Q4gType<IN> Ty;
   typedef typename Ty::Frag Frag;
-  constexpr int STEPS = 4 / UNITS, WR = 4, NT = 4, P = Ty::PARTS;
-  struct Stage {
-    Frag x[NT][4][P][64];
-    typename Ty::Sum total[UNITS][NT * 16];
-    float xs[UNITS][NT * 16];
-  };
+  constexpr int UNITS = PER > M ? PER : M, STEPS = 4 / UNITS, WR = 4, NT = 4, P = Ty::PARTS;
+  typedef Q4gStage<IN, UNITS> Stage;
   extern __shared__ char lds[];  // [WK][2] stages; then the second half's sums
   const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned wr = wave % WR, wk = wave / WR;
@@ -564,13 +609,15 @@ __global__ __launch_bounds__(256 * WK) void k_q4g_many(Q4gArgs a, unsigned token
   const unsigned tile0 = (block * WR + wr) * RT;
   if (block * WR * RT >= tiles) return;  // the whole work-group
 
-  const size_t t = min(tok0 + 16 * wr + i, a.ntok - 1);  // the token that this lane brings
-  const void* row = (const char*)a.x + t * a.x_stride * Ty::SIZE;
-  const float* xscale = IN == Q4G_I8 ? a.x_scales + t * a.x_per : nullptr;
+  // the tokens that this lane brings numbers of, and one whose scales it does
+  const char* row[4];
+#pragma unroll
+  for (int n = 0; n < 4; n++) row[n] = (const char*)a.x + min(tok0 + 16 * wr + 4 * n + g, a.ntok - 1) * a.x_stride * Ty::SIZE;
+  const float* xscale = IN == Q4G_I8 ? a.x_scales + min(tok0 + 16 * wr + i, a.ntok - 1) * a.x_per : nullptr;
 
   struct Tokens {
     Frag x[4][P];
-    float s[UNITS];
+    float s[M];
   } in[2];
   Q4gChunk<PER> q[4][RT];
   // turn k of this half is chunk k WK + wk (the last again where there are no more)
@@ -579,29 +626,27 @@ __global__ __launch_bounds__(256 * WK) void k_q4g_many(Q4gArgs a, unsigned token
 #pragma unroll
     for (int r = 0; r < RT; r++) Q4gTile<PER>(a.g, min(tile0 + r, tiles - 1), lane).load(c, to[r]);
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-      load_x<IN>(a, row, c, j, g, x.x[j]);
-    if constexpr (IN == Q4G_I8) {
-#pragma unroll
-      for (int u = 0; u < UNITS; u++) {
-        x.s[u] = xscale[x_scale_at(a, c * Q4G_CHUNK + u * (128 / UNITS))];
-      }
-    }
+    for (int n = 0; n < 4; n++) load_x<IN>(a, row[n], c, i / 4, i % 4, x.x[n]);
+    if constexpr (IN == Q4G_I8) load_x_scales<M>(a, xscale, c, x.s);
   };
   auto bring = [&](Stage& s, const Tokens& x) {
 #pragma unroll
-    for (int j = 0; j < 4; j++)
+    for (int n = 0; n < 4; n++)
 #pragma unroll
-      for (int p = 0; p < P; p++) s.x[wr][j][p][lane] = x.x[j][p];
+      for (int p = 0; p < P; p++) s.row[16 * wr + 4 * n + g].f[16 * p + i] = x.x[n][p];
 #pragma unroll
     for (int u = 0; u < UNITS; u++) {
-      Frag ones[STEPS];
+      Frag ones[STEPS], mine[STEPS][P];  // of this wave's tokens, which it has just brought
 #pragma unroll
-      for (int e = 0; e < STEPS; e++) ones[e] = ones8<IN>();
-      const typename Ty::Acc total = products<IN, STEPS>(ones, &x.x[u * STEPS]);
+      for (int e = 0; e < STEPS; e++) {
+        ones[e] = ones8<IN>();
+#pragma unroll
+        for (int p = 0; p < P; p++) mine[e][p] = s.row[16 * wr + i].f[16 * p + 4 * (u * STEPS + e) + g];
+      }
+      const typename Ty::Acc total = products<IN, STEPS>(ones, mine);
       if (g == 0) {
         s.total[u][16 * wr + i] = total[0];
-        if constexpr (IN == Q4G_I8) s.xs[u][16 * wr + i] = x.s[u];
+        if constexpr (IN == Q4G_I8) s.xs[u][16 * wr + i] = x.s[u * M / UNITS];
       }
     }
   };
@@ -630,7 +675,7 @@ __global__ __launch_bounds__(256 * WK) void k_q4g_many(Q4gArgs a, unsigned token
 #pragma unroll
         for (int e = 0; e < STEPS; e++)
 #pragma unroll
-          for (int p = 0; p < P; p++) x[e][p] = s.x[n][u * STEPS + e][p][lane];
+          for (int p = 0; p < P; p++) x[e][p] = s.row[16 * n + i].f[16 * p + 4 * (u * STEPS + e) + g];
         const typename Ty::Sum total = s.total[u][16 * n + i];
         const float xs = IN == Q4G_I8 ? s.xs[u][16 * n + i] : 0.0f;
 #pragma unroll
@@ -689,7 +734,12 @@ hipError_t launch_q4g_unpack(const Q4gGeom& g, uint8_t* codes, uint16_t* scales,
   return launch(k_q4g_unpack, dim3(tiles, g.chunks < 1024 ? g.chunks : 1024), 256, 0, st, g, codes, scales, zeros);
 }
 
-template <int IN, int PER, int UNITS, bool BF, int CH, int W>
+// More LDS than a kernel has unasked.
+static hipError_t ask_lds(const void* kernel, uint32_t bytes) {
+  return bytes <= 65536 ? hipSuccess : hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+template <int IN, int PER, int M, bool BF, int CH, int W>
 static hipError_t q4g_few(const Q4gArgs& a, hipStream_t st) {
   const unsigned tiles = (unsigned)((a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS);
   // as many work-groups as there are compute units, each with a chunk a wave at least
@@ -699,72 +749,68 @@ static hipError_t q4g_few(const Q4gArgs& a, hipStream_t st) {
   splits = splits > Q4G_SPLITS ? Q4G_SPLITS : splits;
   const unsigned per = (a.g.chunks + splits - 1) / splits;
   splits = (a.g.chunks + per - 1) / per;
-  return launch(k_q4g_few<IN, PER, UNITS, BF, CH, W>, dim3(tiles, splits), 64 * W, 0, st, a, per);
+  const uint32_t rows = W * CH * (uint32_t)a.ntok * sizeof(Q4gRow<IN>), lds = rows > W * 1024 ? rows : W * 1024;
+  const hipError_t e = ask_lds((const void*)k_q4g_few<IN, PER, M, BF, CH, W>, lds);
+  if (e != hipSuccess) return e;
+  return launch(k_q4g_few<IN, PER, M, BF, CH, W>, dim3(tiles, splits), 64 * W, lds, st, a, per);
 }
 
-template <int IN, int PER, int UNITS, bool BF, int AHEAD>
+template <int IN, int PER, int M, bool BF, int AHEAD>
 static hipError_t q4g_stream(const Q4gArgs& a, uint32_t lds, hipStream_t st) {
   const unsigned tiles = (unsigned)((a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS);
-  if (lds > 65536) {  // more than a kernel has unasked
-    const hipError_t e = hipFuncSetAttribute((const void*)k_q4g_stream<IN, PER, UNITS, BF, AHEAD>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return e;
-  }
-  static const char* env = getenv("Q4W");
+  const hipError_t e = ask_lds((const void*)k_q4g_stream<IN, PER, M, BF, AHEAD>, lds);
+  if (e != hipSuccess) return e;
+  // a work-group per compute unit, of so many waves that all of them have nearly as many tiles
   unsigned waves = 16, best = ~0u;
   for (unsigned w = 16; w >= 8; w--) {
-    const unsigned longest = (tiles + 256 * w - 1) / (256 * w) * w;  // tiles that the waves' time is that of
+    const unsigned longest = (tiles + 256 * w - 1) / (256 * w) * w;
     if (longest < best) best = longest, waves = w;
   }
-  if (env) waves = atoi(env);
-  return launch(k_q4g_stream<IN, PER, UNITS, BF, AHEAD>, 256, 64 * waves, lds, st, a);
+  return launch(k_q4g_stream<IN, PER, M, BF, AHEAD>, 256, 64 * waves, lds, st, a);
 }
 
-template <int IN, int PER, int UNITS, bool BF, int RT, int WK>
+template <int IN, int PER, int M, bool BF, int RT, int WK>
 static hipError_t q4g_many(const Q4gArgs& a, hipStream_t st) {
   const unsigned tiles = (unsigned)((a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS);
   const unsigned blocks = (tiles + 4 * RT - 1) / (4 * RT), token_tiles = (unsigned)((a.ntok + 63) / 64);
-  constexpr uint32_t stage = 4 * 4 * 64 * Q4gType<IN>::PARTS * sizeof(typename Q4gType<IN>::Frag) + 2 * UNITS * 64 * 4;
+  constexpr uint32_t stage = sizeof(Q4gStage<IN, (PER > M ? PER : M)>);
   constexpr uint32_t sums = WK == 2 ? 4 * RT * 4 * 1024 : 0, lds = 2 * WK * stage > sums ? 2 * WK * stage : sums;
   static_assert(lds <= 163840, "LDS of a compute unit");
-  if (lds > 65536) {
-    const hipError_t e = hipFuncSetAttribute((const void*)k_q4g_many<IN, PER, UNITS, BF, RT, WK>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return e;
-  }
+  const hipError_t e = ask_lds((const void*)k_q4g_many<IN, PER, M, BF, RT, WK>, lds);
+  if (e != hipSuccess) return e;
   const size_t grid = (size_t)(blocks + 7) / 8 * 8 * token_tiles;
   if (grid > 0x7fffffffu) return hipErrorInvalidValue;
-  return launch(k_q4g_many<IN, PER, UNITS, BF, RT, WK>, dim3((unsigned)grid), 256 * WK, lds, st, a, token_tiles);
+  return launch(k_q4g_many<IN, PER, M, BF, RT, WK>, dim3((unsigned)grid), 256 * WK, lds, st, a, token_tiles);
 }
 
-template <int IN, int PER, int UNITS, bool BF>
+template <int IN, int PER, int M, bool BF>
 static hipError_t q4g_sized(const Q4gArgs& a, hipStream_t st) {
+  constexpr int UNITS = PER > M ? PER : M;
   if (a.ntok <= 16) {
     const size_t tiles = (a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS, lds = (size_t)a.g.chunks * a.ntok * Q4gTokens<IN, UNITS>::BYTES;
-    if (tiles * a.g.chunks >= 65536 && lds <= 65536) return q4g_stream<IN, PER, UNITS, BF, UNITS == 4 ? 4 : 6>(a, (uint32_t)lds, st);
-    return q4g_few<IN, PER, UNITS, BF, IN == Q4G_F32 ? 1 : 2, 8>(a, st);
+    if (tiles * a.g.chunks >= 65536 && lds <= 65536) return q4g_stream<IN, PER, M, BF, PER == 4 ? (IN == Q4G_F32 ? 2 : 3) : UNITS == 4 || IN == Q4G_F32 ? 4 : 6>(a, (uint32_t)lds, st);
+    return q4g_few<IN, PER, M, BF, IN == Q4G_F32 ? 1 : 2, 8>(a, st);
   }
-  return q4g_many<IN, PER, UNITS, BF, 2, IN == Q4G_F32 ? 1 : 2>(a, st);
+  return q4g_many<IN, PER, M, BF, 2, IN == Q4G_F32 || PER == 4 ? 1 : 2>(a, st);
+}
+
+template <int IN, int PER, bool BF>
+static hipError_t q4g_scaled(const Q4gArgs& a, hipStream_t st) {
+  if constexpr (IN == Q4G_I8) {
+    if (a.x_shift == 5) return q4g_sized<IN, PER, 4, BF>(a, st);
+    if (a.x_shift == 6) return q4g_sized<IN, PER, 2, BF>(a, st);
+  }
+  return q4g_sized<IN, PER, 1, BF>(a, st);
 }
 
 template <int IN, bool BF>
 static hipError_t q4g_units(const Q4gArgs& a, hipStream_t st) {
-  if constexpr (IN == Q4G_I8) {
-    const unsigned unit = a.x_shift < 7 && (1u << a.x_shift) < a.g.group ? 1u << a.x_shift : a.g.group;
-    switch (a.g.per * 8 + 128 / unit) {
-      case 9: return q4g_sized<IN, 1, 1, BF>(a, st);
-      case 10: return q4g_sized<IN, 1, 2, BF>(a, st);
-      case 12: return q4g_sized<IN, 1, 4, BF>(a, st);
-      case 18: return q4g_sized<IN, 2, 2, BF>(a, st);
-      case 20: return q4g_sized<IN, 2, 4, BF>(a, st);
-      case 36: return q4g_sized<IN, 4, 4, BF>(a, st);
-    }
-  } else {
-    switch (a.g.per) {
-      case 1: return q4g_sized<IN, 1, 1, BF>(a, st);
-      case 2: return q4g_sized<IN, 2, 2, BF>(a, st);
-      case 4: return q4g_sized<IN, 4, 4, BF>(a, st);
-    }
+  switch (a.g.per) {
+    case 1: return q4g_scaled<IN, 1, BF>(a, st);
+    case 2: return q4g_scaled<IN, 2, BF>(a, st);
+    case 4: return q4g_scaled<IN, 4, BF>(a, st);
+    default: return hipErrorInvalidValue;
   }
-  return hipErrorInvalidValue;
 }
 
 hipError_t launch_q4g(Q4gInput in, const Q4gArgs& a, hipStream_t st) {
