@@ -16,8 +16,8 @@
 
 namespace hale {
 
-constexpr int LG_THREADS = 256;
-constexpr unsigned LG_OCCURS = 0x80000000u;  // beside the count of generated ones
+constexpr int LG_THREADS = 256, LG_AHEAD = 8;
+constexpr unsigned LG_OCCURS = 0x80000000u;  // in the prompt, beside the count of generated ones
 
 template <typename T> __device__ __forceinline__ T lowest_of();
 template <> __device__ __forceinline__ float lowest_of<float>() { return -__builtin_inff(); }
@@ -26,14 +26,20 @@ template <> __device__ __forceinline__ Bf16 lowest_of<Bf16>() { return {0xff80};
 
 __device__ __forceinline__ int64_t clamped(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 
-// A work-group takes 256 * 8 * C neighbouring tokens of a row: it counts, in LDS, the
-// row's tokens that fall among them, finds the last bias of each, and applies all of it in
-// one pass over the logits, which are on their way meanwhile.  Counts and the biases'
-// places are whole numbers, so the order of the atomics leaves no trace.
+// A work-group takes 256 * 8 * C neighbouring tokens of a row: in LDS it counts the row's
+// tokens that fall among them, and then finds the last bias of each, while the logits are on their
+// way, eight neighbours to a thread.  Counts and the biases' places are whole numbers, so
+// the order of the atomics leaves no trace.  The one table serves both in turn, and tokens
+// are read eight to a thread at a time: 64 rows of 151936 bf16 with up to 4000 tokens and 300 biases each
+// 17.3 us, of which reading and writing the logits alone is 5.8, the mask 0.8, the tokens
+// 5.5 and the biases 3.3 (24 us with a table for each, a token a thread at a time and two atomics for
+// it).  One row of f32 4.9 us, a launch alone 3.5.  Bound by each work-group's passes
+// over the row's lists: sorting them first would take a launch and a workspace
+// of its own.
 template <typename T, int C, bool VEC>
 __global__ __launch_bounds__(LG_THREADS) void k_logits(LogitsArgs a) {
   constexpr unsigned SLICE = LG_THREADS * 8 * C;
-  __shared__ unsigned count[SLICE], place[SLICE];
+  __shared__ unsigned table[SLICE];
   const unsigned t = threadIdx.x;
   const size_t row = blockIdx.x, first = (size_t)blockIdx.y * SLICE;
   const unsigned size = (unsigned)(a.vocab - first < SLICE ? a.vocab - first : SLICE);
@@ -59,73 +65,108 @@ __global__ __launch_bounds__(LG_THREADS) void k_logits(LogitsArgs a) {
     const int64_t m = r.mask_row ? (int64_t)r.mask_row[row] : (int64_t)row;
     if (m >= 0 && m < (int64_t)r.mask_rows) mask = r.mask + (size_t)m * r.mask_stride;
   }
-  unsigned keep[C];
+  unsigned keep[C], named[C];  // a bit per logit: its mask's, and whether a rule has changed it
 #pragma unroll
   for (int c = 0; c < C; c++) {
     const unsigned at = (c * LG_THREADS + t) * 8;
     keep[c] = mask && at < size ? mask[(first + at) / 32] >> at % 32 & 255 : 255;
+    named[c] = 0;
   }
   int64_t b0 = 0, b1 = 0, t0 = 0, t1 = 0, made = 0;
   if (r.tokens) {
     t0 = clamped(r.token_start[row], 0, (int64_t)r.ntokens);
     t1 = clamped(r.token_start[row + 1], t0, (int64_t)r.ntokens);
-    made = r.prompt_len ? clamped(r.prompt_len[row], 0, t1 - t0) : 0;
+    made = t0 + (r.prompt_len ? clamped(r.prompt_len[row], 0, t1 - t0) : 0);
   }
   if (r.bias_tokens) {
     b0 = clamped(r.bias_start[row], 0, (int64_t)r.nbiases);
     b1 = clamped(r.bias_start[row + 1], b0, (int64_t)r.nbiases);
   }
-  const float repetition = r.repetition ? r.repetition[row] : 1.0f;
-  const float frequency = r.frequency ? r.frequency[row] : 0.0f, presence = r.presence ? r.presence[row] : 0.0f;
-  const bool any = t1 > t0 || b1 > b0;
-  if (any) {
-    for (unsigned k = 4 * t; k < SLICE; k += 4 * LG_THREADS) {
-      *(u32x4*)&count[k] = u32x4{0, 0, 0, 0};
-      *(u32x4*)&place[k] = u32x4{0, 0, 0, 0};
-    }
+  float v[C][8];
+  if (t1 > t0 || b1 > b0) {
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) *(u32x4*)&table[(c * LG_THREADS + t) * 8 + j] = u32x4{0, 0, 0, 0};
+  }
+  if (t1 > t0) {
+    const float repetition = r.repetition ? r.repetition[row] : 1.0f;
+    const float frequency = r.frequency ? r.frequency[row] : 0.0f, presence = r.presence ? r.presence[row] : 0.0f;
     __syncthreads();
-    made += t0;
-#pragma unroll 8
-    for (int64_t k = t0 + t; k < t1; k += LG_THREADS) {
-      const size_t at = (size_t)(int64_t)r.tokens[k] - first;  // a token below `first`, or negative, is past all sizes
-      if (at < size) {
-        if (k >= made) atomicAdd(&count[at], 1u);
-        atomicOr(&count[at], LG_OCCURS);
+    // several tokens a thread at a time, on their way together
+    const int32_t* tokens = r.tokens + t0;
+    const unsigned n_tokens = (unsigned)(t1 - t0), n_prompt = (unsigned)(made - t0);
+    for (unsigned from = t; from < n_tokens; from += LG_AHEAD * LG_THREADS) {
+      int32_t token[LG_AHEAD];
+#pragma unroll
+      for (int k = 0; k < LG_AHEAD; k++) token[k] = tokens[min(from + k * LG_THREADS, n_tokens - 1)];
+#pragma unroll
+      for (int k = 0; k < LG_AHEAD; k++) {
+        const size_t at = (size_t)(int64_t)token[k] - first;  // a token below `first`, or negative, is past all sizes
+        if (at < size && from + k * LG_THREADS < n_tokens) {
+          if (from + k * LG_THREADS >= n_prompt) atomicAdd(&table[at], 1u);
+          else atomicOr(&table[at], LG_OCCURS);
+        }
       }
     }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      unsigned n[8];
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) {
+        u32x4* own = (u32x4*)&table[(c * LG_THREADS + t) * 8 + j];
+        *(u32x4*)&n[j] = *own;
+        if (b1 > b0) *own = u32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        if (!n[j]) continue;
+        float y = to_f32(x[c][j]);
+        y = y > 0.0f ? y / repetition : y * repetition;
+        const unsigned g = n[j] & ~LG_OCCURS;
+        if (g) y = (y - frequency * (float)g) - presence;
+        v[c][j] = y;
+        named[c] |= 1u << j;
+      }
+    }
+  }
+  if (b1 > b0) {
+    __syncthreads();
     for (int64_t k = b0 + t; k < b1; k += LG_THREADS) {
       const size_t at = (size_t)(int64_t)r.bias_tokens[k] - first;
-      if (at < size) atomicMax(&place[at], (unsigned)(k - b0 + 1));
+      if (at < size) atomicMax(&table[at], (unsigned)(k - b0 + 1));
     }
     __syncthreads();
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      unsigned p[8];
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) *(u32x4*)&p[j] = *(const u32x4*)&table[(c * LG_THREADS + t) * 8 + j];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        if (!p[j]) continue;
+        v[c][j] = (named[c] >> j & 1 ? v[c][j] : to_f32(x[c][j])) + r.bias[b0 + (int64_t)p[j] - 1];
+        named[c] |= 1u << j;
+      }
+    }
   }
 #pragma unroll
   for (int c = 0; c < C; c++) {
     const unsigned at = (c * LG_THREADS + t) * 8;
     if (at >= size) continue;
-    if (any) {
-      unsigned n[8], p[8];
-#pragma unroll
-      for (int j = 0; j < 8; j += 4) {
-        *(u32x4*)&n[j] = *(const u32x4*)&count[at + j];
-        *(u32x4*)&p[j] = *(const u32x4*)&place[at + j];
-      }
+    if (named[c]) {
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        if (!(n[j] | p[j])) continue;
-        float v = to_f32(x[c][j]);
-        if (n[j]) {
-          v = v > 0.0f ? v / repetition : v * repetition;
-          const unsigned g = n[j] & ~LG_OCCURS;
-          if (g) v = (v - frequency * (float)g) - presence;
-        }
-        if (p[j]) v = v + r.bias[b0 + (int64_t)p[j] - 1];
-        x[c][j] = from_f32<T>(v);
+        const T y = from_f32<T>(v[c][j]);
+        if (named[c] >> j & 1) x[c][j] = y;
       }
     }
+    if (keep[c] != 255) {
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-      if (!(keep[c] >> j & 1)) x[c][j] = lowest_of<T>();
+      for (int j = 0; j < 8; j++)
+        if (!(keep[c] >> j & 1)) x[c][j] = lowest_of<T>();
+    }
     if (VEC && at + 8 <= size) {
 #pragma unroll
       for (int j = 0; j < 8; j += 16 / (int)sizeof(T)) *(u32x4*)(out + at + j) = *(const u32x4*)&x[c][j];
@@ -144,11 +185,18 @@ static hipError_t logits_sized(const LogitsArgs& a, size_t rows, hipStream_t st)
   return a.vec ? launch(k_logits<T, C, true>, grid, LG_THREADS, 0, st, a) : launch(k_logits<T, C, false>, grid, LG_THREADS, 0, st, a);
 }
 
+template <typename T> static hipError_t logits_typed(const LogitsArgs& a, size_t rows, hipStream_t st) {
+  // few rows: as many work-groups as there are compute units; many: fewer passes over the rows' tokens
+  // (64 rows of 151936 17.6 us, 18.4 with half the slice; one 6.3, 4.9 with half)
+  const bool large = rows * a.vocab >= (size_t)1 << 22;
+  return large ? logits_sized<T, 2>(a, rows, st) : logits_sized<T, 1>(a, rows, st);
+}
+
 hipError_t launch_logits(int dtype, const LogitsArgs& a, size_t rows, hipStream_t st) {
   if (rows == 0 || a.vocab == 0) return hipSuccess;
-  if (dtype == F32) return logits_sized<float, 1>(a, rows, st);
-  if (dtype == F16) return logits_sized<_Float16, 1>(a, rows, st);
-  return logits_sized<Bf16, 1>(a, rows, st);
+  if (dtype == F32) return logits_typed<float>(a, rows, st);
+  if (dtype == F16) return logits_typed<_Float16>(a, rows, st);
+  return logits_typed<Bf16>(a, rows, st);
 }
 
 }  // namespace hale
