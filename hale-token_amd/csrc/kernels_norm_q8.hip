@@ -16,36 +16,46 @@
 
 namespace hale {
 
-// Eight numbers of a row as f32.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const void* base, size_t at, float (&v)[8]) {
-  const T* p = (const T*)base + at;
-  T raw[8];
-  if constexpr (VEC) {
-#pragma unroll
-    for (int j = 0; j < 8; j += 16 / (int)sizeof(T)) *(u32x4*)&raw[j] = *(const u32x4*)(p + j);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; j++) raw[j] = p[j];
-  }
-#pragma unroll
-  for (int j = 0; j < 8; j++) v[j] = to_f32(raw[j]);
-}
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(void* base, size_t at, const float (&v)[8]) {
-  T* p = (T*)base + at;
-  T raw[8];
+// Eight numbers of a row as they lie.
+template <typename T> struct Eight {
+  alignas(16) T v[8];
+  template <bool VEC> __device__ __forceinline__ void load(const void* base, size_t at) {
+    const T* p = (const T*)base + at;
+    if constexpr (VEC) {
 #pragma unroll
-  for (int j = 0; j < 8; j++) raw[j] = from_f32<T>(v[j]);
-  if constexpr (VEC) {
+      for (int j = 0; j < 8; j += 16 / (int)sizeof(T)) *(u32x4*)&v[j] = *(const u32x4*)(p + j);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; j += 16 / (int)sizeof(T)) *(u32x4*)(p + j) = *(u32x4*)&raw[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; j++) p[j] = raw[j];
+      for (int j = 0; j < 8; j++) v[j] = p[j];
+    }
   }
-}
+  template <bool VEC> __device__ __forceinline__ void store(void* base, size_t at) const {
+    T* p = (T*)base + at;
+    if constexpr (VEC) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 16 / (int)sizeof(T)) *(u32x4*)(p + j) = *(const u32x4*)&v[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) p[j] = v[j];
+    }
+  }
+  // Rounded to nearest even; a NaN stays one.
+  __device__ __forceinline__ void round(const float (&f)[8]) {
+    if constexpr (sizeof(T) == 2 && !__is_same(T, _Float16)) {  // two at a time, without a branch for NaNs
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const bf16x2 r = __builtin_convertvector(f32x2{f[j], f[j + 1]}, bf16x2);
+        __builtin_memcpy(&v[j], &r, 4);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = from_f32<T>(f[j]);
+    }
+  }
+};
 
 __device__ __forceinline__ double from_words(unsigned lo, unsigned hi) {
   return __longlong_as_double((long long)((unsigned long long)hi << 32 | lo));
@@ -84,8 +94,9 @@ __device__ __forceinline__ int code_of(double u, double top, double inv) {
   return (int)q;
 }
 
-// A work-group of NT threads per row, C groups of eight numbers a thread, all of them
-// read before anything is written.  Blocks of 32, 64 and 128 numbers lie in 4, 8 and 16
+// A work-group of NT threads per row, C groups of eight numbers a thread, all of them on
+// their way at once and read before anything is written.  Four groups a thread spill
+// (64-bit codes of 32 numbers), hence 1024 threads and 16384 numbers at most.  Blocks of 32, 64 and 128 numbers lie in 4, 8 and 16
 // neighbouring lanes.
 template <typename T, int NT, int C, bool VEC>
 __global__ __launch_bounds__(NT) void k_norm_q8(NormQ8Args a) {
@@ -94,22 +105,29 @@ __global__ __launch_bounds__(NT) void k_norm_q8(NormQ8Args a) {
   const int t = threadIdx.x, wave = t >> 6;
   const size_t row = blockIdx.x;
   const unsigned groups = a.n / 8;
+  Eight<T> sum8[C], delta[C];
+  Eight<float> weight[C];
   float s[C][8], w[C][8];
 #pragma unroll
+  for (int c = 0; c < C; c++) {  // groups behind the row are some of it, and count for nothing
+    const unsigned at = 8 * min((unsigned)(t + NT * c), groups - 1);
+    sum8[c].template load<VEC>(a.x, row * a.x_stride + at);
+    if (a.delta) delta[c].template load<VEC>(a.delta, row * a.delta_stride + at);
+    weight[c].template load<VEC>(a.w, at);
+  }
+#pragma unroll
   for (int c = 0; c < C; c++) {
-    const unsigned at = (unsigned)(t + NT * c);
-    if (at < groups) {
-      load8<T, VEC>(a.x, row * a.x_stride + 8 * at, s[c]);
-      load8<float, VEC>(a.w, 8 * at, w[c]);
-      if (a.delta) {
-        float d[8];
-        load8<T, VEC>(a.delta, row * a.delta_stride + 8 * at, d);
+    if (a.delta) {
+      float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) s[c][j] = to_f32(from_f32<T>(s[c][j] + d[j]));
-      }
-    } else {
+      for (int j = 0; j < 8; j++) f[j] = to_f32(sum8[c].v[j]) + to_f32(delta[c].v[j]);
+      sum8[c].round(f);
+    }
+    const bool in = (unsigned)(t + NT * c) < groups;
 #pragma unroll
-      for (int j = 0; j < 8; j++) s[c][j] = w[c][j] = 0.0f;
+    for (int j = 0; j < 8; j++) {
+      s[c][j] = in ? to_f32(sum8[c].v[j]) : 0.0f;
+      w[c][j] = in ? weight[c].v[j] : 0.0f;
     }
   }
   double sum = 0, top[C];
@@ -194,12 +212,14 @@ __global__ __launch_bounds__(NT) void k_norm_q8(NormQ8Args a) {
     } else if (8 * at % a.block == 0) {
       a.scales[row * (a.n / a.block) + 8 * at / a.block] = scale;
     }
-    if (a.sum) store8<T, VEC>(a.sum, row * a.sum_stride + 8 * at, s[c]);
+    if (a.sum) sum8[c].template store<VEC>(a.sum, row * a.sum_stride + 8 * at);
     if (a.y) {
       float y[8];
 #pragma unroll
       for (int j = 0; j < 8; j++) y[j] = (float)((double)s[c][j] * (double)w[c][j] * r);
-      store8<T, VEC>(a.y, row * a.y_stride + 8 * at, y);
+      Eight<T> y8;
+      y8.round(y);
+      y8.template store<VEC>(a.y, row * a.y_stride + 8 * at);
     }
   }
 }
