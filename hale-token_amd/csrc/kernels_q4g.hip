@@ -108,9 +108,8 @@ template <> struct Q4gType<Q4G_I8> {
 };
 
 // A word's eight codes, each 16 + q.  16 .. 31 are consecutive steps of a float's mantissa:
-// the four bits of a code go into it below the pattern of 16.  (A conversion
-// instruction takes four times as long as one of these: a vocabulary's product 41 us with
-// conversions, 28 so.)
+// the four bits of a code go into it below the pattern of 16, one instruction for a pair
+// (conversions to floats are one for each number and another to join a pair).
 template <int IN> __device__ __forceinline__ typename Q4gType<IN>::Frag codes8(unsigned w) {
   if constexpr (IN == Q4G_I8) {
     return u32x2{(w & 0x0f0f0f0fu) | 0x10101010u, (w >> 4 & 0x0f0f0f0fu) | 0x10101010u};
@@ -367,6 +366,13 @@ __device__ __forceinline__ f32x4 get_part(const float* p) {
   return v;
 }
 
+// What a wave's lanes have written to LDS, before others of them read it (they run in
+// step, and LDS serves a wave in its order: nothing to wait for but the compiler).
+__device__ __forceinline__ void lanes_exchange() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Tokens in LDS: a row per token and chunk of operands of eight numbers [part][16], and a gap that
 // puts the same operand of 16 tokens into different banks.
 template <int IN> struct Q4gRow {
@@ -429,6 +435,7 @@ __global__ __launch_bounds__(64 * W) void k_q4g_few(Q4gArgs a, unsigned per_spli
         }
       }
     }
+    lanes_exchange();
 #pragma unroll
     for (int k = 0; k < CH; k++) {
       if (from + W * k >= c1) continue;
@@ -448,6 +455,7 @@ __global__ __launch_bounds__(64 * W) void k_q4g_few(Q4gArgs a, unsigned per_spli
                            q[k].z[u * PER / UNITS], IN == Q4G_I8 ? xs[k][u * M / UNITS] : 0.0f);
       }
     }
+    lanes_exchange();
   }
   __syncthreads();  // the rows are read
   red[wave][lane] = sum;
@@ -634,6 +642,7 @@ __global__ __launch_bounds__(256 * WK) void k_q4g_many(Q4gArgs a, unsigned token
     for (int n = 0; n < 4; n++)
 #pragma unroll
       for (int p = 0; p < P; p++) s.row[16 * wr + 4 * n + g].f[16 * p + i] = x.x[n][p];
+    lanes_exchange();
 #pragma unroll
     for (int u = 0; u < UNITS; u++) {
       Frag ones[STEPS], mine[STEPS][P];  // of this wave's tokens, which it has just brought
@@ -734,6 +743,8 @@ hipError_t launch_q4g_unpack(const Q4gGeom& g, uint8_t* codes, uint16_t* scales,
   return launch(k_q4g_unpack, dim3(tiles, g.chunks < 1024 ? g.chunks : 1024), 256, 0, st, g, codes, scales, zeros);
 }
 
+constexpr uint32_t Q4G_LDS = 163840;  // of a compute unit
+
 // More LDS than a kernel has unasked.
 static hipError_t ask_lds(const void* kernel, uint32_t bytes) {
   return bytes <= 65536 ? hipSuccess : hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
@@ -775,20 +786,41 @@ static hipError_t q4g_many(const Q4gArgs& a, hipStream_t st) {
   const unsigned blocks = (tiles + 4 * RT - 1) / (4 * RT), token_tiles = (unsigned)((a.ntok + 63) / 64);
   constexpr uint32_t stage = sizeof(Q4gStage<IN, (PER > M ? PER : M)>);
   constexpr uint32_t sums = WK == 2 ? 4 * RT * 4 * 1024 : 0, lds = 2 * WK * stage > sums ? 2 * WK * stage : sums;
-  static_assert(lds <= 163840, "LDS of a compute unit");
+  static_assert(lds <= Q4G_LDS, "LDS of a compute unit");
   const hipError_t e = ask_lds((const void*)k_q4g_many<IN, PER, M, BF, RT, WK>, lds);
   if (e != hipSuccess) return e;
-  const size_t grid = (size_t)(blocks + 7) / 8 * 8 * token_tiles;
-  if (grid > 0x7fffffffu) return hipErrorInvalidValue;
-  return launch(k_q4g_many<IN, PER, M, BF, RT, WK>, dim3((unsigned)grid), 256 * WK, lds, st, a, token_tiles);
+  const unsigned grid = (blocks + 7) / 8 * 8 * token_tiles;  // below 2^23 (2^35 results)
+  return launch(k_q4g_many<IN, PER, M, BF, RT, WK>, grid, 256 * WK, lds, st, a, token_tiles);
 }
 
 template <int IN, int PER, int M, bool BF>
 static hipError_t q4g_sized(const Q4gArgs& a, hipStream_t st) {
   constexpr int UNITS = PER > M ? PER : M;
   if (a.ntok <= 16) {
-    const size_t tiles = (a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS, lds = (size_t)a.g.chunks * a.ntok * Q4gTokens<IN, UNITS>::BYTES;
-    if (tiles * a.g.chunks >= 65536 && lds <= 65536) return q4g_stream<IN, PER, M, BF, PER == 4 ? (IN == Q4G_F32 ? 2 : 3) : UNITS == 4 || IN == Q4G_F32 ? 4 : 6>(a, (uint32_t)lds, st);
+    // Each wave of the streaming kernel needs a tile or nearly so: rows of 4096, a token of bf16
+    // (f32), the streaming kernel and the other: 16384 rows 14.3 and 11.1 us (19.1 and 21.6), 24576
+    // 14.7 and 15.8 (19.7 and 31.5), 151936 60 and 87 (82 and 185).  And its tokens have to fit
+    // into LDS: 16 tokens of bf16 and 151936 rows 68 us, 116 without it.  f32 takes three
+    // times the room and the other kernel three times the time for 16 tokens, so that slices
+    // of the tokens, each with all weights, are still faster.
+    constexpr uint32_t BYTES = Q4gTokens<IN, UNITS>::BYTES;
+    const unsigned tiles = (unsigned)((a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS), ntok = (unsigned)a.ntok;
+    const unsigned fit = a.g.chunks <= Q4G_LDS / BYTES ? Q4G_LDS / (a.g.chunks * BYTES) : 0, most = IN == Q4G_F32 ? 3 : 1;
+    if (tiles >= (IN == Q4G_F32 ? 1024u : 1536u) && fit * most >= ntok) {
+      const unsigned slices = (ntok + fit - 1) / fit;
+      for (unsigned k = 0, from = 0; k < slices; k++) {
+        Q4gArgs slice = a;
+        slice.ntok = (ntok - from) / (slices - k);
+        slice.x = (const char*)a.x + from * a.x_stride * Q4gType<IN>::SIZE;
+        slice.out = (char*)a.out + from * a.out_stride * (IN == Q4G_F32 ? 4 : 2);
+        // chunks on their way: as many as registers hold
+        constexpr int AHEAD = PER == 4 ? (IN == Q4G_F32 ? 2 : 3) : UNITS == 4 || IN == Q4G_F32 ? 4 : 6;
+        const hipError_t e = q4g_stream<IN, PER, M, BF, AHEAD>(slices == 1 ? a : slice, a.g.chunks * BYTES * (unsigned)slice.ntok, st);
+        if (e != hipSuccess) return e;
+        from += (unsigned)slice.ntok;
+      }
+      return hipSuccess;
+    }
     return q4g_few<IN, PER, M, BF, IN == Q4G_F32 ? 1 : 2, 8>(a, st);
   }
   return q4g_many<IN, PER, M, BF, 2, IN == Q4G_F32 || PER == 4 ? 1 : 2>(a, st);

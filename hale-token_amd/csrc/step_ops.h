@@ -24,6 +24,7 @@ struct NormQ8Args {
   float eps;
   bool vec;               // all rows (and w) start at multiples of 16 bytes, codes of 8
 };
+constexpr size_t STEP_ROWS = 1u << 22;  // a grid has less than 2^32 threads, a work-group up to 1024
 constexpr size_t NORM_Q8_MAX = 16384;  // numbers per row
 hipError_t launch_norm_q8(int dtype, const NormQ8Args& a, size_t rows, hipStream_t st);
 

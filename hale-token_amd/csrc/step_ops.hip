@@ -30,7 +30,7 @@ extern "C" int hale_rms_norm_q8_device(hale_ctx* c, int dtype, size_t rows, size
   if ((block != 32 && block != 64 && block != 128 && block != n) || n % block)
     return ctx_fail(c, HALE_EINVAL, "rms_norm_q8: blocks of %zu in rows of %zu", block, n);
   if (!(eps >= 0.0f) || !std::isfinite(eps)) return ctx_fail(c, HALE_EINVAL, "rms_norm_q8: eps %g", (double)eps);
-  if (rows >= (1ull << 31)) return ctx_fail(c, HALE_EINVAL, "rms_norm_q8: %zu rows", rows);
+  if (rows >= STEP_ROWS) return ctx_fail(c, HALE_EINVAL, "rms_norm_q8: %zu rows", rows);
   if (rows == 0) return HALE_OK;
   if (!x || !weight || !quants || !scales) return ctx_fail(c, HALE_EINVAL, "rms_norm_q8: NULL argument");
   if (x_stride < n || (delta && delta_stride < n) || (sum && sum_stride < n) || (y && y_stride < n))
@@ -84,7 +84,7 @@ static int q4g_make(hale_ctx* c, size_t rows, size_t cols, size_t group, int sca
     return ctx_fail(c, HALE_EINVAL, "q4g_upload: groups of %zu (32, 64 or 128)", group);
   if (scale_dtype != HALE_F16 && scale_dtype != HALE_BF16)
     return ctx_fail(c, HALE_EINVAL, "q4g_upload: scales of dtype %d are not f16 or bf16", scale_dtype);
-  if (rows == 0 || rows > (1u << 30) || cols == 0 || cols > (1u << 30) || cols % group)
+  if (rows == 0 || rows > (1u << 27) || cols == 0 || cols > (1u << 30) || cols % group)
     return ctx_fail(c, HALE_EINVAL, "q4g_upload: %zu rows of %zu in groups of %zu", rows, cols, group);
   if ((uintptr_t)scales % 2) return ctx_fail(c, HALE_EINVAL, "q4g_upload: scales are not aligned");
   const size_t groups = rows * (cols / group);
@@ -215,6 +215,8 @@ static int q4g_run(hale_q4g* m, Q4gInput in, Q4gArgs& a, int dtype, size_t ntok,
   hale_ctx* c = m->ctx;
   if (!float_type(dtype)) return ctx_fail(c, HALE_EINVAL, "q4g_matmul: dtype %d is not f32, f16 or bf16", dtype);
   if (ntok > (1u << 20)) return ctx_fail(c, HALE_EINVAL, "q4g_matmul: %zu tokens, at most 2^20", ntok);
+  if (ntok * m->g.rows > ((size_t)1 << 35))
+    return ctx_fail(c, HALE_EINVAL, "q4g_matmul: %zu results of %zu tokens, at most 2^35 in all", m->g.rows, ntok);
   if (ntok == 0) return HALE_OK;
   if (!a.x || !out || (in == Q4G_I8 && !a.x_scales)) return ctx_fail(c, HALE_EINVAL, "q4g_matmul: NULL argument");
   if (a.x_stride < m->g.cols || out_stride < m->g.rows)
@@ -267,7 +269,7 @@ extern "C" int hale_logits_device(hale_ctx* c, int dtype, size_t rows, size_t vo
                                   const hale_logits_rules* rules, void* out, size_t out_stride) {
   if (!c || !rules) return ctx_fail(c, HALE_EINVAL, "logits: NULL argument");
   if (!float_type(dtype)) return ctx_fail(c, HALE_EINVAL, "logits: dtype %d is not f32, f16 or bf16", dtype);
-  if (rows >= (1ull << 31) || vocab > (1u << 26)) return ctx_fail(c, HALE_EINVAL, "logits: %zu rows of %zu", rows, vocab);
+  if (rows >= STEP_ROWS || vocab > (1u << 26)) return ctx_fail(c, HALE_EINVAL, "logits: %zu rows of %zu", rows, vocab);
   if (rules->ntokens >= (1ull << 31) || rules->nbiases >= (1ull << 31))
     return ctx_fail(c, HALE_EINVAL, "logits: %zu tokens and %zu biases", rules->ntokens, rules->nbiases);
   if (rows == 0 || vocab == 0) return HALE_OK;

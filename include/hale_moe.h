@@ -572,8 +572,8 @@ int hale_rope_device(hale_rope *rope, int dtype, size_t rows,
  * row with a number that is not finite (or of zeros with eps 0) has scales NaN, codes 0
  * and y NaN; a block whose weights are not finite has scale NaN and codes 0.
  * d_sum and d_y may each be d_x or d_delta with that one's stride (not both the same);
- * otherwise no output may overlap an input or another output.  eps: not negative.
- * Enqueued on the context's stream. */
+ * otherwise no output may overlap an input or another output.  eps: not negative;
+ * rows below 2^22.  Enqueued on the context's stream. */
 int hale_rms_norm_q8_device(hale_ctx *ctx, int dtype, size_t rows, size_t n,
                             const void *d_x, size_t x_stride,
                             const void *d_delta, size_t delta_stride,
@@ -591,8 +591,8 @@ typedef struct hale_q4g hale_q4g;
 /* A matrix of rows x cols weights scale * (code - zero): codes [rows][cols / 2], two to
  * a byte, the first in the low half; scales [rows][cols / group] of scale_dtype
  * (HALE_F16 or HALE_BF16); zeros [rows][cols / group], a byte of 0..15 each, or NULL
- * where all are 8.  group: 32, 64 or 128; cols a multiple of it.  The bytes are laid
- * out anew in device memory; both forms return when they have been read. */
+ * where all are 8.  group: 32, 64 or 128; cols a multiple of it, at most 2^30; rows at
+ * most 2^27.  The bytes are laid out anew in device memory; both forms return when they have been read. */
 int hale_q4g_upload(hale_ctx *ctx, size_t rows, size_t cols, size_t group,
                     int scale_dtype, const uint8_t *codes, const void *scales,
                     const uint8_t *zeros, hale_q4g **out);
@@ -615,7 +615,9 @@ int hale_q4g_download(hale_q4g *m, uint8_t *codes, void *scales, uint8_t *zeros)
  * f32, and the groups' sums in f32; results are rounded once.  Equal calls give equal
  * bits; a token's results do not depend on what the others hold (on how many they are,
  * in their last bits).  A token with a number that is not finite gives results that are
- * not finite (NaN where the formula has an infinity).  d_out may not overlap d_x.
+ * not finite (NaN where the formula has an infinity), and so may one with a number
+ * above 2^115, whose sums of 128 products with 31 leave f32.  ntok at most 2^20, results
+ * at most 2^35.  d_out may not overlap d_x.
  * Enqueued on the context's stream. */
 int hale_q4g_matmul_device(hale_q4g *m, int dtype, size_t ntok, const void *d_x,
                            size_t x_stride, void *d_out, size_t out_stride);
@@ -659,8 +661,8 @@ typedef struct {
  * repetition, or x * repetition where x is not positive; one that occurs g > 0
  * times among the generated ones loses frequency * g, then presence; a bias is added;
  * and a token whose mask bit is 0 becomes -inf.  Tokens outside the vocabulary are passed
- * over.  A logit that no rule names keeps its bits.  vocab at most 2^26, ntokens and
- * nbiases below 2^31.  d_out may be d_logits with the same stride, and may not overlap
+ * over.  A logit that no rule names keeps its bits.  rows below 2^22, vocab at most
+ * 2^26, ntokens and nbiases below 2^31.  d_out may be d_logits with the same stride, and may not overlap
  * anything else.  Enqueued on the context's stream. */
 int hale_logits_device(hale_ctx *ctx, int dtype, size_t rows, size_t vocab,
                        const void *d_logits, size_t stride,

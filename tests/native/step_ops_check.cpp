@@ -111,7 +111,7 @@ void norm_arguments() {
   a = Call(), a.scales = nullptr, refused(a);
   a = Call(), a.x = mem + 2, refused(a);
   a = Call(), a.scales = (float*)(mem + 1), refused(a);
-  a = Call(), a.rows = (size_t)1 << 31, refused(a);
+  for (int bits : {22, 31, 32}) a = Call(), a.rows = (size_t)1 << bits, refused(a);
   for (float eps : {-1.0f, __builtin_nanf(""), __builtin_inff()}) a = Call(), a.eps = eps, refused(a);
   a = Call(), a.rows = 0, a.x = nullptr;
   CHECK(run(a) == HALE_OK && norms == before);
@@ -148,6 +148,7 @@ void matrices() {
   CHECK(q(0, mem, mem, 33) == HALE_EINVAL && q(64, mem, mem, 33) == HALE_EINVAL && q(48, mem, mem, 33) == HALE_EINVAL);
   CHECK(q(32, mem + 4, mem, 33) == HALE_EINVAL && q(32, mem, nullptr, 33) == HALE_EINVAL && q(32, mem, mem + 2, 33) == HALE_EINVAL);
   CHECK(f(HALE_F32, 0, nullptr, 96, nullptr, 33) == HALE_OK && products == before);
+  CHECK(f(HALE_F32, 1 << 20, mem, 96, mem, 33) == HALE_OK && products == before + 1);
   fake.capturing = true;  // what allocates is refused inside a capture, what computes is recorded
   hale_q4g* other = nullptr;
   CHECK(hale_q4g_upload(&c, 33, 96, 32, HALE_F16, codes.data(), scales.data(), nullptr, &other) == HALE_EINVAL && !other);
@@ -158,7 +159,7 @@ void matrices() {
   CHECK(fake.device.empty());
   // refusals and failures leave nothing behind
   CHECK(up(0) == HALE_EINVAL && up(33, 0) == HALE_EINVAL && up(33, 80) == HALE_EINVAL && up(33, 96, 48) == HALE_EINVAL && up(33, 96, 64) == HALE_EINVAL);
-  CHECK(up(33, 96, 32, HALE_F32) == HALE_EINVAL && up(((size_t)1 << 30) + 1) == HALE_EINVAL && !m);
+  CHECK(up(33, 96, 32, HALE_F32) == HALE_EINVAL && up(((size_t)1 << 27) + 1) == HALE_EINVAL && !m);
   zeros[98] = 16;
   CHECK(up() == HALE_EINVAL && !m);
   zeros[98] = 0;

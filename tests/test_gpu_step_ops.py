@@ -251,6 +251,12 @@ Q4 = [
 ]
 
 
+Q4 += [  # many rows: tokens that fill LDS, and f32 ones that do so twice and three times over
+    ("bf16", "f16", 16, 24580, 2112, 64, True, 0, 0, 0), ("f32", "bf16", 16, 16390, 1696, 32, True, 1, 1, 2),
+    ("f32", "f16", 13, 16385, 4224, 128, False, 0, 0, 3), ("f16", "f16", 2, 24577, 160, 32, True, 0, 0, 0),
+]
+
+
 @pytest.mark.parametrize("dtype,scale_dtype,ntok,rows,cols,group,zeros,xpad,xoff,opad", Q4)
 def test_q4_products(ctx, bufs, dtype, scale_dtype, ntok, rows, cols, group, zeros, xpad, xoff, opad):
     rng = np.random.default_rng(rows + cols + ntok)
@@ -284,6 +290,7 @@ def test_q4_weights_from_device_memory(ctx, bufs):
     (5, 100, 544, 32, 544, True, "f16"), (16, 100, 1024, 128, 128, False, "bf16"), (17, 65, 1152, 64, 128, True, "f32"),
     (40, 130, 640, 128, 64, True, "f32"), (100, 257, 512, 64, 32, True, "f16"), (1, 5000, 2048, 128, 32, True, "f32"),
     (130, 300, 896, 128, 896, False, "f32"), (64, 128, 256, 32, 128, True, "bf16"),
+    (16, 24600, 1056, 32, 32, True, "f16"), (7, 24577, 640, 128, 640, False, "f32"),
 ])
 def test_q4_products_of_8_bit_tokens(ctx, bufs, ntok, rows, cols, group, block, zeros, dtype):
     """Whole numbers up to 128 * 127 * 31 < 2^24 within a unit of 32 to 128 numbers; per unit the
