@@ -497,10 +497,15 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
     std::vector<Tile> few, many;
     // each sequence's shared pages, from the whole down, and the tiles of the rest
     std::vector<std::vector<const Shared*>> over(with.size());
+    size_t work = 0;  // pages, for each 16 rows
     for (Shared& d : shared) {
       const KvStepSeq &a = *with[d.first], &b = *with[d.last - 1];
       d.rows = (uint32_t)((b.tok0 + b.ntok - a.tok0) * group);
-      d.few = d.rows <= 16 * (size_t)out->cols;
+      work += ceil_div(d.rows, 16) * (d.page1 - d.page0) * s.kv_heads;
+    }
+    for (Shared& d : shared) {
+      const KvStepSeq& a = *with[d.first];
+      d.few = work <= (f32 ? KV_SHARE_FEW_F32 : KV_SHARE_FEW) || d.rows <= 64;
       const size_t rows = d.few ? 16 * (size_t)out->cols : many_rows;
       for (uint32_t h = 0; h < s.kv_heads; h++)
         for (size_t r = 0; r < d.rows; r += rows)
@@ -521,23 +526,31 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
           (is_few ? few_seq : many_seq).push_back(i);
         }
     }
-    const size_t each[2] = {std::max<size_t>(4, ceil_div(count_pages(few), KV_FEW_GROUPS)), many.empty() ? 1 : many_each(many)};
+    // of few rows: as many pages for each of a work-group's four waves, and about a work-group per
+    // compute unit, for a part costs more here, where joins have several series (32 bf16
+    // sequences of up to 600 behind 8000, 32 heads of 128 on 8, 24.0 us with 256 work-groups, 27.7
+    // with 512; 4 behind 16000, 4 heads, 16.6 and 23.9)
+    const size_t each[2] = {4 * std::max<size_t>(1, ceil_div(count_pages(few), 4 * KV_SHARE_GROUPS)), many.empty() ? 1 : many_each(many)};
     size_t rows = 0, longest = 0;
     for (Shared& d : shared) {
       d.parts = (uint32_t)ceil_div(d.page1 - d.page0, each[!d.few]);
       d.part = (uint32_t)rows;
       rows += (size_t)d.rows * d.parts * s.kv_heads;
-      for (uint32_t h = 0; h < s.kv_heads; h++)
-        for (uint32_t p = 0; p < d.parts; p++) {
-          const size_t n = d.page1 - d.page0, tile = d.few ? 16 * (size_t)out->cols : many_rows;
-          const KvStepSeq& a = *with[d.first];
-          // positions behind the shared ones: every row sees all of these
-          for (size_t r = 0; r < d.rows; r += tile)
+      // A piece's tiles of rows on one die, whose cache then holds its pages: work-groups go to the
+      // eight dies in turn (behind 8000 as above 27.7 us, 34.0 in the pieces' order; behind
+      // 32000 52 and 86).
+      const size_t n = d.page1 - d.page0, tile = d.few ? 16 * (size_t)out->cols : many_rows, pieces = (size_t)s.kv_heads * d.parts;
+      const KvStepSeq& a = *with[d.first];
+      for (size_t from = 0; from < pieces; from += 8)
+        for (size_t r = 0; r < d.rows; r += tile)
+          for (size_t k = from; k < std::min(from + 8, pieces); k++) {
+            const size_t p = k % d.parts;
+            // positions behind the shared ones: every row sees all of these
             (d.few ? out->few : out->many)
-                .push_back({a.row, d.page1 * (uint32_t)KV_PAGE, a.tok0, (uint16_t)h, (uint16_t)std::min(tile, d.rows - r), (uint32_t)r,
-                            (uint32_t)(d.page0 + n * p / d.parts), (uint32_t)(d.page0 + n * (p + 1) / d.parts),
-                            (uint32_t)(d.part + ((size_t)h * d.parts + p) * d.rows + r)});
-        }
+                .push_back({a.row, d.page1 * (uint32_t)KV_PAGE, a.tok0, (uint16_t)(k / d.parts), (uint16_t)std::min(tile, d.rows - r),
+                            (uint32_t)r, (uint32_t)(d.page0 + n * p / d.parts), (uint32_t)(d.page0 + n * (p + 1) / d.parts),
+                            (uint32_t)(d.part + k * d.rows + r)});
+          }
       if (rows > kv_part_rows(s.head_dim)) break;
     }
     for (int kind = 0; kind < 2 && rows <= kv_part_rows(s.head_dim); kind++) {

@@ -132,6 +132,14 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
 // shares what takes up to the square of their number.
 constexpr size_t KV_SHARE_SEQS = 1024;
 constexpr size_t KV_SHARE_PARTS = 1024;  // of a row, over all its series
+// Work-groups of few rows that a step which shares pages is divided into.
+constexpr size_t KV_SHARE_GROUPS = 256;
+// The pages that one launch of the kernel of few rows takes of shared ones, counted for each 16
+// rows.  Above it, runs of more than 64 rows go to the kernel of many, a launch more that
+// converts a page for 128 rows at once (32 sequences, 32 heads of 128 on 8, few and many
+// rows: behind 8000, 8000 pages, bf16 24 and 31 us; behind 32000 bf16 63 and 49, f32 76 and 79;
+// 8 behind 1000 on 4 heads 10.2 and 21.2, f32 11.1 and 27.6).
+constexpr size_t KV_SHARE_FEW = 16384, KV_SHARE_FEW_F32 = 32768;
 
 // Positions that one launch of the reading kernel takes of those first .. first + count - 1: its
 // grid has a work-group of 256 threads per page, and counts threads in 32 bits.

@@ -180,6 +180,23 @@ int main() {
     kv_plan_shared(s, plan, pages, 1, false, &p);
     check_plan(s, pages, plan, p);
   }
+  // few rows' kernel for short shared prompts, many rows' for long ones of many rows
+  for (uint32_t len : {500u, 12000u}) {
+    const KvShape s{64, 8, 128};
+    KvPages pages;
+    pages.init(20000, 110, 13000);
+    uint32_t root, made[100];
+    const std::vector<uint32_t> n(100, 1);
+    CHECK(pages.create(&root, &err) == KvPages::OK && pages.step(1, &root, &len, nullptr, &copies, &err) == KvPages::OK);
+    CHECK(pages.fork(root, 100, made, &err) == KvPages::OK);
+    std::vector<KvStepSeq> plan;
+    CHECK(pages.step(100, made, n.data(), &plan, &copies, &err) == KvPages::OK);
+    KvPlan p;
+    for (bool f32 : {false, true}) {
+      kv_plan_shared(s, plan, pages, 1, f32, &p);
+      CHECK(check_plan(s, pages, plan, p) > 0 && p.many.empty() == (len == 500));
+    }
+  }
   // more sequences than are looked at
   {
     const KvShape s{2, 1, 64};

@@ -84,15 +84,16 @@ def test_prefixes_within_prefixes(rig, dtype):
     r.check_attention(g, 0, dtype, order, [1] * len(order))
 
 
-def test_a_long_prompt_for_many_rows(rig):
-    """Rows over several tiles, pages over many parts."""
-    r = rig(dim=128, heads=16, kv_heads=2, pages=400, seqs=24, max_len=9000)
+@pytest.mark.parametrize("dtype,dim,heads,kv_heads", [("bf16", 128, 16, 2), ("bf16", 128, 32, 4), ("f16", 64, 32, 4), ("f32", 32, 64, 8)])
+def test_a_long_prompt_for_many_rows(rig, dtype, dim, heads, kv_heads):
+    """Rows over several tiles, pages over many parts; from the second on for the kernel of many rows."""
+    r = rig(dim=dim, heads=heads, kv_heads=kv_heads, pages=400, seqs=24, max_len=9000)
     g = np.random.default_rng(5)
     r.kv.share_prefixes(1000)
-    _, seqs = family(r, g, "bf16", 8100, 20, [3 * i for i in range(20)])
+    _, seqs = family(r, g, dtype, 8100, 20, [3 * i for i in range(20)])
     ntok = [1 + (i % 4) * 2 for i in range(20)]
-    r.step(g, "bf16", seqs, ntok)
-    r.check_attention(g, 0, "bf16", seqs, ntok)
+    r.step(g, dtype, seqs, ntok)
+    r.check_attention(g, 0, dtype, seqs, ntok)
 
 
 def test_sequences_that_diverge_truncate_and_move(rig):
