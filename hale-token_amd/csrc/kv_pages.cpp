@@ -472,6 +472,13 @@ void find_shared(const std::vector<const KvStepSeq*>& seqs, const KvPages& pages
 
 }  // namespace
 
+bool kv_share_may_many(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t max_pages, bool f32) {
+  // at any page the runs that share it have two sequences or more each, and a tile of their own begun
+  size_t rows = 0, n = 0;
+  for (const KvStepSeq& q : seqs) rows += q.ntok * s.group(), n += q.ntok > 0;
+  return (rows / 16 + n / 2) * max_pages * s.kv_heads > (f32 ? KV_SHARE_FEW_F32 : KV_SHARE_FEW);
+}
+
 void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const KvPages& pages, size_t min_pages, bool f32,
                     KvPlan* out) {
   const size_t group = s.group(), few_rows = kv_few_rows(s.head_dim), many_rows = kv_many_rows(s.head_dim);

@@ -140,6 +140,9 @@ constexpr size_t KV_SHARE_GROUPS = 256;
 // rows: behind 8000, 8000 pages, bf16 24 and 31 us; behind 32000 bf16 63 and 49, f32 76 and 79;
 // 8 behind 1000 on 4 heads 10.2 and 21.2, f32 11.1 and 27.6).
 constexpr size_t KV_SHARE_FEW = 16384, KV_SHARE_FEW_F32 = 32768;
+// Whether shared pages may go to the kernel of many rows, whatever the sequences of this step's
+// numbers of tokens come to share later: a captured launch of it that finds nothing costs 4 us.
+bool kv_share_may_many(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t max_pages, bool f32);
 
 // Positions that one launch of the reading kernel takes of those first .. first + count - 1: its
 // grid has a work-group of 256 threads per page, and counts threads in 32 bits.

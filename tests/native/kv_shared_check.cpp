@@ -151,6 +151,9 @@ int main() {
       const bool f32 = below(2);
       kv_plan_shared(s, plan, pages, 1 + below(6), f32, &shared);
       const size_t a = check_plan(s, pages, plan, shared);
+      // what a captured launch may leave out
+      const bool own = std::any_of(plan.begin(), plan.end(), [&](const KvStepSeq& q) { return q.ntok * s.group() > kv_few_limit(s, plan, f32); });
+      CHECK(shared.many.empty() || own || kv_share_may_many(s, plan, pages.max_pages(), f32));
       kv_plan_shared(s, plan, pages, 1u << 20, f32, &apart);
       const size_t b = check_plan(s, pages, plan, apart);
       fewer += a < b;
@@ -195,6 +198,7 @@ int main() {
     for (bool f32 : {false, true}) {
       kv_plan_shared(s, plan, pages, 1, f32, &p);
       CHECK(check_plan(s, pages, plan, p) > 0 && p.many.empty() == (len == 500));
+      CHECK(kv_share_may_many(s, plan, pages.max_pages(), f32) && !kv_share_may_many(s, plan, 20, f32));
     }
   }
   // more sequences than are looked at
