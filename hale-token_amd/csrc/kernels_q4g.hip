@@ -381,7 +381,7 @@ template <int IN> struct Q4gRow {
   Frag f[SIZE];
 };
 
-// Up to 16 tokens.  A work-group of W waves computes a tile of 16 rows; its waves take CH
+// A work-group of W waves computes a tile of 16 rows for 16 tokens (blockIdx.z); its waves take CH
 // chunks of 128 numbers at a time, all of them on their way before the first is used,
 // and join their sums in LDS, in the waves' order.  A token's numbers of a chunk are read by 16
 // neighbouring lanes and change lanes through LDS (16 tokens of 4096, 8-bit: 11.0 us where each
@@ -397,10 +397,12 @@ __global__ __launch_bounds__(64 * W) void k_q4g_few(Q4gArgs a, unsigned per_spli
   extern __shared__ char lds[];  // [W][CH][ntok] rows; then [W][64] sums
   f32x4(*red)[64] = (f32x4(*)[64])lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned i = lane & 15, g = lane >> 4, tile = blockIdx.x, ntok = (unsigned)a.ntok;
+  const unsigned i = lane & 15, g = lane >> 4, tile = blockIdx.x, tok0 = 16 * blockIdx.z;
+  const unsigned ntok = min((unsigned)a.ntok - tok0, 16u);
   const unsigned c0 = blockIdx.y * per_split, c1 = min(c0 + per_split, a.g.chunks);
   const unsigned t = min(i, ntok - 1);  // tokens that are missing are the last one
-  const float* xscale = IN == Q4G_I8 ? a.x_scales + t * a.x_per : nullptr;
+  const char* x0 = (const char*)a.x + tok0 * a.x_stride * Ty::SIZE;
+  const float* xscale = IN == Q4G_I8 ? a.x_scales + (size_t)(tok0 + t) * a.x_per : nullptr;
   const Q4gTile<PER> weights(a.g, tile, lane);
   Q4gRow<IN>* rows = (Q4gRow<IN>*)lds + wave * CH * ntok;
 
@@ -419,7 +421,7 @@ __global__ __launch_bounds__(64 * W) void k_q4g_few(Q4gArgs a, unsigned per_spli
 #pragma unroll
       for (int n = 0; n < 4; n++) {  // four tokens at a time
         if (4 * n >= (int)ntok) break;
-        load_x<IN>(a, (const char*)a.x + min(4 * n + g, ntok - 1) * a.x_stride * Ty::SIZE, c, i / 4, i % 4, in[k][n]);
+        load_x<IN>(a, x0 + min(4 * n + g, ntok - 1) * a.x_stride * Ty::SIZE, c, i / 4, i % 4, in[k][n]);
       }
       if constexpr (IN == Q4G_I8) load_x_scales<M>(a, xscale, c, xs[k]);
     }
@@ -466,17 +468,18 @@ __global__ __launch_bounds__(64 * W) void k_q4g_few(Q4gArgs a, unsigned per_spli
   for (int o = 1; o < W; o++) v = v + red[o][lane];
   if (gridDim.y > 1) {
     const size_t step = (size_t)gridDim.x * 256;
-    float* part = a.g.parts + ((size_t)tile * 64 + lane) * 4;
+    float* part = a.g.parts + blockIdx.z * gridDim.y * step + ((size_t)tile * 64 + lane) * 4;
+    unsigned* done = a.g.done + blockIdx.z * gridDim.x + tile;
     put_part(part + blockIdx.y * step, v);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the sums are where the others look before they are counted
     unsigned before = 0;
-    if (lane == 0) before = atomicAdd(&a.g.done[tile], 1u);
+    if (lane == 0) before = atomicAdd(done, 1u);
     if (__builtin_amdgcn_readfirstlane(before) != gridDim.y - 1) return;
     v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     for (unsigned o = 0; o < gridDim.y; o++) v = v + get_part(part + o * step);
-    if (lane == 0) a.g.done[tile] = 0;
+    if (lane == 0) *done = 0;
   }
-  if (i < a.ntok) store_rows<IN>(a, i, tile * Q4G_ROWS + 4 * g, v);
+  if (i < ntok) store_rows<IN>(a, tok0 + i, tile * Q4G_ROWS + 4 * g, v);
 }
 
 // The tokens in LDS: [chunk][token] operands [j][part][g] and then a gap that puts 16 tokens'
@@ -753,17 +756,20 @@ static hipError_t ask_lds(const void* kernel, uint32_t bytes) {
 template <int IN, int PER, int M, bool BF, int CH, int W>
 static hipError_t q4g_few(const Q4gArgs& a, hipStream_t st) {
   const unsigned tiles = (unsigned)((a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS);
-  // as many work-groups as there are compute units, each with a chunk a wave at least
-  unsigned splits = 256 / tiles, most = (a.g.chunks + W - 1) / W;
-  splits = splits < 1 ? 1 : splits;
+  // As many work-groups as there are compute units, and twice all waves' chunks at least for each
+  // of them: the join takes 1 us and 0.2 a split, as long as the chunks of two turns (1024 rows, a
+  // token of bf16: of 4096 numbers 4.3 us whole, 6.0 in four; of 14336 8.4 whole, 6.9 in three).
+  const unsigned slices = (unsigned)((a.ntok + 15) / 16);
+  unsigned splits = 256 / (tiles * slices), most = a.g.chunks / (2 * W * CH);
   splits = splits > most ? most : splits;
-  splits = splits > Q4G_SPLITS ? Q4G_SPLITS : splits;
+  splits = splits > Q4G_SPLITS / slices ? Q4G_SPLITS / slices : splits;
+  splits = splits < 1 ? 1 : splits;
   const unsigned per = (a.g.chunks + splits - 1) / splits;
   splits = (a.g.chunks + per - 1) / per;
-  const uint32_t rows = W * CH * (uint32_t)a.ntok * sizeof(Q4gRow<IN>), lds = rows > W * 1024 ? rows : W * 1024;
+  const uint32_t rows = W * CH * (uint32_t)(a.ntok < 16 ? a.ntok : 16) * sizeof(Q4gRow<IN>), lds = rows > W * 1024 ? rows : W * 1024;
   const hipError_t e = ask_lds((const void*)k_q4g_few<IN, PER, M, BF, CH, W>, lds);
   if (e != hipSuccess) return e;
-  return launch(k_q4g_few<IN, PER, M, BF, CH, W>, dim3(tiles, splits), 64 * W, lds, st, a, per);
+  return launch(k_q4g_few<IN, PER, M, BF, CH, W>, dim3(tiles, splits, slices), 64 * W, lds, st, a, per);
 }
 
 template <int IN, int PER, int M, bool BF, int AHEAD>
@@ -793,37 +799,49 @@ static hipError_t q4g_many(const Q4gArgs& a, hipStream_t st) {
   return launch(k_q4g_many<IN, PER, M, BF, RT, WK>, grid, 256 * WK, lds, st, a, token_tiles);
 }
 
+// Which kernel: rates of each, on 4-bit rows of 4096, a token and 16, 32 and 128 of bf16 (f32), us:
+//   rows     streaming                    few                          many
+//   4096                                  4.3, 5.3, 7.1, 19 (5.6, 9.5, 16, 59)    28 to 29 (75)
+//   14336    14.3 (18)                    10.7, 12, 22, 83 (20, 32, 57, 228)      29 to 30 (75)
+//   24576    14.7 (19.7)                  15.8 (31.5)
+//   151936   60, 68 (81, 252 in slices)   87, 116 (185, 306)
+// The streaming kernel gives each wave a tile or nearly so, and its tokens have to fit into LDS
+// (Q4G_LDS), f32 ones in three slices at most, each with all weights: still faster than the other of
+// few, whose time grows with the tokens.  Beyond 16 tokens the others work in slices of 16
+// (the streaming kernel in as many launches), while that of many takes as long for 64 tokens as
+// for one, and rounds of 256 work-groups: chunk by chunk a round of it is as long as some 2304 tiles
+// of few, and 3840 (f32 7680) of the streaming kernel.  With four groups or blocks to a chunk it is
+// slower, the others hardly: 3840 and 4608 (32768 rows of 2048, groups of 32, 32 tokens of f16:
+// streaming 26.4, many 33.4; 8-bit 29.8 and 44.8).
 template <int IN, int PER, int M, bool BF>
 static hipError_t q4g_sized(const Q4gArgs& a, hipStream_t st) {
   constexpr int UNITS = PER > M ? PER : M;
-  if (a.ntok <= 16) {
-    // Each wave of the streaming kernel needs a tile or nearly so: rows of 4096, a token of bf16
-    // (f32), the streaming kernel and the other: 16384 rows 14.3 and 11.1 us (19.1 and 21.6), 24576
-    // 14.7 and 15.8 (19.7 and 31.5), 151936 60 and 87 (82 and 185).  And its tokens have to fit
-    // into LDS: 16 tokens of bf16 and 151936 rows 68 us, 116 without it.  f32 takes three
-    // times the room and the other kernel three times the time for 16 tokens, so that slices
-    // of the tokens, each with all weights, are still faster.
-    constexpr uint32_t BYTES = Q4gTokens<IN, UNITS>::BYTES;
-    const unsigned tiles = (unsigned)((a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS), ntok = (unsigned)a.ntok;
-    const unsigned fit = a.g.chunks <= Q4G_LDS / BYTES ? Q4G_LDS / (a.g.chunks * BYTES) : 0, most = IN == Q4G_F32 ? 3 : 1;
-    if (tiles >= (IN == Q4G_F32 ? 1024u : 1536u) && fit * most >= ntok) {
-      const unsigned slices = (ntok + fit - 1) / fit;
-      for (unsigned k = 0, from = 0; k < slices; k++) {
+  constexpr bool WIDE = IN == Q4G_F32;
+  constexpr uint32_t BYTES = Q4gTokens<IN, UNITS>::BYTES;
+  const size_t tiles = (a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS, rounds = ((tiles + 7) / 8 * ((a.ntok + 63) / 64) + 255) / 256;
+  size_t fit = a.g.chunks <= Q4G_LDS / BYTES ? Q4G_LDS / (a.g.chunks * BYTES) : 0;
+  fit = fit > 16 ? 16 : fit;
+  if (tiles >= (WIDE ? 1024 : 1536) && fit) {
+    const size_t slices = (a.ntok + fit - 1) / fit;
+    if (a.ntok <= 16 ? slices <= (WIDE ? 3 : 1) : slices * tiles <= (WIDE ? 7680 : UNITS == 4 ? 4608 : 3840) * rounds) {
+      for (size_t k = 0, from = 0; k < slices; k++) {
         Q4gArgs slice = a;
-        slice.ntok = (ntok - from) / (slices - k);
+        slice.ntok = (a.ntok - from) / (slices - k);
         slice.x = (const char*)a.x + from * a.x_stride * Q4gType<IN>::SIZE;
-        slice.out = (char*)a.out + from * a.out_stride * (IN == Q4G_F32 ? 4 : 2);
+        if (IN == Q4G_I8) slice.x_scales = a.x_scales + from * a.x_per;
+        slice.out = (char*)a.out + from * a.out_stride * (a.out_dtype == F32 ? 4 : 2);
         // chunks on their way: as many as registers hold
-        constexpr int AHEAD = PER == 4 ? (IN == Q4G_F32 ? 2 : 3) : UNITS == 4 || IN == Q4G_F32 ? 4 : 6;
-        const hipError_t e = q4g_stream<IN, PER, M, BF, AHEAD>(slices == 1 ? a : slice, a.g.chunks * BYTES * (unsigned)slice.ntok, st);
+        constexpr int AHEAD = PER == 4 ? (WIDE ? 2 : 3) : UNITS == 4 || WIDE ? 4 : 6;
+        const hipError_t e = q4g_stream<IN, PER, M, BF, AHEAD>(slice, a.g.chunks * BYTES * (unsigned)slice.ntok, st);
         if (e != hipSuccess) return e;
-        from += (unsigned)slice.ntok;
+        from += slice.ntok;
       }
       return hipSuccess;
     }
-    return q4g_few<IN, PER, M, BF, IN == Q4G_F32 ? 1 : 2, 8>(a, st);
   }
-  return q4g_many<IN, PER, M, BF, 2, IN == Q4G_F32 || PER == 4 ? 1 : 2>(a, st);
+  if (a.ntok <= 16 || tiles * ((a.ntok + 15) / 16) <= (UNITS == 4 && !WIDE ? 3840 : 2304) * rounds)
+    return q4g_few<IN, PER, M, BF, WIDE ? 1 : 2, 8>(a, st);
+  return q4g_many<IN, PER, M, BF, 2, WIDE || PER == 4 ? 1 : 2>(a, st);
 }
 
 template <int IN, int PER, bool BF>

@@ -27,6 +27,9 @@ class Bufs:
             b.upload(arr, offset)
         return b.address + offset
 
+    def set(self, address, arr):
+        next(b for b in self.all if b.address == address).upload(arr)
+
     def get(self, address, dtype, count):
         b = next(b for b in self.all if b.address <= address < b.address + max(b.nbytes, 1))
         return b.download(dtype, count, address - b.address)
@@ -254,6 +257,14 @@ Q4 = [
 Q4 += [  # many rows: tokens that fill LDS, and f32 ones that do so twice and three times over
     ("bf16", "f16", 16, 24580, 2112, 64, True, 0, 0, 0), ("f32", "bf16", 16, 16390, 1696, 32, True, 1, 1, 2),
     ("f32", "f16", 13, 16385, 4224, 128, False, 0, 0, 3), ("f16", "f16", 2, 24577, 160, 32, True, 0, 0, 0),
+    ("bf16", "f16", 27, 32780, 320, 32, True, 0, 0, 1), ("f32", "f16", 40, 24590, 256, 64, True, 0, 0, 0),
+    # many tokens
+    ("f16", "f16", 1130, 520, 384, 64, True, 2, 0, 1), ("bf16", "bf16", 965, 1040, 352, 32, False, 0, 0, 0),
+    ("f32", "f16", 1141, 520, 416, 32, True, 1, 1, 0), ("bf16", "f16", 1121, 517, 896, 128, True, 1, 1, 1),
+    ("f32", "bf16", 1122, 517, 640, 128, False, 0, 0, 0),
+    # few rows of many numbers
+    ("bf16", "f16", 3, 40, 14336, 64, True, 0, 0, 0), ("f32", "f16", 5, 100, 8192, 32, True, 0, 0, 1),
+    ("f16", "bf16", 40, 33, 8224, 32, False, 0, 0, 0),
 ]
 
 
@@ -276,6 +287,39 @@ def test_q4_products(ctx, bufs, dtype, scale_dtype, ntok, rows, cols, group, zer
     m.close()
 
 
+@pytest.mark.parametrize("dtype,ntok,rows,cols", [("bf16", 2, 40, 14336), ("f32", 16, 100, 4096), ("f16", 40, 33, 8192), ("f32", 16, 16400, 1792)])
+def test_q4_calls_in_turn(ctx, bufs, dtype, ntok, rows, cols):
+    """Divided rows count their parts in memory of the matrix: eager calls and replays one behind the
+    other, of other tokens each time, give the bits of calls apart."""
+    rng = np.random.default_rng(cols)
+    codes, raw, _, z = q4_weights(rng, rows, cols, 128, True, "f16")
+    m = H.GroupQ4Matrix.new(ctx, rows, cols, 128, codes, raw, z)
+    xs = [encode(rng.normal(size=(ntok, cols)), dtype)[0] for _ in range(3)]
+    dxs, dx = [bufs.put(x) for x in xs], bufs.put(xs[0])
+    outs = [bufs.put(np.zeros((ntok, rows), NP[dtype])) for _ in range(4)]
+    want = []
+    for d, o in zip(dxs, outs):
+        m.matmul_device(dtype, ntok, d, o)
+        want.append(bufs.get(o, NP[dtype], ntok * rows))
+    for _ in range(5):
+        for d, o in zip(dxs, outs):
+            m.matmul_device(dtype, ntok, d, o)
+    assert all((bufs.get(o, NP[dtype], ntok * rows) == w).all() for o, w in zip(outs, want))
+
+    def calls():
+        for o in outs:
+            m.matmul_device(dtype, ntok, dx, o)
+
+    graph = ctx.capture(calls)
+    for x, w in list(zip(xs, want)) * 2:
+        bufs.set(dx, x)
+        graph.launch()
+        assert all((bufs.get(o, NP[dtype], ntok * rows) == w).all() for o in outs)
+        m.matmul_device(dtype, ntok, dxs[1], outs[0])
+    graph.close()
+    m.close()
+
+
 def test_q4_weights_from_device_memory(ctx, bufs):
     rng = np.random.default_rng(8)
     codes, raw, scales, z = q4_weights(rng, 37, 320, 64, True, "f16")
@@ -290,7 +334,9 @@ def test_q4_weights_from_device_memory(ctx, bufs):
     (5, 100, 544, 32, 544, True, "f16"), (16, 100, 1024, 128, 128, False, "bf16"), (17, 65, 1152, 64, 128, True, "f32"),
     (40, 130, 640, 128, 64, True, "f32"), (100, 257, 512, 64, 32, True, "f16"), (1, 5000, 2048, 128, 32, True, "f32"),
     (130, 300, 896, 128, 896, False, "f32"), (64, 128, 256, 32, 128, True, "bf16"),
-    (16, 24600, 1056, 32, 32, True, "f16"), (7, 24577, 640, 128, 640, False, "f32"),
+    (16, 24600, 1056, 32, 32, True, "f16"), (7, 24577, 640, 128, 640, False, "f32"), (23, 32770, 192, 64, 32, True, "bf16"),
+    (965, 1040, 352, 32, 32, True, "f16"), (1130, 520, 640, 128, 64, False, "f32"), (1121, 517, 896, 128, 896, True, "bf16"),
+    (9, 50, 8192, 128, 64, True, "f32"), (60, 20, 9216, 64, 128, True, "f16"),
 ])
 def test_q4_products_of_8_bit_tokens(ctx, bufs, ntok, rows, cols, group, block, zeros, dtype):
     """Whole numbers up to 128 * 127 * 31 < 2^24 within a unit of 32 to 128 numbers; per unit the
