@@ -16,7 +16,7 @@
 
 namespace hale {
 
-constexpr int LG_THREADS = 256, LG_AHEAD = 8;
+constexpr int LG_THREADS = 512, LG_AHEAD = 8;
 constexpr unsigned LG_OCCURS = 0x80000000u;  // in the prompt, beside the count of generated ones
 
 template <typename T> __device__ __forceinline__ T lowest_of();
@@ -26,20 +26,21 @@ template <> __device__ __forceinline__ Bf16 lowest_of<Bf16>() { return {0xff80};
 
 __device__ __forceinline__ int64_t clamped(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 
-// A work-group takes 256 * 8 * C neighbouring tokens of a row: in LDS it counts the row's
+// A work-group takes 512 * 8 * C neighbouring tokens of a row: in LDS it counts the row's
 // tokens that fall among them, and then finds the last bias of each, while the logits are on their
 // way, eight neighbours to a thread.  Counts and the biases' places are whole numbers, so
 // the order of the atomics leaves no trace.  The one table serves both in turn, and tokens
-// are read eight to a thread at a time: 64 rows of 151936 bf16 with up to 4000 tokens and 300 biases each
-// 17.3 us, of which reading and writing the logits alone is 5.8, the mask 0.8, the tokens
-// 5.5 and the biases 3.3 (24 us with a table for each, a token a thread at a time and two atomics for
-// it).  One row of f32 4.9 us, a launch alone 3.5.  Bound by each work-group's passes
-// over the row's lists: sorting them first would take a launch and a workspace
-// of its own.
+// are read eight to a thread at a time: 64 rows of 151936 bf16 with up to 4000 tokens and 300 biases
+// each 17.0 us (15.3 where the logits stay in the caches; 24 with a table for each, a token a thread
+// at a time and two atomics for it; 15.9 with 256 threads).  Of the 15.3 reading and writing the
+// logits alone takes 5.9, the mask 0.9, the tokens 5.4 and the biases 3.  Bound by each
+// work-group's chain of reads (offsets, tokens, table) in little more than one round of them.  One row
+// of f32 4.7 us, a launch alone 3.5.
 template <typename T, int C, bool VEC>
 __global__ __launch_bounds__(LG_THREADS) void k_logits(LogitsArgs a) {
   constexpr unsigned SLICE = LG_THREADS * 8 * C;
   __shared__ unsigned table[SLICE];
+  __shared__ float biases[LG_THREADS];  // the first ones
   const unsigned t = threadIdx.x;
   const size_t row = blockIdx.x, first = (size_t)blockIdx.y * SLICE;
   const unsigned size = (unsigned)(a.vocab - first < SLICE ? a.vocab - first : SLICE);
@@ -81,6 +82,12 @@ __global__ __launch_bounds__(LG_THREADS) void k_logits(LogitsArgs a) {
   if (r.bias_tokens) {
     b0 = clamped(r.bias_start[row], 0, (int64_t)r.nbiases);
     b1 = clamped(r.bias_start[row + 1], b0, (int64_t)r.nbiases);
+  }
+  int32_t bias_token = 0;
+  if (b1 > b0) {  // on their way beside the row's tokens
+    const int64_t k = b0 + t < b1 ? b0 + t : b1 - 1;
+    bias_token = r.bias_tokens[k];
+    biases[t] = r.bias[k];
   }
   float v[C][8];
   if (t1 > t0 || b1 > b0) {
@@ -134,7 +141,7 @@ __global__ __launch_bounds__(LG_THREADS) void k_logits(LogitsArgs a) {
   if (b1 > b0) {
     __syncthreads();
     for (int64_t k = b0 + t; k < b1; k += LG_THREADS) {
-      const size_t at = (size_t)(int64_t)r.bias_tokens[k] - first;
+      const size_t at = (size_t)(int64_t)(k < b0 + LG_THREADS ? bias_token : r.bias_tokens[k]) - first;
       if (at < size) atomicMax(&table[at], (unsigned)(k - b0 + 1));
     }
     __syncthreads();
@@ -146,7 +153,8 @@ __global__ __launch_bounds__(LG_THREADS) void k_logits(LogitsArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         if (!p[j]) continue;
-        v[c][j] = (named[c] >> j & 1 ? v[c][j] : to_f32(x[c][j])) + r.bias[b0 + (int64_t)p[j] - 1];
+        const float bias = p[j] <= LG_THREADS ? biases[p[j] - 1] : r.bias[b0 + (int64_t)p[j] - 1];
+        v[c][j] = (named[c] >> j & 1 ? v[c][j] : to_f32(x[c][j])) + bias;
         named[c] |= 1u << j;
       }
     }
@@ -186,8 +194,8 @@ static hipError_t logits_sized(const LogitsArgs& a, size_t rows, hipStream_t st)
 }
 
 template <typename T> static hipError_t logits_typed(const LogitsArgs& a, size_t rows, hipStream_t st) {
-  // few rows: as many work-groups as there are compute units; many: fewer passes over the rows' tokens
-  // (64 rows of 151936 17.6 us, 18.4 with half the slice; one 6.3, 4.9 with half)
+  // few rows: short work-groups; many: fewer passes over the rows' tokens (64 rows of 151936 15.1 us, 16.6
+  // with half the slice; one 6.1, 4.7 with half)
   const bool large = rows * a.vocab >= (size_t)1 << 22;
   return large ? logits_sized<T, 2>(a, rows, st) : logits_sized<T, 1>(a, rows, st);
 }
