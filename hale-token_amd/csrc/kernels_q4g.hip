@@ -604,9 +604,14 @@ template <int IN, int UNITS> struct Q4gStage {
 // A work-group computes 4 RT tiles of 16 rows for 64 tokens; its waves divide the rows, and
 // (WK) the chunks of 128 numbers.  For each chunk the tokens' numbers go through LDS (wave k of
 // four brings tokens 16 k .., each by 16 neighbouring lanes, and their sums); they are read
-// from memory two chunks ahead, and so are the weights, to registers.
+// from memory two chunks ahead, and the weights one, to registers: so two waves share a SIMD (with
+// weights two ahead, one of them where groups are of 32: 512 tokens, 4096 x 4096, 69 us, 47 now).
+// 512 tokens of f16, 4096 x 4096, groups of 128, take 29 us, 592 TFLOP/s; 2048 100, 688.  Bound by the
+// vector units: for 512 cycles of products of a chunk and wave they work for 830, laying codes
+// out and scaling the groups' sums, and half of that is hidden.  128 tokens for each reading
+// of the weights leave room for one wave (120 us for 2048).
 template <int IN, int PER, int M, bool BF, int RT, int WK>
-__global__ __launch_bounds__(256 * WK) void k_q4g_many(Q4gArgs a, unsigned token_tiles) {
+__global__ __launch_bounds__(256 * WK, IN == Q4G_F32 ? 1 : 2) void k_q4g_many(Q4gArgs a, unsigned token_tiles) {
   typedef Q4gType<IN> Ty;
   typedef typename Ty::Frag Frag;
   constexpr int UNITS = PER > M ? PER : M, STEPS = 4 / UNITS, WR = 4, NT = 4, P = Ty::PARTS;
@@ -633,12 +638,15 @@ __global__ __launch_bounds__(256 * WK) void k_q4g_many(Q4gArgs a, unsigned token
     Frag x[4][P];
     float s[M];
   } in[2];
-  Q4gChunk<PER> q[4][RT];
+  Q4gChunk<PER> q[2][RT];
   // turn k of this half is chunk k WK + wk (the last again where there are no more)
-  auto load = [&](unsigned turn, Tokens& x, Q4gChunk<PER> (&to)[RT]) {
+  auto load_weights = [&](unsigned turn, Q4gChunk<PER> (&to)[RT]) {
     const unsigned c = min(turn * WK + wk, a.g.chunks - 1);
 #pragma unroll
     for (int r = 0; r < RT; r++) Q4gTile<PER>(a.g, min(tile0 + r, tiles - 1), lane).load(c, to[r]);
+  };
+  auto load_tokens = [&](unsigned turn, Tokens& x) {
+    const unsigned c = min(turn * WK + wk, a.g.chunks - 1);
 #pragma unroll
     for (int n = 0; n < 4; n++) load_x<IN>(a, row[n], c, i / 4, i % 4, x.x[n]);
     if constexpr (IN == Q4G_I8) load_x_scales<M>(a, xscale, c, x.s);
@@ -701,17 +709,19 @@ __global__ __launch_bounds__(256 * WK) void k_q4g_many(Q4gArgs a, unsigned token
   };
   // the halves make as many turns; a chunk that is missing is not computed
   const unsigned turns = (a.g.chunks + WK - 1) / WK;
-  load(0, in[0], q[0]);
-  load(1, in[1], q[1]);
+  load_weights(0, q[0]);
+  load_tokens(0, in[0]);
+  load_tokens(1, in[1]);
   bring(stage[0], in[0]);
   __syncthreads();
-  for (unsigned from = 0; from < turns; from += 4) {
+  for (unsigned from = 0; from < turns; from += 2) {
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
+    for (int k = 0; k < 2; k++) {
       if (from + k >= turns) break;
-      load(from + k + 2, in[k % 2], q[(k + 2) % 4]);
+      load_weights(from + k + 1, q[(k + 1) % 2]);
+      load_tokens(from + k + 2, in[k]);
       __builtin_amdgcn_sched_barrier(0);  // on their way first
-      if ((from + k) * WK + wk < a.g.chunks) compute(stage[k % 2], q[k]);
+      if ((from + k) * WK + wk < a.g.chunks) compute(stage[k], q[k]);
       bring(stage[(k + 1) % 2], in[(k + 1) % 2]);
       __syncthreads();
     }
@@ -844,7 +854,12 @@ static hipError_t q4g_sized(const Q4gArgs& a, hipStream_t st) {
   }
   if (a.ntok <= 16 || tiles * ((a.ntok + 15) / 16) <= (UNITS == 4 && !WIDE ? 3840 : 2304) * rounds)
     return q4g_few<IN, PER, M, BF, WIDE ? 1 : 2, 8>(a, st);
-  return q4g_many<IN, PER, M, BF, 2, WIDE || PER == 4 ? 1 : 2>(a, st);
+  // The chunks divided over two halves of a work-group where there would be few of them, f16, groups of
+  // 128 (64): 512 tokens, 4096 x 4096, 29.0 us (35.4), undivided 32.8 (44.2); 2048 113 (141) and 100 (119).
+  if constexpr (!WIDE) {
+    if ((tiles + 7) / 8 * ((a.ntok + 63) / 64) < 512) return q4g_many<IN, PER, M, BF, 2, 2>(a, st);
+  }
+  return q4g_many<IN, PER, M, BF, 2, 1>(a, st);
 }
 
 template <int IN, int PER, bool BF>

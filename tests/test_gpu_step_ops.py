@@ -261,7 +261,7 @@ Q4 += [  # many rows: tokens that fill LDS, and f32 ones that do so twice and th
     # many tokens
     ("f16", "f16", 1130, 520, 384, 64, True, 2, 0, 1), ("bf16", "bf16", 965, 1040, 352, 32, False, 0, 0, 0),
     ("f32", "f16", 1141, 520, 416, 32, True, 1, 1, 0), ("bf16", "f16", 1121, 517, 896, 128, True, 1, 1, 1),
-    ("f32", "bf16", 1122, 517, 640, 128, False, 0, 0, 0),
+    ("f32", "bf16", 1122, 517, 640, 128, False, 0, 0, 0), ("bf16", "bf16", 1901, 2170, 384, 128, True, 0, 0, 0),
     # few rows of many numbers
     ("bf16", "f16", 3, 40, 14336, 64, True, 0, 0, 0), ("f32", "f16", 5, 100, 8192, 32, True, 0, 0, 1),
     ("f16", "bf16", 40, 33, 8224, 32, False, 0, 0, 0),
@@ -336,6 +336,7 @@ def test_q4_weights_from_device_memory(ctx, bufs):
     (130, 300, 896, 128, 896, False, "f32"), (64, 128, 256, 32, 128, True, "bf16"),
     (16, 24600, 1056, 32, 32, True, "f16"), (7, 24577, 640, 128, 640, False, "f32"), (23, 32770, 192, 64, 32, True, "bf16"),
     (965, 1040, 352, 32, 32, True, "f16"), (1130, 520, 640, 128, 64, False, "f32"), (1121, 517, 896, 128, 896, True, "bf16"),
+    (1901, 2170, 384, 64, 128, True, "f32"),
     (9, 50, 8192, 128, 64, True, "f32"), (60, 20, 9216, 64, 128, True, "f16"),
 ])
 def test_q4_products_of_8_bit_tokens(ctx, bufs, ntok, rows, cols, group, block, zeros, dtype):
