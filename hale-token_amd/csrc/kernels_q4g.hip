@@ -823,20 +823,20 @@ static hipError_t q4g_many(const Q4gArgs& a, hipStream_t st) {
 // few, whose time grows with the tokens.  Beyond 16 tokens the others work in slices of 16
 // (the streaming kernel in as many launches), while that of many takes as long for 64 tokens as
 // for one, and rounds of 256 work-groups: chunk by chunk a round of it is as long as some 2304 tiles
-// of few, and 3840 (f32 7680) of the streaming kernel.  With four groups or blocks to a chunk it is
-// slower, the others hardly: 3840 and 4608 (32768 rows of 2048, groups of 32, 32 tokens of f16:
-// streaming 26.4, many 33.4; 8-bit 29.8 and 44.8).
+// of few, and 3840 (f32 7680) of the streaming kernel.  Of 8-bit tokens with four groups or blocks to a
+// chunk it is slower, the others hardly: 3840 and 4608 (groups of 32: 32768 rows of 2048, 32 tokens,
+// streaming 29.8, many 35.1; 14336 rows of 4096, 64 tokens, few 57.8, many 64.7).
 template <int IN, int PER, int M, bool BF>
 static hipError_t q4g_sized(const Q4gArgs& a, hipStream_t st) {
   constexpr int UNITS = PER > M ? PER : M;
-  constexpr bool WIDE = IN == Q4G_F32;
+  constexpr bool WIDE = IN == Q4G_F32, FOUR8 = IN == Q4G_I8 && UNITS == 4;
   constexpr uint32_t BYTES = Q4gTokens<IN, UNITS>::BYTES;
   const size_t tiles = (a.g.rows + Q4G_ROWS - 1) / Q4G_ROWS, rounds = ((tiles + 7) / 8 * ((a.ntok + 63) / 64) + 255) / 256;
   size_t fit = a.g.chunks <= Q4G_LDS / BYTES ? Q4G_LDS / (a.g.chunks * BYTES) : 0;
   fit = fit > 16 ? 16 : fit;
   if (tiles >= (WIDE ? 1024 : 1536) && fit) {
     const size_t slices = (a.ntok + fit - 1) / fit;
-    if (a.ntok <= 16 ? slices <= (WIDE ? 3 : 1) : slices * tiles <= (WIDE ? 7680 : UNITS == 4 ? 4608 : 3840) * rounds) {
+    if (a.ntok <= 16 ? slices <= (WIDE ? 3 : 1) : slices * tiles <= (WIDE ? 7680 : FOUR8 ? 4608 : 3840) * rounds) {
       for (size_t k = 0, from = 0; k < slices; k++) {
         Q4gArgs slice = a;
         slice.ntok = (a.ntok - from) / (slices - k);
@@ -852,7 +852,7 @@ static hipError_t q4g_sized(const Q4gArgs& a, hipStream_t st) {
       return hipSuccess;
     }
   }
-  if (a.ntok <= 16 || tiles * ((a.ntok + 15) / 16) <= (UNITS == 4 && !WIDE ? 3840 : 2304) * rounds)
+  if (a.ntok <= 16 || tiles * ((a.ntok + 15) / 16) <= (FOUR8 ? 3840 : 2304) * rounds)
     return q4g_few<IN, PER, M, BF, WIDE ? 1 : 2, 8>(a, st);
   // The chunks divided over two halves of a work-group where there would be few of them, f16, groups of
   // 128 (64): 512 tokens, 4096 x 4096, 29.0 us (35.4), undivided 32.8 (44.2); 2048 113 (141) and 100 (119).
