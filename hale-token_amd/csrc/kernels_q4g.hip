@@ -387,8 +387,8 @@ template <int IN> struct Q4gRow {
 // A work-group of W waves computes a tile of 16 rows for 16 tokens (blockIdx.z); its waves take CH
 // chunks of 128 numbers at a time, all of them on their way before the first is used,
 // and join their sums in LDS, in the waves' order.  A token's numbers of a chunk are read by 16
-// neighbouring lanes and change lanes through LDS (16 tokens of 4096, 8-bit: 11.0 us where each
-// lane read its operands itself).  Long rows of few tiles are divided over gridDim.y
+// neighbouring lanes and change lanes through LDS (4096 x 4096, 16 tokens of 8 bits: 7.3 us, 11.0 where each
+// lane read its operands itself; a launch alone 3.5).  Bound by latency: two turns of 4096 numbers.  Long rows of few tiles are divided over gridDim.y
 // work-groups: the last of a tile's to finish adds their sums up in the splits' order.
 // UNITS: units per chunk, within which the scales (PER of the weights, M of 8-bit codes) are the
 // same.
@@ -495,7 +495,10 @@ template <int IN, int UNITS> struct Q4gTokens {
 
 // Up to 16 tokens and many tiles.  The tokens' numbers are laid out in LDS as the operands
 // lie, with their sums; then each wave streams through tiles of its own, one behind the
-// other in memory, AHEAD chunks of weights on their way, and meets no other wave.
+// other in memory, AHEAD chunks of weights on their way, and meets no other wave.  A vocabulary of
+// 151936 x 2048, groups of 64 with zeros, a token of bf16, is 37.6 us: 4.5 TB/s where plain reads reach 6.25.
+// The reads would take 27 us and the vector instructions (77 a chunk) 19; their loads come
+// just in time, and the longest wave has 5 % more tiles than the mean.
 template <int IN, int PER, int M, bool BF, int AHEAD>
 __global__ __launch_bounds__(1024) void k_q4g_stream(Q4gArgs a) {
   typedef Q4gType<IN> Ty;
