@@ -855,7 +855,8 @@ static hipError_t q4g_sized(const Q4gArgs& a, hipStream_t st) {
       return hipSuccess;
     }
   }
-  if (a.ntok <= 16 || tiles * ((a.ntok + 15) / 16) <= (FOUR8 ? 3840 : 2304) * rounds)
+  const size_t slices = (a.ntok + 15) / 16;
+  if (slices == 1 || (slices < 65536 && tiles * slices <= (FOUR8 ? 3840 : 2304) * rounds))  // (a grid's third side)
     return q4g_few<IN, PER, M, BF, WIDE ? 1 : 2, 8>(a, st);
   // The chunks divided over two halves of a work-group where there would be few of them, f16, groups of
   // 128 (64): 512 tokens, 4096 x 4096, 29.0 us (35.4), undivided 32.8 (44.2); 2048 113 (141) and 100 (119).

@@ -262,6 +262,7 @@ Q4 += [  # many rows: tokens that fill LDS, and f32 ones that do so twice and th
     ("f16", "f16", 1130, 520, 384, 64, True, 2, 0, 1), ("bf16", "bf16", 965, 1040, 352, 32, False, 0, 0, 0),
     ("f32", "f16", 1141, 520, 416, 32, True, 1, 1, 0), ("bf16", "f16", 1121, 517, 896, 128, True, 1, 1, 1),
     ("f32", "bf16", 1122, 517, 640, 128, False, 0, 0, 0), ("bf16", "bf16", 1901, 2170, 384, 128, True, 0, 0, 0),
+    ("bf16", "f16", 40001, 9, 64, 32, True, 0, 0, 0), ("f32", "f16", 1 << 20, 3, 32, 32, False, 0, 0, 0),
     # few rows of many numbers
     ("bf16", "f16", 3, 40, 14336, 64, True, 0, 0, 0), ("f32", "f16", 5, 100, 8192, 32, True, 0, 0, 1),
     ("f16", "bf16", 40, 33, 8224, 32, False, 0, 0, 0),
