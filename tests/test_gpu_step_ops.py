@@ -1,6 +1,7 @@
 """Norms that hand on 8 bits, products of 4-bit weights with group scales, and
 rules on logits, on the GPU, against their formulas in 64 bits and more."""
 import ctypes as C
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 import pytest
@@ -648,3 +649,40 @@ def test_captured_norm_product_and_rules(ctx, bufs):
         check(x, d)
     graph.close()
     head.close()
+
+
+def test_two_contexts_at_once(ctx, bufs):
+    """Two contexts on one device, a thread each, the same calls many times over: each has the
+    results of calls apart (divided rows, whose parts are counted in memory of the matrix)."""
+    rng = np.random.default_rng(31)
+    ntok, rows, cols, vocab = 3, 40, 14336, 5000
+    codes, raw, _, z = q4_weights(rng, rows, cols, 128, True, "f16")
+    x = rng.normal(size=(ntok, cols)).astype(np.float32)
+    w = np.ones(2048, np.float32)
+    logits = rng.normal(size=(4, vocab)).astype(np.float32)
+    tokens, start = rng.integers(0, vocab, 4000).astype(np.int32), np.array([0, 500, 500, 3000, 4000], np.int64)
+    repetition = np.full(4, 1.3, np.float32)
+
+    def work(c, times):
+        mine = Bufs(c)
+        m = H.GroupQ4Matrix.new(c, rows, cols, 128, codes, raw, z)
+        dx, dw, dl = mine.put(x), mine.put(w), mine.put(logits)
+        R = H.LogitsRules(tokens=mine.put(tokens), token_start=mine.put(start), ntokens=4000, repetition=mine.put(repetition))
+        o, q, s, lo = (mine.put(np.zeros(n, t)) for n, t in ((ntok * rows, np.float32), (7 * 2048, np.int8), (7, np.float32), (4 * vocab, np.float32)))
+        for _ in range(times):
+            m.matmul_device("f32", ntok, dx, o)
+            H.rms_norm_q8_device(c, "f32", 7, 2048, dx, dw, 1e-6, q, s, block=2048)
+            H.logits_device(c, "f32", 4, vocab, dl, R, lo)
+        got = [mine.get(o, np.float32, ntok * rows), mine.get(q, np.int8, 7 * 2048), mine.get(s, np.float32, 7), mine.get(lo, np.float32, 4 * vocab)]
+        m.close()
+        for b in mine.all:
+            b.free()
+        return got
+
+    want = work(ctx, 1)
+    other = H.Context(0)
+    with ThreadPoolExecutor(2) as pool:
+        both = list(pool.map(work, (ctx, other), (200, 200)))
+    for got in both:
+        assert all((a == b).all() for a, b in zip(got, want))
+    other.close()
