@@ -365,10 +365,11 @@ def test_q4_products_of_8_bit_tokens(ctx, bufs, ntok, rows, cols, group, block, 
     m.close()
 
 
-@pytest.mark.parametrize("dtype,ntok", [("f32", 3), ("bf16", 5), ("f16", 20), ("bf16", 80), ("f32", 70)])
-def test_q4_tokens_that_are_not_finite_stay_apart(ctx, bufs, dtype, ntok):
+@pytest.mark.parametrize("dtype,ntok,rows", [("f32", 3, 50), ("bf16", 5, 50), ("f16", 20, 50), ("bf16", 80, 50), ("f32", 70, 50),
+                                             ("f16", 9300, 50), ("f32", 9300, 50), ("bf16", 4, 24600), ("f32", 12, 16400)])
+def test_q4_tokens_that_are_not_finite_stay_apart(ctx, bufs, dtype, ntok, rows):
     rng = np.random.default_rng(9)
-    rows, cols = 50, 256
+    cols = 256
     codes, raw, _, z = q4_weights(rng, rows, cols, 64, True, "f16")
     m = H.GroupQ4Matrix.new(ctx, rows, cols, 64, codes, raw, z)
     x = rng.normal(size=(ntok, cols)).astype(np.float32)
@@ -519,6 +520,9 @@ LOGITS = [
     ("f32", 2, 10000, 20000, 500, 0, 0, False, 2),
     ("f32", 7, 5001, 0, 0, 0, 3, False, 3),
     ("bf16", 300, 1000, 20, 4, 0, 0, False, 10),
+    # more biases than a work-group has threads; work-groups of longer slices
+    ("f32", 3, 6000, 100, 4000, 0, 0, False, 0), ("f16", 2, 300, 9000, 3000, 0, 0, True, 2),
+    ("bf16", 33, 131080, 6000, 1500, 0, 0, False, 7), ("f32", 40, 106003, 200, 30, 2, 1, True, 0),
 ]
 
 
