@@ -815,18 +815,20 @@ static hipError_t q4g_many(const Q4gArgs& a, hipStream_t st) {
   return launch(k_q4g_many<IN, PER, M, BF, RT, WK>, grid, 256 * WK, lds, st, a, token_tiles);
 }
 
-// Which kernel: rates of each, on 4-bit rows of 4096, a token and 16, 32 and 128 of bf16 (f32), us:
-//   rows     streaming                    few                          many
-//   4096                                  4.3, 5.3, 7.1, 19 (5.6, 9.5, 16, 59)    28 to 29 (75)
-//   14336    14.3 (18)                    10.7, 12, 22, 83 (20, 32, 57, 228)      29 to 30 (75)
-//   24576    14.7 (19.7)                  15.8 (31.5)
-//   151936   60, 68 (81, 252 in slices)   87, 116 (185, 306)
+// Which kernel: 4-bit rows of 4096, bf16 (f32), us:
+//   rows     tokens   streaming      few            many
+//   4096     1, 16                   4.3, 5.2 (5.6, 8.9)
+//            32, 128                 6.9, 19 (14.8, 43)    28, 28 (76, 77)
+//   14336    1, 16    14.3 (18)      9.4, 13 (19, 28)
+//            32                      21 (43)               29 (76)
+//   24576    1        14.7 (19.7)    15.8 (31.5)
+//   151936   1, 16    60, 68 (81, 252 in slices)   87, 116 (185, 306)
 // The streaming kernel gives each wave a tile or nearly so, and its tokens have to fit into LDS
 // (Q4G_LDS), f32 ones in three slices at most, each with all weights: still faster than the other of
 // few, whose time grows with the tokens.  Beyond 16 tokens the others work in slices of 16
 // (the streaming kernel in as many launches), while that of many takes as long for 64 tokens as
 // for one, and rounds of 256 work-groups: chunk by chunk a round of it is as long as some 2304 tiles
-// of few, and 3840 (f32 7680) of the streaming kernel.  Of 8-bit tokens with four groups or blocks to a
+// (f32 3328) of few, and 3840 (f32 7680) of the streaming kernel.  Of 8-bit tokens with four groups or blocks to a
 // chunk it is slower, the others hardly: 3840 and 4608 (groups of 32: 32768 rows of 2048, 32 tokens,
 // streaming 29.8, many 35.1; 14336 rows of 4096, 64 tokens, few 57.8, many 64.7).
 template <int IN, int PER, int M, bool BF>
@@ -856,8 +858,13 @@ static hipError_t q4g_sized(const Q4gArgs& a, hipStream_t st) {
     }
   }
   const size_t slices = (a.ntok + 15) / 16;
-  if (slices == 1 || (slices < 65536 && tiles * slices <= (FOUR8 ? 3840 : 2304) * rounds))  // (a grid's third side)
+  if (slices == 1 || (slices < 65536 && tiles * slices <= (FOUR8 ? 3840 : WIDE ? 3328 : 2304) * rounds)) {  // (a grid's third side)
+    // work-groups of half as many waves, which follow each other more closely, where there are enough of them
+    // (14336 rows of 4096, a token 9.4 and 10.7 us, 8192 7.2 and 6.0; f32, 16 tokens, 27.8 and 33.0, 4096 rows 11.9
+    // and 8.9)
+    if (tiles * slices >= (WIDE ? 384 : 640)) return q4g_few<IN, PER, M, BF, WIDE ? 1 : 2, 4>(a, st);
     return q4g_few<IN, PER, M, BF, WIDE ? 1 : 2, 8>(a, st);
+  }
   // The chunks divided over two halves of a work-group where there would be few of them, f16, groups of
   // 128 (64): 512 tokens, 4096 x 4096, 29.0 us (35.4), undivided 32.8 (44.2); 2048 113 (141) and 100 (119).
   if constexpr (!WIDE) {

@@ -264,6 +264,9 @@ Q4 += [  # many rows: tokens that fill LDS, and f32 ones that do so twice and th
     ("f32", "f16", 1141, 520, 416, 32, True, 1, 1, 0), ("bf16", "f16", 1121, 517, 896, 128, True, 1, 1, 1),
     ("f32", "bf16", 1122, 517, 640, 128, False, 0, 0, 0), ("bf16", "bf16", 1901, 2170, 384, 128, True, 0, 0, 0),
     ("bf16", "f16", 40001, 9, 64, 32, True, 0, 0, 0), ("f32", "f16", 1 << 20, 3, 32, 32, False, 0, 0, 0),
+    # work-groups of four waves
+    ("bf16", "f16", 1, 10250, 1120, 32, True, 0, 0, 0), ("f16", "bf16", 37, 4100, 640, 64, False, 1, 1, 1), ("f32", "f16", 50, 2000, 1056, 32, True, 0, 0, 0),
+    ("f32", "f16", 5, 6150, 896, 128, True, 0, 0, 0),
     # few rows of many numbers
     ("bf16", "f16", 3, 40, 14336, 64, True, 0, 0, 0), ("f32", "f16", 5, 100, 8192, 32, True, 0, 0, 1),
     ("f16", "bf16", 40, 33, 8224, 32, False, 0, 0, 0),
@@ -339,7 +342,7 @@ def test_q4_weights_from_device_memory(ctx, bufs):
     (16, 24600, 1056, 32, 32, True, "f16"), (7, 24577, 640, 128, 640, False, "f32"), (23, 32770, 192, 64, 32, True, "bf16"),
     (965, 1040, 352, 32, 32, True, "f16"), (1130, 520, 640, 128, 64, False, "f32"), (1121, 517, 896, 128, 896, True, "bf16"),
     (1901, 2170, 384, 64, 128, True, "f32"),
-    (9, 50, 8192, 128, 64, True, "f32"), (60, 20, 9216, 64, 128, True, "f16"),
+    (20, 5200, 416, 32, 32, True, "bf16"), (9, 50, 8192, 128, 64, True, "f32"), (60, 20, 9216, 64, 128, True, "f16"),
 ])
 def test_q4_products_of_8_bit_tokens(ctx, bufs, ntok, rows, cols, group, block, zeros, dtype):
     """Whole numbers up to 128 * 127 * 31 < 2^24 within a unit of 32 to 128 numbers; per unit the
