@@ -24,22 +24,20 @@ ProfEvents& prof_events();
 
 // kernel<<<grid, block, shmem, st>>>(args...), or the same launch with the
 // open bracket's events.  Arguments are converted to the kernel's parameter
-// types before their addresses are taken.
+// types before their addresses are taken.  The status is the launch's own: the
+// thread's last error may be that of an earlier call, of whatever library.
 template <typename... P, typename... A>
 hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, uint32_t shmem, hipStream_t st,
                   A... args) {
   static_assert(sizeof...(P) == sizeof...(A), "kernel argument count");
   ProfEvents& pe = prof_events();
-  if (!pe.stop) {
-    kernel<<<grid, block, shmem, st>>>(args...);
-    return hipGetLastError();
-  }
   std::tuple<P...> typed{static_cast<P>(args)...};
   void* ptrs[sizeof...(P) ? sizeof...(P) : 1];
   std::apply([&](auto&... v) {
     int i = 0;
     ((ptrs[i++] = (void*)&v), ...);
   }, typed);
+  if (!pe.stop) return hipLaunchKernel((const void*)kernel, grid, block, ptrs, shmem, st);
   hipError_t e = hipExtLaunchKernel((const void*)kernel, grid, block, ptrs, shmem, st,
                                     pe.started ? nullptr : pe.start, pe.stop, 0);
   pe.started = true;

@@ -89,7 +89,10 @@ struct hale_moe {
 
 static thread_local std::string g_create_err;
 
+// A HIP error that is reported here is not left behind as the thread's last one, where the
+// caller's next look at that would find it.
 static int fail(hale_ctx* c, int code, const char* fmt, ...) {
+  if (code == HALE_ENOMEM || code == HALE_EHIP) (void)hipGetLastError();
   char buf[512];
   va_list ap;
   va_start(ap, fmt);
