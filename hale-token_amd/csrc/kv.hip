@@ -877,14 +877,14 @@ extern "C" int hale_kv_attention_device(hale_kv_cache* kv, size_t layer, int dty
   bool few = false, many = false;
   for (const KvStepSeq& s : kv->seqs) (s.ntok * kv->shape.group() <= limit ? few : many) |= s.ntok > 0;
   if (v.plan.shared) {
-    // captured: later steps of these tokens may share otherwise, so both kinds (where their pages can
-    // be enough for that) and their joins
+    // captured: later steps of these tokens may share otherwise, so both kinds (few rows where a sequence
+    // has few, many where one has or where few rows' pages can be enough for that) and their joins
     a.nitems = a.njoins = 0xffffffffu;
     unsigned rows = 0;
     for (const KvStepSeq& q : kv->seqs) rows = std::max(rows, std::min<unsigned>(q.ntok * kv->shape.group(), kv_many_rows(kv->shape.head_dim)));
     for (int kind = 0; kind < 2; kind++) {
       const size_t n = (kind ? v.plan.many : v.plan.few).size();
-      const bool later = kind == 0 || many || kv_share_may_many(kv->shape, kv->seqs, kv->pages.max_pages(), f32);
+      const bool later = kind == 0 ? few : many || kv_share_may_many(kv->shape, kv->seqs, kv->pages.max_pages(), f32);
       if (!n && !(cap && later)) continue;
       a.kind = kind;
       a.items = kind ? items + kv->at.many * 4 / sizeof(KvItem) : items;

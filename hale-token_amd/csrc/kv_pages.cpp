@@ -440,14 +440,28 @@ struct Shared {
 
 // Which sequences share which pages, from the whole step downward: a run of sequences
 // shares what its least similar neighbours have in common, and falls into the runs
-// between those.
-void find_shared(const std::vector<const KvStepSeq*>& seqs, const KvPages& pages, size_t min_pages, std::vector<Shared>* out) {
-  const size_t n = seqs.size();
+// between those.  All of a run are of few rows (limit at most) or all of many: the few rows of
+// one token beside a prompt's would otherwise go to the kernel of many, or the prompt's, in more
+// tiles than its own, to that of few (8 sequences of 40 rows behind 4000, 4 heads, bf16: apart 23.3 us, shared
+// in tiles of 16 rows 31.3, in tiles of 128 20.8).
+// Many rows fill tiles of their own already, and partial results cost their rows about as
+// much as half a page for each: such a run shares where that is less than the pages that it saves
+// (rows, sequences, positions, pages saved for each row, time of apart, bf16 and f32: 40 x 8 behind
+// 4000 1.0 0.89 0.71, x 32 1.1 0.80 0.62; 40 x 8 behind 1000 0.23 1.13 1.11, x 32 0.26 1.26 0.89; 96 x 8
+// behind 4000 0.16 1.12 0.99; 320 x 8 0.10 1.06 1.05; 2400 x 4 0.006 1.16 1.03).  Few rows always fill
+// tiles better together.
+void find_shared(const std::vector<const KvStepSeq*>& seqs, const KvShape& s, size_t limit, const KvPages& pages,
+                 size_t min_pages, std::vector<Shared>* out) {
+  const size_t n = seqs.size(), group = s.group(), many_rows = kv_many_rows(s.head_dim);
   out->clear();
   if (n < 2 || n > KV_SHARE_SEQS) return;
-  std::vector<size_t> common(n - 1);
+  std::vector<size_t> common(n - 1), tiles(n + 1, 0);  // tiles: of the sequences before, each by itself, of many rows
+  const auto is_few = [&](size_t i) { return seqs[i]->ntok * group <= limit; };
+  for (size_t i = 0; i < n; i++) tiles[i + 1] = tiles[i] + ceil_div(seqs[i]->ntok * group, many_rows);
   for (size_t i = 0; i + 1 < n; i++)  // whole pages that neither writes to in this step
-    common[i] = pages.common(seqs[i]->row, seqs[i + 1]->row, std::min(seqs[i]->len0, seqs[i + 1]->len0) / KV_PAGE);
+    common[i] = is_few(i) != is_few(i + 1)
+                    ? 0
+                    : pages.common(seqs[i]->row, seqs[i + 1]->row, std::min(seqs[i]->len0, seqs[i + 1]->len0) / KV_PAGE);
   struct Run {
     size_t first, last, page0;
     int level;
@@ -457,7 +471,13 @@ void find_shared(const std::vector<const KvStepSeq*>& seqs, const KvPages& pages
     Run r = todo.back();
     todo.pop_back();
     const size_t least = *std::min_element(common.begin() + r.first, common.begin() + r.last - 1);
-    if (least >= r.page0 + min_pages) {
+    bool share = least >= r.page0 + min_pages;
+    if (share && !is_few(r.first)) {
+      const size_t rows = (seqs[r.last - 1]->tok0 + seqs[r.last - 1]->ntok - seqs[r.first]->tok0) * group;
+      const size_t apart = tiles[r.last] - tiles[r.first], together = ceil_div(rows, many_rows);
+      share = (apart - together) * (least - r.page0) * 2 >= rows;
+    }
+    if (share) {
       out->push_back({r.first, r.last, (uint32_t)r.page0, (uint32_t)least});
       r.page0 = least;
       if (++r.level == KV_SHARE_LEVELS) continue;
@@ -492,7 +512,7 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
   }
   const size_t room = kv_max_items(s, tokens, seqs.size());
   std::vector<Shared> shared;
-  find_shared(with, pages, min_pages, &shared);
+  find_shared(with, s, limit, pages, min_pages, &shared);
   for (;;) {  // without sharing where its partial results or lists exceed what there is room for
     out->few.clear();
     out->many.clear();
@@ -508,11 +528,11 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
     for (Shared& d : shared) {
       const KvStepSeq &a = *with[d.first], &b = *with[d.last - 1];
       d.rows = (uint32_t)((b.tok0 + b.ntok - a.tok0) * group);
-      work += ceil_div(d.rows, 16) * (d.page1 - d.page0) * s.kv_heads;
+      if (a.ntok * group <= limit) work += ceil_div(d.rows, 16) * (d.page1 - d.page0) * s.kv_heads;
     }
     for (Shared& d : shared) {
       const KvStepSeq& a = *with[d.first];
-      d.few = work <= (f32 ? KV_SHARE_FEW_F32 : KV_SHARE_FEW) || d.rows <= 64;
+      d.few = a.ntok * group <= limit && (work <= (f32 ? KV_SHARE_FEW_F32 : KV_SHARE_FEW) || d.rows <= 64);
       const size_t rows = d.few ? 16 * (size_t)out->cols : many_rows;
       for (uint32_t h = 0; h < s.kv_heads; h++)
         for (size_t r = 0; r < d.rows; r += rows)

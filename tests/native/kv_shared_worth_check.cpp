@@ -1,0 +1,118 @@
+// Checks that sharing pages is worth it where a plan shares them
+// (hale-token_amd/csrc/kv_pages.cpp): a step never reads more pages than with each sequence
+// by itself, whatever its numbers of rows.  The argument names the check; exits 1 with a
+// message where it fails.
+#include <stdio.h>
+#include <stdlib.h>
+
+#include <algorithm>
+#include <random>
+#include <string>
+
+#include "kv_pages.h"
+
+using namespace hale;
+
+#define CHECK(cond)                                                    \
+  do {                                                                 \
+    if (!(cond)) {                                                     \
+      fprintf(stderr, "line %d: %s does not hold\n", __LINE__, #cond); \
+      exit(1);                                                         \
+    }                                                                  \
+  } while (0)
+
+namespace {
+
+std::string err;
+std::vector<KvCopy> copies;
+
+size_t reads(const KvPlan& p) {
+  size_t n = 0;
+  for (const KvItem& it : p.few) n += it.page1 - it.page0;
+  for (const KvItem& it : p.many) n += it.page1 - it.page0;
+  return n;
+}
+
+// A step of forks behind a prompt, ntok tokens each, and its plans apart and shared.
+struct Step {
+  std::vector<KvStepSeq> seqs;
+  KvPlan apart, shared;
+};
+Step forks(const KvShape& s, uint32_t prompt, const std::vector<uint32_t>& ntok, bool f32, const std::vector<uint32_t>& tails = {}) {
+  KvPages pages;
+  pages.init(40000, ntok.size() + 1, prompt + 2000);
+  uint32_t root;
+  std::vector<uint32_t> made(ntok.size());
+  CHECK(pages.create(&root, &err) == KvPages::OK && pages.step(1, &root, &prompt, nullptr, &copies, &err) == KvPages::OK);
+  CHECK(pages.fork(root, made.size(), made.data(), &err) == KvPages::OK);
+  if (!tails.empty()) CHECK(pages.step(made.size(), made.data(), tails.data(), nullptr, &copies, &err) == KvPages::OK);
+  Step t;
+  CHECK(pages.step(made.size(), made.data(), ntok.data(), &t.seqs, &copies, &err) == KvPages::OK);
+  kv_plan(s, t.seqs, 0, f32, &t.apart);
+  kv_plan_shared(s, t.seqs, pages, 1, f32, &t.shared);
+  return t;
+}
+std::vector<uint32_t> each(size_t n, uint32_t v) { return std::vector<uint32_t>(n, v); }
+
+void no_more_pages() {
+  for (bool f32 : {false, true})
+    for (size_t kv : {1, 4, 8})
+      for (size_t group : {1, 4, 8, 16})
+        for (size_t dim : {128, 256})
+          for (uint32_t ntok : {1, 2, 3, 5, 10, 12, 20, 40, 75, 200, 600})
+            for (uint32_t n : {2, 3, 8, 32})
+              for (uint32_t prompt : {70u, 1000u, 9000u}) {
+                const Step t = forks({kv * group, kv, dim}, prompt, each(n, ntok), f32);
+                CHECK(reads(t.shared) <= reads(t.apart));
+              }
+  std::mt19937 rng(5);
+  for (int k = 0; k < 400; k++) {  // of all kinds side by side
+    std::vector<uint32_t> ntok, tails;
+    for (size_t n = 2 + rng() % 30; ntok.size() < n;) {
+      ntok.push_back(rng() % 6 == 0 ? rng() % 700 : rng() % 9 == 0 ? 0 : 1 + rng() % 12);
+      tails.push_back(rng() % 400);
+    }
+    const size_t kv = 1 + rng() % 8, group = (size_t)1 << rng() % 5;
+    const uint32_t prompt = rng() % 9000;
+    const bool f32 = rng() % 2;
+    const Step t = forks({kv * group, kv, 64u << rng() % 3}, prompt, ntok, f32, tails);
+    CHECK(reads(t.shared) <= reads(t.apart));
+    // two neighbours whose rows fit into one tile of the 16 that the kernel of few takes at least
+    bool saves = false;
+    size_t before = 1000;
+    for (uint32_t n : ntok)
+      if (n) saves |= (n + before) * group <= 16, before = n;
+    CHECK(!(saves && prompt >= KV_PAGE) || reads(t.shared) < reads(t.apart));
+  }
+}
+
+// Sequences of many rows stay with the kernel of many, and share where that saves enough.
+void many_rows() {
+  const KvShape s{32, 4, 128};
+  for (bool f32 : {false, true}) {
+    const Step five = forks(s, 4000, each(8, 5), f32);  // 40 rows each: three tiles in place of eight
+    CHECK(five.shared.few.empty() && !five.shared.many.empty() && reads(five.shared) * 2 < reads(five.apart));
+    for (uint32_t ntok : {12, 40, 600}) {  // tiles that are full already, or nearly
+      const Step t = forks(s, 4000, each(4, ntok), f32);
+      CHECK(t.shared.few.empty() && reads(t.shared) == reads(t.apart) && t.shared.many.size() == t.apart.many.size());
+    }
+    // a prompt among decoding sequences: those on either side share, in tiles of few rows
+    std::vector<uint32_t> ntok = each(21, 1);
+    ntok[10] = 300;
+    const Step t = forks(s, 4000, ntok, f32);
+    size_t most = 0;
+    for (const KvItem& it : t.shared.few) most = std::max<size_t>(most, it.rows);
+    CHECK(most == 16 && reads(t.shared) < reads(t.apart));
+    for (const KvItem& it : t.shared.many) CHECK(it.tok0 == t.seqs[10].tok0);
+  }
+}
+
+}  // namespace
+
+int main(int argc, char** argv) {
+  const std::string what = argc > 1 ? argv[1] : "";
+  if (what == "no_more_pages") no_more_pages();
+  else if (what == "many_rows") many_rows();
+  else return 2;
+  return 0;
+}
