@@ -700,24 +700,38 @@ constexpr unsigned JOIN_PARTS = 2 * (KV_FEW_GROUPS > KV_MANY_GROUPS ? KV_FEW_GRO
 constexpr int JOIN_BITS = 10;
 static_assert(JOIN_PARTS <= 1u << JOIN_BITS, "the sum of a row's parts");
 
+// The joins of a launch and their one series: of steps apart, or of those that may share and do not
+// (a.kind 2).
+template <typename Join> __device__ __forceinline__ Join join_of(const KvAttnArgs& a, unsigned it) {
+  if constexpr (__is_same(Join, KvJoin)) return a.joins[it];
+  else return a.share_joins[it];
+}
+__device__ __forceinline__ KvSeries series_of(const KvJoin& j) { return {j.part0, j.parts, j.step}; }
+__device__ __forceinline__ KvSeries series_of(const KvShareJoin& j) { return j.of[0]; }
+template <typename Join> __device__ __forceinline__ unsigned joins_of(const KvAttnArgs& a) {
+  return a.njoins != 0xffffffffu ? a.njoins : a.counts[__is_same(Join, KvJoin) ? a.kind + 2 : 2];
+}
+
 // Joins of few parts, or of many rows: a work-group takes as many rows as its
 // threads hold at four numbers each, the parts one behind the other.  A chain of three
 // reads: 5.1 us for 32 sequences of up to 7 parts, 4 rows of 128 each.
+template <typename Join>
 __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a) {
   const int t = threadIdx.x;
   const int quads = a.g.hd / 4, lanes = quads <= 16 ? 16 : quads <= 32 ? 32 : 64, x = t % lanes;
-  const unsigned njoins = a.njoins != 0xffffffffu ? a.njoins : a.counts[a.kind + 2];
+  const unsigned njoins = joins_of<Join>(a);
   for (unsigned it = blockIdx.x; it < njoins; it += gridDim.x) {
-    const KvJoin join = a.joins[it];
+    const Join join = join_of<Join>(a, it);
+    const KvSeries of = series_of(join);
     const unsigned row = blockIdx.y * (256 / lanes) + t / lanes;
     if (row >= join.rows || x >= quads) continue;
-    const float2* ml = a.part_ml + (size_t)join.part0 + row;
-    const float* po = a.part_o + ((size_t)join.part0 + row) * a.g.hd + 4 * x;
-    const size_t step = (size_t)join.step * a.g.hd;
+    const float2* ml = a.part_ml + (size_t)of.part0 + row;
+    const float* po = a.part_o + ((size_t)of.part0 + row) * a.g.hd + 4 * x;
+    const size_t step = (size_t)of.step * a.g.hd;
     float top = -__builtin_inff(), most = 0.0f, total = 0.0f;
 #pragma unroll 4
-    for (unsigned k = 0; k < join.parts; k++) {
-      const float2 part = ml[(size_t)k * join.step];
+    for (unsigned k = 0; k < of.parts; k++) {
+      const float2 part = ml[(size_t)k * of.step];
       top = fmaxf(top, part.x);
       most = fmaxf(most, part.y);
     }
@@ -725,8 +739,8 @@ __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a) {
     const float base2 = top == -__builtin_inff() ? 0.0f : top;
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (unsigned k = 0; k < join.parts; k++) {
-      const float2 part = ml[(size_t)k * join.step];
+    for (unsigned k = 0; k < of.parts; k++) {
+      const float2 part = ml[(size_t)k * of.step];
       const float w = exp2_fast(part.x - base2);
       total += w * part.y;
       v = v + *(const f32x4*)(po + k * step) * (w * pow2(above(part.y) - e));
@@ -741,6 +755,7 @@ __global__ __launch_bounds__(256) void k_kv_join_rows(KvAttnArgs a) {
 // Joins the partial results of one row: a work-group, whose threads take four
 // numbers each of every so many'th part; the slices are added in their order.  16 parts
 // a slice are read while the weights are found.  5.5 us for 128 parts of 32 rows of 128.
+template <typename Join>
 __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a) {
   constexpr int AHEAD = 16;
   __shared__ float sw[JOIN_PARTS];
@@ -749,20 +764,21 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a) {
   const int t = threadIdx.x, wave = t >> 6;
   const int quads = a.g.hd / 4, lanes = quads <= 16 ? 16 : quads <= 32 ? 32 : 64, slices = 256 / lanes;
   const int x = t % lanes, slice = t / lanes;
-  const unsigned njoins = a.njoins != 0xffffffffu ? a.njoins : a.counts[a.kind + 2];
+  const unsigned njoins = joins_of<Join>(a);
   for (unsigned it = blockIdx.x; it < njoins; it += gridDim.x) {
-    const KvJoin join = a.joins[it];
+    const Join join = join_of<Join>(a, it);
+    const KvSeries of = series_of(join);
     const unsigned row = blockIdx.y;
     if (row >= join.rows) continue;
-    const float2* ml = a.part_ml + (size_t)join.part0 + row;
-    const float* po = a.part_o + ((size_t)join.part0 + row) * a.g.hd + 4 * x;
-    const size_t step = (size_t)join.step * a.g.hd;
+    const float2* ml = a.part_ml + (size_t)of.part0 + row;
+    const float* po = a.part_o + ((size_t)of.part0 + row) * a.g.hd + 4 * x;
+    const size_t step = (size_t)of.step * a.g.hd;
     f32x4 early[AHEAD];  // the first parts, on their way while the weights are found
     if (x < quads) {
 #pragma unroll
       for (int k = 0; k < AHEAD; k++) {
         const unsigned part = slice + slices * k;
-        early[k] = *(const f32x4*)(po + (part < join.parts ? part : 0) * step);
+        early[k] = *(const f32x4*)(po + (part < of.parts ? part : 0) * step);
       }
     }
     float2 mine[JOIN_PARTS / 256];
@@ -770,7 +786,7 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a) {
 #pragma unroll
     for (int k = 0; k < (int)JOIN_PARTS / 256; k++) {
       const unsigned part = t + 256 * k;
-      mine[k] = part < join.parts ? ml[(size_t)part * join.step] : float2{-__builtin_inff(), 0.0f};
+      mine[k] = part < of.parts ? ml[(size_t)part * of.step] : float2{-__builtin_inff(), 0.0f};
       top = fmaxf(top, mine[k].x);
     }
     top = wave_max_f32(top);
@@ -783,7 +799,7 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a) {
     for (int k = 0; k < (int)JOIN_PARTS / 256; k++) {
       const unsigned part = t + 256 * k;
       const float w = exp2_fast(mine[k].x - base2);
-      if (part < join.parts) sw[part] = w * pow2(above(mine[k].y));
+      if (part < of.parts) sw[part] = w * pow2(above(mine[k].y));
       total += w * mine[k].y;
     }
 #pragma unroll
@@ -798,10 +814,10 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a) {
 #pragma unroll
       for (int k = 0; k < AHEAD; k++) {
         const unsigned part = slice + slices * k;
-        if (part < join.parts) v = v + early[k] * (sw[part] * down);
+        if (part < of.parts) v = v + early[k] * (sw[part] * down);
       }
 #pragma unroll 8
-      for (unsigned k = slice + slices * AHEAD; k < join.parts; k += slices) v = v + *(const f32x4*)(po + k * step) * (sw[k] * down);
+      for (unsigned k = slice + slices * AHEAD; k < of.parts; k += slices) v = v + *(const f32x4*)(po + k * step) * (sw[k] * down);
     }
     sv[t] = v;
     __syncthreads();
@@ -940,16 +956,17 @@ hipError_t launch_kv_attend_many(const KvAttnArgs& a, unsigned grid, hipStream_t
 
 hipError_t launch_kv_join(const KvAttnArgs& a, unsigned grid, unsigned rows, unsigned parts, hipStream_t st) {
   if (grid == 0) return hipSuccess;
-  if (a.kind == 2) {
+  if (a.kind == 2 && !a.alone) {
     const unsigned lanes = a.g.hd <= 64 ? 16 : a.g.hd <= 128 ? 32 : 64, per = 256 / lanes / SHARE_SLICES;
     return launch(k_kv_join_shared, dim3(grid, (rows + per - 1) / per), 256, 0, st, a);
   }
   // (with the attention, by row / rows together: 16 sequences of 1000, 4 parts 13.3 / 11.9 us;
   // of 6000, 8 parts 25.1 / 24.1; 4 of 3000, 12 parts 11.5 / 11.7; one of 131000, 512 parts
   // 31.1 / 54.5.  Many rows are the more work-groups: 300 behind 8000 102 / 68.)
-  if (a.kind == 0 && parts > 8) return launch(k_kv_join, dim3(grid, rows), 256, 0, st, a);
+  if (a.kind != 1 && rows <= kv_few_rows(a.g.hd) && parts > 8)
+    return launch(a.alone ? k_kv_join<KvShareJoin> : k_kv_join<KvJoin>, dim3(grid, rows), 256, 0, st, a);
   const unsigned per = a.g.hd <= 64 ? 16 : a.g.hd <= 128 ? 8 : 4;
-  return launch(k_kv_join_rows, dim3(grid, (rows + per - 1) / per), 256, 0, st, a);
+  return launch(a.alone ? k_kv_join_rows<KvShareJoin> : k_kv_join_rows<KvJoin>, dim3(grid, (rows + per - 1) / per), 256, 0, st, a);
 }
 
 }  // namespace hale

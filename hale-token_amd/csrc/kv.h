@@ -112,6 +112,7 @@ struct KvAttnArgs {
   const uint32_t* counts;      // {few, many, joins of few (or all, of kind 2), of many} of the plan, on the device
   unsigned nitems, njoins;     // the same, or 0xffffffff: read counts (captured calls)
   int kind;                    // 0: items and joins of few rows, 1: of many; 2: joins of shared pages
+  bool alone;                  // kind 2: each join has one series, its row's own pages
   float* part_o;               // [row][hd], times a power of two that follows from the sum
   float2* part_ml;             // [row] running maximum (base 2) and sum
   bool vec;                    // q and out rows start at multiples of four elements
@@ -121,7 +122,8 @@ struct KvAttnArgs {
 hipError_t launch_kv_attend_few(const KvAttnArgs& a, int cols, unsigned grid, hipStream_t st);
 // Of many rows: kv_many_rows per work-group.
 hipError_t launch_kv_attend_many(const KvAttnArgs& a, unsigned grid, hipStream_t st);
-// Joins of one kind, of at most `rows` rows each; parts: of a row, at most (kinds 0 and 1).
+// Joins of one kind, of at most `rows` rows each; parts: of a row, at most (but for joins
+// of several series).
 hipError_t launch_kv_join(const KvAttnArgs& a, unsigned grid, unsigned rows, unsigned parts, hipStream_t st);
 
 // ---- rotary positions --------------------------------------------------------

@@ -588,9 +588,10 @@ extern "C" int hale_kv_resize(hale_kv_cache* kv, size_t num_pages) {
 // steps
 // ---------------------------------------------------------------------------
 
-// A step's attention in one of the views.
+// A step's attention in one of the views.  What kind of plan follows from the tokens per sequence, so
+// that captured launches hold for later steps.
 static void make_plan(const hale_kv_cache* kv, const std::vector<KvStepSeq>& seqs, const View& v, KvPlan* out) {
-  if (kv->share && v.window == 0) kv_plan_shared(kv->shape, seqs, kv->pages, kv->share, v.f32, out);
+  if (kv->share && v.window == 0 && kv_may_share(seqs)) kv_plan_shared(kv->shape, seqs, kv->pages, kv->share, v.f32, out);
   else kv_plan(kv->shape, seqs, v.window, v.f32, out);
 }
 static size_t plan_bytes(const KvPlan& p) {
@@ -895,9 +896,14 @@ extern "C" int hale_kv_attention_device(hale_kv_cache* kv, size_t layer, int dty
     a.kind = 2;
     a.share_joins = (const KvShareJoin*)joins;
     const size_t n = v.plan.share_joins.size();
-    if (!cap) a.njoins = (unsigned)n;
+    unsigned parts = 0;
+    if (!cap) {  // a captured join takes what later steps share
+      a.njoins = (unsigned)n;
+      a.alone = v.plan.alone;
+      for (const KvShareJoin& j : v.plan.share_joins) parts = std::max(parts, j.of[0].parts);
+    }
     if (n || cap)
-      CALL_LAUNCH(c, K_KV_ATTENTION, launch_kv_join(a, (unsigned)(cap ? std::min<size_t>(tiles, 256) : std::min<size_t>(n, 1u << 20)), rows, 0, c->stream));
+      CALL_LAUNCH(c, K_KV_ATTENTION, launch_kv_join(a, (unsigned)(cap ? std::min<size_t>(tiles, 256) : std::min<size_t>(n, 1u << 20)), rows, parts, c->stream));
     return HALE_OK;
   }
   for (int kind = 0; kind < 2; kind++) {

@@ -394,7 +394,7 @@ void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window
   out->few_joins.clear();
   out->many_joins.clear();
   out->share_joins.clear();
-  out->shared = false;
+  out->shared = out->alone = false;
   out->part_rows = 0;
   const size_t group = s.group(), few_rows = kv_few_rows(s.head_dim), many_rows = kv_many_rows(s.head_dim);
   const size_t limit = kv_few_limit(s, seqs, f32);
@@ -492,6 +492,12 @@ void find_shared(const std::vector<const KvStepSeq*>& seqs, const KvShape& s, si
 
 }  // namespace
 
+bool kv_may_share(const std::vector<KvStepSeq>& seqs) {
+  size_t n = 0;
+  for (const KvStepSeq& q : seqs) n += q.ntok > 0;
+  return n > 1 && n <= KV_SHARE_SEQS;
+}
+
 bool kv_share_may_many(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t max_pages, bool f32) {
   // at any page the runs that share it have two sequences or more each, and a tile of their own begun
   size_t rows = 0, n = 0;
@@ -556,7 +562,9 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
     // of few rows: as many pages for each of a work-group's four waves, and about a work-group per
     // compute unit, for a part costs more here, where joins have several series (32 bf16
     // sequences of up to 600 behind 8000, 32 heads of 128 on 8, 24.0 us with 256 work-groups, 27.7
-    // with 512; 4 behind 16000, 4 heads, 16.6 and 23.9)
+    // with 512; 4 behind 16000, 4 heads, 16.6 and 23.9; of 18 steps that share nothing 16 are as fast or faster
+    // with 256, f32, 16 of 1000 15.8 and 21.4, 2 of 16000 20.3 and 25.0, and 32 of 4000, whose 270 MB come from
+    // memory, 79 and 65)
     const size_t each[2] = {4 * std::max<size_t>(1, ceil_div(count_pages(few), 4 * KV_SHARE_GROUPS)), many.empty() ? 1 : many_each(many)};
     size_t rows = 0, longest = 0;
     for (Shared& d : shared) {
@@ -609,6 +617,7 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
       }
     }
     out->part_rows = (uint32_t)rows;
+    out->alone = shared.empty();
     if (shared.empty() || (rows <= kv_part_rows(s.head_dim) && longest <= KV_SHARE_PARTS && out->few.size() <= room && out->many.size() <= room))
       break;
     shared.clear();

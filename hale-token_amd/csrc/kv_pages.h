@@ -80,6 +80,7 @@ struct KvPlan {
   std::vector<KvJoin> few_joins, many_joins;
   bool shared = false;  // made by kv_plan_shared: all joins are these
   std::vector<KvShareJoin> share_joins;
+  bool alone = false;  // and no pages are shared
   uint32_t part_rows = 0;
 };
 
@@ -131,6 +132,8 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
 // Sequences with new tokens in a step up to which pages are shared: finding out who
 // shares what takes up to the square of their number.
 constexpr size_t KV_SHARE_SEQS = 1024;
+// Whether sequences of a step of these numbers of tokens may share pages at all.
+bool kv_may_share(const std::vector<KvStepSeq>& seqs);
 constexpr size_t KV_SHARE_PARTS = 1024;  // of a row, over all its series
 // Work-groups of few rows that a step which shares pages is divided into.
 constexpr size_t KV_SHARE_GROUPS = 256;

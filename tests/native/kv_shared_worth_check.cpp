@@ -107,12 +107,45 @@ void many_rows() {
   }
 }
 
+// A plan says whether it shares any pages: without, each join has the one series of its row's own.
+void nothing_shared() {
+  for (uint32_t ntok : {1, 300})
+    for (uint32_t pair : {0, 1}) {
+      const KvShape s{32, 8, 128};
+      KvPages pages;
+      pages.init(4000, 40, 6000);
+      std::vector<uint32_t> seqs(30), n(30);
+      for (uint32_t k = 0; k < 30; k++) {
+        CHECK(pages.create(&seqs[k], &err) == KvPages::OK);
+        n[k] = 3900 + 7 * k;
+      }
+      CHECK(pages.step(30, seqs.data(), n.data(), nullptr, &copies, &err) == KvPages::OK);
+      if (pair) {  // two forks beside them
+        uint32_t made[2];
+        CHECK(pages.fork(seqs[4], 2, made, &err) == KvPages::OK);
+        seqs.insert(seqs.begin() + 5, made, made + 2);
+      }
+      n.assign(seqs.size(), ntok);
+      std::vector<KvStepSeq> plan;
+      CHECK(pages.step(seqs.size(), seqs.data(), n.data(), &plan, &copies, &err) == KvPages::OK);
+      KvPlan p;
+      kv_plan_shared(s, plan, pages, 1, false, &p);
+      CHECK(p.alone == !(pair && ntok == 1));  // (tiles of 300 tokens are full already, and so many that none is divided)
+      size_t most = 0;
+      for (const KvShareJoin& j : p.share_joins) most = std::max<size_t>(most, j.n);
+      CHECK(ntok == 1 ? p.alone == (most == 1) && most : most <= 1);
+      kv_plan(s, plan, 0, false, &p);
+      CHECK(!p.alone && !p.shared);
+    }
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
   const std::string what = argc > 1 ? argv[1] : "";
   if (what == "no_more_pages") no_more_pages();
   else if (what == "many_rows") many_rows();
+  else if (what == "nothing_shared") nothing_shared();
   else return 2;
   return 0;
 }

@@ -32,3 +32,7 @@ def test_sharing_reads_no_more_pages(check):
 
 def test_sequences_of_many_rows(check):
     check("many_rows")
+
+
+def test_plans_that_share_nothing_say_so(check):
+    check("nothing_shared")
