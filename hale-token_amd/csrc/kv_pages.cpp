@@ -449,9 +449,9 @@ struct Shared {
 // (rows, sequences, positions, pages saved for each row, time of apart, bf16 and f32: 40 x 8 behind
 // 4000 1.0 0.89 0.71, x 32 1.1 0.80 0.62; 40 x 8 behind 1000 0.23 1.13 1.11, x 32 0.26 1.26 0.89; 96 x 8
 // behind 4000 0.16 1.12 0.99; 320 x 8 0.10 1.06 1.05; 2400 x 4 0.006 1.16 1.03).  Few rows always fill
-// tiles better together.
+// tiles better together.  levels: how often a run's rows may share pages behind others.
 void find_shared(const std::vector<const KvStepSeq*>& seqs, const KvShape& s, size_t limit, const KvPages& pages,
-                 size_t min_pages, std::vector<Shared>* out) {
+                 size_t min_pages, int levels, std::vector<Shared>* out) {
   const size_t n = seqs.size(), group = s.group(), many_rows = kv_many_rows(s.head_dim);
   out->clear();
   if (n < 2 || n > KV_SHARE_SEQS) return;
@@ -480,7 +480,7 @@ void find_shared(const std::vector<const KvStepSeq*>& seqs, const KvShape& s, si
     if (share) {
       out->push_back({r.first, r.last, (uint32_t)r.page0, (uint32_t)least});
       r.page0 = least;
-      if (++r.level == KV_SHARE_LEVELS) continue;
+      if (++r.level == levels) continue;
     }
     for (size_t i = r.first, from = r.first; i < r.last; i++)
       if (i + 1 == r.last || common[i] == least) {
@@ -517,9 +517,10 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
     tokens += q.ntok;
   }
   const size_t room = kv_max_items(s, tokens, seqs.size());
+  int levels = KV_SHARE_LEVELS;
   std::vector<Shared> shared;
-  find_shared(with, s, limit, pages, min_pages, &shared);
-  for (;;) {  // without sharing where its partial results or lists exceed what there is room for
+  find_shared(with, s, limit, pages, min_pages, levels, &shared);
+  for (;;) {  // with less sharing where its partial results or lists exceed what there is room for
     out->few.clear();
     out->many.clear();
     out->few_joins.clear();
@@ -566,11 +567,43 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
     // with 256, f32, 16 of 1000 15.8 and 21.4, 2 of 16000 20.3 and 25.0, and 32 of 4000, whose 270 MB come from
     // memory, 79 and 65)
     const size_t each[2] = {4 * std::max<size_t>(1, ceil_div(count_pages(few), 4 * KV_SHARE_GROUPS)), many.empty() ? 1 : many_each(many)};
-    size_t rows = 0, longest = 0;
+    // what that comes to: partial results, parts of a row at most, items
+    size_t rows = 0, longest = 0, items[2] = {0, 0};
     for (Shared& d : shared) {
       d.parts = (uint32_t)ceil_div(d.page1 - d.page0, each[!d.few]);
       d.part = (uint32_t)rows;
       rows += (size_t)d.rows * d.parts * s.kv_heads;
+      items[!d.few] += ceil_div(d.rows, d.few ? 16 * (size_t)out->cols : many_rows) * d.parts * s.kv_heads;
+    }
+    const size_t own = rows;  // partial results of sequences' own pages from here on
+    for (int kind = 0; kind < 2; kind++) {
+      const auto& tiles = kind ? many : few;
+      for (size_t k = kind ? many_shared : few_shared; k < tiles.size(); k++) {
+        const auto& above = over[(kind ? many_seq : few_seq)[k - (kind ? many_shared : few_shared)]];
+        const size_t parts = ceil_div(tiles[k].page1 - tiles[k].page0, each[kind]);
+        size_t sum = parts;
+        for (const Shared* d : above) sum += d->parts;
+        if (sum > 1) rows += parts * tiles[k].rows, longest = std::max(longest, sum);
+        items[kind] += parts;
+      }
+    }
+    const size_t most_rows = kv_part_rows(s.head_dim);
+    if (!shared.empty() && (rows > most_rows || longest > KV_SHARE_PARTS || items[0] > room || items[1] > room)) {
+      // the deepest level first, then of the runs those of the fewest pages (what a row saves by its partial
+      // results), as many as they are for too many rows
+      if (--levels > 0) {
+        find_shared(with, s, limit, pages, min_pages, levels, &shared);
+        continue;
+      }
+      levels = 1;
+      std::stable_sort(shared.begin(), shared.end(), [](const Shared& a, const Shared& b) { return a.page1 < b.page1; });
+      size_t n = 0;
+      do rows -= std::min(rows, (size_t)shared[n].rows * (shared[n].parts + 1) * s.kv_heads);
+      while (++n < shared.size() && rows > most_rows);
+      shared.erase(shared.begin(), shared.begin() + (long)n);
+      continue;
+    }
+    for (const Shared& d : shared) {
       // A piece's tiles of rows on one die, whose cache then holds its pages: work-groups go to the
       // eight dies in turn (behind 8000 as above 27.7 us, 34.0 in the pieces' order; behind
       // 32000 52 and 86).
@@ -586,9 +619,9 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
                             (uint32_t)r, (uint32_t)(d.page0 + n * p / d.parts), (uint32_t)(d.page0 + n * (p + 1) / d.parts),
                             (uint32_t)(d.part + k * d.rows + r)});
           }
-      if (rows > kv_part_rows(s.head_dim)) break;
     }
-    for (int kind = 0; kind < 2 && rows <= kv_part_rows(s.head_dim); kind++) {
+    rows = own;
+    for (int kind = 0; kind < 2; kind++) {
       const auto& tiles = kind ? many : few;
       for (size_t k = kind ? many_shared : few_shared; k < tiles.size(); k++) {
         const Tile& t = tiles[k];
@@ -597,14 +630,11 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
         const bool joined = parts > 1 || !over[i].empty();
         if (joined) {
           KvShareJoin j{t.q->tok0, (uint16_t)t.head, (uint16_t)t.rows, t.row0, 0, {}};
-          size_t sum = parts;
           for (const Shared* d : over[i]) {
             const size_t row = (t.q->tok0 - with[d->first]->tok0) * group + t.row0;
             j.of[j.n++] = {(uint32_t)(d->part + (size_t)t.head * d->parts * d->rows + row), d->parts, d->rows};
-            sum += d->parts;
           }
           j.of[j.n++] = {(uint32_t)rows, (uint32_t)parts, t.rows};
-          longest = std::max(longest, sum);
           out->share_joins.push_back(j);
         }
         for (size_t p = 0; p < parts; p++) {
@@ -613,14 +643,11 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
                           (uint32_t)(t.page0 + n * (p + 1) / parts), joined ? (uint32_t)rows : KV_WHOLE});
           if (joined) rows += t.rows;
         }
-        if (rows > kv_part_rows(s.head_dim)) break;
       }
     }
     out->part_rows = (uint32_t)rows;
     out->alone = shared.empty();
-    if (shared.empty() || (rows <= kv_part_rows(s.head_dim) && longest <= KV_SHARE_PARTS && out->few.size() <= room && out->many.size() <= room))
-      break;
-    shared.clear();
+    break;
   }
   spread(&out->many);
 }

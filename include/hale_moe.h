@@ -745,13 +745,19 @@ int hale_kv_compact(hale_kv_cache *kv, size_t *moved);
 int hale_kv_resize(hale_kv_cache *kv, size_t num_pages);
 
 /* From the next step on, attention without a window computes over pages that sequences
- * have in common once for all of them: where sequences that stand side by side in a step
+ * have in common for all of them together: where sequences that stand side by side in a step
  * (those without new tokens aside) hold the same whole pages from their start, min_len
- * positions of them or more, the pages are read for all of their rows together, and those
- * that some of them share behind these likewise (on up to three levels, each of min_len
- * positions more; in steps of up to 1024 sequences with tokens).  Forks
- * (hale_kv_seq_fork) share so what their origin held.  Results are the same but for the order
- * of sums, so for their last bits.  0, the default: never.  A changed setting ends the current
+ * positions of them or more, the pages are read once for every 16 rows of all of them (rows: of a
+ * key/value head, tokens times the heads that share it; 32 where a sequence of the step has more than 16), or
+ * for every 128 (head_dim above 128: 64) where that is much, and not for each sequence apart; and those that
+ * some of them share behind these likewise (on up to three levels, each of min_len positions more; in steps of
+ * up to 1024 sequences with tokens).  Sequences of few rows (up to 16, in small steps up to 64) and of more
+ * share among their like, the latter where the pages saved are worth it: prompts of several hundred tokens fill
+ * tiles of their own and share nothing.  Where the cache's workspace has no room for all partial results the
+ * deepest levels, then the shortest prefixes are not shared.  Sharing costs a launch that joins the
+ * results, some 4 us, which short prefixes need not have: from about 1000 positions on it is
+ * worth it.  Forks (hale_kv_seq_fork) share so what their origin held.  Results are the same but for
+ * the order of sums, so for their last bits.  0, the default: never.  A changed setting ends the current
  * step, and graphs that use the cache have to be captured anew. */
 int hale_kv_share_prefixes(hale_kv_cache *kv, size_t min_len);
 

@@ -139,6 +139,52 @@ void nothing_shared() {
     }
 }
 
+// Where there is no room for the partial results of all levels, or of all runs, the others are shared.
+void as_much_as_there_is_room_for() {
+  const KvShape s{64, 8, 256};  // room for 81920 rows of partial results, 64 a token and part
+  KvPages pages;
+  pages.init(60000, 1100, 6000);
+  auto check = [&](const std::vector<uint32_t>& seqs) {
+    std::vector<KvStepSeq> plan;
+    const std::vector<uint32_t> n(seqs.size(), 1);
+    CHECK(pages.step(seqs.size(), seqs.data(), n.data(), &plan, &copies, &err) == KvPages::OK);
+    KvPlan apart, shared;
+    kv_plan(s, plan, 0, false, &apart);
+    kv_plan_shared(s, plan, pages, 1, false, &shared);
+    CHECK(shared.part_rows <= kv_part_rows(s.head_dim));
+    return std::pair<size_t, KvPlan>(reads(apart) - reads(shared), shared);
+  };
+  // 20 talks of 30 behind one prompt: 38400 rows for each level and for the sequences' own pages
+  uint32_t root;
+  uint32_t len = 2000;
+  CHECK(pages.create(&root, &err) == KvPages::OK && pages.step(1, &root, &len, nullptr, &copies, &err) == KvPages::OK);
+  std::vector<uint32_t> talks(20), seqs;
+  CHECK(pages.fork(root, 20, talks.data(), &err) == KvPages::OK);
+  const std::vector<uint32_t> more(20, 640);
+  CHECK(pages.step(20, talks.data(), more.data(), nullptr, &copies, &err) == KvPages::OK);
+  for (uint32_t t : talks) {
+    uint32_t made[30];
+    CHECK(pages.fork(t, 30, made, &err) == KvPages::OK);
+    seqs.insert(seqs.end(), made, made + 30);
+  }
+  auto got = check(seqs);
+  // 31 pages of 8 heads, so many that they go to the kernel of many: tiles of 64 rows, 8 a sequence
+  CHECK(got.first == (600 - 600 / 8) * 31u * 8);
+  // two prompts with 500 answers each, 64000 rows of partial results each: the longer one's are shared
+  for (uint32_t s : seqs) CHECK(pages.free(s, &err) == KvPages::OK);
+  seqs.clear();
+  for (uint32_t prompt : {1000u, 2000u}) {
+    uint32_t a;
+    std::vector<uint32_t> made(500);
+    CHECK(pages.create(&a, &err) == KvPages::OK && pages.step(1, &a, &prompt, nullptr, &copies, &err) == KvPages::OK);
+    CHECK(pages.fork(a, 500, made.data(), &err) == KvPages::OK);
+    seqs.insert(seqs.end(), made.begin(), made.end());
+  }
+  got = check(seqs);
+  CHECK(got.first == (500 - (500 + 7) / 8) * 31u * 8);
+  for (const KvShareJoin& j : got.second.share_joins) CHECK(j.tok0 >= 500 && j.n == 2);
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -146,6 +192,7 @@ int main(int argc, char** argv) {
   if (what == "no_more_pages") no_more_pages();
   else if (what == "many_rows") many_rows();
   else if (what == "nothing_shared") nothing_shared();
+  else if (what == "as_much_as_there_is_room_for") as_much_as_there_is_room_for();
   else return 2;
   return 0;
 }

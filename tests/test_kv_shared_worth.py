@@ -36,3 +36,7 @@ def test_sequences_of_many_rows(check):
 
 def test_plans_that_share_nothing_say_so(check):
     check("nothing_shared")
+
+
+def test_as_much_is_shared_as_there_is_room_for(check):
+    check("as_much_as_there_is_room_for")
