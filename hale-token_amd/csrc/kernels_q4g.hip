@@ -776,10 +776,7 @@ static hipError_t q4g_few(const Q4gArgs& a, hipStream_t st) {
   // of them: the join takes 1 us and 0.2 a split, as long as the chunks of two turns (1024 rows, a
   // token of bf16: of 4096 numbers 4.3 us whole, 6.0 in four; of 14336 8.4 whole, 6.9 in three).
   const unsigned slices = (unsigned)((a.ntok + 15) / 16);
-  unsigned splits = 256 / (tiles * slices), most = a.g.chunks / (2 * W * CH);
-  splits = splits > most ? most : splits;
-  splits = splits > Q4G_SPLITS / slices ? Q4G_SPLITS / slices : splits;
-  splits = splits < 1 ? 1 : splits;
+  unsigned splits = q4g_splits(tiles, slices, a.g.chunks / (2 * W * CH));
   const unsigned per = (a.g.chunks + splits - 1) / splits;
   splits = (a.g.chunks + per - 1) / per;
   const uint32_t rows = W * CH * (uint32_t)(a.ntok < 16 ? a.ntok : 16) * sizeof(Q4gRow<IN>), lds = rows > W * 1024 ? rows : W * 1024;

@@ -61,8 +61,21 @@ struct Q4gGeom {
   float* parts;
   unsigned* done;
 };
-// Most work-groups that a tile's row is divided over.
-constexpr unsigned Q4G_SPLITS = 8;
+// Most work-groups that a tile's row is divided over, and that the divided rows of a launch come to.
+constexpr unsigned Q4G_SPLITS = 8, Q4G_GROUPS = 256;
+// Over how many work-groups a launch of `tiles` tiles for `slices` times 16 tokens divides rows of which
+// `most` parts are worth it.
+inline unsigned q4g_splits(size_t tiles, size_t slices, unsigned most) {
+  size_t n = Q4G_GROUPS / (tiles * slices);
+  n = n > most ? most : n;
+  n = n > Q4G_SPLITS / slices ? Q4G_SPLITS / slices : n;
+  return n < 1 ? 1 : (unsigned)n;
+}
+// The partial sums of tiles that a launch can need room for: a matrix of more tiles is never divided.
+inline size_t q4g_part_tiles(size_t tiles) {
+  if (2 * tiles > Q4G_GROUPS) return 0;
+  return tiles * Q4G_SPLITS < Q4G_GROUPS ? tiles * Q4G_SPLITS : Q4G_GROUPS;
+}
 
 hipError_t launch_q4g_pack(const Q4gGeom& g, const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros,
                            hipStream_t st);

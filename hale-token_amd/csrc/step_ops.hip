@@ -112,7 +112,7 @@ static int q4g_make(hale_ctx* c, size_t rows, size_t cols, size_t group, int sca
   const size_t zeros_at = g.scales_at + (size_t)g.chunks * 32 * g.per;
   g.tile_bytes = round_up(zeros_at + (g.zeros ? (size_t)g.chunks * 16 * g.per : 0), 128);
   const size_t tiles = (rows + Q4G_ROWS - 1) / Q4G_ROWS, bytes = tiles * g.tile_bytes;
-  const size_t parts = Q4G_SPLITS * tiles * 1024, done = round_up(Q4G_SPLITS * tiles * 4, 256);
+  const size_t parts = q4g_part_tiles(tiles) * 1024, done = round_up(q4g_part_tiles(tiles) * 4, 256);
   if (hipMalloc(&g.data, bytes + parts + done + 64) != hipSuccess)
     return ctx_fail(c, HALE_ENOMEM, "q4g_upload: %zu bytes of weights and workspace", bytes + parts + done + 64);
   g.parts = (float*)(g.data + bytes);
@@ -121,7 +121,7 @@ static int q4g_make(hale_ctx* c, size_t rows, size_t cols, size_t group, int sca
   g.zero_chunk = g.zeros ? 16 * g.per : 0;
   g.zero_tile = g.zeros ? g.tile_bytes : 0;
   uint8_t* sent = nullptr;
-  hipError_t e = hipMemsetAsync(g.done, 0, done, c->stream);
+  hipError_t e = done ? hipMemsetAsync(g.done, 0, done, c->stream) : hipSuccess;
   if (e == hipSuccess) e = hipMemsetAsync(g.data + bytes + parts + done, Q4G_OFFSET + 8, 64, c->stream);
   if (host) {
     const size_t cb = round_up(rows * (cols / 2), 256), sb = round_up(groups * 2, 256);

@@ -592,7 +592,9 @@ typedef struct hale_q4g hale_q4g;
  * a byte, the first in the low half; scales [rows][cols / group] of scale_dtype
  * (HALE_F16 or HALE_BF16); zeros [rows][cols / group], a byte of 0..15 each, or NULL
  * where all are 8.  group: 32, 64 or 128; cols a multiple of it, at most 2^30; rows at
- * most 2^27.  The bytes are laid out anew in device memory; both forms return when they have been read. */
+ * most 2^27.  The bytes are laid out anew in device memory, rows filled up to a multiple of 16 and
+ * columns to one of 128, with up to 260 KiB of workspace where rows are at most 2048; both forms return when
+ * they have been read. */
 int hale_q4g_upload(hale_ctx *ctx, size_t rows, size_t cols, size_t group,
                     int scale_dtype, const uint8_t *codes, const void *scales,
                     const uint8_t *zeros, hale_q4g **out);
