@@ -764,9 +764,10 @@ hipError_t launch_q4g_unpack(const Q4gGeom& g, uint8_t* codes, uint16_t* scales,
 
 constexpr uint32_t Q4G_LDS = 163840;  // of a compute unit
 
-// More LDS than a kernel has unasked.
+// More LDS than a kernel has unasked.  The limit is the process's, and calls of other contexts
+// run beside: each asks for the same, all there is, whatever its own launch takes.
 static hipError_t ask_lds(const void* kernel, uint32_t bytes) {
-  return bytes <= 65536 ? hipSuccess : hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  return bytes <= 65536 ? hipSuccess : hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)Q4G_LDS);
 }
 
 template <int IN, int PER, int M, bool BF, int CH, int W>
