@@ -60,6 +60,16 @@ template <typename T> struct Eight {
 __device__ __forceinline__ double from_words(unsigned lo, unsigned hi) {
   return __longlong_as_double((long long)((unsigned long long)hi << 32 | lo));
 }
+// A number of 64 bits as an f32 that rounds to f16 and bf16 as it does itself: the leading 13
+// bits, the last of them set where anything was cut off (11 for f16, the next, and whether there are more).
+// The nearest f32 would be rounded a second time, and a number beside a border of the 16 bits could
+// come to lie on it.  f32 holds 13 bits down to 2^-137, below what bf16 rounds to 0.
+__device__ __forceinline__ float odd_f32(double d) {
+  const unsigned long long b = (unsigned long long)__double_as_longlong(d);
+  const unsigned hi = (unsigned)(b >> 32), rest = (hi & 0xffu) | (unsigned)b;
+  return (float)from_words(0, (hi & ~0xffu) | (rest ? 0x100u : 0u));
+}
+
 template <int CTRL> __device__ __forceinline__ double dpp64(double v) {
   const unsigned long long b = (unsigned long long)__double_as_longlong(v);
   return from_words((unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)b, CTRL, 0xF, 0xF, false),
@@ -216,7 +226,11 @@ __global__ __launch_bounds__(NT) void k_norm_q8(NormQ8Args a) {
     if (a.y) {
       float y[8];
 #pragma unroll
-      for (int j = 0; j < 8; j++) y[j] = (float)((double)s[c][j] * (double)w[c][j] * r);
+      for (int j = 0; j < 8; j++) {
+        const double d = (double)s[c][j] * (double)w[c][j] * r;
+        if constexpr (sizeof(T) == 2) y[j] = odd_f32(d);
+        else y[j] = (float)d;
+      }
       Eight<T> y8;
       y8.round(y);
       y8.template store<VEC>(a.y, row * a.y_stride + 8 * at);
