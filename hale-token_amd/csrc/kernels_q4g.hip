@@ -9,6 +9,8 @@
 // step_ops.h.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "hale_device.h"
 #include "kernels.h"
 #include "kv_device.h"
@@ -156,10 +158,12 @@ __device__ __forceinline__ typename Q4gType<IN>::Acc products(const typename Q4g
       }
     }
   } else {
+    // the least parts of f32 numbers first: sums of them round far below the number's, and only STEPS
+    // additions at its size
 #pragma unroll
-    for (int k = 0; k < STEPS; k++)
+    for (int p = Q4gType<IN>::PARTS - 1; p >= 0; p--)
 #pragma unroll
-      for (int p = 0; p < Q4gType<IN>::PARTS; p++) {
+      for (int k = 0; k < STEPS; k++) {
         if constexpr (IN == Q4G_F16)
           acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[k], x[k][p], acc, 0, 0, 0);
         else
@@ -540,18 +544,21 @@ __global__ __launch_bounds__(1024) void k_q4g_stream(Q4gArgs a) {
     for (int p = 0; p < P; p++) xl[(c * ntok + t) * Tok::ROW + (j * P + p) * 4 + gg] = x[p];
   }
   __syncthreads();
+  // f32 numbers, put together again, in 64 bits: what their sum is off by counts 16 + zero times
   for (unsigned k = threadIdx.x; k < chunks * ntok * UNITS; k += blockDim.x) {
     const unsigned u = k % UNITS, t = k / UNITS % ntok, c = k / UNITS / ntok;
-    typename Ty::Sum sum = 0;
-    for (int e = 0; e < STEPS * P * 4; e++) {
-      const Frag f = xl[(c * ntok + t) * Tok::ROW + u * STEPS * P * 4 + e];
+    const Frag* from = xl + (c * ntok + t) * Tok::ROW + u * STEPS * P * 4;
+    typename std::conditional<IN == Q4G_F32, double, typename Ty::Sum>::type sum = 0;
+    for (int e = 0; e < STEPS * 4; e++) {
+      const Frag* f = from + e / 4 * P * 4 + e % 4;
 #pragma unroll
       for (int b = 0; b < 8; b++) {
-        if constexpr (IN == Q4G_I8) sum += (int)(int8_t)(f[b / 4] >> (8 * (b % 4)));
-        else sum += (float)f[b];
+        if constexpr (IN == Q4G_I8) sum += (int)(int8_t)(f[0][b / 4] >> (8 * (b % 4)));
+        else if constexpr (IN == Q4G_F32) sum += (double)((float)f[0][b] + ((float)f[4][b] + (float)f[8][b]));
+        else sum += (float)f[0][b];
       }
     }
-    totals[k] = sum;
+    totals[k] = (typename Ty::Sum)sum;
     if constexpr (IN == Q4G_I8) {
       xsl[k] = a.x_scales[(size_t)t * a.x_per + (a.x_per == 1 ? 0 : min(c * M + u * M / UNITS, a.x_per - 1))];
     }

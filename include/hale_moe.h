@@ -614,7 +614,9 @@ int hale_q4g_download(hale_q4g *m, uint8_t *codes, void *scales, uint8_t *zeros)
 /* out[t][r] = sum_k weight[r][k] * x[t][k] for ntok tokens: d_x [ntok][cols] and d_out
  * [ntok][rows] of dtype (HALE_F32, HALE_F16, HALE_BF16), strides in elements from token
  * to token.  Each group's sum of products, and of x, is formed of exact products in
- * f32, and the groups' sums in f32; results are rounded once.  Equal calls give equal
+ * f32, and the groups' sums in f32; results are rounded once.  The products are with 16 + code, of
+ * which 16 + zero times the sum of x is taken off, so that f32 results are off by what three to
+ * ten roundings of 24 |scale| |x| come to (|x|: the root of a group's squares' sum).  Equal calls give equal
  * bits; a token's results do not depend on what the others hold (on how many they are,
  * in their last bits).  A token with a number that is not finite gives results that are
  * not finite (NaN where the formula has an infinity), and so may one with a number

@@ -5,7 +5,7 @@ import pytest
 
 import hale_moe as H
 from kv_model import NP, decode, encode
-from test_gpu_step_ops import bufs  # noqa: F401
+from test_gpu_step_ops import bufs, q4_model  # noqa: F401
 from test_gpu_step_ops_rounding import rounded
 
 pytestmark = pytest.mark.gpu
@@ -59,4 +59,29 @@ def test_q4_keeps_all_bits_of_a_token(ctx, bufs, dtype, ntok, rows, cols, group,
         low = ((np.abs(x).astype(np.float32) - top).view(np.uint32) & 0xffff0000).view(np.float32)
         lost = np.sign(x) * (top.astype(np.float64) + low)
         assert ((exact(lost) != exact(x)) | (q.T == 0)).mean() > 0.5
+    m.close()
+
+
+@pytest.mark.parametrize("ntok,rows,cols,group", [(16, 63, 2048, 128), (16, 63, 2048, 32), (16, 1000, 512, 64), (5, 100, 8192, 64), (50, 2000, 1056, 32),
+                                                  (5, 6150, 896, 128), (16, 16390, 1696, 32), (13, 16385, 4224, 128), (3, 20000, 1024, 64),
+                                                  (1141, 520, 416, 32), (1122, 517, 640, 128), (512, 2050, 384, 64)])
+def test_q4_errors_of_f32_tokens_in_the_mean(ctx, bufs, ntok, rows, cols, group):
+    """A group's sum of (16 + q) x is some 24 times the root of its squares' sum (16 + q is 24 in the mean of
+    squares), and so is (16 + zero) times its sum of x.  Each addition of 32 numbers' first parts rounds at that
+    size, group / 32 of them for either sum (those of the second and third parts round 2^-8 below, or in
+    64 bits), then the difference and the sum over groups: 2 group / 32 + 2 roundings of at
+    most 2^-24 of it each, evenly spread, 2^-24 / sqrt(3) in the mean of squares, and independent."""
+    rng = np.random.default_rng(ntok + rows + cols)
+    codes = rng.integers(0, 256, (rows, cols // 2), dtype=np.uint8)
+    raw, scales = encode(0.02 * np.exp(0.5 * rng.normal(size=(rows, cols // group))) * rng.choice([-1, 1], (rows, cols // group)), "f16")
+    z = rng.integers(0, 16, (rows, cols // group), dtype=np.uint8)
+    m = H.GroupQ4Matrix.new(ctx, rows, cols, group, codes, raw.view(np.uint16), z)
+    x = rng.normal(size=(ntok, cols)).astype(np.float32)
+    out = bufs.put(np.zeros((ntok, rows), np.float32))
+    m.matmul_device("f32", ntok, bufs.put(x), out)
+    got = bufs.get(out, np.float32, ntok * rows).reshape(ntok, rows).astype(np.float64)
+    want, _ = q4_model(codes, scales.astype(np.float64), z, group, x)
+    size = np.sqrt(np.square(x.astype(np.float64)).reshape(ntok, -1, group).sum(2) @ np.square(24 * scales.astype(np.float64)).T)
+    error = np.sqrt(np.square((got - want) / size).mean())
+    assert error <= 2.0 ** -24 / np.sqrt(3) * np.sqrt(2 * group / 32 + 2)
     m.close()
