@@ -185,6 +185,31 @@ void as_much_as_there_is_room_for() {
   for (const KvShareJoin& j : got.second.share_joins) CHECK(j.tok0 >= 500 && j.n == 2);
 }
 
+// 24 sequences of 16 rows each, whose shared pages go to the kernel of many rows and whose own, also where
+// they have nothing in common, do not: what a captured step has to launch both kernels for.
+void many_rows_by_sharing() {
+  const KvShape s{128, 16, 32};
+  for (bool f32 : {false, true}) {
+    const Step t = forks(s, f32 ? 5700 : 3000, each(24, 2), f32);
+    CHECK(!t.shared.many.empty() && !t.shared.few.empty() && t.apart.many.empty());
+    CHECK(kv_share_may_many(s, t.seqs, 94, f32));
+    KvPages pages;
+    pages.init(400, 24, 6000);
+    std::vector<uint32_t> seqs(24), n(24);
+    for (uint32_t k = 0; k < 24; k++) {
+      CHECK(pages.create(&seqs[k], &err) == KvPages::OK);
+      n[k] = 30 * k;
+    }
+    CHECK(pages.step(24, seqs.data(), n.data(), nullptr, &copies, &err) == KvPages::OK);
+    n = each(24, 2);
+    std::vector<KvStepSeq> plan;
+    CHECK(pages.step(24, seqs.data(), n.data(), &plan, &copies, &err) == KvPages::OK);
+    KvPlan p;
+    kv_plan_shared(s, plan, pages, 1, f32, &p);
+    CHECK(p.many.empty() && p.alone && p.share_joins.empty());
+  }
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -193,6 +218,7 @@ int main(int argc, char** argv) {
   else if (what == "many_rows") many_rows();
   else if (what == "nothing_shared") nothing_shared();
   else if (what == "as_much_as_there_is_room_for") as_much_as_there_is_room_for();
+  else if (what == "many_rows_by_sharing") many_rows_by_sharing();
   else return 2;
   return 0;
 }

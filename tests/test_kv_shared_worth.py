@@ -40,3 +40,7 @@ def test_plans_that_share_nothing_say_so(check):
 
 def test_as_much_is_shared_as_there_is_room_for(check):
     check("as_much_as_there_is_room_for")
+
+
+def test_steps_whose_many_rows_come_from_sharing(check):
+    check("many_rows_by_sharing")
