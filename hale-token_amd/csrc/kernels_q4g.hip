@@ -5,7 +5,9 @@
 // sum_k x[t][k]).  Within a group both sums are matrix products of whole numbers (16 + q, and
 // ones; the 16 goes with the zero) with x: of f16 and bf16 exactly, of f32 as three
 // bf16 parts that add up to it, of 8-bit codes in whole numbers.  Their accumulators and
-// the sum over groups are f32 (i32 within a unit of 8-bit codes).  Layout of the weights:
+// the sum over groups are f32 (i32 within a unit of 8-bit codes), rounded at the size of sums of 16 + q, some
+// five times that of q - zero: for f16 and bf16 far below a result's own rounding, for f32 what
+// products() and the streaming kernel's sums keep to few roundings.  Layout of the weights:
 // step_ops.h.
 #include <hip/hip_runtime.h>
 
@@ -616,9 +618,10 @@ template <int IN, int UNITS> struct Q4gStage {
 // four brings tokens 16 k .., each by 16 neighbouring lanes, and their sums); they are read
 // from memory two chunks ahead, and the weights one, to registers: so two waves share a SIMD (with
 // weights two ahead, one of them where groups are of 32: 512 tokens, 4096 x 4096, 69 us, 47 now).
-// 512 tokens of f16, 4096 x 4096, groups of 128, take 29 us, 592 TFLOP/s; 2048 100, 688.  Bound by the
-// vector units: for 512 cycles of products of a chunk and wave they work for 830, laying codes
-// out and scaling the groups' sums, and half of that is hidden.  128 tokens for each reading
+// 512 tokens of f16, 4096 x 4096, groups of 128, take 29 us, 592 TFLOP/s; 2048 100, 688.  By the
+// counters the vector units work for 43 % of the time, the matrix units for 30, and waves wait for 37: for
+// 512 cycles of products of a chunk and wave there are 830 of vector instructions, laying codes out and
+// scaling the groups' sums, and at its end a barrier that two waves a SIMD do not cover.  128 tokens for each reading
 // of the weights leave room for one wave (120 us for 2048).
 template <int IN, int PER, int M, bool BF, int RT, int WK>
 __global__ __launch_bounds__(256 * WK, IN == Q4G_F32 ? 1 : 2) void k_q4g_many(Q4gArgs a, unsigned token_tiles) {
@@ -826,8 +829,8 @@ static hipError_t q4g_many(const Q4gArgs& a, hipStream_t st) {
 //            32, 128                 6.9, 19 (14.8, 43)    28, 28 (76, 77)
 //   14336    1, 16    14.3 (18)      9.4, 13 (19, 28)
 //            32                      21 (43)               29 (76)
-//   24576    1        14.7 (19.7)    15.8 (31.5)
-//   151936   1, 16    60, 68 (81, 252 in slices)   87, 116 (185, 306)
+//   24576    1        14.9 (20.8)    15.8 (31.5)
+//   151936   1, 16    60, 68 (81, 253 in slices)   87, 116 (185, 306)
 // The streaming kernel gives each wave a tile or nearly so, and its tokens have to fit into LDS
 // (Q4G_LDS), f32 ones in three slices at most, each with all weights: still faster than the other of
 // few, whose time grows with the tokens.  Beyond 16 tokens the others work in slices of 16

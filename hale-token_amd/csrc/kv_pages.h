@@ -125,8 +125,10 @@ class KvPages;
 void kv_plan(const KvShape& s, const std::vector<KvStepSeq>& seqs, size_t window, bool f32, KvPlan* out);
 
 // The same for window 0 where sequences that stand side by side in the step hold the same
-// first pages, at least min_pages of them: the pages are attended over once for all of
-// the sequences' rows, and again so among those that share more behind them.
+// first pages, at least min_pages of them: the pages are attended over for all of
+// the sequences' rows together, once for each tile of them (16 rows, or 32, in the kernel of few, kv_many_rows in
+// that of many), and again so among those that share more behind them.  Runs that this does not
+// save pages for, and what there is no room for, stay apart.
 void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const KvPages& pages, size_t min_pages,
                     bool f32, KvPlan* out);
 // Sequences with new tokens in a step up to which pages are shared: finding out who
@@ -135,7 +137,9 @@ constexpr size_t KV_SHARE_SEQS = 1024;
 // Whether sequences of a step of these numbers of tokens may share pages at all.
 bool kv_may_share(const std::vector<KvStepSeq>& seqs);
 constexpr size_t KV_SHARE_PARTS = 1024;  // of a row, over all its series
-// Work-groups of few rows that a step which shares pages is divided into.
+// Work-groups of few rows that a step's pages are divided for where it may share them: the longest part has
+// as many pages as this makes; what is left over of shared pages and of each sequence's own, mostly shorter, adds
+// others (32 sequences behind 8000, 8 heads: 256 of shared pages, 256 of their own).
 constexpr size_t KV_SHARE_GROUPS = 256;
 // The pages that one launch of the kernel of few rows takes of shared ones, counted for each 16
 // rows.  Above it, runs of more than 64 rows go to the kernel of many, a launch more that

@@ -943,7 +943,8 @@ class KvCache:
 
     def share_prefixes(self, min_len: int):
         """Attention over pages that neighbours in a step have in common, min_len
-        positions or more, is computed once for all of them (0: never)."""
+        positions or more, is computed for all of them together (0: never); worth it
+        from about 1000 positions on."""
         self._check(lib().hale_kv_share_prefixes(self.handle, min_len), "share_prefixes")
 
     def step(self, seqs, ntok):

@@ -615,7 +615,7 @@ int hale_q4g_download(hale_q4g *m, uint8_t *codes, void *scales, uint8_t *zeros)
  * [ntok][rows] of dtype (HALE_F32, HALE_F16, HALE_BF16), strides in elements from token
  * to token.  Each group's sum of products, and of x, is formed of exact products in
  * f32, and the groups' sums in f32; results are rounded once.  The products are with 16 + code, of
- * which 16 + zero times the sum of x is taken off, so that f32 results are off by what three to
+ * which 16 + zero times the sum of x is taken off, so that f32 results are off by what four to
  * ten roundings of 24 |scale| |x| come to (|x|: the root of a group's squares' sum).  Equal calls give equal
  * bits; a token's results do not depend on what the others hold (on how many they are,
  * in their last bits).  A token with a number that is not finite gives results that are
@@ -755,13 +755,14 @@ int hale_kv_resize(hale_kv_cache *kv, size_t num_pages);
  * key/value head, tokens times the heads that share it; 32 where a sequence of the step has more than 16), or
  * for every 128 (head_dim above 128: 64) where that is much, and not for each sequence apart; and those that
  * some of them share behind these likewise (on up to three levels, each of min_len positions more; in steps of
- * up to 1024 sequences with tokens).  Sequences of few rows (up to 16, in small steps up to 64) and of more
+ * up to 1024 sequences with tokens).  Sequences of few rows (up to 16 to 64, by the step's size and type) and of more
  * share among their like, the latter where the pages saved are worth it: prompts of several hundred tokens fill
  * tiles of their own and share nothing.  Where the cache's workspace has no room for all partial results the
  * deepest levels, then the shortest prefixes are not shared.  Sharing costs a launch that joins the
  * results, some 4 us, which short prefixes need not have: from about 1000 positions on it is
  * worth it.  Forks (hale_kv_seq_fork) share so what their origin held.  Results are the same but for
- * the order of sums, so for their last bits.  0, the default: never.  A changed setting ends the current
+ * the order of sums, so for their last bits (a captured step's too, beside an eager one's, where nothing is shared).
+ * 0, the default: never.  A changed setting ends the current
  * step, and graphs that use the cache have to be captured anew. */
 int hale_kv_share_prefixes(hale_kv_cache *kv, size_t min_len);
 
