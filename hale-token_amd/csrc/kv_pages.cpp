@@ -517,9 +517,8 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
     tokens += q.ntok;
   }
   const size_t room = kv_max_items(s, tokens, seqs.size());
-  int levels = KV_SHARE_LEVELS;
   std::vector<Shared> shared;
-  find_shared(with, s, limit, pages, min_pages, levels, &shared);
+  find_shared(with, s, limit, pages, min_pages, KV_SHARE_LEVELS, &shared);
   for (;;) {  // with less sharing where its partial results or lists exceed what there is room for
     out->few.clear();
     out->many.clear();
@@ -591,11 +590,12 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
     if (!shared.empty() && (rows > most_rows || longest > KV_SHARE_PARTS || items[0] > room || items[1] > room)) {
       // the deepest level first, then of the runs those of the fewest pages (what a row saves by its partial
       // results), as many as they are for too many rows
-      if (--levels > 0) {
-        find_shared(with, s, limit, pages, min_pages, levels, &shared);
+      size_t depth = 0;
+      for (const auto& o : over) depth = std::max(depth, o.size());
+      if (depth > 1) {
+        find_shared(with, s, limit, pages, min_pages, (int)depth - 1, &shared);
         continue;
       }
-      levels = 1;
       std::stable_sort(shared.begin(), shared.end(), [](const Shared& a, const Shared& b) { return a.page1 < b.page1; });
       size_t n = 0;
       do rows -= std::min(rows, (size_t)shared[n].rows * (shared[n].parts + 1) * s.kv_heads);
