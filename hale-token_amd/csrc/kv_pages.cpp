@@ -517,8 +517,17 @@ void kv_plan_shared(const KvShape& s, const std::vector<KvStepSeq>& seqs, const 
     tokens += q.ntok;
   }
   const size_t room = kv_max_items(s, tokens, seqs.size());
+  // A step whose tiles apart are all of up to four pages, a page to a wave, and run at once has no joins and
+  // nothing to gain: sharing would only add the launch of one (8 sequences behind 128, 32 heads of 128 on
+  // 4, bf16, 6.3 us and 9.9).
+  size_t longest_apart = 0, pages_apart = 0;
+  for (const KvStepSeq* q : with) {
+    const size_t n = (q->len0 + q->ntok - 1) / KV_PAGE + 1, rows = q->ntok * group;
+    longest_apart = std::max(longest_apart, n);
+    pages_apart += n * ceil_div(rows, rows <= limit ? few_rows : many_rows) * s.kv_heads;
+  }
   std::vector<Shared> shared;
-  find_shared(with, s, limit, pages, min_pages, KV_SHARE_LEVELS, &shared);
+  if (longest_apart > 4 || pages_apart > 4 * KV_FEW_GROUPS) find_shared(with, s, limit, pages, min_pages, KV_SHARE_LEVELS, &shared);
   for (;;) {  // with less sharing where its partial results or lists exceed what there is room for
     out->few.clear();
     out->many.clear();

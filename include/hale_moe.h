@@ -759,8 +759,8 @@ int hale_kv_resize(hale_kv_cache *kv, size_t num_pages);
  * share among their like, the latter where the pages saved are worth it: prompts of several hundred tokens fill
  * tiles of their own and share nothing.  Where the cache's workspace has no room for all partial results the
  * deepest levels, then the shortest prefixes are not shared.  Sharing costs a launch that joins the
- * results, some 4 us, which short prefixes need not have: from about 1000 positions on it is
- * worth it.  Forks (hale_kv_seq_fork) share so what their origin held.  Results are the same but for
+ * results, some 4 us, which steps of short sequences (up to 256 positions each, 2048 pages of all rows' tiles)
+ * need not have: these share nothing.  Prefixes of about 1000 positions and more are worth it.  Forks (hale_kv_seq_fork) share so what their origin held.  Results are the same but for
  * the order of sums, so for their last bits (a captured step's too, beside an eager one's, where nothing is shared).
  * 0, the default: never.  A changed setting ends the current
  * step, and graphs that use the cache have to be captured anew. */

@@ -77,12 +77,16 @@ void no_more_pages() {
     const bool f32 = rng() % 2;
     const Step t = forks({kv * group, kv, 64u << rng() % 3}, prompt, ntok, f32, tails);
     CHECK(reads(t.shared) <= reads(t.apart));
-    // two neighbours whose rows fit into one tile of the 16 that the kernel of few takes at least
-    bool saves = false;
+    // two neighbours whose rows fit into one tile of the 16 that the kernel of few takes at least, in a step
+    // that is long enough
+    bool saves = false, long_one = false;
     size_t before = 1000;
-    for (uint32_t n : ntok)
-      if (n) saves |= (n + before) * group <= 16, before = n;
-    CHECK(!(saves && prompt >= KV_PAGE) || reads(t.shared) < reads(t.apart));
+    for (size_t i = 0; i < ntok.size(); i++)
+      if (ntok[i]) {
+        saves |= (ntok[i] + before) * group <= 16, before = ntok[i];
+        long_one |= prompt + tails[i] + ntok[i] > 4 * KV_PAGE;
+      }
+    CHECK(!(saves && long_one && prompt >= KV_PAGE) || reads(t.shared) < reads(t.apart));
   }
 }
 
@@ -210,6 +214,21 @@ void many_rows_by_sharing() {
   }
 }
 
+// Steps of short sequences, a few pages each, stay apart and need no joins; more or longer ones share.
+void short_steps() {
+  const KvShape s{32, 4, 128};
+  for (bool f32 : {false, true}) {
+    const Step a = forks(s, 200, each(8, 1), f32, each(8, 55));  // 256 positions with the new token
+    CHECK(a.shared.alone && a.shared.share_joins.empty() && reads(a.shared) == reads(a.apart) && a.apart.few_joins.empty());
+    std::vector<uint32_t> tails = each(8, 55);
+    tails[3] = 56;
+    const Step b = forks(s, 200, each(8, 1), f32, tails);  // one of 257
+    CHECK(!b.shared.alone && reads(b.shared) < reads(b.apart));
+    const Step c = forks(s, 200, each(200, 1), f32, each(200, 55));  // 800 tiles of four pages
+    CHECK(!c.shared.alone && reads(c.shared) < reads(c.apart));
+  }
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -219,6 +238,7 @@ int main(int argc, char** argv) {
   else if (what == "nothing_shared") nothing_shared();
   else if (what == "as_much_as_there_is_room_for") as_much_as_there_is_room_for();
   else if (what == "many_rows_by_sharing") many_rows_by_sharing();
+  else if (what == "short_steps") short_steps();
   else return 2;
   return 0;
 }

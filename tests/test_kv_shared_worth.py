@@ -44,3 +44,7 @@ def test_as_much_is_shared_as_there_is_room_for(check):
 
 def test_steps_whose_many_rows_come_from_sharing(check):
     check("many_rows_by_sharing")
+
+
+def test_steps_of_short_sequences_stay_apart(check):
+    check("short_steps")
