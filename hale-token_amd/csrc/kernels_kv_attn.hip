@@ -835,14 +835,21 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a) {
 // groups of threads take every so many'th part of the series laid end to end, four numbers of
 // the head dimension a thread, and put theirs together in LDS in the slices' order.  A chain of
 // three reads: 4.7 us for 32 sequences, 32 heads of 128, four shared parts and one or two of their own
-// (a launch alone 3.5).
+// (a launch alone 3.5).  Of many parts the places, maxima and sums are brought to LDS by all of a row's threads
+// first, which changes no result: 2 sequences behind 11000, 2 heads of 128, f16, 45 parts, with the attention 12.9
+// us, 13.8 where each slice looks for its own.  (A work-group a row, as in k_kv_join, or eight parts at a
+// time take 100 registers for 70: 11.2, but 32 sequences of 40 rows behind 4000 40.9 for 37.5.)
 constexpr int SHARE_SLICES = 4;
+constexpr unsigned SHARE_WIDE = 16, SHARE_STAGED = 256;  // many: more than the first, up to the second
 static_assert(KV_SHARE_PARTS <= 1u << JOIN_BITS, "the sum of a row's parts");
 
 __global__ __launch_bounds__(256) void k_kv_join_shared(KvAttnArgs a) {
   constexpr int S = SHARE_SLICES;
+  constexpr int PER = 256 / 16 / S;  // rows at most
   __shared__ f32x4 sv[256];
   __shared__ float2 sml[256];
+  __shared__ unsigned at_part[PER][SHARE_STAGED];
+  __shared__ float2 ml_part[PER][SHARE_STAGED];
   const int t = threadIdx.x;
   const int quads = a.g.hd / 4, lanes = quads <= 16 ? 16 : quads <= 32 ? 32 : 64, x = t % lanes;
   const int slice = t / lanes % S, per = 256 / lanes / S;
@@ -851,36 +858,65 @@ __global__ __launch_bounds__(256) void k_kv_join_shared(KvAttnArgs a) {
     const KvShareJoin join = a.share_joins[it];
     const unsigned row = blockIdx.y * per + t / lanes / S;
     const bool mine = row < join.rows && x < quads;
+    unsigned parts = 0;
+#pragma unroll
+    for (int s = 0; s <= KV_SHARE_LEVELS; s++) parts += s < (int)join.n ? join.of[s].parts : 0;
     float top = -__builtin_inff(), most = 0.0f, total = 0.0f;
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     int e = 0;
-    if (mine) {
-      auto each = [&](auto&& f) {
-        unsigned from = slice;
-#pragma unroll
-        for (int s = 0; s <= KV_SHARE_LEVELS; s++) {
-          if (s >= (int)join.n) break;
-          const KvSeries& r = join.of[s];
-#pragma unroll 4
-          for (; from < r.parts; from += S) f((size_t)r.part0 + row + (size_t)from * r.step);
-          from -= r.parts;
-        }
-      };
-      each([&](size_t at) {
-        const float2 part = a.part_ml[at];
+    // the slice's parts, each by its place and its maximum and sum
+    auto slice_of = [&](auto&& each) {
+      each([&](size_t, float2 part) {
         top = fmaxf(top, part.x);
         most = fmaxf(most, part.y);
       });
       e = above(most) + JOIN_BITS;  // 2^e is above the sum
       const float base2 = top == -__builtin_inff() ? 0.0f : top;
-      each([&](size_t at) {
-        const float2 part = a.part_ml[at];
+      each([&](size_t at, float2 part) {
         const float w = exp2_fast(part.x - base2);
         total += w * part.y;
         v = v + *(const f32x4*)(a.part_o + at * a.g.hd + 4 * x) * (w * pow2(above(part.y) - e));
       });
       // as large as values, times 2^-above(total)
       v = scaled(v, e - above(total));
+    };
+    if (parts > SHARE_WIDE && parts <= SHARE_STAGED) {
+      const int here = t / lanes / S, threads = lanes * S;
+      if (row < join.rows) {
+        for (unsigned k = t % threads; k < parts; k += threads) {
+          unsigned from = k, at = 0;
+#pragma unroll
+          for (int s = 0; s <= KV_SHARE_LEVELS; s++) {
+            const KvSeries& r = join.of[s];
+            const bool in = s < (int)join.n && from < r.parts;
+            if (in) at = r.part0 + row + from * r.step;
+            from = in || s >= (int)join.n ? 0xffffffffu : from - r.parts;
+          }
+          at_part[here][k] = at;
+          ml_part[here][k] = a.part_ml[at];
+        }
+      }
+      __syncthreads();
+      if (mine)
+        slice_of([&](auto&& f) {
+#pragma unroll 4
+          for (unsigned k = slice; k < parts; k += S) f((size_t)at_part[here][k], ml_part[here][k]);
+        });
+    } else if (mine) {
+      slice_of([&](auto&& f) {
+        unsigned from = slice;
+#pragma unroll
+        for (int s = 0; s <= KV_SHARE_LEVELS; s++) {
+          if (s >= (int)join.n) break;
+          const KvSeries& r = join.of[s];
+#pragma unroll 4
+          for (; from < r.parts; from += S) {
+            const size_t at = (size_t)r.part0 + row + (size_t)from * r.step;
+            f(at, a.part_ml[at]);
+          }
+          from -= r.parts;
+        }
+      });
     }
     __syncthreads();  // the join before is read
     sv[t] = v;

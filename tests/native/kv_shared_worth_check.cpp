@@ -229,6 +229,35 @@ void short_steps() {
   }
 }
 
+// Rows of more parts than the join brings to LDS at once (256), over three levels of a long history.
+void many_parts() {
+  const KvShape s{2, 1, 16};
+  KvPages pages;
+  pages.init(1100, 8, 66000);
+  uint32_t root, two[2], three[2], four;
+  const auto step = [&](std::vector<uint32_t> seqs, std::vector<uint32_t> n, std::vector<KvStepSeq>* plan = nullptr) {
+    CHECK(pages.step(seqs.size(), seqs.data(), n.data(), plan, &copies, &err) == KvPages::OK);
+  };
+  CHECK(pages.create(&root, &err) == KvPages::OK);
+  step({root}, {337 * 64});
+  CHECK(pages.fork(root, 2, two, &err) == KvPages::OK);
+  step({two[1]}, {341 * 64});
+  CHECK(pages.fork(two[1], 2, three, &err) == KvPages::OK);
+  step({three[1]}, {341 * 64});
+  CHECK(pages.fork(three[1], 1, &four, &err) == KvPages::OK);
+  std::vector<KvStepSeq> plan;
+  step({two[0], three[0], three[1], four}, each(4, 1), &plan);
+  KvPlan p;
+  kv_plan_shared(s, plan, pages, 1, true, &p);
+  size_t most = 0;
+  for (const KvShareJoin& j : p.share_joins) {
+    size_t n = 0;
+    for (uint32_t k = 0; k < j.n; k++) n += j.of[k].parts;
+    most = std::max(most, n);
+  }
+  CHECK(most == 258);
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -239,6 +268,7 @@ int main(int argc, char** argv) {
   else if (what == "as_much_as_there_is_room_for") as_much_as_there_is_room_for();
   else if (what == "many_rows_by_sharing") many_rows_by_sharing();
   else if (what == "short_steps") short_steps();
+  else if (what == "many_parts") many_parts();
   else return 2;
   return 0;
 }

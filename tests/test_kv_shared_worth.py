@@ -48,3 +48,7 @@ def test_steps_whose_many_rows_come_from_sharing(check):
 
 def test_steps_of_short_sequences_stay_apart(check):
     check("short_steps")
+
+
+def test_rows_of_many_parts(check):
+    check("many_parts")
